@@ -32,6 +32,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -50,6 +51,11 @@ CUDA_SOURCES = [
     os.path.join(CSRC, "conv_simt.cu"),
     os.path.join(CSRC, "stage_heads.cu"),
     os.path.join(CSRC, "engine.cu"),
+    os.path.join(CSRC, "ops_api.cu"),
+    os.path.join(CSRC, "ops_gemm.cu"),
+    os.path.join(CSRC, "ops_embed.cu"),
+    os.path.join(CSRC, "ops_linear.cu"),
+    os.path.join(CSRC, "ops_cross_entropy.cu"),
     os.path.join(HOST, "net_weights.cpp"),
     os.path.join(HOST, "onnx_reader.cpp"),
 ]
@@ -59,7 +65,10 @@ CUDA_HEADERS = [
     os.path.join(CSRC, "trunk_schedule.cuh"),
     os.path.join(HOST, "net_weights.h"),
     os.path.join(HOST, "onnx_reader.h"),
+    os.path.join(CSRC, "ops_common.cuh"),
+    os.path.join(CSRC, "ops_gemm.cuh"),
     os.path.join(INCLUDE, "minigo_cuda.h"),
+    os.path.join(INCLUDE, "minigo_ops.h"),
 ]
 HOST_SOURCES = [
     os.path.join(HOST, "go_positions.cpp"),
@@ -143,10 +152,22 @@ def build_cuda(force: bool = False) -> str:
         if not os.path.exists(NVCC) and shutil.which("nvcc") is None:
             raise RuntimeError("nvcc not found; set CUDA_HOME")
         nvcc = NVCC if os.path.exists(NVCC) else "nvcc"
+        flags = [GENCODE, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
+                 "-Xcompiler", "-Wall"]
+        objects = os.path.join(LIB, "obj")
+        os.makedirs(objects, exist_ok=True)
+
+        def compile_one(source: str) -> str:
+            obj = os.path.join(objects, os.path.basename(source) + ".o")
+            if force or _stale(obj, [source] + CUDA_HEADERS):
+                _run([nvcc] + flags + ["-c", "-o", obj + ".tmp", source])
+                os.replace(obj + ".tmp", obj)
+            return obj
+
+        with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+            made = list(pool.map(compile_one, CUDA_SOURCES))
         tmp = CUDA_LIB + ".tmp"
-        _run([nvcc, GENCODE, "-O3", "-lineinfo", "-std=c++17", "-shared",
-              "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
-              "-o", tmp] + CUDA_SOURCES)
+        _run([nvcc, GENCODE, "-shared", "-o", tmp] + made)
         os.replace(tmp, CUDA_LIB)
     return CUDA_LIB
 

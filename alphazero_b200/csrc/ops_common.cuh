@@ -1,0 +1,127 @@
+// Shared by the training operators (include/minigo_ops.h): element types,
+// argument checks, workspace layout and errors.
+#pragma once
+
+#include "../../include/minigo_ops.h"
+
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <string>
+
+namespace mgb {
+namespace ops {
+
+// ---- element types ----
+
+template <int DT>
+struct Elem;
+template <>
+struct Elem<MG_PREC_BF16> {
+    using T = __nv_bfloat16;
+    static __device__ __forceinline__ float get(T v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ T put(float v) { return __float2bfloat16_rn(v); }
+};
+template <>
+struct Elem<MG_PREC_FP16> {
+    using T = __half;
+    static __device__ __forceinline__ float get(T v) { return __half2float(v); }
+    static __device__ __forceinline__ T put(float v) { return __float2half_rn(v); }
+};
+template <>
+struct Elem<MG_PREC_FP32> {
+    using T = float;
+    static __device__ __forceinline__ float get(T v) { return v; }
+    static __device__ __forceinline__ T put(float v) { return v; }
+};
+
+inline int elem_bytes(int dtype) { return dtype == MG_PREC_FP32 ? 4 : 2; }
+
+// A token or target, or -1 where it lies outside [0, limit).
+__device__ __forceinline__ int64_t index_at(const void* p, int bytes, int64_t i, int64_t limit) {
+    const int64_t t = bytes == 8 ? static_cast<const int64_t*>(p)[i]
+                                 : (int64_t)static_cast<const int32_t*>(p)[i];
+    return t >= 0 && t < limit ? t : -1;
+}
+
+// ---- host side ----
+
+struct OpFailure {
+    int code;
+    std::string what;
+};
+[[noreturn]] inline void fail(int code, const std::string& what) { throw OpFailure{code, what}; }
+inline void need(bool ok, const char* what) {
+    if (!ok) fail(MG_E_ARG, what);
+}
+inline void check(cudaError_t e, const char* where) {
+    if (e != cudaSuccess) fail(MG_E_CUDA, std::string(where) + ": " + cudaGetErrorString(e));
+}
+inline void launched(const char* kernel) { check(cudaGetLastError(), kernel); }
+
+// Makes args->device current for one call.
+class OnDevice {
+public:
+    explicit OnDevice(int device) {
+        check(cudaGetDevice(&prev_), "cudaGetDevice");
+        if (prev_ != device) check(cudaSetDevice(device), "cudaSetDevice");
+        now_ = device;
+    }
+    ~OnDevice() {
+        if (prev_ != now_) cudaSetDevice(prev_);
+    }
+
+private:
+    int prev_ = 0, now_ = 0;
+};
+
+// Lays buffers out one after another.  With a null base it only adds up the
+// bytes, so the size query and the call run the same code.
+class Workspace {
+public:
+    Workspace() = default;
+    Workspace(void* base, size_t bytes) : base_(static_cast<char*>(base)), bytes_(bytes) {}
+    template <class T = void>
+    T* take(size_t bytes) {
+        const size_t at = used_;
+        used_ += (bytes + 255) & ~size_t(255);
+        return base_ ? reinterpret_cast<T*>(base_ + at) : nullptr;
+    }
+    size_t used() const { return used_; }
+    void require() const {
+        need(used_ == 0 || base_ != nullptr, "workspace is null");
+        need((reinterpret_cast<uintptr_t>(base_) & 255) == 0, "workspace is not 256-byte aligned");
+        need(used_ <= bytes_, "workspace is smaller than the matching *_workspace call reports");
+    }
+
+private:
+    char* base_ = nullptr;
+    size_t bytes_ = 0, used_ = 0;
+};
+
+std::string& last_op_error();  // of the calling thread
+
+// Runs a C entry's body: any failure becomes a code and a message.
+template <class F>
+int guarded(F&& body) noexcept {
+    try {
+        body();
+        return MG_OK;
+    } catch (const OpFailure& f) {
+        try {
+            last_op_error() = f.what;
+        } catch (...) {
+        }
+        return f.code;
+    } catch (...) {
+        return MG_E_STATE;
+    }
+}
+
+// The device status word of these kernels (0, or a DeviceError of
+// ptx_sm100.cuh from a wait that gave up) on the current device.
+int* op_status_word();
+
+}  // namespace ops
+}  // namespace mgb

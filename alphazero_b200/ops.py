@@ -1,0 +1,400 @@
+"""Training operators of a move-sequence policy over torch CUDA tensors:
+embedding lookup, linear layer and linear cross entropy, each with its
+gradient, over the C ABI of include/minigo_ops.h (libminigo_cuda.so).
+
+Every function enqueues its kernels on the current stream of the tensors'
+device and returns without waiting, like torch's own; scratch comes from
+torch's allocator.  Inputs are read where they lie, with any strides; outputs
+are new dense tensors of the inputs' type.  Arguments that do not fit raise
+ValueError (wrong shapes or values) or TypeError (wrong types or devices);
+failures of the library raise RuntimeError.  There is no CPU fallback.
+
+``embedding``, ``linear_layer`` and ``cross_entropy_loss`` are the same
+operators for torch's autograd.  The reference trains with torch on its own
+(scripts/train.py) and has no counterpart.
+"""
+from __future__ import annotations
+
+import ctypes
+import struct
+
+import torch
+
+from . import engine
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_INDEX_BYTES = {torch.int64: 8, torch.int32: 4}
+
+# The argument structs of minigo_ops.h, field by field.
+_EMBED = struct.Struct("3P5qf3i")
+_EMBED_BACKWARD = struct.Struct("3P5qf3i")
+_LINEAR = struct.Struct("6P9qf3i")
+_LINEAR_BACKWARD = struct.Struct("7P11q4i")
+_CROSS_ENTROPY = struct.Struct("9P8qf3i")
+
+_LIB = None
+
+
+def lib() -> ctypes.CDLL:
+    """libminigo_cuda.so with the operators' signatures."""
+    global _LIB
+    if _LIB is None:
+        L = engine.lib()
+        vp = ctypes.c_void_p
+        size = ctypes.POINTER(ctypes.c_size_t)
+        L.mg_op_error.restype = ctypes.c_char_p
+        L.mg_op_error.argtypes = []
+        L.mg_op_synchronize.argtypes = [ctypes.c_int, vp]
+        L.mg_embed.argtypes = [vp, vp]
+        for name in ("mg_embed_backward", "mg_linear", "mg_linear_backward", "mg_cross_entropy"):
+            getattr(L, name).argtypes = [vp, vp, ctypes.c_size_t, vp]
+            getattr(L, name + "_workspace").argtypes = [vp, size]
+        _LIB = L
+    return _LIB
+
+
+def _raise(code: int):
+    message = lib().mg_op_error().decode() or f"error {code}"
+    raise ValueError(message) if code == -1 else RuntimeError(message)
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _call(name: str, args: bytes, device: torch.device) -> None:
+    L = lib()
+    need = ctypes.c_size_t()
+    code = getattr(L, name + "_workspace")(args, ctypes.byref(need))
+    if code:
+        _raise(code)
+    stream = torch.cuda.current_stream(device)
+    # torch's allocator orders the block's reuse after this stream's work
+    w = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+    code = getattr(L, name)(args, w.data_ptr() if w is not None else None, need.value,
+                            stream.cuda_stream)
+    if code:
+        _raise(code)
+
+
+def synchronize(device=None) -> None:
+    """Waits for the current stream; raises RuntimeError if a kernel of these
+    operators gave up a bounded wait (its outputs are then invalid)."""
+    d = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    code = lib().mg_op_synchronize(d.index if d.index is not None else torch.cuda.current_device(),
+                                   _stream(d))
+    if code:
+        _raise(code)
+
+
+# ---- argument checks ----
+
+def _on_gpu(t, name: str) -> torch.device:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor, not {type(t).__name__}")
+    if t.device.type != "cuda":
+        raise TypeError(f"{name} must be a CUDA tensor (it is on {t.device})")
+    return t.device
+
+
+def _same(t, name: str, like, what: str) -> None:
+    if _on_gpu(t, name) != like.device:
+        raise TypeError(f"{name} is on {t.device}, {what} on {like.device}")
+    if t.dtype != like.dtype:
+        raise TypeError(f"{name} is {t.dtype}, {what} {like.dtype}")
+
+
+def _dtype(t, name: str, wide: bool) -> int:
+    code = _DTYPES.get(t.dtype)
+    if code is None or (code == 2 and not wide):
+        raise TypeError(f"{name} must be bfloat16{', float16 or float32' if wide else ' or float16'}, "
+                        f"not {t.dtype}")
+    return code
+
+
+def _indices(t, name: str, like) -> int:
+    if _on_gpu(t, name) != like.device:
+        raise TypeError(f"{name} is on {t.device}, expected {like.device}")
+    b = _INDEX_BYTES.get(t.dtype)
+    if b is None:
+        raise TypeError(f"{name} must be int64 or int32, not {t.dtype}")
+    return b
+
+
+def _matrix(t, name: str, cols=None):
+    """t [..., cols] as [rows, cols]; a copy only where the leading
+    dimensions cannot be one."""
+    if t.dim() < 1:
+        raise ValueError(f"{name} must have at least one dimension")
+    if cols is not None and t.shape[-1] != cols:
+        raise ValueError(f"{name} has {t.shape[-1]} columns, expected {cols}")
+    if t.dim() == 2:
+        return t
+    if t.shape[-1] == 0:
+        raise ValueError(f"{name} has no columns")
+    return t.reshape(-1, t.shape[-1])
+
+
+def _weight(t, name: str, like, what: str):
+    _same(t, name, like, what)
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be a matrix, not {tuple(t.shape)}")
+    return t
+
+
+def _vector(t, name: str, n: int, like, what: str):
+    _same(t, name, like, what)
+    if t.shape != (n,):
+        raise ValueError(f"{name} must have shape ({n},), not {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def _rows(t):
+    """t with unit column stride."""
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _activation(name: str) -> int:
+    if name not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, not {name!r}")
+    return ACTIVATIONS[name]
+
+
+# ---- embedding ----
+
+def embed(tokens, table, scale: float = 1.0):
+    """``scale * table[tokens]``: tokens [...] int64 or int32, table
+    [vocab, dim] bfloat16, float16 or float32 -> [..., dim].  A token outside
+    [0, vocab) is padding and gives a zero row."""
+    _on_gpu(table, "table")
+    dt = _dtype(table, "table", True)
+    tb = _indices(tokens, "tokens", table)
+    if table.dim() != 2:
+        raise ValueError(f"table must be a matrix, not {tuple(table.shape)}")
+    vocab, dim = table.shape
+    t = tokens.reshape(-1)
+    table = _rows(table)
+    out = torch.empty(tokens.shape + (dim,), dtype=table.dtype, device=table.device)
+    n = t.numel()
+    code = lib().mg_embed(_EMBED.pack(t.data_ptr(), table.data_ptr(), out.data_ptr(), n, vocab, dim,
+                                      t.stride(0) if n > 1 else 1, table.stride(0), scale, dt, tb,
+                                      table.device.index), _stream(table.device))
+    if code:
+        _raise(code)
+    return out
+
+
+def embed_backward(grad, tokens, vocab: int, scale: float = 1.0):
+    """Gradient of ``embed`` with respect to its table: [vocab, dim], the
+    rows of grad [..., dim] summed by token in 32 bits, times scale."""
+    _on_gpu(grad, "grad")
+    dt = _dtype(grad, "grad", True)
+    tb = _indices(tokens, "tokens", grad)
+    if grad.shape[:-1] != tokens.shape:
+        raise ValueError(f"grad {tuple(grad.shape)} does not match tokens {tuple(tokens.shape)}")
+    g = _rows(_matrix(grad, "grad"))
+    t = tokens.reshape(-1)
+    n, dim = g.shape
+    out = torch.empty((vocab, dim), dtype=grad.dtype, device=grad.device)
+    _call("mg_embed_backward",
+          _EMBED_BACKWARD.pack(t.data_ptr(), g.data_ptr(), out.data_ptr(), n, vocab, dim,
+                               t.stride(0) if n > 1 else 1, g.stride(0), scale, dt, tb,
+                               grad.device.index), grad.device)
+    return out
+
+
+# ---- linear layer ----
+
+def linear(x, weight, bias=None, residual=None, activation: str = "none",
+           residual_scale: float = 1.0, keep_preactivation: bool = False):
+    """``act(x @ weight.T + bias) + residual_scale * residual`` in one pass:
+    x [..., k], weight [n, k], bias [n], residual [..., n] -> [..., n], in
+    bfloat16 or float16 with 32-bit sums.  activation is "none", "relu",
+    "silu" or "gelu" (the erf form).  With keep_preactivation returns
+    (y, z), z = x @ weight.T + bias being what ``linear_backward`` needs."""
+    _on_gpu(x, "x")
+    dt = _dtype(x, "x", False)
+    act = _activation(activation)
+    _weight(weight, "weight", x, "x")
+    n, k = weight.shape
+    x2 = _matrix(x, "x", k)
+    m = x2.shape[0]
+    b = None if bias is None else _vector(bias, "bias", n, x, "x")
+    shape = x.shape[:-1] + (n,)
+    r, r_row, r_col = None, 0, 0
+    if residual is not None:
+        _same(residual, "residual", x, "x")
+        if residual.shape != shape:
+            raise ValueError(f"residual must have shape {tuple(shape)}, not {tuple(residual.shape)}")
+        r = _matrix(residual, "residual")
+        r_row, r_col = r.stride()
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    z = torch.empty(shape, dtype=x.dtype, device=x.device) if keep_preactivation else None
+    x_row, x_col = x2.stride()
+    w_row, w_col = weight.stride()
+    _call("mg_linear",
+          _LINEAR.pack(x2.data_ptr(), weight.data_ptr(), _ptr(b), _ptr(r), y.data_ptr(), _ptr(z),
+                       m, n, k, x_row, x_col, w_row, w_col, r_row, r_col, residual_scale, act, dt,
+                       x.device.index), x.device)
+    return (y, z) if keep_preactivation else y
+
+
+def linear_backward(grad, x, weight, preactivation=None, activation: str = "none", bias: bool = True):
+    """Gradients (dx, dw, db) of ``linear`` from grad = dL/dy [..., n] and
+    the z that it kept (needed unless activation is "none"); db is None with
+    bias=False.  The residual's gradient is residual_scale * grad."""
+    _on_gpu(grad, "grad")
+    dt = _dtype(grad, "grad", False)
+    act = _activation(activation)
+    _same(x, "x", grad, "grad")
+    _weight(weight, "weight", grad, "grad")
+    n, k = weight.shape
+    g, x2 = _matrix(grad, "grad", n), _matrix(x, "x", k)
+    if grad.shape[:-1] != x.shape[:-1]:
+        raise ValueError(f"grad {tuple(grad.shape)} does not match x {tuple(x.shape)}")
+    z, z_row, z_col = None, 0, 0
+    if act:
+        if preactivation is None:
+            raise ValueError(f"the backward pass of {activation!r} needs the preactivation")
+        _same(preactivation, "preactivation", grad, "grad")
+        if preactivation.shape != grad.shape:
+            raise ValueError(f"preactivation must have shape {tuple(grad.shape)}, not "
+                             f"{tuple(preactivation.shape)}")
+        z = _matrix(preactivation, "preactivation")
+        z_row, z_col = z.stride()
+    m = g.shape[0]
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dw = torch.empty((n, k), dtype=x.dtype, device=x.device)
+    db = torch.empty((n,), dtype=x.dtype, device=x.device) if bias else None
+    g_row, g_col = g.stride()
+    x_row, x_col = x2.stride()
+    w_row, w_col = weight.stride()
+    _call("mg_linear_backward",
+          _LINEAR_BACKWARD.pack(g.data_ptr(), x2.data_ptr(), weight.data_ptr(), _ptr(z),
+                                dx.data_ptr(), dw.data_ptr(), _ptr(db), m, n, k, g_row, g_col,
+                                x_row, x_col, w_row, w_col, z_row, z_col, act, dt, x.device.index,
+                                0), x.device)
+    return dx, dw, db
+
+
+# ---- linear cross entropy ----
+
+def _cross_entropy(x, weight, targets, bias, grad_scale, gradients):
+    _on_gpu(x, "x")
+    dt = _dtype(x, "x", False)
+    _weight(weight, "weight", x, "x")
+    vocab, dim = weight.shape
+    x2 = _matrix(x, "x", dim)
+    tb = _indices(targets, "targets", x)
+    if targets.shape != x.shape[:-1]:
+        raise ValueError(f"targets {tuple(targets.shape)} do not match x {tuple(x.shape)}")
+    t = targets.reshape(-1)
+    n = t.numel()
+    b = None if bias is None else _vector(bias, "bias", vocab, x, "x")
+    # the loss and the row losses in one allocation
+    both = torch.empty(n + 1, dtype=torch.float32, device=x.device)
+    loss, rows = both[n], both[:n].view(targets.shape)
+    dx = dw = db = None
+    if gradients:
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dw = torch.empty((vocab, dim), dtype=x.dtype, device=x.device)
+        db = torch.empty((vocab,), dtype=x.dtype, device=x.device) if b is not None else None
+    x_row, x_col = x2.stride()
+    w_row, w_col = weight.stride()
+    _call("mg_cross_entropy",
+          _CROSS_ENTROPY.pack(x2.data_ptr(), weight.data_ptr(), _ptr(b), t.data_ptr(),
+                              loss.data_ptr(), rows.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db),
+                              n, vocab, dim, x_row, x_col, w_row, w_col,
+                              t.stride(0) if n > 1 else 1, grad_scale, dt, tb, x.device.index),
+          x.device)
+    return loss, rows, dx, dw, db
+
+
+def linear_cross_entropy(x, weight, targets, bias=None):
+    """(loss, row_loss) of softmax(x @ weight.T + bias) against target
+    indices, without keeping the logits: x [..., dim], weight [vocab, dim],
+    bias [vocab] (-inf bans an entry), targets [...] int64 or int32; the
+    losses are float32.  A target outside [0, vocab) leaves its row out
+    (row_loss 0); loss is the mean over the other rows, 0 if there is none."""
+    return _cross_entropy(x, weight, targets, bias, 1.0, False)[:2]
+
+
+def linear_cross_entropy_grad(x, weight, targets, bias=None, grad_scale: float = 1.0):
+    """(loss, row_loss, dx, dw, db): ``linear_cross_entropy`` and the
+    gradients of grad_scale * loss (db None without a bias) in one call.
+    float16 gradients need a grad_scale that keeps them in range."""
+    return _cross_entropy(x, weight, targets, bias, float(grad_scale), True)
+
+
+# ---- autograd ----
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, table, scale):
+        ctx.save_for_backward(tokens)
+        ctx.vocab, ctx.scale = table.shape[0], scale
+        return embed(tokens, table, scale)
+
+    @staticmethod
+    def backward(ctx, grad):
+        (tokens,) = ctx.saved_tensors
+        return None, embed_backward(grad, tokens, ctx.vocab, ctx.scale), None
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation, residual_scale):
+        keep = activation != "none"
+        out = linear(x, weight, bias, residual, activation, residual_scale, keep)
+        y, z = out if keep else (out, None)
+        ctx.save_for_backward(x, weight, z)
+        ctx.activation, ctx.residual_scale = activation, residual_scale
+        ctx.has_bias, ctx.has_residual = bias is not None, residual is not None
+        return y
+
+    @staticmethod
+    def backward(ctx, grad):
+        x, weight, z = ctx.saved_tensors
+        dx, dw, db = linear_backward(grad, x, weight, z, ctx.activation, ctx.has_bias)
+        dr = grad * ctx.residual_scale if ctx.has_residual else None
+        return dx, dw, db, dr, None, None
+
+
+class _CrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, targets, grad_scale):
+        if not any(ctx.needs_input_grad):
+            return linear_cross_entropy(x, weight, targets, bias)[0]
+        loss, _, dx, dw, db = linear_cross_entropy_grad(x, weight, targets, bias, grad_scale)
+        ctx.save_for_backward(dx, dw, db)
+        ctx.grad_scale = grad_scale
+        return loss
+
+    @staticmethod
+    def backward(ctx, grad):
+        factor = grad / ctx.grad_scale
+        dx, dw, db = (None if t is None else (t * factor).to(t.dtype) for t in ctx.saved_tensors)
+        return dx, dw, db, None, None
+
+
+def embedding(tokens, table, scale: float = 1.0):
+    """``embed`` for autograd."""
+    return _Embedding.apply(tokens, table, float(scale))
+
+
+def linear_layer(x, weight, bias=None, residual=None, activation: str = "none",
+                 residual_scale: float = 1.0):
+    """``linear`` for autograd."""
+    return _Linear.apply(x, weight, bias, residual, activation, float(residual_scale))
+
+
+def cross_entropy_loss(x, weight, targets, bias=None, grad_scale: float = 1.0):
+    """The loss of ``linear_cross_entropy`` for autograd.  The gradients are
+    made with the loss, of grad_scale * loss, and multiplied by the incoming
+    gradient / grad_scale when the backward pass reaches them."""
+    return _CrossEntropy.apply(x, weight, bias, targets, float(grad_scale))
