@@ -10,11 +10,34 @@ namespace {
 __device__ int g_op_status;
 constexpr int kMaxDevices = 64;
 
+template <int DT>
+__global__ void __launch_bounds__(256) add_rows_kernel(const float* sums, int64_t rows, int64_t cols, float alpha,
+                                                       const int* count, typename Elem<DT>::T* out) {
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= cols) return;
+    float s = 0.0f;
+#pragma unroll 8
+    for (int64_t r = 0; r < rows; ++r) s += sums[r * cols + c];
+    out[c] = Elem<DT>::put(s * (count ? alpha / (float)max(*count, 1) : alpha));
+}
+
 }  // namespace
 
 std::string& last_op_error() {
     thread_local std::string message;
     return message;
+}
+
+void add_rows(int dtype, const float* sums, int64_t rows, int64_t cols, float alpha, const int* count,
+              void* out, cudaStream_t stream) {
+    const unsigned grid = (unsigned)((cols + 255) / 256);
+    if (dtype == MG_PREC_BF16)
+        add_rows_kernel<MG_PREC_BF16><<<grid, 256, 0, stream>>>(sums, rows, cols, alpha, count,
+                                                                static_cast<__nv_bfloat16*>(out));
+    else
+        add_rows_kernel<MG_PREC_FP16><<<grid, 256, 0, stream>>>(sums, rows, cols, alpha, count,
+                                                                static_cast<__half*>(out));
+    launched("add_rows_kernel");
 }
 
 int* op_status_word() {

@@ -123,5 +123,10 @@ int guarded(F&& body) noexcept {
 // ptx_sm100.cuh from a wait that gave up) on the current device.
 int* op_status_word();
 
+// out[c] = alpha / max(*count, 1) * sum over `rows` rows of sums[r * cols + c],
+// in row order (count may be null: 1).
+void add_rows(int dtype, const float* sums, int64_t rows, int64_t cols, float alpha, const int* count,
+              void* out, cudaStream_t stream);
+
 }  // namespace ops
 }  // namespace mgb

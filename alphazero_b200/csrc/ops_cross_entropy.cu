@@ -1,26 +1,42 @@
 // Linear softmax cross entropy without the logits, with its gradients
 // (include/minigo_ops.h).
 //
-// Rows are taken in pieces: a piece's logits are written to the workspace,
-// turned into the row losses and (with gradients) into d, and used up by the
-// two products before the next piece overwrites them.
+// Forward: the product's epilogue turns each tile of logits into a maximum
+// and a sum per row and block of 128 columns; the logits leave the chip in
+// no form.  combine_kernel joins the blocks of a row.
+//
+// With gradients each tile also leaves exp(l - its block's maximum) in 16
+// bits (Prob16, ops_gemm.cuh), for a piece of the rows at a time.  Once a
+// row's logsumexp is known, d_kernel turns the piece into d in place, and
+// two products use it up: dx = d W and dw += d^T x.  So the product x W^T is
+// computed once (6 n V D operations in all), where making d from the inputs
+// again after the forward pass would compute it twice (8 n V D).
 #include "ops_gemm.cuh"
 
 #include <algorithm>
-#include <cfloat>
 #include <cmath>
 
 namespace mgb {
 namespace ops {
 namespace {
 
-constexpr size_t kPieceBytes = size_t(512) << 20;  // of logits at a time
+// Of a piece of the rows' probabilities at a time.  Each further piece costs
+// the fp32 sums of dw a trip through memory.
+constexpr size_t kPieceBytes = size_t(1) << 30;
 
-__global__ void __launch_bounds__(1024) count_kernel(mg_cross_entropy_args a, int* count) {
+// d is kept times 2^14 in fp16, so that small probabilities keep their bits.
+template <int DT>
+constexpr float kDScale = DT == MG_PREC_FP16 ? 16384.0f : 1.0f;
+
+// target[i] (-1: not counted) and their number.
+__global__ void __launch_bounds__(1024) target_kernel(mg_cross_entropy_args a, int* target, int* count) {
     __shared__ int part[32];
     int c = 0;
-    for (int64_t i = threadIdx.x; i < a.n; i += 1024)
-        c += index_at(a.targets, a.target_bytes, i * a.target_stride, a.vocab) >= 0;
+    for (int64_t i = threadIdx.x; i < a.n; i += 1024) {
+        const int t = (int)index_at(a.targets, a.target_bytes, i * a.target_stride, a.vocab);
+        target[i] = t;
+        c += t >= 0;
+    }
     c = __reduce_add_sync(~0u, c);
     if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = c;
     __syncthreads();
@@ -30,148 +46,215 @@ __global__ void __launch_bounds__(1024) count_kernel(mg_cross_entropy_args a, in
     }
 }
 
-// d is kept times 2^14 in fp16, so that small probabilities keep their bits.
-template <int DT>
-constexpr float kDScale = DT == MG_PREC_FP16 ? 16384.0f : 1.0f;
-
-// One block per row: its loss, and its d.
-template <int DT>
-__global__ void __launch_bounds__(256)
-    row_kernel(mg_cross_entropy_args a, int64_t row0, const float* logits, void* d) {
-    using E = Elem<DT>;
-    using T = typename E::T;
-    __shared__ float sm[256], ss[256];
-    const int64_t i = row0 + blockIdx.x;
-    const float* l = logits + (int64_t)blockIdx.x * a.vocab;
-    T* out = static_cast<T*>(d) + (int64_t)blockIdx.x * a.vocab;
-    const int64_t t = index_at(a.targets, a.target_bytes, i * a.target_stride, a.vocab);
-    if (t < 0) {
-        if (threadIdx.x == 0) a.row_loss[i] = 0.0f;
-        if (d)
-            for (int64_t v = threadIdx.x; v < a.vocab; v += 256) out[v] = E::put(0.0f);
-        return;
-    }
+// logsumexp and loss of 32 rows per block: 32 threads share a row's blocks.
+// A row of -inf has lse -inf.
+__global__ void __launch_bounds__(1024)
+    combine_kernel(int64_t rows, int blocks, const float2* part, int64_t part_ld, const int* target,
+                   const float* logit, float* lse, float* row_loss) {
+    __shared__ float2 mine[32][33];
+    const int64_t row = (int64_t)blockIdx.x * 32 + threadIdx.x % 32;
+    const int slice = threadIdx.x / 32;
     float m = -INFINITY, s = 0.0f;
-    for (int64_t v = threadIdx.x; v < a.vocab; v += 256) m = fmaxf(m, l[v]);
-    sm[threadIdx.x] = m;
-    __syncthreads();
-    for (int w = 128; w > 0; w /= 2) {
-        if (threadIdx.x < w) sm[threadIdx.x] = fmaxf(sm[threadIdx.x], sm[threadIdx.x + w]);
-        __syncthreads();
-    }
-    m = sm[0];
-    const float ref = m == -INFINITY ? 0.0f : m;
-    for (int64_t v = threadIdx.x; v < a.vocab; v += 256) s += expf(l[v] - ref);
-    ss[threadIdx.x] = s;
-    __syncthreads();
-    for (int w = 128; w > 0; w /= 2) {
-        if (threadIdx.x < w) ss[threadIdx.x] += ss[threadIdx.x + w];
-        __syncthreads();
-    }
-    s = ss[0];
-    const float lse = ref + logf(s);
-    if (threadIdx.x == 0) a.row_loss[i] = l[t] == -INFINITY ? INFINITY : lse - l[t];
-    if (d)
-        for (int64_t v = threadIdx.x; v < a.vocab; v += 256) {
-            const float p = s == 0.0f ? 0.0f : expf(l[v] - lse);
-            out[v] = E::put((p - (v == t ? 1.0f : 0.0f)) * kDScale<DT>);
+    if (row < rows)
+        for (int b = slice; b < blocks; b += 32) {
+            const float2 p = part[(int64_t)b * part_ld + row];
+            const float top = fmaxf(m, p.x), ref = top == -INFINITY ? 0.0f : top;
+            s = s * exp2f((m - ref) * 1.4426950408889634f) + p.y * exp2f((p.x - ref) * 1.4426950408889634f);
+            m = top;
         }
+    mine[slice][threadIdx.x % 32] = make_float2(m, s);
+    __syncthreads();
+    if (threadIdx.x >= 32 || row >= rows) return;
+    float top = -INFINITY, sum = 0.0f;
+    for (int i = 0; i < 32; ++i) top = fmaxf(top, mine[i][threadIdx.x].x);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    for (int i = 0; i < 32; ++i) {
+        const float2 p = mine[i][threadIdx.x];
+        sum += p.y * exp2f((p.x - ref) * 1.4426950408889634f);
+    }
+    const float l = sum == 0.0f ? -INFINITY : ref + logf(sum);
+    lse[row] = l;
+    const float at = logit[row];
+    row_loss[row] = target[row] < 0 ? 0.0f : at == -INFINITY ? INFINITY : l - at;
 }
 
-__global__ void __launch_bounds__(1024) loss_kernel(mg_cross_entropy_args a, const int* count) {
+// probs (Prob16, per block of `block` columns) -> d = (softmax - onehot) in
+// place, and its column sums before rounding per block of rows.  A thread
+// has 8 adjacent columns of every eighth row; the factor from the block's
+// maximum to the row's logsumexp is one exp per thread and row.
+template <int DT>
+__global__ void __launch_bounds__(256)
+    d_kernel(int64_t rows, int64_t vocab, int block, uint16_t* probs, int64_t ld, const float2* part,
+             int64_t part_ld, const float* lse, const int* target, int rows_per_block, float* sums) {
+    using E = Elem<DT>;
+    using T = typename E::T;
+    __shared__ float acc[8][256];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 256 + lane * 8;
+    const int64_t r0 = (int64_t)blockIdx.y * rows_per_block, r1 = min(rows, r0 + rows_per_block);
+    float sum[8] = {};
+    if (c < vocab) {
+        const float2* mine = part + c / block * part_ld;
+#pragma unroll 4
+        for (int64_t r = r0 + warp; r < r1; r += 8) {
+            const int t = target[r];
+            const float l = lse[r];
+            uint4* p = reinterpret_cast<uint4*>(probs + r * ld + c);
+            const uint4 u = *p;
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            const float f = l == -INFINITY ? 0.0f : exp2f((mine[r].x - l) * 1.4426950408889634f);
+            alignas(16) T d[8];
+            const int64_t hot = t < 0 ? -1 : t - c;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float v = prob16_value(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu) * f;
+                if (hot == i) v -= 1.0f;
+                if (t < 0) v = 0.0f;
+                sum[i] += v;
+                d[i] = E::put(v * kDScale<DT>);
+            }
+            *p = *reinterpret_cast<uint4*>(d);
+        }
+    }
+    if (sums == nullptr) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[warp][lane * 8 + i] = sum[i];
+    __syncthreads();
+    const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (col >= vocab) return;
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += acc[i][threadIdx.x];
+    sums[(int64_t)blockIdx.y * vocab + col] = s;
+}
+
+__global__ void __launch_bounds__(1024) loss_kernel(int64_t n, const float* row_loss, const int* count, float* loss) {
     __shared__ float part[1024];
     float s = 0.0f;
-    for (int64_t i = threadIdx.x; i < a.n; i += 1024) s += a.row_loss[i];
+    for (int64_t i = threadIdx.x; i < n; i += 1024) s += row_loss[i];
     part[threadIdx.x] = s;
     __syncthreads();
     for (int w = 512; w > 0; w /= 2) {
         if (threadIdx.x < w) part[threadIdx.x] += part[threadIdx.x + w];
         __syncthreads();
     }
-    if (threadIdx.x == 0) *a.loss = part[0] / (float)max(*count, 1);
-}
-
-// db = sum of d over the piece's rows, added to what earlier pieces gave.
-template <int DT>
-__global__ void __launch_bounds__(256)
-    column_kernel(int64_t vocab, int64_t rows, const void* d, float* sums, bool first, void* db,
-                  float alpha, const int* count) {
-    using E = Elem<DT>;
-    using T = typename E::T;
-    const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (v >= vocab) return;
-    float s = first ? 0.0f : sums[v];
-    for (int64_t i = 0; i < rows; ++i) s += E::get(static_cast<const T*>(d)[i * vocab + v]);
-    sums[v] = s;
-    if (db) static_cast<T*>(db)[v] = E::put(s * alpha / (float)max(*count, 1));
-}
-
-// dw = alpha / count * (sums of the pieces).
-template <int DT>
-__global__ void __launch_bounds__(256)
-    weight_kernel(int64_t total, float* sums, const float* piece, bool first, void* dw, float alpha,
-                  const int* count) {
-    using E = Elem<DT>;
-    using T = typename E::T;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= total) return;
-    const float s = (first ? 0.0f : sums[i]) + piece[i];
-    sums[i] = s;
-    if (dw) static_cast<T*>(dw)[i] = E::put(s * alpha / (float)max(*count, 1));
+    if (threadIdx.x == 0) *loss = part[0] / (float)max(*count, 1);
 }
 
 template <int DT>
 void run(const mg_cross_entropy_args& a, Workspace& w, bool go, cudaStream_t s) {
     using T = typename Elem<DT>::T;
     const bool grads = a.dw != nullptr;  // an empty dx may be null
-    const int64_t piece = std::min<int64_t>(std::max<int64_t>(a.n, 1),
-                                            std::max<int64_t>(1, kPieceBytes / 4 / a.vocab));
-    int* count = w.take<int>(4);
-    float* logits = w.take<float>((size_t)piece * a.vocab * 4);
-    T* d = grads ? w.take<T>((size_t)piece * a.vocab * 2) : nullptr;
-    float* sums = grads ? w.take<float>((size_t)a.vocab * 4) : nullptr;
-    float* part = grads ? w.take<float>((size_t)a.vocab * a.dim * 4) : nullptr;
-    float* total = grads ? w.take<float>((size_t)a.vocab * a.dim * 4) : nullptr;
-    if (!go) return;
-    w.require();
-    count_kernel<<<1, 1024, 0, s>>>(a, count);
-    launched("count_kernel");
-    const GemmOperand weight{a.weight, a.w_row, a.w_col};
-    const float alpha = a.grad_scale / kDScale<DT>;
-    if (grads && a.n == 0) {
-        check(cudaMemsetAsync(a.dw, 0, (size_t)a.vocab * a.dim * 2, s), "cudaMemsetAsync");
-        if (a.db) check(cudaMemsetAsync(a.db, 0, (size_t)a.vocab * 2, s), "cudaMemsetAsync");
+    if (a.n == 0) {
+        if (!go) return;
+        ops::check(cudaMemsetAsync(a.loss, 0, 4, s), "cudaMemsetAsync");
+        if (grads) ops::check(cudaMemsetAsync(a.dw, 0, (size_t)a.vocab * a.dim * 2, s), "cudaMemsetAsync");
+        if (a.db) ops::check(cudaMemsetAsync(a.db, 0, (size_t)a.vocab * 2, s), "cudaMemsetAsync");
+        return;
     }
+    const int64_t ld = (a.vocab + 7) / 8 * 8;
+    // pieces of equal length, whole tiles
+    const int64_t most = std::max<int64_t>(256, (int64_t)(kPieceBytes / 2) / ld / 256 * 256);
+    const int64_t count_pieces = grads ? (a.n + most - 1) / most : 1;
+    const int64_t piece = std::min(a.n, ((a.n + count_pieces - 1) / count_pieces + 255) / 256 * 256);
+    const int block = gemm_softmax_block(piece, a.vocab);
+    const int blocks = (int)((a.vocab + block - 1) / block);
+
+    int* count = w.take<int>(4);
+    int* target = w.take<int>((size_t)a.n * 4);
+    float* logit = w.take<float>((size_t)piece * 4);
+    float* lse = w.take<float>((size_t)piece * 4);
+    float2* part = w.take<float2>((size_t)blocks * piece * 8);
+    uint16_t* probs = grads ? w.take<uint16_t>((size_t)piece * ld * 2) : nullptr;
+    const int64_t across = (a.vocab + 255) / 256;
+    const int64_t want = std::max<int64_t>(1, 148 * 16 / across);
+    const int down_rows = (int)std::max<int64_t>(32, (piece + want - 1) / want);
+    const int64_t down = (piece + down_rows - 1) / down_rows;  // of a whole piece
+    float* sums = a.db ? w.take<float>((size_t)down * count_pieces * a.vocab * 4) : nullptr;
+    const int64_t ld32 = (a.dim + 7) / 8 * 8;
+    float* dw32 = grads && count_pieces > 1 ? w.take<float>((size_t)a.vocab * ld32 * 4) : nullptr;
+
+    StagedOperand x = stage_operand(w, go, {a.x, a.x_row, a.x_col}, a.n, a.dim, s);
+    const StagedOperand weight = stage_operand(w, go, {a.weight, a.w_row, a.w_col}, a.vocab, a.dim, s);
+    if (go) {
+        w.require();
+        target_kernel<<<1, 1024, 0, s>>>(a, target, count);
+        launched("target_kernel");
+    }
+    const float alpha = a.grad_scale / kDScale<DT>;
+    int64_t sum_rows = 0;
+    size_t piece_scratch = 0;
     for (int64_t row0 = 0; row0 < a.n; row0 += piece) {
         const int64_t rows = std::min(piece, a.n - row0);
-        const bool last = row0 + rows == a.n;
-        const T* x = static_cast<const T*>(a.x) + row0 * a.x_row;
-        GemmEpilogue e;
-        e.bias = a.bias;
-        e.out32 = logits;
-        e.ld = a.vocab;
-        launch_gemm(DT, {x, a.x_row, a.x_col}, weight, rows, a.vocab, a.dim, e, s);
-        row_kernel<DT><<<(unsigned)rows, 256, 0, s>>>(a, row0, logits, d);
-        launched("row_kernel");
+        const bool first = row0 == 0, last = row0 + rows == a.n;
+        StagedOperand xp = x;  // row0 is a multiple of 256: still aligned
+        xp.data = static_cast<const uint16_t*>(x.data) + row0 * (x.mn ? 1 : x.ld);
+        if (go) {
+            SoftmaxJob f;
+            f.a = xp;
+            f.b = weight;
+            f.m = rows;
+            f.n = a.vocab;
+            f.k = a.dim;
+            f.e.bias = a.bias;
+            f.e.target = target + row0;
+            f.e.logit = logit;
+            f.e.part = part;
+            f.e.part_ld = piece;
+            f.e.probs = probs;
+            f.e.probs_ld = ld;
+            gemm_softmax(DT, f, block, s);
+            combine_kernel<<<(unsigned)((rows + 31) / 32), 1024, 0, s>>>(rows, blocks, part, piece, target + row0,
+                                                                       logit, lse, a.row_loss + row0);
+            launched("combine_kernel");
+        }
         if (!grads) continue;
-        GemmEpilogue ex;
-        ex.out = static_cast<T*>(a.dx) + row0 * a.dim;
-        ex.ld = a.dim;
-        ex.alpha = alpha;
-        ex.count = count;
-        launch_gemm(DT, {d, a.vocab, 1}, {a.weight, a.w_col, a.w_row}, rows, a.dim, a.vocab, ex, s);
-        GemmEpilogue ew;
-        ew.out32 = part;
-        ew.ld = a.dim;
-        launch_gemm(DT, {d, 1, a.vocab}, {x, a.x_col, a.x_row}, a.vocab, a.dim, rows, ew, s);
-        weight_kernel<DT><<<(unsigned)((a.vocab * a.dim + 255) / 256), 256, 0, s>>>(
-            a.vocab * a.dim, total, part, row0 == 0, last ? a.dw : nullptr, alpha, count);
-        launched("weight_kernel");
-        column_kernel<DT><<<(unsigned)((a.vocab + 255) / 256), 256, 0, s>>>(
-            a.vocab, rows, d, sums, row0 == 0, last ? a.db : nullptr, alpha, count);
-        launched("column_kernel");
+        const int64_t these = (rows + down_rows - 1) / down_rows;
+        if (go) {
+            d_kernel<DT><<<dim3((unsigned)across, (unsigned)these), 256, 0, s>>>(
+                rows, a.vocab, block, probs, ld, part, piece, lse, target + row0, down_rows,
+                sums ? sums + sum_rows * a.vocab : nullptr);
+            launched("d_kernel");
+        }
+        sum_rows += these;
+        StagedOperand d;
+        d.data = probs;
+        d.ld = ld;
+        GemmJob jobs[2];
+        GemmJob& jx = jobs[0];
+        jx.a = d;
+        jx.b = transposed(weight);
+        jx.m = rows;
+        jx.n = a.dim;
+        jx.k = a.vocab;
+        jx.e.out = static_cast<T*>(a.dx) + row0 * a.dim;
+        jx.e.ld = a.dim;
+        jx.e.alpha = alpha;
+        jx.e.count = count;
+        GemmJob& jw = jobs[1];
+        jw.a = transposed(d);
+        jw.b = transposed(xp);
+        jw.m = a.vocab;
+        jw.n = a.dim;
+        jw.k = rows;
+        jw.e.ld32 = ld32;
+        jw.e.acc32 = first ? nullptr : dw32;
+        jw.e.out32 = last ? nullptr : dw32;
+        jw.e.out = a.dw;
+        jw.e.ld = a.dim;
+        jw.e.alpha = alpha;
+        jw.e.count = count;
+        Workspace again = w;  // every piece's scratch is the same
+        gemm(again, go, DT, jobs, 2, s);
+        if (go) continue;
+        piece_scratch = std::max(piece_scratch, again.used() - w.used());
     }
-    loss_kernel<<<1, 1024, 0, s>>>(a, count);
+    if (!go) {
+        w.take(piece_scratch);
+        return;
+    }
+    if (a.db) add_rows(DT, sums, sum_rows, a.vocab, alpha * kDScale<DT>, count, a.db, s);
+    loss_kernel<<<1, 1024, 0, s>>>(a.n, a.row_loss, count, a.loss);
     launched("loss_kernel");
 }
 

@@ -1,65 +1,722 @@
-// 64 x 64 tiles, 4 x 4 outputs per thread, operands of any strides.
+// Tensor-core products of the training operators on pairs of SMs.
+//
+// C = A B^T by tiles of 256 x BN (BN 256 or 128), a CTA pair
+// (tcgen05, cta_group::2) per tile: each CTA holds 128 rows of A, half of
+// the BN rows of B and 128 x BN fp32 sums in TMEM, so a K step of 64 moves
+// 16 + BN / 16 KB per CTA for 128 x BN x 64 multiply-adds.  One CTA with a
+// 128 x 256 tile of its own would move 48 KB for the same work: more than
+// L2 gives 148 SMs at the tensor cores' rate.
+//
+// Either operand may lie along k (K-major) or along its own rows (MN-major):
+// TMA writes both with the 128-byte swizzle, and the instruction and matrix
+// descriptors say which, so the gradients' products read x, the weight and
+// g where they are, with no transposing pass.
+//
+// Warps of each CTA (persistent over its tiles):
+//   warp 0     TMA producer (one thread), a ring of kStages K steps
+//   warp 1     TMEM; in the even CTA also the MMA issuer (one thread)
+//   warps 2-9  epilogue: warp w reads TMEM lanes 32 (w % 4) .. + 31 (a thread
+//              owns a row) and half of the columns, 32 at a time
+// The sums are double-buffered in TMEM: a tile's epilogue overlaps the next
+// tile's products.  Every wait is bounded (ptx_sm100.cuh).
 #include "ops_gemm.cuh"
+#include "ptx_sm100.cuh"
+
+#include <algorithm>
+#include <cmath>
+#include <cudaTypedefs.h>
 
 namespace mgb {
 namespace ops {
 namespace {
 
-constexpr int kTile = 64, kStep = 16;
+constexpr int kRowsCta = 128;          // rows of a tile per CTA
+constexpr int kRowsPair = 256;
+constexpr int kBK = 64;                // K elements per stage
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 32 * (2 + kEpiWarps);
+constexpr int kPairs = 74;             // of SMs on a B200 (148)
+constexpr int kGroup = 8;              // row tiles walked together (their B tiles stay in L2)
+constexpr int kStagePitch = 34;        // 16-bit elements per staged row (17 words: no bank conflicts)
+
+template <int BN>
+struct Config {
+    static constexpr int kStages = BN == 256 ? 6 : 8;
+    static constexpr uint32_t kABytes = kRowsCta * kBK * 2;
+    static constexpr uint32_t kBBytes = BN / 2 * kBK * 2;
+    static constexpr uint32_t kStageBytes = kABytes + kBBytes;
+    static constexpr uint32_t kTmemCols = 2 * BN;
+    static constexpr int kBarriers = 2 * kStages + 5;
+    // ring + per epilogue warp a staged block and a bias row + barriers + alignment slack
+    static constexpr int kSmem = kStages * kStageBytes + kEpiWarps * (32 * kStagePitch * 2 + BN / 2 * 4) +
+                                 kBarriers * 8 + 16 + 1024;
+};
+
+enum Epi : int { kStore, kSoftmax };
+
+struct JobArgs {
+    int m, n, kblocks;
+    int tiles_m, tiles_n, splits, kb_split;
+    int a_mn, b_mn;
+    int vec;  // outputs, z and residual take 16-byte accesses
+    GemmEpilogue e;
+    SoftmaxEpilogue s;
+};
+
+struct alignas(64) KernelArgs {
+    CUtensorMap ta[2], tb[2];
+    JobArgs job[2];
+    int units[2];
+    int head_start;  // units of job 1 that a pair does while others finish their last unit of job 0
+    int* err;
+};
+
+// The units of a pair: job 0's round robin, then job 1's, handed out in the
+// order in which the pairs come free (pairs with one unit of job 0 fewer
+// start head_start units of job 1 earlier).
+struct UnitWalk {
+    int pairs, p, n0, n1, extra, ahead, c0, step = 0;
+    __device__ UnitWalk(const KernelArgs& a, int pair, int total) : pairs(total), p(pair) {
+        n0 = a.units[0];
+        n1 = a.units[1];
+        extra = n0 % pairs;
+        ahead = extra ? a.head_start : 0;
+        c0 = p < n0 ? (n0 - p + pairs - 1) / pairs : 0;
+    }
+    __device__ bool next(int* job, int* unit) {
+        const int i = step++;
+        if (i < c0) {
+            *job = 0;
+            *unit = p + i * pairs;
+            return true;
+        }
+        const int j = i - c0, early = pairs - extra;
+        int u;
+        if (p >= extra && j < ahead) u = j * early + (p - extra);
+        else if (p >= extra) u = ahead * early + (j - ahead) * pairs + p;
+        else u = ahead * early + j * pairs + p;
+        *job = 1;
+        *unit = u;
+        return u < n1;
+    }
+};
+
+struct Tile {
+    int m0, n0, kb0, kb1, split;
+    __device__ Tile(const JobArgs& j, int unit, int bn) {
+        const int tiles = j.tiles_m * j.tiles_n;
+        split = unit / tiles;
+        const int t = unit % tiles, per = kGroup * j.tiles_n;
+        const int first = t / per * kGroup, rows = min(kGroup, j.tiles_m - first);
+        m0 = (first + t % per % rows) * kRowsPair;
+        n0 = t % per / rows * bn;
+        kb0 = split * j.kb_split;
+        kb1 = min(kb0 + j.kb_split, j.kblocks);
+    }
+};
 
 template <int DT>
-__global__ void __launch_bounds__(256)
-    gemm_kernel(GemmOperand a, GemmOperand b, int64_t m, int64_t n, int64_t k, GemmEpilogue e) {
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (DT == MG_PREC_BF16) {
+        __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<uint32_t*>(&h);
+    } else {
+        __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<uint32_t*>(&h);
+    }
+}
+template <int DT>
+__device__ __forceinline__ float2 unpack2(uint32_t u) {
+    if constexpr (DT == MG_PREC_BF16) return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&u));
+    else return __half22float2(*reinterpret_cast<__half2*>(&u));
+}
+
+// The 32 x 32 block of 16-bit values at p (row stride `row`, column stride
+// `col`) <-> one row per lane.  vec: 16-byte accesses, a row per lane;
+// otherwise through the warp's staging block, a row at a time, coalesced.
+template <int DT>
+__device__ __forceinline__ void load_block(const void* base, int64_t row, int64_t col, bool vec, int rows,
+                                           int cols, int lane, uint16_t* stage, float (&v)[32]) {
+    const uint16_t* p = static_cast<const uint16_t*>(base);
+    if (vec) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (lane < rows && q * 8 < cols)
+                u = __ldg(reinterpret_cast<const uint4*>(p + lane * row + q * 8));
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = unpack2<DT>(w[i]);
+                v[q * 8 + 2 * i] = f.x;
+                v[q * 8 + 2 * i + 1] = f.y;
+            }
+        }
+        return;
+    }
+    __syncwarp();
+    for (int r = 0; r < rows; ++r)
+        if (lane < cols) stage[r * kStagePitch + lane] = p[r * row + lane * col];
+    __syncwarp();
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(stage + lane * kStagePitch);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float2 f = unpack2<DT>(w[i]);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ void store_block(void* base, int64_t row, bool vec, int rows, int cols, int lane,
+                                            uint16_t* stage, const float (&v)[32]) {
+    uint16_t* p = static_cast<uint16_t*>(base);
+    if (vec) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            uint4 u;
+            u.x = pack2<DT>(v[q * 8], v[q * 8 + 1]);
+            u.y = pack2<DT>(v[q * 8 + 2], v[q * 8 + 3]);
+            u.z = pack2<DT>(v[q * 8 + 4], v[q * 8 + 5]);
+            u.w = pack2<DT>(v[q * 8 + 6], v[q * 8 + 7]);
+            if (lane < rows && q * 8 < cols) *reinterpret_cast<uint4*>(p + lane * row + q * 8) = u;
+        }
+        return;
+    }
+    __syncwarp();
+    uint32_t* w = reinterpret_cast<uint32_t*>(stage + lane * kStagePitch);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = pack2<DT>(v[2 * i], v[2 * i + 1]);
+    __syncwarp();
+    for (int r = 0; r < rows; ++r)
+        if (lane < cols) p[r * row + lane] = stage[r * kStagePitch + lane];
+}
+
+__device__ __forceinline__ void activate_all(float (&v)[32], int act) {
+    if (act == MG_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = activate(v[i], MG_ACT_RELU);
+    } else if (act == MG_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = activate(v[i], MG_ACT_SILU);
+    } else if (act == MG_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = activate(v[i], MG_ACT_GELU);
+    }
+}
+
+// Columns [n0 + c0, + BN / 2) of rows [m0, + 32) of a finished tile.
+template <int BN, int DT>
+__device__ __forceinline__ void epilogue(const JobArgs& j, const Tile& t, int m0, int c0, uint32_t taddr,
+                                         int lane, uint16_t* stage, const float* sbias, float alpha) {
+    const GemmEpilogue& e = j.e;
+    const int rows = min(32, j.m - m0);
+#pragma unroll 1
+    for (int c = 0; c < BN / 2; c += 32) {
+        const int64_t col = t.n0 + c0 + c;
+        const int cols = (int)min((int64_t)32, j.n - col);
+        if (cols <= 0) break;
+        uint32_t r[32];
+        tmem_ld_32cols(taddr + c, r);
+        tmem_ld_wait();
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+        if (rows <= 0) continue;
+        if (e.acc32 != nullptr && lane < rows) {
+            const float* p = e.acc32 + (int64_t)(m0 + lane) * e.ld32 + col;
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (q * 4 < cols) {
+                    const float4 f = *reinterpret_cast<const float4*>(p + q * 4);
+                    v[q * 4] += f.x;
+                    v[q * 4 + 1] += f.y;
+                    v[q * 4 + 2] += f.z;
+                    v[q * 4 + 3] += f.w;
+                }
+        }
+        if (e.out32 != nullptr) {
+            if (lane < rows) {
+                float* p = e.out32 + ((int64_t)t.split * j.m + m0 + lane) * e.ld32 + col;
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (q * 4 < cols)
+                        *reinterpret_cast<float4*>(p + q * 4) =
+                            make_float4(v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]);
+            }
+            continue;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = v[i] * alpha + sbias[c + i];
+        const bool vec = j.vec != 0;
+        if (e.z != nullptr)
+            store_block<DT>(static_cast<uint16_t*>(e.z) + (int64_t)m0 * e.ld + col, e.ld, vec, rows, cols,
+                            lane, stage, v);
+        activate_all(v, e.act);
+        if (e.res != nullptr) {
+            float x[32];
+            load_block<DT>(static_cast<const uint16_t*>(e.res) + m0 * e.r_row + col * e.r_col, e.r_row,
+                           e.r_col, vec, rows, cols, lane, stage, x);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] += e.res_scale * x[i];
+        }
+        store_block<DT>(static_cast<uint16_t*>(e.out) + (int64_t)m0 * e.ld + col, e.ld, vec, rows, cols,
+                        lane, stage, v);
+    }
+}
+
+// The same columns and rows as softmax statistics.  A thread has its row's
+// block to itself, so the maximum and the sum need no exchange; the sums are
+// read from TMEM twice rather than held in BN / 2 registers.
+template <int BN>
+__device__ __forceinline__ void softmax_epilogue(const JobArgs& j, const Tile& t, int m0, int c0,
+                                                 uint32_t taddr, int lane, const float* sbias) {
+    const SoftmaxEpilogue& e = j.s;
+    const int row = m0 + lane;
+    const int first = t.n0 + c0;
+    if (first >= j.n) return;
+    const int width = min(BN / 2, j.n - first);
+    const int target = row < j.m ? e.target[row] - first : -1;
+    float top = -INFINITY, logit = 0.0f;
+#pragma unroll 1
+    for (int c = 0; c < width; c += 32) {
+        uint32_t r[32];
+        tmem_ld_32cols(taddr + c, r);
+        tmem_ld_wait();
+        const bool here = target >= c && target < c + 32;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const float l = __uint_as_float(r[i]) + sbias[c + i];  // -inf past the last column
+            top = fmaxf(top, l);
+            if (here && target == c + i) logit = l;
+        }
+    }
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+    for (int c = 0; c < width; c += 32) {
+        uint32_t r[32];
+        tmem_ld_32cols(taddr + c, r);
+        tmem_ld_wait();
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            // the difference first: exact near the maximum, and in range for any finite logits
+            v[i] = exp2f((__uint_as_float(r[i]) + sbias[c + i] - ref) * 1.4426950408889634f);
+            sum[i & 3] += v[i];
+        }
+        if (e.probs != nullptr && row < j.m) {
+            uint16_t* p = e.probs + (int64_t)row * e.probs_ld + first + c;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (c + q * 8 < width) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        w[i] = prob16x2(v[q * 8 + 2 * i], v[q * 8 + 2 * i + 1]);
+                    *reinterpret_cast<uint4*>(p + q * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+        }
+    }
+    if (row < j.m) {
+        if (target >= 0 && target < width) e.logit[row] = logit;
+        e.part[(int64_t)(first / (BN / 2)) * e.part_ld + row] =
+            make_float2(top, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+    }
+}
+
+template <int BN, int DT, int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    gemm_kernel(const __grid_constant__ KernelArgs a) {
+    using Cfg = Config<BN>;
+    constexpr int S = Cfg::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    // the same offset in both CTAs: the dynamic segment starts at the same address in each
+    uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
+    uint8_t* ring = smem;
+    float* sbias_all = reinterpret_cast<float*>(ring + S * Cfg::kStageBytes);
+    uint16_t* stage_all = reinterpret_cast<uint16_t*>(sbias_all + kEpiWarps * (BN / 2));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(stage_all + kEpiWarps * 32 * kStagePitch);
+    uint64_t* full = bars;           // even CTA's: a stage has landed in both CTAs
+    uint64_t* empty = bars + S;      // each CTA's: the products have read a stage
+    uint64_t* tfull = bars + 2 * S;  // [2] each CTA's: a tile's sums are complete
+    uint64_t* tempty = tfull + 2;    // [2] even CTA's: both CTAs have read them
+    uint64_t* done = tempty + 2;     // even CTA's: drain after a wait gave up
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::kBarriers);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(smem_u32(&full[s]), 1);
+            mbar_init(smem_u32(&empty[s]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&tfull[i]), 1);
+            mbar_init(smem_u32(&tempty[i]), 2 * kEpiWarps);
+        }
+        mbar_init(smem_u32(done), 1);
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(smem_u32(tmem_slot), Cfg::kTmemCols);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    UnitWalk walk(a, pair, pairs);
+    int job, unit;
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            while (ok && walk.next(&job, &unit)) {
+                const JobArgs& j = a.job[job];
+                const Tile t(j, unit, BN);
+                const int am = t.m0 + (int)rank * kRowsCta, bn = t.n0 + (int)rank * (BN / 2);
+                for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+                    const int s = it % S;
+                    if (!mbar_wait_cluster(smem_u32(&empty[s]), ((it / S) & 1) ^ 1, a.err, kErrWaitProducer)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t bar = map_to_rank(smem_u32(&full[s]), 0);
+                    if (rank == 0) mbar_arrive_expect_tx(smem_u32(&full[s]), 2 * Cfg::kStageBytes);
+                    const uint32_t da = smem_u32(ring + s * Cfg::kStageBytes), db = da + Cfg::kABytes;
+                    const int k0 = kb * kBK;
+                    if (j.a_mn) {
+                        tma_load_2d_pair(da, &a.ta[job], bar, am, k0);
+                        tma_load_2d_pair(da + 8192, &a.ta[job], bar, am + 64, k0);
+                    } else {
+                        tma_load_2d_pair(da, &a.ta[job], bar, k0, am);
+                    }
+                    if (j.b_mn) {
+                        tma_load_2d_pair(db, &a.tb[job], bar, bn, k0);
+                        if (BN == 256) tma_load_2d_pair(db + 8192, &a.tb[job], bar, bn + 64, k0);
+                    } else {
+                        tma_load_2d_pair(db, &a.tb[job], bar, k0, bn);
+                    }
+                }
+            }
+            // Every load has landed and every stage has been released (the
+            // release comes from the peer's commits) before this CTA ends.
+            for (int i = max(0, it - S); i < it; ++i) {
+                const int s = i % S;
+                if (rank == 0) mbar_wait_cluster(smem_u32(&full[s]), (i / S) & 1, a.err, kErrWaitDrain);
+                if (ok) mbar_wait_cluster(smem_u32(&empty[s]), (i / S) & 1, a.err, kErrWaitDrain);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (rank == 0 && lane == 0) {
+            int it = 0, tile = 0;
+            bool ok = true;
+            while (ok && walk.next(&job, &unit)) {
+                const JobArgs& j = a.job[job];
+                const Tile t(j, unit, BN);
+                const uint32_t idesc = idesc_f16(kRowsPair, BN, DT == MG_PREC_BF16) |
+                                       (j.a_mn ? kIdescAMn : 0) | (j.b_mn ? kIdescBMn : 0);
+                const uint64_t step_a = j.a_mn ? 2048 >> 4 : 32 >> 4, step_b = j.b_mn ? 2048 >> 4 : 32 >> 4;
+                const int buf = tile & 1;
+                if (!mbar_wait_cluster(smem_u32(&tempty[buf]), ((tile >> 1) & 1) ^ 1, a.err, kErrWaitMma)) break;
+                tc_fence_after();
+                const uint32_t acc = tmem_base + buf * BN;
+                for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+                    const int s = it % S;
+                    if (!mbar_wait_cluster(smem_u32(&full[s]), (it / S) & 1, a.err, kErrWaitMma)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t da = smem_u32(ring + s * Cfg::kStageBytes), db = da + Cfg::kABytes;
+                    uint64_t xa = j.a_mn ? smem_desc_sw128_mn(da) : smem_desc_sw128(da);
+                    uint64_t xb = j.b_mn ? smem_desc_sw128_mn(db) : smem_desc_sw128(db);
+#pragma unroll
+                    for (int kk = 0; kk < kBK / 16; ++kk) {
+                        mma_f16_pair(acc, xa, xb, idesc, kb > t.kb0 || kk > 0);
+                        xa += step_a;
+                        xb += step_b;
+                    }
+                    mma_commit_pair(smem_u32(&empty[s]));
+                }
+                if (!ok) break;
+                mma_commit_pair(smem_u32(&tfull[buf]));
+                ++tile;
+            }
+            // Products still in flight finish before TMEM is freed.
+            asm volatile(
+                "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(done))
+                : "memory");
+            mbar_wait_cluster(smem_u32(done), 0, a.err, kErrWaitDrain);
+        }
+        __syncwarp();
+    } else {
+        const int ew = warp - 2, quarter = warp & 3, half = ew >> 2;
+        uint16_t* stage = stage_all + ew * 32 * kStagePitch;
+        float* sbias = sbias_all + ew * (BN / 2);
+        const int c0 = half * (BN / 2);
+        int tile = 0;
+        while (walk.next(&job, &unit)) {
+            const JobArgs& j = a.job[job];
+            const Tile t(j, unit, BN);
+            __syncwarp();
+            for (int i = lane; i < BN / 2; i += 32) {
+                const int64_t col = t.n0 + c0 + i;
+                const void* bias = EPI == kSoftmax ? j.s.bias : j.e.out32 == nullptr ? j.e.bias : nullptr;
+                float b = EPI == kSoftmax ? -INFINITY : 0.0f;
+                if (col < j.n)
+                    b = bias != nullptr ? Elem<DT>::get(static_cast<const typename Elem<DT>::T*>(bias)[col]) : 0.0f;
+                sbias[i] = b;
+            }
+            __syncwarp();
+            const int buf = tile & 1;
+            // one answer for the warp, which goes on or stops together
+            if (!__all_sync(~0u, mbar_wait_cluster(smem_u32(&tfull[buf]), (tile >> 1) & 1, a.err, kErrWaitEpilogue)))
+                break;
+            tc_fence_after();
+            const int m0 = t.m0 + (int)rank * kRowsCta + quarter * 32;
+            const uint32_t taddr = tmem_base + buf * BN + c0 + ((uint32_t)quarter << 21);
+            if constexpr (EPI == kSoftmax) {
+                softmax_epilogue<BN>(j, t, m0, c0, taddr, lane, sbias);
+            } else {
+                const float alpha = j.e.count ? j.e.alpha / (float)max(*j.e.count, 1) : j.e.alpha;
+                epilogue<BN, DT>(j, t, m0, c0, taddr, lane, stage, sbias, alpha);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&tempty[buf]), 0));
+            ++tile;
+        }
+    }
+    // Neither CTA ends, or frees TMEM, while the other may still read its
+    // shared memory or signal its barriers.
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc_pair(tmem_base, Cfg::kTmemCols);
+}
+
+// Sums the splits of a product and applies its epilogue.
+template <int DT>
+__global__ void __launch_bounds__(256) finish_kernel(const float* part, int splits, int64_t m, int64_t n,
+                                                     int64_t ld32, GemmEpilogue e) {
     using E = Elem<DT>;
     using T = typename E::T;
-    __shared__ float sa[kStep][kTile + 1], sb[kStep][kTile + 1];
-    const int64_t i0 = (int64_t)blockIdx.x * kTile, j0 = (int64_t)blockIdx.y * kTile;
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    const T* pa = static_cast<const T*>(a.data);
-    const T* pb = static_cast<const T*>(b.data);
-    float acc[4][4] = {};
-    for (int64_t k0 = 0; k0 < k; k0 += kStep) {
-        for (int t = threadIdx.x; t < kTile * kStep; t += 256) {
-            const int r = t / kStep, c = t % kStep;
-            const int64_t i = i0 + r, j = j0 + r, kk = k0 + c;
-            sa[c][r] = i < m && kk < k ? E::get(pa[i * a.row + kk * a.col]) : 0.0f;
-            sb[c][r] = j < n && kk < k ? E::get(pb[j * b.row + kk * b.col]) : 0.0f;
-        }
-        __syncthreads();
-        for (int c = 0; c < kStep; ++c)
-            for (int r = 0; r < 4; ++r)
-                for (int s = 0; s < 4; ++s) acc[r][s] += sa[c][ty * 4 + r] * sb[c][tx * 4 + s];
-        __syncthreads();
-    }
     const float alpha = e.count ? e.alpha / (float)max(*e.count, 1) : e.alpha;
-    for (int r = 0; r < 4; ++r)
-        for (int s = 0; s < 4; ++s) {
-            const int64_t i = i0 + ty * 4 + r, j = j0 + tx * 4 + s;
-            if (i >= m || j >= n) continue;
-            float v = acc[r][s] * alpha;
-            if (e.bias) v += E::get(static_cast<const T*>(e.bias)[j]);
-            if (e.out32) {
-                e.out32[i * e.ld + j] = v;
-                continue;
-            }
-            if (e.z) static_cast<T*>(e.z)[i * e.ld + j] = E::put(v);
-            v = activate(v, e.act);
-            if (e.res)
-                v += e.res_scale * E::get(static_cast<const T*>(e.res)[i * e.r_row + j * e.r_col]);
-            static_cast<T*>(e.out)[i * e.ld + j] = E::put(v);
+    const int64_t total = m * n;
+    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * 256) {
+        const int64_t i = at / n, c = at % n;
+        float v = e.acc32 ? e.acc32[i * e.ld32 + c] : 0.0f;
+        for (int s = 0; s < splits; ++s) v += part[((int64_t)s * m + i) * ld32 + c];
+        if (e.out32) {
+            e.out32[i * e.ld32 + c] = v;
+            continue;
         }
+        v *= alpha;
+        if (e.bias) v += E::get(static_cast<const T*>(e.bias)[c]);
+        if (e.z) static_cast<T*>(e.z)[i * e.ld + c] = E::put(v);
+        v = activate(v, e.act);
+        if (e.res) v += e.res_scale * E::get(static_cast<const T*>(e.res)[i * e.r_row + c * e.r_col]);
+        static_cast<T*>(e.out)[i * e.ld + c] = E::put(v);
+    }
+}
+
+// Copies `rows` lines of `len` 16-bit elements (strides line, step) to lines of ld.
+__global__ void __launch_bounds__(256) pack_kernel(const uint16_t* in, int64_t line, int64_t step, int64_t rows,
+                                                   int64_t len, int64_t ld, uint16_t* out) {
+    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y)
+        for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < len; c += (int64_t)gridDim.x * 256)
+            out[r * ld + c] = in[r * line + c * step];
+}
+
+bool encode(CUtensorMap* map, int dtype, const StagedOperand& s, int64_t rows, int64_t k, int tile_rows) {
+    static PFN_cuTensorMapEncodeTiled_v12000 enc = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                       q == cudaDriverEntryPointSuccess
+                   ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p)
+                   : nullptr;
+    }();
+    if (enc == nullptr) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)(s.mn ? rows : k), (cuuint64_t)(s.mn ? k : rows)};
+    cuuint64_t strides[1] = {(cuuint64_t)s.ld * 2};
+    cuuint32_t box[2] = {64, (cuuint32_t)(s.mn ? kBK : tile_rows)};
+    cuuint32_t one[2] = {1, 1};
+    return enc(map, dtype == MG_PREC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+               const_cast<void*>(s.data), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+int64_t up8(int64_t v) { return (v + 7) / 8 * 8; }
+
+template <int BN, int DT, int EPI>
+void launch_one(const KernelArgs& a, int pairs, cudaStream_t stream) {
+    check(cudaFuncSetAttribute(gemm_kernel<BN, DT, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               Config<BN>::kSmem),
+          "cudaFuncSetAttribute(gemm_kernel)");
+    gemm_kernel<BN, DT, EPI><<<2 * pairs, kThreads, Config<BN>::kSmem, stream>>>(a);
+    launched("gemm_kernel");
+}
+
+template <int EPI>
+void launch(KernelArgs& a, int bn, int dtype, cudaStream_t stream) {
+    a.err = op_status_word();
+    const int pairs = (int)std::min<int64_t>(kPairs, (int64_t)a.units[0] + a.units[1]);
+    if (bn == 256) {
+        if (dtype == MG_PREC_BF16) launch_one<256, MG_PREC_BF16, EPI>(a, pairs, stream);
+        else launch_one<256, MG_PREC_FP16, EPI>(a, pairs, stream);
+    } else {
+        if (dtype == MG_PREC_BF16) launch_one<128, MG_PREC_BF16, EPI>(a, pairs, stream);
+        else launch_one<128, MG_PREC_FP16, EPI>(a, pairs, stream);
+    }
+}
+
+// Fills in what a job's tiles are, for tiles of bn columns.
+template <class Job>
+void lay_out(JobArgs& j, const Job& g, int bn) {
+    j.m = (int)g.m;
+    j.n = (int)g.n;
+    j.kblocks = (int)((g.k + kBK - 1) / kBK);
+    j.tiles_m = (int)((g.m + kRowsPair - 1) / kRowsPair);
+    j.tiles_n = (int)((g.n + bn - 1) / bn);
+    j.splits = 1;
+    j.kb_split = j.kblocks;
+    j.a_mn = g.a.mn;
+    j.b_mn = g.b.mn;
+    need((int64_t)j.tiles_m * j.tiles_n < (int64_t(1) << 24), "too many tiles");
+}
+
+template <class Job>
+void encode_operands(KernelArgs& a, int i, int dtype, const Job& g, int bn) {
+    if (!encode(&a.ta[i], dtype, g.a, g.m, g.k, kRowsCta) || !encode(&a.tb[i], dtype, g.b, g.n, g.k, bn / 2))
+        fail(MG_E_CUDA, "cuTensorMapEncodeTiled rejected an operand's tensor map");
+}
+
+// Narrow tiles where wide ones would leave pairs idle or mostly compute
+// padding; a narrow tile costs more than half a wide one, since it reads A
+// as often.
+template <class Job>
+int tile_columns(const Job* jobs, int count) {
+    const auto cost = [&](int bn) {
+        double work = 0;
+        int64_t units = 0;
+        for (int i = 0; i < count; ++i) {
+            const int64_t t = (jobs[i].m + 255) / 256 * ((jobs[i].n + bn - 1) / bn);
+            work += (double)t * (double)jobs[i].k;
+            units += t;
+        }
+        const double waves = std::max(1.0, (double)units / kPairs);
+        return work / units * waves * (bn == 256 ? 1.0 : 0.6);
+    };
+    return cost(128) < cost(256) ? 128 : 256;
 }
 
 }  // namespace
 
-void launch_gemm(int dtype, const GemmOperand& a, const GemmOperand& b, int64_t m, int64_t n,
-                 int64_t k, const GemmEpilogue& e, cudaStream_t stream) {
-    const dim3 grid((unsigned)((m + kTile - 1) / kTile), (unsigned)((n + kTile - 1) / kTile));
-    if (dtype == MG_PREC_BF16)
-        gemm_kernel<MG_PREC_BF16><<<grid, 256, 0, stream>>>(a, b, m, n, k, e);
-    else
-        gemm_kernel<MG_PREC_FP16><<<grid, 256, 0, stream>>>(a, b, m, n, k, e);
-    launched("gemm_kernel");
+StagedOperand stage_operand(Workspace& w, bool go, const GemmOperand& op, int64_t rows, int64_t k,
+                            cudaStream_t stream) {
+    // a dimension of one element has no stride of its own
+    const int64_t row = rows == 1 ? up8(std::max(k, op.row)) : op.row, col = k == 1 ? up8(std::max(rows, op.col)) : op.col;
+    const int64_t top = int64_t(1) << 38;
+    StagedOperand s;
+    s.data = op.data;
+    if (op.col == 1 || k == 1) {
+        s.ld = row;
+        if (row % 8 == 0 && row >= k && row < top && aligned16(op.data)) return s;
+    }
+    if (op.row == 1 || rows == 1) {
+        s.ld = col;
+        s.mn = true;
+        if (col % 8 == 0 && col >= rows && col < top && aligned16(op.data)) return s;
+    }
+    // copied along the way it lies, so that reads and writes are both in order
+    s.mn = op.row == 1 && op.col != 1;
+    const int64_t lines = s.mn ? k : rows, len = s.mn ? rows : k;
+    s.ld = up8(len);
+    uint16_t* out = w.take<uint16_t>((size_t)lines * s.ld * 2);
+    s.data = out;
+    if (go) {
+        w.require();
+        const dim3 grid((unsigned)std::min<int64_t>((len + 255) / 256, 1024), (unsigned)std::min<int64_t>(lines, 65535));
+        pack_kernel<<<grid, 256, 0, stream>>>(static_cast<const uint16_t*>(op.data), s.mn ? op.col : op.row,
+                                              s.mn ? op.row : op.col, lines, len, s.ld, out);
+        launched("pack_kernel");
+    }
+    return s;
+}
+
+void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, cudaStream_t stream) {
+    if (count == 2 && jobs[1].k > jobs[0].k) std::swap(jobs[0], jobs[1]);
+    const int bn = tile_columns(jobs, count);
+    KernelArgs a{};
+    GemmEpilogue finish[2];
+    double len[2] = {0, 0};
+    for (int i = 0; i < count; ++i) {
+        JobArgs& j = a.job[i];
+        const GemmJob& g = jobs[i];
+        lay_out(j, g, bn);
+        j.e = finish[i] = g.e;
+        j.vec = g.e.ld % 8 == 0 && g.n % 8 == 0 && aligned16(g.e.out) && aligned16(g.e.z) &&
+                (g.e.res == nullptr || (aligned16(g.e.res) && g.e.r_col == 1 && g.e.r_row % 8 == 0));
+        const int64_t tiles = (int64_t)j.tiles_m * j.tiles_n;
+        // Few tiles: their K steps are shared out over the idle pairs, at least 8 steps each.
+        const int splits = tiles * 2 <= kPairs ? (int)std::min<int64_t>(kPairs / tiles, j.kblocks / 8) : 1;
+        j.kb_split = (j.kblocks + std::max(splits, 1) - 1) / std::max(splits, 1);
+        j.splits = (j.kblocks + j.kb_split - 1) / j.kb_split;
+        if (j.splits > 1) {
+            j.e = GemmEpilogue{};
+            j.e.ld32 = up8(g.n);
+            j.e.out32 = w.take<float>((size_t)j.splits * g.m * j.e.ld32 * 4);
+        }
+        a.units[i] = (int)(tiles * j.splits);
+        len[i] = j.kb_split + 4.0;  // a tile's epilogue is worth a few K steps
+    }
+    if (!go) return;
+    w.require();
+    for (int i = 0; i < count; ++i) encode_operands(a, i, dtype, jobs[i], bn);
+    a.head_start = count == 2 ? (int)(len[0] / len[1] + 0.5) : 0;
+    launch<kStore>(a, bn, dtype, stream);
+    for (int i = 0; i < count; ++i)
+        if (a.job[i].splits > 1) {
+            const int64_t total = jobs[i].m * jobs[i].n;
+            const unsigned grid = (unsigned)std::min<int64_t>((total + 255) / 256, 148 * 8);
+            const float* part = a.job[i].e.out32;
+            if (dtype == MG_PREC_BF16)
+                finish_kernel<MG_PREC_BF16><<<grid, 256, 0, stream>>>(part, a.job[i].splits, jobs[i].m, jobs[i].n,
+                                                                      a.job[i].e.ld32, finish[i]);
+            else
+                finish_kernel<MG_PREC_FP16><<<grid, 256, 0, stream>>>(part, a.job[i].splits, jobs[i].m, jobs[i].n,
+                                                                      a.job[i].e.ld32, finish[i]);
+            launched("finish_kernel");
+        }
+}
+
+int gemm_softmax_block(int64_t m, int64_t n) {
+    SoftmaxJob g;
+    g.m = m;
+    g.n = n;
+    g.k = 1;
+    return tile_columns(&g, 1) / 2;
+}
+
+void gemm_softmax(int dtype, const SoftmaxJob& g, int block, cudaStream_t stream) {
+    const int bn = 2 * block;
+    KernelArgs a{};
+    lay_out(a.job[0], g, bn);
+    a.job[0].s = g.e;
+    a.units[0] = a.job[0].tiles_m * a.job[0].tiles_n;
+    encode_operands(a, 0, dtype, g, bn);
+    launch<kSoftmax>(a, bn, dtype, stream);
 }
 
 }  // namespace ops

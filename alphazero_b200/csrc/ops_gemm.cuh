@@ -1,5 +1,5 @@
 // Matrix products of the training operators: C[i][j] = sum_k A[i][k] B[j][k]
-// with a fused epilogue.
+// in bf16 or fp16 with 32-bit sums, with a fused epilogue.
 #pragma once
 
 #include "ops_common.cuh"
@@ -13,23 +13,88 @@ struct GemmOperand {
     int64_t row, col;
 };
 
-// out = act(alpha * acc + bias) + res_scale * res; z = alpha * acc + bias.
+// An operand a TMA map can describe: 16-byte aligned, one unit stride, the
+// other (ld) a multiple of 8.  mn: the unit stride runs along i, not k.
+struct StagedOperand {
+    const void* data = nullptr;
+    int64_t ld = 0;
+    bool mn = false;
+};
+
+// z = alpha * acc + bias; out = act(z) + res_scale * res, both 16-bit.
 struct GemmEpilogue {
     const void* bias = nullptr;      // [n]
     const void* res = nullptr;       // [m][n]
     int64_t r_row = 0, r_col = 0;
     void* out = nullptr;             // [m][n], row stride ld
     void* z = nullptr;               // [m][n], row stride ld
-    float* out32 = nullptr;          // [m][n] fp32 instead of out
-    int64_t ld = 0;
+    float* out32 = nullptr;          // acc + acc32 in fp32, row stride ld32 (a multiple of 8), and nothing else
+    const float* acc32 = nullptr;    // fp32 sums of earlier pieces, added to acc
+    int64_t ld = 0, ld32 = 0;
     float res_scale = 0.0f;
     int act = MG_ACT_NONE;
     float alpha = 1.0f;
     const int* count = nullptr;      // alpha is divided by max(*count, 1)
 };
 
-void launch_gemm(int dtype, const GemmOperand& a, const GemmOperand& b, int64_t m, int64_t n,
-                 int64_t k, const GemmEpilogue& e, cudaStream_t stream);
+struct GemmJob {
+    StagedOperand a, b;
+    int64_t m = 0, n = 0, k = 0;
+    GemmEpilogue e;
+};
+
+// Softmax statistics of l = acc + bias instead of a product (the forward
+// half of the cross entropy).  A row's columns are taken in blocks of
+// `block` (gemm_softmax_block()); per block and row
+//   part[block * part_ld + row] = (max, sum of exp(l - max)),
+// (-inf, 0) for a block of -inf; logit[row] = l at the row's target; and, if
+// probs is set, probs[row * probs_ld + col] = exp(l - max) as a Prob16.
+struct SoftmaxEpilogue {
+    const void* bias = nullptr;       // [n]
+    const int* target = nullptr;      // [m], -1 for none
+    float* logit = nullptr;           // [m]
+    float2* part = nullptr;
+    int64_t part_ld = 0;
+    uint16_t* probs = nullptr;
+    int64_t probs_ld = 0;             // a multiple of 8, at least n
+};
+struct SoftmaxJob {
+    StagedOperand a, b;
+    int64_t m = 0, n = 0, k = 0;
+    SoftmaxEpilogue e;
+};
+int gemm_softmax_block(int64_t m, int64_t n);
+// `block`: gemm_softmax_block of the largest m that shares part's layout.
+void gemm_softmax(int dtype, const SoftmaxJob& job, int block, cudaStream_t stream);
+
+// A number in [0, 1] in 16 bits: 4 bits of exponent and 12 of fraction, no
+// sign (relative error 2^-14 from 2^-14 up, absolute 2^-28 below).  A block's
+// largest is 1, so the range is where the block's probabilities are, and the
+// rounding is far below the one to bf16 or fp16 that follows.  It is an fp32
+// value scaled by 2^-112, whose exponent then has four bits, cut to its top
+// 16 bits below the exponent's fourth.
+__device__ __forceinline__ uint32_t prob16(float v) {
+    return (__float_as_uint(v * 0x1p-112f) + 0x400u) >> 11;
+}
+// Two of them in one word.  (The byte permutation is written out: as shifts
+// and an or, nvcc 12.9 -O3 drops the high half.)
+__device__ __forceinline__ uint32_t prob16x2(float low, float high) {
+    return __byte_perm(prob16(low), prob16(high), 0x5410);
+}
+__device__ __forceinline__ float prob16_value(uint32_t u) { return __uint_as_float(u << 11) * 0x1p112f; }
+
+// Gives an operand of `rows` x k in a form the products read: itself where
+// it lies right, else a copy in the workspace (made now if `go`).
+StagedOperand stage_operand(Workspace& w, bool go, const GemmOperand& op, int64_t rows, int64_t k,
+                            cudaStream_t stream);
+// The same matrix with i and k exchanged.
+inline StagedOperand transposed(StagedOperand s) {
+    s.mn = !s.mn;
+    return s;
+}
+
+// One or two products in one launch (the one with more k first).
+void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, cudaStream_t stream);
 
 __device__ __forceinline__ float activate(float z, int act) {
     switch (act) {

@@ -22,22 +22,58 @@ __device__ __forceinline__ float slope(float z, int act) {
     }
 }
 
-// g = grad * act'(z) and db = sum of g over rows; one thread per column.
-template <int DT>
-__global__ void __launch_bounds__(256) slope_kernel(mg_linear_backward_args a, void* g) {
+// g = grad * act'(z) (if g is set) and, per block of rows, the column sums of
+// grad * act'(z) before their rounding.  One pass; a thread has V adjacent
+// columns (V = 8: 16-byte accesses) of every eighth row of its block, the
+// eight sums of a column meet in shared memory.
+template <int DT, int V>
+__global__ void __launch_bounds__(256)
+    slope_kernel(mg_linear_backward_args a, uint16_t* g, int64_t ldg, int rows_per_block, float* sums) {
     using E = Elem<DT>;
     using T = typename E::T;
-    const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (j >= a.n) return;
-    float sum = 0.0f;
-    for (int64_t i = 0; i < a.m; ++i) {
-        float v = E::get(static_cast<const T*>(a.grad)[i * a.g_row + j * a.g_col]);
-        if (a.activation != MG_ACT_NONE)
-            v *= slope(E::get(static_cast<const T*>(a.z)[i * a.z_row + j * a.z_col]), a.activation);
-        if (g) static_cast<T*>(g)[i * a.n + j] = E::put(v);
-        sum += v;
+    __shared__ float part[8][32 * V];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * (32 * V) + lane * V;
+    const int64_t r0 = (int64_t)blockIdx.y * rows_per_block, r1 = min(a.m, r0 + rows_per_block);
+    const T* dy = static_cast<const T*>(a.grad);
+    const T* z = static_cast<const T*>(a.z);
+    float sum[V] = {};
+    if (c < a.n)
+        for (int64_t r = r0 + warp; r < r1; r += 8) {
+            alignas(16) T dv[V], zv[V];
+            if constexpr (V == 8) {
+                *reinterpret_cast<uint4*>(dv) = __ldg(reinterpret_cast<const uint4*>(dy + r * a.g_row + c));
+                if (g) *reinterpret_cast<uint4*>(zv) = __ldg(reinterpret_cast<const uint4*>(z + r * a.z_row + c));
+            } else {
+                dv[0] = dy[r * a.g_row + c * a.g_col];
+                if (g) zv[0] = z[r * a.z_row + c * a.z_col];
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float v = E::get(dv[i]);
+                if (g) {
+                    v *= slope(E::get(zv[i]), a.activation);
+                    dv[i] = E::put(v);
+                }
+                sum[i] += v;
+            }
+            if (g) {
+                if constexpr (V == 8) *reinterpret_cast<uint4*>(g + r * ldg + c) = *reinterpret_cast<uint4*>(dv);
+                else reinterpret_cast<T*>(g)[r * ldg + c] = dv[0];
+            }
+        }
+    if (sums == nullptr) return;
+#pragma unroll
+    for (int i = 0; i < V; ++i) part[warp][lane * V + i] = sum[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * V; i += 256) {
+        const int64_t col = (int64_t)blockIdx.x * (32 * V) + i;
+        if (col >= a.n) continue;
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) s += part[w][i];
+        sums[(int64_t)blockIdx.y * a.n + col] = s;
     }
-    if (a.db) static_cast<T*>(a.db)[j] = E::put(sum);
 }
 
 void check_sizes(int64_t m, int64_t n, int64_t k) {
@@ -69,43 +105,85 @@ void check(const mg_linear_backward_args& a) {
 }
 
 void linear(const mg_linear_args& a, Workspace& w, bool go, cudaStream_t s) {
-    if (!go || a.m == 0) return;
-    w.require();
-    GemmEpilogue e;
-    e.bias = a.bias;
-    e.res = a.residual;
-    e.r_row = a.r_row;
-    e.r_col = a.r_col;
-    e.out = a.y;
-    e.z = a.z;
-    e.ld = a.n;
-    e.res_scale = a.residual_scale;
-    e.act = a.activation;
-    launch_gemm(a.dtype, {a.x, a.x_row, a.x_col}, {a.weight, a.w_row, a.w_col}, a.m, a.n, a.k, e, s);
+    if (a.m == 0) return;
+    GemmJob job;
+    job.a = stage_operand(w, go, {a.x, a.x_row, a.x_col}, a.m, a.k, s);
+    job.b = stage_operand(w, go, {a.weight, a.w_row, a.w_col}, a.n, a.k, s);
+    job.m = a.m;
+    job.n = a.n;
+    job.k = a.k;
+    job.e.bias = a.bias;
+    job.e.res = a.residual;
+    job.e.r_row = a.r_row;
+    job.e.r_col = a.r_col;
+    job.e.out = a.y;
+    job.e.z = a.z;
+    job.e.ld = a.n;
+    job.e.res_scale = a.residual_scale;
+    job.e.act = a.activation;
+    gemm(w, go, a.dtype, &job, 1, s);
 }
 
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
 void linear_backward(const mg_linear_backward_args& a, Workspace& w, bool go, cudaStream_t s) {
-    const bool has_g = a.activation != MG_ACT_NONE && a.m > 0;
-    void* g = has_g ? w.take((size_t)a.m * a.n * 2) : nullptr;
-    if (!go) return;
-    w.require();
-    if (a.db || has_g) {
-        const unsigned blocks = (unsigned)((a.n + 255) / 256);
-        if (a.dtype == MG_PREC_BF16) slope_kernel<MG_PREC_BF16><<<blocks, 256, 0, s>>>(a, g);
-        else slope_kernel<MG_PREC_FP16><<<blocks, 256, 0, s>>>(a, g);
-        launched("slope_kernel");
+    if (a.m == 0) {
+        if (!go) return;
+        if (a.dw) ops::check(cudaMemsetAsync(a.dw, 0, (size_t)a.n * a.k * 2, s), "cudaMemsetAsync");
+        if (a.db) ops::check(cudaMemsetAsync(a.db, 0, (size_t)a.n * 2, s), "cudaMemsetAsync");
+        return;
     }
-    const GemmOperand gr = has_g ? GemmOperand{g, a.n, 1} : GemmOperand{a.grad, a.g_row, a.g_col};
-    GemmEpilogue e;
-    e.ld = a.k;
-    if (a.dx && a.m > 0) {
-        e.out = a.dx;
-        launch_gemm(a.dtype, gr, {a.weight, a.w_col, a.w_row}, a.m, a.k, a.n, e, s);
+    const bool has_g = a.activation != MG_ACT_NONE;
+    const int64_t ldg = (a.n + 7) / 8 * 8;
+    uint16_t* g = has_g ? w.take<uint16_t>((size_t)a.m * ldg * 2) : nullptr;
+    if (a.db || has_g) {
+        const bool vec = a.n % 8 == 0 && aligned16(a.grad) && a.g_col == 1 && a.g_row % 8 == 0 &&
+                         (!has_g || (aligned16(a.z) && a.z_col == 1 && a.z_row % 8 == 0));
+        const int64_t across = (a.n + (vec ? 255 : 31)) / (vec ? 256 : 32);
+        // about eight blocks per SM, at least 32 rows each
+        const int64_t want = std::max<int64_t>(1, 148 * 8 / across);
+        const int rows = (int)std::max<int64_t>(32, (a.m + want - 1) / want);
+        const int64_t down = (a.m + rows - 1) / rows;
+        float* sums = a.db ? w.take<float>((size_t)down * a.n * 4) : nullptr;
+        if (go) {
+            w.require();
+            const dim3 grid((unsigned)across, (unsigned)down);
+            const bool bf = a.dtype == MG_PREC_BF16;
+            if (vec && bf) slope_kernel<MG_PREC_BF16, 8><<<grid, 256, 0, s>>>(a, g, ldg, rows, sums);
+            else if (vec) slope_kernel<MG_PREC_FP16, 8><<<grid, 256, 0, s>>>(a, g, ldg, rows, sums);
+            else if (bf) slope_kernel<MG_PREC_BF16, 1><<<grid, 256, 0, s>>>(a, g, ldg, rows, sums);
+            else slope_kernel<MG_PREC_FP16, 1><<<grid, 256, 0, s>>>(a, g, ldg, rows, sums);
+            launched("slope_kernel");
+            if (a.db) add_rows(a.dtype, sums, down, a.n, 1.0f, nullptr, a.db, s);
+        }
+    }
+    StagedOperand gs;
+    gs.data = g;
+    gs.ld = ldg;
+    if (!has_g) gs = stage_operand(w, go, {a.grad, a.g_row, a.g_col}, a.m, a.n, s);
+    GemmJob jobs[2];
+    int count = 0;
+    if (a.dx) {
+        GemmJob& j = jobs[count++];
+        j.a = gs;
+        j.b = stage_operand(w, go, {a.weight, a.w_col, a.w_row}, a.k, a.n, s);
+        j.m = a.m;
+        j.n = a.k;
+        j.k = a.n;
+        j.e.out = a.dx;
+        j.e.ld = a.k;
     }
     if (a.dw) {
-        e.out = a.dw;
-        launch_gemm(a.dtype, {gr.data, gr.col, gr.row}, {a.x, a.x_col, a.x_row}, a.n, a.k, a.m, e, s);
+        GemmJob& j = jobs[count++];
+        j.a = transposed(gs);
+        j.b = stage_operand(w, go, {a.x, a.x_col, a.x_row}, a.k, a.m, s);
+        j.m = a.n;
+        j.n = a.k;
+        j.k = a.m;
+        j.e.out = a.dw;
+        j.e.ld = a.k;
     }
+    if (count > 0) gemm(w, go, a.dtype, jobs, count, s);
 }
 
 }  // namespace
