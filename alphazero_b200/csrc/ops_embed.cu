@@ -14,7 +14,6 @@
 // over as many warps as its rows deserve, there are no atomics on sums, and
 // the result does not depend on the order in which blocks run.
 #include "ops_common.cuh"
-#include "ptx_sm100.cuh"
 
 #include <algorithm>
 
@@ -110,125 +109,165 @@ void embed(const mg_embed_args& a, cudaStream_t s) {
 }
 
 // ---- sort ----
+//
+// Stable least-significant-digit radix sort of (token, position), padding
+// last as token `vocab`: two launches per digit.  rank_kernel gives each
+// token its place among its block's tokens of the same digit and counts the
+// block's digits; scatter_kernel adds up the counts of smaller digits and
+// earlier blocks and moves the tokens.  The moves are scattered 8-byte
+// writes, which one SM does at about one a clock: so the sort uses up to 148
+// blocks rather than one cluster (16 CTAs: 22 us a digit for 65536 tokens,
+// where these two take 7).
 
-constexpr int kSortWarps = 32;
-constexpr int kSortCtas = 8;   // of the cluster
-constexpr int kMaxBits = 10;   // of the key per pass
+constexpr int kSortWarps = 16;
+constexpr int kSortThreads = 32 * kSortWarps;
+constexpr int kMaxBits = 10;  // of the key per pass
+constexpr int kBatch = 4;     // steps of 32 tokens whose loads a warp issues together
 
 struct SortArgs {
     const void* tokens;
     int token_bytes;
     int64_t token_stride, vocab;
     int n, passes, bits;
-    uint32_t* key[2];
-    uint32_t* pos[2];
+    int blocks, steps;    // steps of 32 tokens per warp
+    uint2* pair[2];       // [n] (token, position)
+    uint32_t* place;      // [n]
+    uint32_t* counts;     // [blocks][bins]
 };
 
-// Stable least-significant-digit radix sort of (token, position), padding
-// last as token `vocab`, by one cluster: its barriers order the passes, and
-// the digit counts travel through distributed shared memory.  Warp w of CTA
-// c has the (32 c + w)-th stretch of the input and its own row of counts,
-// which after a scan over digits, CTAs and warps are the places its tokens
-// go to.  The result is in key[passes & 1], pos[passes & 1].
-__global__ void __launch_bounds__(32 * kSortWarps) sort_kernel(SortArgs a) {
-    extern __shared__ uint32_t counts[];  // [warps][bins], then [bins] sums of the CTA
-    const int bins = 1 << a.bits;
-    uint32_t* total = counts + kSortWarps * bins;
-    __shared__ uint32_t warp_sum[kSortWarps];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = cluster_rank();
-    uint32_t ctas;
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
-    const int64_t per = ((int64_t)a.n + ctas * kSortWarps * 32 - 1) / (ctas * kSortWarps * 32) * 32;
-    const int64_t begin = min((int64_t)a.n, ((int64_t)rank * kSortWarps + warp) * per);
-    const int64_t end = min((int64_t)a.n, begin + per);
-    uint32_t* mine = counts + warp * bins;
+__device__ __forceinline__ uint32_t sort_key(const SortArgs& a, int pass, int64_t i, uint32_t* pos) {
+    if (pass > 0) {
+        const uint2 u = a.pair[pass & 1][i];
+        *pos = u.y;
+        return u.x;
+    }
+    *pos = (uint32_t)i;
+    const int64_t t = index_at(a.tokens, a.token_bytes, i * a.token_stride, a.vocab);
+    return (uint32_t)(t < 0 ? a.vocab : t);
+}
 
-    for (int pass = 0; pass < a.passes; ++pass) {
-        const uint32_t* kin = a.key[pass & 1];
-        const uint32_t* pin = a.pos[pass & 1];
-        uint32_t* kout = a.key[(pass + 1) & 1];
-        uint32_t* pout = a.pos[(pass + 1) & 1];
-        const int shift = pass * a.bits;
-        const auto key_at = [&](int64_t i) -> uint32_t {
-            if (pass > 0) return __ldcg(kin + i);
-            const int64_t t = index_at(a.tokens, a.token_bytes, i * a.token_stride, a.vocab);
-            return (uint32_t)(t < 0 ? a.vocab : t);
-        };
-        for (int b = threadIdx.x; b < kSortWarps * bins; b += blockDim.x) counts[b] = 0;
-        __syncthreads();
-#pragma unroll 4
-        for (int64_t i = begin + lane; i < end; i += 32) atomicAdd(&mine[key_at(i) >> shift & (bins - 1)], 1u);
-        __syncthreads();
-        // bin `threadIdx.x`: counts of the warps before each warp, sum of the CTA
-        if (threadIdx.x < bins) {
-            uint32_t s = 0;
-            for (int w = 0; w < kSortWarps; ++w) {
-                const uint32_t c = counts[w * bins + threadIdx.x];
-                counts[w * bins + threadIdx.x] = s;
-                s += c;
-            }
-            total[threadIdx.x] = s;
+// Equal digits of a warp find one another with match_any, so places follow
+// the order of the input.
+__global__ void __launch_bounds__(kSortThreads) rank_kernel(SortArgs a, int pass) {
+    extern __shared__ uint32_t rows[];  // [warps][bins]
+    const int bins = 1 << a.bits, shift = pass * a.bits;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t begin = ((int64_t)blockIdx.x * kSortWarps + warp) * a.steps * 32;
+    const int64_t end = min((int64_t)a.n, begin + (int64_t)a.steps * 32);
+    uint32_t* mine = rows + warp * bins;
+    uint32_t k[kBatch], at[kBatch], pos;
+    for (int b = threadIdx.x; b < kSortWarps * bins; b += kSortThreads) rows[b] = 0;
+    __syncthreads();
+    const auto load = [&](int64_t i0) {
+#pragma unroll
+        for (int q = 0; q < kBatch; ++q) {
+            const int64_t i = i0 + 32 * q + lane;
+            // past the end: a digit of its own
+            k[q] = i < end ? sort_key(a, pass, i, &pos) >> shift & (bins - 1) : (uint32_t)bins + lane;
         }
-        cluster_sync();
+    };
+    const auto rank = [&]() {
+#pragma unroll
+        for (int q = 0; q < kBatch; ++q) {
+            const uint32_t peers = __match_any_sync(~0u, k[q]);
+            const uint32_t below = __popc(peers & ((1u << lane) - 1));
+            const uint32_t before = k[q] < bins ? mine[k[q]] : 0;
+            __syncwarp();
+            if (k[q] < bins && below == 0) mine[k[q]] = before + __popc(peers);
+            __syncwarp();
+            at[q] = before + below;
+        }
+    };
+    for (int64_t i0 = begin; i0 < end; i0 += 32 * kBatch) {
+        load(i0);
+        rank();
+#pragma unroll
+        for (int q = 0; q < kBatch; ++q)
+            if (i0 + 32 * q + lane < end) a.place[i0 + 32 * q + lane] = at[q];
+    }
+    __syncthreads();
+    // per digit: the counts of the warps before each warp, and of the block
+    for (int b = threadIdx.x; b < bins; b += kSortThreads) {
+        uint32_t s = 0;
+#pragma unroll
+        for (int w = 0; w < kSortWarps; ++w) {
+            const uint32_t c = rows[w * bins + b];
+            rows[w * bins + b] = s;
+            s += c;
+        }
+        a.counts[(int64_t)blockIdx.x * bins + b] = s;
+    }
+    __syncthreads();
+    for (int64_t i0 = begin; i0 < end; i0 += 32 * kBatch) {
+        if (a.steps > kBatch) load(i0);  // else still in k and at
+#pragma unroll
+        for (int q = 0; q < kBatch; ++q) {
+            const int64_t i = i0 + 32 * q + lane;
+            if (i < end) a.place[i] = (a.steps > kBatch ? a.place[i] : at[q]) + mine[k[q]];
+        }
+    }
+}
+
+__global__ void __launch_bounds__(kSortThreads) scatter_kernel(SortArgs a, int pass) {
+    extern __shared__ uint32_t rows[];  // [slices][2][bins]: counts of earlier blocks, of all
+    __shared__ uint32_t warp_sum[kSortWarps];
+    const int bins = 1 << a.bits, shift = pass * a.bits;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // four adjacent digits per thread, the blocks in `slices` interleaved shares
+    const int quads = bins / 4, slices = max(1, kSortThreads / quads);
+    if (threadIdx.x < slices * quads) {
+        const int quad = threadIdx.x % quads, slice = threadIdx.x / quads;
+        uint4 before = make_uint4(0, 0, 0, 0), all = before;
+#pragma unroll 8
+        for (int b = slice; b < a.blocks; b += slices) {
+            const uint4 c = *reinterpret_cast<const uint4*>(a.counts + (int64_t)b * bins + quad * 4);
+            all.x += c.x, all.y += c.y, all.z += c.z, all.w += c.w;
+            if (b < blockIdx.x) before.x += c.x, before.y += c.y, before.z += c.z, before.w += c.w;
+        }
+        *reinterpret_cast<uint4*>(rows + (slice * 2) * bins + quad * 4) = before;
+        *reinterpret_cast<uint4*>(rows + (slice * 2 + 1) * bins + quad * 4) = all;
+    }
+    __syncthreads();
+    uint32_t carry = 0;
+    for (int b0 = 0; b0 < bins; b0 += kSortThreads) {
+        const int b = b0 + threadIdx.x;
         uint32_t before = 0, all = 0;
-        if (threadIdx.x < bins)
-            for (uint32_t r = 0; r < ctas; ++r) {
-                uint32_t c;
-                asm volatile("ld.shared::cluster.u32 %0, [%1];"
-                             : "=r"(c)
-                             : "r"(map_to_rank(smem_u32(&total[threadIdx.x]), r))
-                             : "memory");
-                if (r < rank) before += c;
-                all += c;
+        if (b < bins)
+            for (int s = 0; s < slices; ++s) {
+                before += rows[s * 2 * bins + b];
+                all += rows[(s * 2 + 1) * bins + b];
             }
         uint32_t scan = all;
+#pragma unroll
         for (int d = 1; d < 32; d *= 2) {
             const uint32_t up = __shfl_up_sync(~0u, scan, d);
             if (lane >= d) scan += up;
         }
         if (lane == 31) warp_sum[warp] = scan;
         __syncthreads();
-        if (warp == 0) {
-            uint32_t v = warp_sum[lane], inc = v;
-            for (int d = 1; d < 32; d *= 2) {
-                const uint32_t up = __shfl_up_sync(~0u, inc, d);
-                if (lane >= d) inc += up;
-            }
-            warp_sum[lane] = inc - v;
+        uint32_t lower = carry;
+#pragma unroll
+        for (int w = 0; w < kSortWarps; ++w) {
+            if (w < warp) lower += warp_sum[w];
+            carry += warp_sum[w];
         }
+        if (b < bins) rows[b] = lower + scan - all + before;  // slice 0's counts of earlier blocks are used up
         __syncthreads();
-        if (threadIdx.x < bins) {
-            const uint32_t base = warp_sum[warp] + scan - all + before;
-            for (int w = 0; w < kSortWarps; ++w) counts[w * bins + threadIdx.x] += base;
-        }
-        __syncthreads();
-        for (int64_t i0 = begin; i0 < end; i0 += 32) {
-            const int64_t i = i0 + lane;
-            const bool in = i < end;
-            const uint32_t k = in ? key_at(i) : 0;
-            const uint32_t p = !in ? 0 : pass > 0 ? __ldcg(pin + i) : (uint32_t)i;
-            const uint32_t digit = in ? k >> shift & (bins - 1) : (uint32_t)bins + lane;
-            const uint32_t peers = __match_any_sync(~0u, digit);
-            const uint32_t below = __popc(peers & ((1u << lane) - 1));
-            const uint32_t to = in ? mine[digit] + below : 0;
-            __syncwarp();
-            if (in && below == 0) mine[digit] += __popc(peers);
-            __syncwarp();
-            if (in) {
-                kout[to] = k;
-                pout[to] = p;
-            }
-        }
-        cluster_sync();  // before the next pass reads what this one wrote (and reuses the counts)
+    }
+    const int64_t begin = (int64_t)blockIdx.x * a.steps * kSortThreads;
+    const int64_t end = min((int64_t)a.n, begin + (int64_t)a.steps * kSortThreads);
+#pragma unroll 4
+    for (int64_t i = begin + threadIdx.x; i < end; i += kSortThreads) {
+        uint32_t pos;
+        const uint32_t k = sort_key(a, pass, i, &pos);
+        a.pair[(pass + 1) & 1][rows[k >> shift & (bins - 1)] + a.place[i]] = make_uint2(k, pos);
     }
 }
 
 // ---- sums ----
 
 struct SumArgs {
-    const uint32_t* key;  // sorted
-    const uint32_t* pos;
+    const uint2* pair;  // sorted (token, position)
     int n, window, windows;
     int64_t segments;
     const void* grad;
@@ -297,32 +336,33 @@ struct Columns {
 
 constexpr int kAhead = 8;  // rows in flight per warp
 
-// First place in the sorted keys whose key is at least v.
-__device__ __forceinline__ int lower_bound(const uint32_t* key, int n, uint32_t v) {
+// First place in the sorted tokens whose token is at least v.
+__device__ __forceinline__ int lower_bound(const uint2* pair, int n, uint32_t v) {
     int lo = 0, hi = n;
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (key[mid] < v) lo = mid + 1;
+        if (pair[mid].x < v) lo = mid + 1;
         else hi = mid;
     }
     return lo;
 }
 
-// Blocks [0, sum_blocks) sum the windows, a warp per window and segment; the
-// others write zeros to the rows of 256 entries each that no token names.
+// The first zero_blocks blocks write zeros to the rows, of 256 entries each,
+// that no token names (first, so that their searches overlap the sums); the
+// others sum the windows, a warp per window and segment.
 template <int DT, bool VEC>
-__global__ void __launch_bounds__(256) sum_kernel(SumArgs a, int64_t sum_blocks) {
+__global__ void __launch_bounds__(256, 3) sum_kernel(SumArgs a, int64_t zero_blocks) {
     using C = Columns<DT, VEC>;
     using T = typename C::T;
     constexpr int N = C::N;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (blockIdx.x >= sum_blocks) {
+    if (blockIdx.x < zero_blocks) {
         __shared__ bool empty[256];
-        const int64_t v0 = (blockIdx.x - sum_blocks) * 256, v = v0 + threadIdx.x;
+        const int64_t v0 = (int64_t)blockIdx.x * 256, v = v0 + threadIdx.x;
         bool none = false;
         if (v < a.vocab) {
-            const int at = lower_bound(a.key, a.n, (uint32_t)v);
-            none = at == a.n || a.key[at] != (uint32_t)v;
+            const int at = lower_bound(a.pair, a.n, (uint32_t)v);
+            none = at == a.n || a.pair[at].x != (uint32_t)v;
         }
         empty[threadIdx.x] = none;
         __syncthreads();
@@ -333,128 +373,146 @@ __global__ void __launch_bounds__(256) sum_kernel(SumArgs a, int64_t sum_blocks)
                     C(s, a.dim).store(static_cast<T*>(a.d_table) + (v0 + r) * a.dim, zero, 1.0f);
         return;
     }
-    const int64_t task = (int64_t)blockIdx.x * 8 + warp;
+    const int64_t task = (blockIdx.x - zero_blocks) * 8 + warp;
     const int64_t window = task / a.segments;
     if (window >= a.windows) return;
     const C c(task % a.segments, a.dim);
     const int s0 = (int)window * a.window, s1 = min(a.n, s0 + a.window);
-    uint32_t run = a.key[s0];
-    bool from_prev = s0 > 0 && a.key[s0 - 1] == run;
+    uint32_t run = a.pair[s0].x;
+    const uint32_t before = s0 > 0 ? a.pair[s0 - 1].x : ~0u, after = s1 < a.n ? a.pair[s1].x : ~0u;
+    if (run >= a.vocab) return;
+    bool from_prev = before == run;
     float sum[N] = {};
-    const auto flush = [&](bool to_next) {
-        if (from_prev) c.store32(a.head + window * a.dim, sum);
-        else if (to_next) c.store32(a.tail + window * a.dim, sum);
-        else c.store(static_cast<T*>(a.d_table) + (int64_t)run * a.dim, sum, a.scale);
-    };
-    for (int j0 = s0; j0 < s1 && run < a.vocab; j0 += 32) {
-        const int have = min(32, s1 - j0);
-        const uint32_t k = lane < have ? a.key[j0 + lane] : ~0u;
-        const uint32_t p = lane < have ? a.pos[j0 + lane] : 0;
-        for (int j = 0; j < have; j += kAhead) {
+    for (int j0 = s0; j0 < s1; j0 += 32) {
+        const uint2 u = j0 + lane < s1 ? a.pair[j0 + lane] : make_uint2(~0u, 0);
+        const int valid = __popc(__ballot_sync(~0u, u.x < a.vocab));  // padding comes last
+        uint32_t up = __shfl_up_sync(~0u, u.x, 1);
+        if (lane == 0) up = run;
+        const uint32_t starts = __ballot_sync(~0u, u.x != up);
+        for (int j = 0; j < valid; j += kAhead) {
             alignas(16) T v[kAhead][N];
 #pragma unroll
             for (int q = 0; q < kAhead; ++q) {
-                const uint32_t at = __shfl_sync(~0u, p, j + q), key = __shfl_sync(~0u, k, j + q);
-                if (key < a.vocab) c.load(static_cast<const T*>(a.grad) + (int64_t)at * a.grad_row, v[q]);
+                const uint32_t at = __shfl_sync(~0u, u.y, j + q);
+                if (j + q < valid) c.load(static_cast<const T*>(a.grad) + at * a.grad_row, v[q]);
             }
 #pragma unroll
             for (int q = 0; q < kAhead; ++q) {
-                const uint32_t key = __shfl_sync(~0u, k, j + q);
-                if (key >= a.vocab && key != run && j + q >= have) continue;  // past the window
-                if (key != run) {
-                    if (run < a.vocab) flush(false);
-                    run = key;
+                if (j + q >= valid) break;
+                if (starts >> (j + q) & 1) {
+                    if (from_prev) c.store32(a.head + window * a.dim, sum);
+                    else c.store(static_cast<T*>(a.d_table) + run * a.dim, sum, a.scale);
                     from_prev = false;
+                    run = __shfl_sync(~0u, u.x, j + q);
 #pragma unroll
                     for (int i = 0; i < N; ++i) sum[i] = 0.0f;
                 }
-                if (key < a.vocab)
 #pragma unroll
-                    for (int i = 0; i < N; ++i) sum[i] += C::E::get(v[q][i]);
+                for (int i = 0; i < N; ++i) sum[i] += C::E::get(v[q][i]);
             }
         }
+        if (valid < 32) break;
     }
-    if (run < a.vocab) flush(s1 < a.n && a.key[s1] == run);
+    if (from_prev) c.store32(a.head + window * a.dim, sum);
+    else if (after == run) c.store32(a.tail + window * a.dim, sum);
+    else c.store(static_cast<T*>(a.d_table) + run * a.dim, sum, a.scale);
 }
 
-// Adds the parts of the run that begins in window blockIdx.x and goes past
-// its end; the block's warps take equal stretches of its windows.
+// Adds the parts of the runs that begin in windows 8 blockIdx.x .. + 7 and
+// go past their end; the block's warps take equal stretches of a run's
+// windows.
 template <int DT, bool VEC>
-__global__ void __launch_bounds__(256) join_kernel(SumArgs a) {
+__global__ void __launch_bounds__(256, 3) join_kernel(SumArgs a) {
     using C = Columns<DT, VEC>;
     using T = typename C::T;
     constexpr int N = C::N;
-    const int64_t window = blockIdx.x;
-    const int s0 = (int)window * a.window, s1 = s0 + a.window;
-    if (s1 >= a.n) return;
-    const uint32_t run = a.key[s1 - 1];
-    if (run >= a.vocab || a.key[s1] != run) return;                                // ends here
-    if (a.key[s0] == run && s0 > 0 && a.key[s0 - 1] == run) return;                // began earlier
-    const int warp = threadIdx.x >> 5;
     __shared__ float part[8][32][N + 1];
-    const int64_t last = (lower_bound(a.key + s1, a.n - s1, run + 1) + s1 - 1) / a.window;
-    const int64_t per = (last - window + 7) / 8;
-    const C c(blockIdx.y, a.dim);
-    float sum[N] = {};
-    const int64_t from = window + 1 + warp * per, to = min(last + 1, from + per);
-    for (int64_t w0 = from; w0 < to; w0 += kAhead) {
-        float v[kAhead][N];
-#pragma unroll
-        for (int q = 0; q < kAhead; ++q)
-            if (w0 + q < to) c.load32(a.head + (w0 + q) * a.dim, v[q]);
-#pragma unroll
-        for (int q = 0; q < kAhead; ++q)
-            if (w0 + q < to)
-#pragma unroll
-                for (int i = 0; i < N; ++i) sum[i] += v[q][i];
+    __shared__ uint32_t runs[8];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x < 8) {
+        const int64_t w = (int64_t)blockIdx.x * 8 + threadIdx.x;
+        const int64_t s0 = w * a.window, s1 = s0 + a.window;
+        uint32_t run = ~0u;
+        if (s1 < a.n) {
+            const uint32_t k = a.pair[s1 - 1].x, next = a.pair[s1].x, before = s0 > 0 ? a.pair[s0 - 1].x : ~0u;
+            if (k < a.vocab && next == k && before != k) run = k;
+        }
+        runs[threadIdx.x] = run;
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) part[warp][threadIdx.x & 31][i] = sum[i];
     __syncthreads();
-    if (warp > 0) return;
-    c.load32(a.tail + window * a.dim, sum);
-    for (int w = 0; w < 8; ++w)
+    const C c(blockIdx.y, a.dim);
+    for (int r = 0; r < 8; ++r) {
+        const uint32_t run = runs[r];
+        if (run == ~0u) continue;
+        const int64_t window = (int64_t)blockIdx.x * 8 + r;
+        // the windows that go on with the run: those whose first token is its own
+        int64_t last = window;
+        for (int more = 256; more == 256; last += more) {
+            const int64_t x = last + 1 + threadIdx.x;
+            more = __syncthreads_count(x < a.windows && a.pair[x * a.window].x == run);
+        }
+        const int64_t per = (last - window + 7) / 8;
+        const int64_t from = window + 1 + warp * per, to = min(last + 1, from + per);
+        float sum[N] = {};
+        for (int64_t w0 = from; w0 < to; w0 += 4) {
+            float v[4][N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) sum[i] += part[w][threadIdx.x][i];
-    c.store(static_cast<T*>(a.d_table) + (int64_t)run * a.dim, sum, a.scale);
+            for (int q = 0; q < 4; ++q)
+                if (w0 + q < to) c.load32(a.head + (w0 + q) * a.dim, v[q]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (w0 + q < to)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) sum[i] += v[q][i];
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) part[warp][lane][i] = sum[i];
+        __syncthreads();
+        if (warp == 0) {
+            c.load32(a.tail + window * a.dim, sum);
+            for (int w = 0; w < 8; ++w)
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum[i] += part[w][lane][i];
+            c.store(static_cast<T*>(a.d_table) + run * a.dim, sum, a.scale);
+        }
+        __syncthreads();
+    }
 }
 
 template <int DT, bool VEC>
 void sum_rows(SumArgs a, cudaStream_t s) {
     const int64_t sum_blocks = ((int64_t)a.windows * a.segments + 7) / 8;
-    const int64_t blocks = sum_blocks + (a.vocab + 255) / 256;
+    const int64_t zero_blocks = (a.vocab + 255) / 256, blocks = zero_blocks + sum_blocks;
     need(blocks < (int64_t(1) << 31) && a.segments <= 65535, "n times dim is too large");
-    sum_kernel<DT, VEC><<<(unsigned)blocks, 256, 0, s>>>(a, sum_blocks);
+    sum_kernel<DT, VEC><<<(unsigned)blocks, 256, 0, s>>>(a, zero_blocks);
     launched("sum_kernel");
     if (a.windows > 1) {
-        join_kernel<DT, VEC><<<dim3((unsigned)a.windows, (unsigned)a.segments), 256, 0, s>>>(a);
+        join_kernel<DT, VEC><<<dim3((unsigned)((a.windows + 7) / 8), (unsigned)a.segments), 256, 0, s>>>(a);
         launched("join_kernel");
     }
 }
 
-void sort(SortArgs& a, cudaStream_t s) {
-    int total = 1;
+void plan_sort(SortArgs& a) {
+    int total = 2;
     while ((int64_t(1) << total) <= a.vocab) ++total;  // vocab itself is a key
     a.passes = (total + kMaxBits - 1) / kMaxBits;
     a.bits = (total + a.passes - 1) / a.passes;
-    const int smem = (kSortWarps + 1) * (4 << a.bits);
-    check(cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (kSortWarps + 1) * (4 << kMaxBits)),
-          "cudaFuncSetAttribute(sort_kernel)");
-    cudaLaunchConfig_t cfg{};
-    // one CTA while each of its warps has at most a few steps of 32 tokens
-    const unsigned ctas = a.n <= 4096 ? 1 : kSortCtas;
-    cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(32 * kSortWarps);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = ctas;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    check(cudaLaunchKernelEx(&cfg, sort_kernel, a), "sort_kernel");
+    const int64_t per_step = kSortThreads;
+    a.steps = (int)std::max<int64_t>(2, (a.n + 148 * per_step - 1) / (148 * per_step));
+    a.blocks = (int)((a.n + a.steps * per_step - 1) / (a.steps * per_step));
+}
+
+void sort(const SortArgs& a, cudaStream_t s) {
+    const int bins = 1 << a.bits, slices = std::max(1, kSortThreads / (bins / 4));
+    const int most = kSortWarps * (4 << kMaxBits);
+    check(cudaFuncSetAttribute(rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most),
+          "cudaFuncSetAttribute(rank_kernel)");
+    for (int pass = 0; pass < a.passes; ++pass) {
+        rank_kernel<<<a.blocks, kSortThreads, kSortWarps * bins * 4, s>>>(a, pass);
+        launched("rank_kernel");
+        scatter_kernel<<<a.blocks, kSortThreads, slices * 2 * bins * 4, s>>>(a, pass);
+        launched("scatter_kernel");
+    }
 }
 
 template <int DT>
@@ -470,10 +528,10 @@ void embed_backward(const mg_embed_backward_args& a, Workspace& w, bool go, cuda
     sort_args.token_stride = a.token_stride;
     sort_args.vocab = a.vocab;
     sort_args.n = (int)a.n;
-    for (int i = 0; i < 2; ++i) {
-        sort_args.key[i] = w.take<uint32_t>((size_t)a.n * 4);
-        sort_args.pos[i] = w.take<uint32_t>((size_t)a.n * 4);
-    }
+    plan_sort(sort_args);
+    for (int i = 0; i < 2; ++i) sort_args.pair[i] = w.take<uint2>((size_t)a.n * 8);
+    sort_args.place = w.take<uint32_t>((size_t)a.n * 4);
+    sort_args.counts = w.take<uint32_t>((size_t)sort_args.blocks * 4 << sort_args.bits);
     const bool vec = widest(e, a.dim * e, a.grad_row * e, 0, a.grad, a.d_table) == 16;
     SumArgs sum{};
     sum.n = (int)a.n;
@@ -487,8 +545,7 @@ void embed_backward(const mg_embed_backward_args& a, Workspace& w, bool go, cuda
     if (!go) return;
     w.require();
     sort(sort_args, s);
-    sum.key = sort_args.key[sort_args.passes & 1];
-    sum.pos = sort_args.pos[sort_args.passes & 1];
+    sum.pair = sort_args.pair[sort_args.passes & 1];
     sum.grad = a.grad;
     sum.grad_row = a.grad_row;
     sum.dim = a.dim;
