@@ -60,6 +60,27 @@ inline void check(cudaError_t e, const char* where) {
 }
 inline void launched(const char* kernel) { check(cudaGetLastError(), kernel); }
 
+// Launches a kernel that may begin while the one before it in the stream is
+// finishing (programmatic dependent launch).  Such a kernel calls
+// griddep_wait() in every thread before it touches global memory, and so
+// does every kernel it can follow; the first kernel of a call is launched in
+// the ordinary way, after everything before it.
+template <class... P, class... A>
+void launch_next(const char* name, void (*kernel)(P...), dim3 grid, int block, int smem, cudaStream_t stream,
+                 A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)block);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    check(cudaLaunchKernelEx(&cfg, kernel, P(args)...), name);
+}
+
 // Makes args->device current for one call.
 class OnDevice {
 public:

@@ -14,6 +14,7 @@
 // over as many warps as its rows deserve, there are no atomics on sums, and
 // the result does not depend on the order in which blocks run.
 #include "ops_common.cuh"
+#include "ptx_sm100.cuh"
 
 #include <algorithm>
 
@@ -130,14 +131,16 @@ struct SortArgs {
     int64_t token_stride, vocab;
     int n, passes, bits;
     int blocks, steps;    // steps of 32 tokens per warp
-    uint2* pair[2];       // [n] (token, position)
+    uint2* pair[2];       // [n] (token, position); host side
+    const uint2* in;      // of this pass (the first reads tokens)
+    uint2* out;
     uint32_t* place;      // [n]
     uint32_t* counts;     // [blocks][bins]
 };
 
 __device__ __forceinline__ uint32_t sort_key(const SortArgs& a, int pass, int64_t i, uint32_t* pos) {
     if (pass > 0) {
-        const uint2 u = a.pair[pass & 1][i];
+        const uint2 u = a.in[i];
         *pos = u.y;
         return u.x;
     }
@@ -156,8 +159,10 @@ __global__ void __launch_bounds__(kSortThreads) rank_kernel(SortArgs a, int pass
     const int64_t end = min((int64_t)a.n, begin + (int64_t)a.steps * 32);
     uint32_t* mine = rows + warp * bins;
     uint32_t k[kBatch], at[kBatch], pos;
+    griddep_launch_dependents();
     for (int b = threadIdx.x; b < kSortWarps * bins; b += kSortThreads) rows[b] = 0;
     __syncthreads();
+    griddep_wait();
     const auto load = [&](int64_t i0) {
 #pragma unroll
         for (int q = 0; q < kBatch; ++q) {
@@ -213,6 +218,8 @@ __global__ void __launch_bounds__(kSortThreads) scatter_kernel(SortArgs a, int p
     __shared__ uint32_t warp_sum[kSortWarps];
     const int bins = 1 << a.bits, shift = pass * a.bits;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    griddep_launch_dependents();
+    griddep_wait();
     // four adjacent digits per thread, the blocks in `slices` interleaved shares
     const int quads = bins / 4, slices = max(1, kSortThreads / quads);
     if (threadIdx.x < slices * quads) {
@@ -260,7 +267,7 @@ __global__ void __launch_bounds__(kSortThreads) scatter_kernel(SortArgs a, int p
     for (int64_t i = begin + threadIdx.x; i < end; i += kSortThreads) {
         uint32_t pos;
         const uint32_t k = sort_key(a, pass, i, &pos);
-        a.pair[(pass + 1) & 1][rows[k >> shift & (bins - 1)] + a.place[i]] = make_uint2(k, pos);
+        a.out[rows[k >> shift & (bins - 1)] + a.place[i]] = make_uint2(k, pos);
     }
 }
 
@@ -356,6 +363,8 @@ __global__ void __launch_bounds__(256, 3) sum_kernel(SumArgs a, int64_t zero_blo
     using T = typename C::T;
     constexpr int N = C::N;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    griddep_launch_dependents();
+    griddep_wait();
     if (blockIdx.x < zero_blocks) {
         __shared__ bool empty[256];
         const int64_t v0 = (int64_t)blockIdx.x * 256, v = v0 + threadIdx.x;
@@ -419,52 +428,66 @@ __global__ void __launch_bounds__(256, 3) sum_kernel(SumArgs a, int64_t zero_blo
 }
 
 // Adds the parts of the runs that begin in windows 8 blockIdx.x .. + 7 and
-// go past their end; the block's warps take equal stretches of a run's
-// windows.
+// go past their end.  A run of up to 32 windows more is its warp's own work;
+// for a longer one the block's warps take equal stretches of its windows.
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(256, 3) join_kernel(SumArgs a) {
     using C = Columns<DT, VEC>;
     using T = typename C::T;
     constexpr int N = C::N;
     __shared__ float part[8][32][N + 1];
-    __shared__ uint32_t runs[8];
+    __shared__ uint32_t runs[8];  // the long ones
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (threadIdx.x < 8) {
-        const int64_t w = (int64_t)blockIdx.x * 8 + threadIdx.x;
+    const C c(blockIdx.y, a.dim);
+    griddep_wait();
+    const auto add_windows = [&](int64_t from, int64_t to, float (&sum)[N]) {
+        constexpr int kMore = 32 / N;
+        for (int64_t w0 = from; w0 < to; w0 += kMore) {
+            float v[kMore][N];
+#pragma unroll
+            for (int q = 0; q < kMore; ++q)
+                if (w0 + q < to) c.load32(a.head + (w0 + q) * a.dim, v[q]);
+#pragma unroll
+            for (int q = 0; q < kMore; ++q)
+                if (w0 + q < to)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) sum[i] += v[q][i];
+        }
+    };
+    {
+        const int64_t w = (int64_t)blockIdx.x * 8 + warp;
         const int64_t s0 = w * a.window, s1 = s0 + a.window;
         uint32_t run = ~0u;
         if (s1 < a.n) {
             const uint32_t k = a.pair[s1 - 1].x, next = a.pair[s1].x, before = s0 > 0 ? a.pair[s0 - 1].x : ~0u;
             if (k < a.vocab && next == k && before != k) run = k;
         }
-        runs[threadIdx.x] = run;
+        // the windows that go on with the run: those whose first token is its own
+        const int64_t x = w + 1 + lane;
+        const uint32_t first = x < a.windows ? a.pair[x * a.window].x : ~0u;
+        const int more = __popc(__ballot_sync(~0u, run != ~0u && first == run));
+        if (lane == 0) runs[warp] = more == 32 ? run : ~0u;
+        if (run != ~0u && more < 32) {
+            float sum[N];
+            c.load32(a.tail + w * a.dim, sum);
+            add_windows(w + 1, w + 1 + more, sum);
+            c.store(static_cast<T*>(a.d_table) + run * a.dim, sum, a.scale);
+        }
     }
     __syncthreads();
-    const C c(blockIdx.y, a.dim);
     for (int r = 0; r < 8; ++r) {
         const uint32_t run = runs[r];
         if (run == ~0u) continue;
         const int64_t window = (int64_t)blockIdx.x * 8 + r;
-        // the windows that go on with the run: those whose first token is its own
         int64_t last = window;
         for (int more = 256; more == 256; last += more) {
             const int64_t x = last + 1 + threadIdx.x;
             more = __syncthreads_count(x < a.windows && a.pair[x * a.window].x == run);
         }
         const int64_t per = (last - window + 7) / 8;
-        const int64_t from = window + 1 + warp * per, to = min(last + 1, from + per);
+        const int64_t from = window + 1 + warp * per;
         float sum[N] = {};
-        for (int64_t w0 = from; w0 < to; w0 += 4) {
-            float v[4][N];
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (w0 + q < to) c.load32(a.head + (w0 + q) * a.dim, v[q]);
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (w0 + q < to)
-#pragma unroll
-                    for (int i = 0; i < N; ++i) sum[i] += v[q][i];
-        }
+        add_windows(from, min(last + 1, from + per), sum);
 #pragma unroll
         for (int i = 0; i < N; ++i) part[warp][lane][i] = sum[i];
         __syncthreads();
@@ -484,12 +507,10 @@ void sum_rows(SumArgs a, cudaStream_t s) {
     const int64_t sum_blocks = ((int64_t)a.windows * a.segments + 7) / 8;
     const int64_t zero_blocks = (a.vocab + 255) / 256, blocks = zero_blocks + sum_blocks;
     need(blocks < (int64_t(1) << 31) && a.segments <= 65535, "n times dim is too large");
-    sum_kernel<DT, VEC><<<(unsigned)blocks, 256, 0, s>>>(a, zero_blocks);
-    launched("sum_kernel");
-    if (a.windows > 1) {
-        join_kernel<DT, VEC><<<dim3((unsigned)((a.windows + 7) / 8), (unsigned)a.segments), 256, 0, s>>>(a);
-        launched("join_kernel");
-    }
+    launch_next("sum_kernel", sum_kernel<DT, VEC>, dim3((unsigned)blocks), 256, 0, s, a, zero_blocks);
+    if (a.windows > 1)
+        launch_next("join_kernel", join_kernel<DT, VEC>,
+                    dim3((unsigned)((a.windows + 7) / 8), (unsigned)a.segments), 256, 0, s, a);
 }
 
 void plan_sort(SortArgs& a) {
@@ -502,16 +523,22 @@ void plan_sort(SortArgs& a) {
     a.blocks = (int)((a.n + a.steps * per_step - 1) / (a.steps * per_step));
 }
 
-void sort(const SortArgs& a, cudaStream_t s) {
+void sort(SortArgs a, cudaStream_t s) {
     const int bins = 1 << a.bits, slices = std::max(1, kSortThreads / (bins / 4));
     const int most = kSortWarps * (4 << kMaxBits);
     check(cudaFuncSetAttribute(rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most),
           "cudaFuncSetAttribute(rank_kernel)");
     for (int pass = 0; pass < a.passes; ++pass) {
-        rank_kernel<<<a.blocks, kSortThreads, kSortWarps * bins * 4, s>>>(a, pass);
-        launched("rank_kernel");
-        scatter_kernel<<<a.blocks, kSortThreads, slices * 2 * bins * 4, s>>>(a, pass);
-        launched("scatter_kernel");
+        a.in = a.pair[pass & 1];
+        a.out = a.pair[(pass + 1) & 1];
+        if (pass == 0) {
+            rank_kernel<<<a.blocks, kSortThreads, kSortWarps * bins * 4, s>>>(a, pass);
+            launched("rank_kernel");
+        } else {
+            launch_next("rank_kernel", rank_kernel, dim3(a.blocks), kSortThreads, kSortWarps * bins * 4, s, a, pass);
+        }
+        launch_next("scatter_kernel", scatter_kernel, dim3(a.blocks), kSortThreads, slices * 2 * bins * 4, s, a,
+                    pass);
     }
 }
 
@@ -537,8 +564,8 @@ void embed_backward(const mg_embed_backward_args& a, Workspace& w, bool go, cuda
     sum.n = (int)a.n;
     const int segment = 32 * 16 / e;
     sum.segments = (a.dim + segment - 1) / segment;
-    // windows long enough that few runs cross them, short enough for 24 warps per SM
-    sum.window = (int)std::clamp<int64_t>(a.n * sum.segments / (148 * 24) / 8 * 8, 16, 128);
+    // windows long enough that few runs cross them, short enough for 24 warps on each SM at once
+    sum.window = (int)std::clamp<int64_t>((a.n * sum.segments / (148 * 24) + 7) / 8 * 8, 16, 128);
     sum.windows = (int)((a.n + sum.window - 1) / sum.window);
     sum.head = w.take<float>((size_t)sum.windows * a.dim * 4);
     sum.tail = w.take<float>((size_t)sum.windows * a.dim * 4);

@@ -59,21 +59,19 @@ def _raise(code: int):
     raise ValueError(message) if code == -1 else RuntimeError(message)
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# The current stream of a device by index, without a Stream object.
+_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _call(name: str, args: bytes, device: torch.device) -> None:
+def _call(name: str, args: bytes, like, device: int) -> None:
     L = lib()
     need = ctypes.c_size_t()
     code = getattr(L, name + "_workspace")(args, ctypes.byref(need))
     if code:
         _raise(code)
-    stream = torch.cuda.current_stream(device)
     # torch's allocator orders the block's reuse after this stream's work
-    w = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
-    code = getattr(L, name)(args, w.data_ptr() if w is not None else None, need.value,
-                            stream.cuda_stream)
+    w = like.new_empty(need.value, dtype=torch.uint8) if need.value else None
+    code = getattr(L, name)(args, w.data_ptr() if w is not None else None, need.value, _stream(device))
     if code:
         _raise(code)
 
@@ -81,25 +79,26 @@ def _call(name: str, args: bytes, device: torch.device) -> None:
 def synchronize(device=None) -> None:
     """Waits for the current stream; raises RuntimeError if a kernel of these
     operators gave up a bounded wait (its outputs are then invalid)."""
-    d = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    code = lib().mg_op_synchronize(d.index if d.index is not None else torch.cuda.current_device(),
-                                   _stream(d))
+    d = torch.device("cuda" if device is None else device)
+    index = d.index if d.index is not None else torch.cuda.current_device()
+    code = lib().mg_op_synchronize(index, _stream(index))
     if code:
         _raise(code)
 
 
 # ---- argument checks ----
 
-def _on_gpu(t, name: str) -> torch.device:
+def _on_gpu(t, name: str) -> int:
+    """The index of the tensor's device."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor, not {type(t).__name__}")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA tensor (it is on {t.device})")
-    return t.device
+    return t.get_device()
 
 
-def _same(t, name: str, like, what: str) -> None:
-    if _on_gpu(t, name) != like.device:
+def _same(t, name: str, like, what: str, device: int) -> None:
+    if _on_gpu(t, name) != device:
         raise TypeError(f"{name} is on {t.device}, {what} on {like.device}")
     if t.dtype != like.dtype:
         raise TypeError(f"{name} is {t.dtype}, {what} {like.dtype}")
@@ -113,13 +112,19 @@ def _dtype(t, name: str, wide: bool) -> int:
     return code
 
 
-def _indices(t, name: str, like) -> int:
-    if _on_gpu(t, name) != like.device:
+def _indices(t, name: str, like, device: int) -> int:
+    if _on_gpu(t, name) != device:
         raise TypeError(f"{name} is on {t.device}, expected {like.device}")
     b = _INDEX_BYTES.get(t.dtype)
     if b is None:
         raise TypeError(f"{name} must be int64 or int32, not {t.dtype}")
     return b
+
+
+def _flat(t):
+    """t as a vector, and its stride."""
+    v = t if t.dim() == 1 else t.reshape(-1)
+    return v, v.stride(0)
 
 
 def _matrix(t, name: str, cols=None):
@@ -136,16 +141,15 @@ def _matrix(t, name: str, cols=None):
     return t.reshape(-1, t.shape[-1])
 
 
-def _weight(t, name: str, like, what: str):
-    _same(t, name, like, what)
+def _weight(t, name: str, like, what: str, device: int) -> None:
+    _same(t, name, like, what, device)
     if t.dim() != 2:
         raise ValueError(f"{name} must be a matrix, not {tuple(t.shape)}")
-    return t
 
 
-def _vector(t, name: str, n: int, like, what: str):
-    _same(t, name, like, what)
-    if t.shape != (n,):
+def _vector(t, name: str, n: int, like, what: str, device: int):
+    _same(t, name, like, what, device)
+    if t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{name} must have shape ({n},), not {tuple(t.shape)}")
     return t.contiguous()
 
@@ -160,9 +164,10 @@ def _ptr(t) -> int:
 
 
 def _activation(name: str) -> int:
-    if name not in ACTIVATIONS:
+    code = ACTIVATIONS.get(name)
+    if code is None:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, not {name!r}")
-    return ACTIVATIONS[name]
+    return code
 
 
 # ---- embedding ----
@@ -171,19 +176,17 @@ def embed(tokens, table, scale: float = 1.0):
     """``scale * table[tokens]``: tokens [...] int64 or int32, table
     [vocab, dim] bfloat16, float16 or float32 -> [..., dim].  A token outside
     [0, vocab) is padding and gives a zero row."""
-    _on_gpu(table, "table")
+    d = _on_gpu(table, "table")
     dt = _dtype(table, "table", True)
-    tb = _indices(tokens, "tokens", table)
+    tb = _indices(tokens, "tokens", table, d)
     if table.dim() != 2:
         raise ValueError(f"table must be a matrix, not {tuple(table.shape)}")
     vocab, dim = table.shape
-    t = tokens.reshape(-1)
+    t, t_stride = _flat(tokens)
     table = _rows(table)
-    out = torch.empty(tokens.shape + (dim,), dtype=table.dtype, device=table.device)
-    n = t.numel()
-    code = lib().mg_embed(_EMBED.pack(t.data_ptr(), table.data_ptr(), out.data_ptr(), n, vocab, dim,
-                                      t.stride(0) if n > 1 else 1, table.stride(0), scale, dt, tb,
-                                      table.device.index), _stream(table.device))
+    out = table.new_empty((*tokens.shape, dim))
+    code = lib().mg_embed(_EMBED.pack(t.data_ptr(), table.data_ptr(), out.data_ptr(), t.shape[0], vocab,
+                                      dim, t_stride, table.stride(0), scale, dt, tb, d), _stream(d))
     if code:
         _raise(code)
     return out
@@ -192,19 +195,18 @@ def embed(tokens, table, scale: float = 1.0):
 def embed_backward(grad, tokens, vocab: int, scale: float = 1.0):
     """Gradient of ``embed`` with respect to its table: [vocab, dim], the
     rows of grad [..., dim] summed by token in 32 bits, times scale."""
-    _on_gpu(grad, "grad")
+    d = _on_gpu(grad, "grad")
     dt = _dtype(grad, "grad", True)
-    tb = _indices(tokens, "tokens", grad)
+    tb = _indices(tokens, "tokens", grad, d)
     if grad.shape[:-1] != tokens.shape:
         raise ValueError(f"grad {tuple(grad.shape)} does not match tokens {tuple(tokens.shape)}")
     g = _rows(_matrix(grad, "grad"))
-    t = tokens.reshape(-1)
+    t, t_stride = _flat(tokens)
     n, dim = g.shape
-    out = torch.empty((vocab, dim), dtype=grad.dtype, device=grad.device)
+    out = grad.new_empty((vocab, dim))
     _call("mg_embed_backward",
-          _EMBED_BACKWARD.pack(t.data_ptr(), g.data_ptr(), out.data_ptr(), n, vocab, dim,
-                               t.stride(0) if n > 1 else 1, g.stride(0), scale, dt, tb,
-                               grad.device.index), grad.device)
+          _EMBED_BACKWARD.pack(t.data_ptr(), g.data_ptr(), out.data_ptr(), n, vocab, dim, t_stride,
+                               g.stride(0), scale, dt, tb, d), grad, d)
     return out
 
 
@@ -217,30 +219,27 @@ def linear(x, weight, bias=None, residual=None, activation: str = "none",
     bfloat16 or float16 with 32-bit sums.  activation is "none", "relu",
     "silu" or "gelu" (the erf form).  With keep_preactivation returns
     (y, z), z = x @ weight.T + bias being what ``linear_backward`` needs."""
-    _on_gpu(x, "x")
+    d = _on_gpu(x, "x")
     dt = _dtype(x, "x", False)
     act = _activation(activation)
-    _weight(weight, "weight", x, "x")
+    _weight(weight, "weight", x, "x", d)
     n, k = weight.shape
     x2 = _matrix(x, "x", k)
-    m = x2.shape[0]
-    b = None if bias is None else _vector(bias, "bias", n, x, "x")
-    shape = x.shape[:-1] + (n,)
+    b = None if bias is None else _vector(bias, "bias", n, x, "x", d)
+    shape = (*x.shape[:-1], n)
     r, r_row, r_col = None, 0, 0
     if residual is not None:
-        _same(residual, "residual", x, "x")
+        _same(residual, "residual", x, "x", d)
         if residual.shape != shape:
             raise ValueError(f"residual must have shape {tuple(shape)}, not {tuple(residual.shape)}")
         r = _matrix(residual, "residual")
         r_row, r_col = r.stride()
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    z = torch.empty(shape, dtype=x.dtype, device=x.device) if keep_preactivation else None
-    x_row, x_col = x2.stride()
-    w_row, w_col = weight.stride()
+    y = x.new_empty(shape)
+    z = x.new_empty(shape) if keep_preactivation else None
     _call("mg_linear",
           _LINEAR.pack(x2.data_ptr(), weight.data_ptr(), _ptr(b), _ptr(r), y.data_ptr(), _ptr(z),
-                       m, n, k, x_row, x_col, w_row, w_col, r_row, r_col, residual_scale, act, dt,
-                       x.device.index), x.device)
+                       x2.shape[0], n, k, *x2.stride(), *weight.stride(), r_row, r_col,
+                       residual_scale, act, dt, d), x, d)
     return (y, z) if keep_preactivation else y
 
 
@@ -248,11 +247,11 @@ def linear_backward(grad, x, weight, preactivation=None, activation: str = "none
     """Gradients (dx, dw, db) of ``linear`` from grad = dL/dy [..., n] and
     the z that it kept (needed unless activation is "none"); db is None with
     bias=False.  The residual's gradient is residual_scale * grad."""
-    _on_gpu(grad, "grad")
+    d = _on_gpu(grad, "grad")
     dt = _dtype(grad, "grad", False)
     act = _activation(activation)
-    _same(x, "x", grad, "grad")
-    _weight(weight, "weight", grad, "grad")
+    _same(x, "x", grad, "grad", d)
+    _weight(weight, "weight", grad, "grad", d)
     n, k = weight.shape
     g, x2 = _matrix(grad, "grad", n), _matrix(x, "x", k)
     if grad.shape[:-1] != x.shape[:-1]:
@@ -261,57 +260,48 @@ def linear_backward(grad, x, weight, preactivation=None, activation: str = "none
     if act:
         if preactivation is None:
             raise ValueError(f"the backward pass of {activation!r} needs the preactivation")
-        _same(preactivation, "preactivation", grad, "grad")
+        _same(preactivation, "preactivation", grad, "grad", d)
         if preactivation.shape != grad.shape:
             raise ValueError(f"preactivation must have shape {tuple(grad.shape)}, not "
                              f"{tuple(preactivation.shape)}")
         z = _matrix(preactivation, "preactivation")
         z_row, z_col = z.stride()
-    m = g.shape[0]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dw = torch.empty((n, k), dtype=x.dtype, device=x.device)
-    db = torch.empty((n,), dtype=x.dtype, device=x.device) if bias else None
-    g_row, g_col = g.stride()
-    x_row, x_col = x2.stride()
-    w_row, w_col = weight.stride()
+    dx = x.new_empty(x.shape)
+    dw = x.new_empty((n, k))
+    db = x.new_empty((n,)) if bias else None
     _call("mg_linear_backward",
           _LINEAR_BACKWARD.pack(g.data_ptr(), x2.data_ptr(), weight.data_ptr(), _ptr(z),
-                                dx.data_ptr(), dw.data_ptr(), _ptr(db), m, n, k, g_row, g_col,
-                                x_row, x_col, w_row, w_col, z_row, z_col, act, dt, x.device.index,
-                                0), x.device)
+                                dx.data_ptr(), dw.data_ptr(), _ptr(db), g.shape[0], n, k,
+                                *g.stride(), *x2.stride(), *weight.stride(), z_row, z_col, act, dt,
+                                d, 0), x, d)
     return dx, dw, db
 
 
 # ---- linear cross entropy ----
 
 def _cross_entropy(x, weight, targets, bias, grad_scale, gradients):
-    _on_gpu(x, "x")
+    d = _on_gpu(x, "x")
     dt = _dtype(x, "x", False)
-    _weight(weight, "weight", x, "x")
+    _weight(weight, "weight", x, "x", d)
     vocab, dim = weight.shape
     x2 = _matrix(x, "x", dim)
-    tb = _indices(targets, "targets", x)
+    tb = _indices(targets, "targets", x, d)
     if targets.shape != x.shape[:-1]:
         raise ValueError(f"targets {tuple(targets.shape)} do not match x {tuple(x.shape)}")
-    t = targets.reshape(-1)
-    n = t.numel()
-    b = None if bias is None else _vector(bias, "bias", vocab, x, "x")
-    # the loss and the row losses in one allocation
-    both = torch.empty(n + 1, dtype=torch.float32, device=x.device)
-    loss, rows = both[n], both[:n].view(targets.shape)
+    t, t_stride = _flat(targets)
+    b = None if bias is None else _vector(bias, "bias", vocab, x, "x", d)
+    loss = x.new_empty((), dtype=torch.float32)
+    rows = x.new_empty(targets.shape, dtype=torch.float32)
     dx = dw = db = None
     if gradients:
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dw = torch.empty((vocab, dim), dtype=x.dtype, device=x.device)
-        db = torch.empty((vocab,), dtype=x.dtype, device=x.device) if b is not None else None
-    x_row, x_col = x2.stride()
-    w_row, w_col = weight.stride()
+        dx = x.new_empty(x.shape)
+        dw = x.new_empty((vocab, dim))
+        db = x.new_empty((vocab,)) if b is not None else None
     _call("mg_cross_entropy",
           _CROSS_ENTROPY.pack(x2.data_ptr(), weight.data_ptr(), _ptr(b), t.data_ptr(),
                               loss.data_ptr(), rows.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db),
-                              n, vocab, dim, x_row, x_col, w_row, w_col,
-                              t.stride(0) if n > 1 else 1, grad_scale, dt, tb, x.device.index),
-          x.device)
+                              t.shape[0], vocab, dim, *x2.stride(), *weight.stride(), t_stride,
+                              grad_scale, dt, tb, d), x, d)
     return loss, rows, dx, dw, db
 
 
