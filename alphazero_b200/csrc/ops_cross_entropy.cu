@@ -172,7 +172,7 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, cudaStream_t s) 
     const int64_t down = (piece + down_rows - 1) / down_rows;  // of a whole piece
     float* sums = a.db ? w.take<float>((size_t)down * count_pieces * a.vocab * 4) : nullptr;
     const int64_t ld32 = (a.dim + 7) / 8 * 8;
-    float* dw32 = grads && count_pieces > 1 ? w.take<float>((size_t)a.vocab * ld32 * 4) : nullptr;
+    float* dw32 = grads && count_pieces > 1 ? w.take<float>((size_t)((a.vocab + 255) / 256 * 256) * ld32 * 4) : nullptr;
 
     StagedOperand x = stage_operand(w, go, {a.x, a.x_row, a.x_col}, a.n, a.dim, s);
     const StagedOperand weight = stage_operand(w, go, {a.weight, a.w_row, a.w_col}, a.vocab, a.dim, s);

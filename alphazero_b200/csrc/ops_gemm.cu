@@ -16,7 +16,11 @@
 //   warp 0     TMA producer (one thread), a ring of kStages K steps
 //   warp 1     TMEM; in the even CTA also the MMA issuer (one thread)
 //   warps 2-9  epilogue: warp w reads TMEM lanes 32 (w % 4) .. + 31 (a thread
-//              owns a row) and half of the columns, 32 at a time
+//              owns a row) and half of the columns, 32 at a time, through
+//              swizzled blocks of shared memory that TMA stores (and, for the
+//              residual, loads): a lane's own 16-byte stores to 32 rows at
+//              once cost 8.4 us for a 128 x 256 tile (184832 x 256 x 256:
+//              82 us)
 // The sums are double-buffered in TMEM: a tile's epilogue overlaps the next
 // tile's products.  Every wait is bounded (ptx_sm100.cuh).
 #include "ops_gemm.cuh"
@@ -37,19 +41,22 @@ constexpr int kEpiWarps = 8;
 constexpr int kThreads = 32 * (2 + kEpiWarps);
 constexpr int kPairs = 74;             // of SMs on a B200 (148)
 constexpr int kGroup = 8;              // row tiles walked together (their B tiles stay in L2)
-constexpr int kStagePitch = 34;        // 16-bit elements per staged row (17 words: no bank conflicts)
+constexpr int kStagePitch = 34;        // 16-bit elements per row staged without TMA (17 words: no bank conflicts)
+constexpr int kOutBytes = 4096;        // per epilogue warp: two 32 x 32 blocks of 16-bit, or one of fp32
+constexpr int kResBytes = 2048;        // a 32 x 32 block of the residual
+constexpr int kWarpBytes = kOutBytes + kResBytes;
 
 template <int BN>
 struct Config {
-    static constexpr int kStages = BN == 256 ? 6 : 8;
+    static constexpr int kStages = BN == 256 ? 5 : 7;
     static constexpr uint32_t kABytes = kRowsCta * kBK * 2;
     static constexpr uint32_t kBBytes = BN / 2 * kBK * 2;
     static constexpr uint32_t kStageBytes = kABytes + kBBytes;
     static constexpr uint32_t kTmemCols = 2 * BN;
-    static constexpr int kBarriers = 2 * kStages + 5;
-    // ring + per epilogue warp a staged block and a bias row + barriers + alignment slack
-    static constexpr int kSmem = kStages * kStageBytes + kEpiWarps * (32 * kStagePitch * 2 + BN / 2 * 4) +
-                                 kBarriers * 8 + 16 + 1024;
+    static constexpr int kBarriers = 2 * kStages + 5 + kEpiWarps;
+    // ring + per epilogue warp its blocks and a bias row + barriers + alignment slack
+    static constexpr int kSmem = kStages * kStageBytes + kEpiWarps * (kWarpBytes + BN / 2 * 4) + kBarriers * 8 +
+                                 16 + 1024;
 };
 
 enum Epi : int { kStore, kSoftmax };
@@ -58,13 +65,16 @@ struct JobArgs {
     int m, n, kblocks;
     int tiles_m, tiles_n, splits, kb_split;
     int a_mn, b_mn;
-    int vec;  // outputs, z and residual take 16-byte accesses
+    int by_tma;  // outputs, z and residual go through their tensor maps
+    int m_pad;   // rows of out32 per split
     GemmEpilogue e;
     SoftmaxEpilogue s;
 };
 
 struct alignas(64) KernelArgs {
     CUtensorMap ta[2], tb[2];
+    CUtensorMap to[2];   // out, out32 or probs
+    CUtensorMap tz, tr;  // z and residual of job 0
     JobArgs job[2];
     int units[2];
     int head_start;  // units of job 1 that a pair does while others finish their last unit of job 0
@@ -131,29 +141,78 @@ __device__ __forceinline__ float2 unpack2(uint32_t u) {
     else return __half22float2(*reinterpret_cast<__half2*>(&u));
 }
 
-// The 32 x 32 block of 16-bit values at p (row stride `row`, column stride
-// `col`) <-> one row per lane.  vec: 16-byte accesses, a row per lane;
-// otherwise through the warp's staging block, a row at a time, coalesced.
-template <int DT>
-__device__ __forceinline__ void load_block(const void* base, int64_t row, int64_t col, bool vec, int rows,
-                                           int cols, int lane, uint16_t* stage, float (&v)[32]) {
-    const uint16_t* p = static_cast<const uint16_t*>(base);
-    if (vec) {
+// Byte offset of 16-byte chunk q of row r in a block of 64-byte (128-byte)
+// rows as TMA swizzles it.
+__device__ __forceinline__ uint32_t swizzle64(int r, int q) { return r * 64 + ((q ^ (r >> 1 & 3)) << 4); }
+__device__ __forceinline__ uint32_t swizzle128(int r, int q) { return r * 128 + ((q ^ (r & 7)) << 4); }
+
+// An epilogue warp's shared memory, and which of its blocks are in use.
+struct WarpBlocks {
+    uint8_t* out;      // [2][2048], or [4096]
+    uint8_t* res;
+    uint64_t* landed;  // the residual block has arrived
+    int lane;
+    int next = 0;      // out block to write
+    int parity = 0;
+    bool pending = false;  // a residual block is on its way
+
+    // Writes v (a row per lane) to the next block and starts its store.
+    template <class Words>
+    __device__ __forceinline__ void store16(const CUtensorMap* map, int col, int row, Words word) {
+        if (lane == 0) bulk_wait_read_n<1>();  // the store before last is done with this block
+        __syncwarp();
+        uint8_t* p = out + next * 2048;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            uint4 u = make_uint4(0, 0, 0, 0);
-            if (lane < rows && q * 8 < cols)
-                u = __ldg(reinterpret_cast<const uint4*>(p + lane * row + q * 8));
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 f = unpack2<DT>(w[i]);
-                v[q * 8 + 2 * i] = f.x;
-                v[q * 8 + 2 * i + 1] = f.y;
-            }
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint4*>(p + swizzle64(lane, q)) =
+                make_uint4(word(4 * q), word(4 * q + 1), word(4 * q + 2), word(4 * q + 3));
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            tma_store_2d(map, smem_u32(p), col, row);
+            bulk_commit();
         }
-        return;
+        next ^= 1;
     }
+    __device__ __forceinline__ void store32(const CUtensorMap* map, int col, int row, const float (&v)[32]) {
+        if (lane == 0) bulk_wait_read_n<0>();
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            *reinterpret_cast<float4*>(out + swizzle128(lane, q)) =
+                make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            tma_store_2d(map, smem_u32(out), col, row);
+            bulk_commit();
+        }
+    }
+    // The residual's block at (row, col): started, and (after a wait) read.
+    __device__ __forceinline__ void start_res(const CUtensorMap* map, int col, int row) {
+        __syncwarp();  // every lane has read the last one
+        pending = true;
+        if (lane == 0) {
+            mbar_arrive_expect_tx(smem_u32(landed), kResBytes);
+            tma_load_2d(smem_u32(res), map, smem_u32(landed), col, row);
+        }
+    }
+    __device__ __forceinline__ bool read_res(uint4 (&u)[4], int* err) {
+        const bool ok = __all_sync(~0u, mbar_wait(smem_u32(landed), parity, err, kErrWaitEpilogue));
+        parity ^= 1;
+        pending = false;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) u[q] = *reinterpret_cast<const uint4*>(res + swizzle64(lane, q));
+        return ok;
+    }
+};
+
+// The same blocks for matrices that no tensor map describes (any strides and
+// alignment): a row at a time, coalesced, through a staging block.
+template <int DT>
+__device__ __forceinline__ void load_block(const void* base, int64_t row, int64_t col, int rows, int cols, int lane,
+                                           uint16_t* stage, float (&v)[32]) {
+    const uint16_t* p = static_cast<const uint16_t*>(base);
     __syncwarp();
     for (int r = 0; r < rows; ++r)
         if (lane < cols) stage[r * kStagePitch + lane] = p[r * row + lane * col];
@@ -168,21 +227,9 @@ __device__ __forceinline__ void load_block(const void* base, int64_t row, int64_
 }
 
 template <int DT>
-__device__ __forceinline__ void store_block(void* base, int64_t row, bool vec, int rows, int cols, int lane,
-                                            uint16_t* stage, const float (&v)[32]) {
+__device__ __forceinline__ void store_block(void* base, int64_t row, int rows, int cols, int lane, uint16_t* stage,
+                                            const float (&v)[32]) {
     uint16_t* p = static_cast<uint16_t*>(base);
-    if (vec) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            uint4 u;
-            u.x = pack2<DT>(v[q * 8], v[q * 8 + 1]);
-            u.y = pack2<DT>(v[q * 8 + 2], v[q * 8 + 3]);
-            u.z = pack2<DT>(v[q * 8 + 4], v[q * 8 + 5]);
-            u.w = pack2<DT>(v[q * 8 + 6], v[q * 8 + 7]);
-            if (lane < rows && q * 8 < cols) *reinterpret_cast<uint4*>(p + lane * row + q * 8) = u;
-        }
-        return;
-    }
     __syncwarp();
     uint32_t* w = reinterpret_cast<uint32_t*>(stage + lane * kStagePitch);
 #pragma unroll
@@ -205,24 +252,26 @@ __device__ __forceinline__ void activate_all(float (&v)[32], int act) {
     }
 }
 
-// Columns [n0 + c0, + BN / 2) of rows [m0, + 32) of a finished tile.
+// Columns [n0 + c0, + BN / 2) of rows [m0, + 32) of a finished tile.  False
+// if a wait gave up.
 template <int BN, int DT>
-__device__ __forceinline__ void epilogue(const JobArgs& j, const Tile& t, int m0, int c0, uint32_t taddr,
-                                         int lane, uint16_t* stage, const float* sbias, float alpha) {
+__device__ __forceinline__ bool epilogue(const KernelArgs& a, int job, const Tile& t, int m0, int c0, uint32_t taddr,
+                                         WarpBlocks& blocks, const float* sbias, float alpha) {
+    const JobArgs& j = a.job[job];
     const GemmEpilogue& e = j.e;
-    const int rows = min(32, j.m - m0);
+    const int rows = min(32, j.m - m0), lane = blocks.lane;
+    const bool res_tma = e.res != nullptr && j.by_tma;
 #pragma unroll 1
     for (int c = 0; c < BN / 2; c += 32) {
-        const int64_t col = t.n0 + c0 + c;
-        const int cols = (int)min((int64_t)32, j.n - col);
-        if (cols <= 0) break;
+        const int col = t.n0 + c0 + c;
+        const int cols = min(32, j.n - col);
+        if (cols <= 0 || rows <= 0) break;
         uint32_t r[32];
         tmem_ld_32cols(taddr + c, r);
         tmem_ld_wait();
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-        if (rows <= 0) continue;
         if (e.acc32 != nullptr && lane < rows) {
             const float* p = e.acc32 + (int64_t)(m0 + lane) * e.ld32 + col;
 #pragma unroll
@@ -236,45 +285,60 @@ __device__ __forceinline__ void epilogue(const JobArgs& j, const Tile& t, int m0
                 }
         }
         if (e.out32 != nullptr) {
-            if (lane < rows) {
-                float* p = e.out32 + ((int64_t)t.split * j.m + m0 + lane) * e.ld32 + col;
-#pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    if (q * 4 < cols)
-                        *reinterpret_cast<float4*>(p + q * 4) =
-                            make_float4(v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]);
-            }
+            blocks.store32(&a.to[job], col, t.split * j.m_pad + m0, v);
             continue;
         }
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = v[i] * alpha + sbias[c + i];
-        const bool vec = j.vec != 0;
-        if (e.z != nullptr)
-            store_block<DT>(static_cast<uint16_t*>(e.z) + (int64_t)m0 * e.ld + col, e.ld, vec, rows, cols,
-                            lane, stage, v);
+        if (e.z != nullptr) {
+            if (j.by_tma)
+                blocks.store16(&a.tz, col, m0, [&](int i) { return pack2<DT>(v[2 * i], v[2 * i + 1]); });
+            else
+                store_block<DT>(static_cast<uint16_t*>(e.z) + (int64_t)m0 * e.ld + col, e.ld, rows, cols, lane,
+                                reinterpret_cast<uint16_t*>(blocks.out), v);
+        }
         activate_all(v, e.act);
-        if (e.res != nullptr) {
+        if (res_tma) {
+            uint4 u[4];
+            if (!blocks.read_res(u, a.err)) return false;
+            if (c + 32 < BN / 2 && col + 32 < j.n) blocks.start_res(&a.tr, col + 32, m0);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t w[4] = {u[q].x, u[q].y, u[q].z, u[q].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = unpack2<DT>(w[i]);
+                    v[q * 8 + 2 * i] += e.res_scale * f.x;
+                    v[q * 8 + 2 * i + 1] += e.res_scale * f.y;
+                }
+            }
+        } else if (e.res != nullptr) {
             float x[32];
-            load_block<DT>(static_cast<const uint16_t*>(e.res) + m0 * e.r_row + col * e.r_col, e.r_row,
-                           e.r_col, vec, rows, cols, lane, stage, x);
+            load_block<DT>(static_cast<const uint16_t*>(e.res) + m0 * e.r_row + col * e.r_col, e.r_row, e.r_col, rows,
+                           cols, lane, reinterpret_cast<uint16_t*>(blocks.out), x);
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] += e.res_scale * x[i];
         }
-        store_block<DT>(static_cast<uint16_t*>(e.out) + (int64_t)m0 * e.ld + col, e.ld, vec, rows, cols,
-                        lane, stage, v);
+        if (j.by_tma)
+            blocks.store16(&a.to[job], col, m0, [&](int i) { return pack2<DT>(v[2 * i], v[2 * i + 1]); });
+        else
+            store_block<DT>(static_cast<uint16_t*>(e.out) + (int64_t)m0 * e.ld + col, e.ld, rows, cols, lane,
+                            reinterpret_cast<uint16_t*>(blocks.out), v);
     }
+    return true;
 }
 
 // The same columns and rows as softmax statistics.  A thread has its row's
 // block to itself, so the maximum and the sum need no exchange; the sums are
 // read from TMEM twice rather than held in BN / 2 registers.
 template <int BN>
-__device__ __forceinline__ void softmax_epilogue(const JobArgs& j, const Tile& t, int m0, int c0,
-                                                 uint32_t taddr, int lane, const float* sbias) {
+__device__ __forceinline__ void softmax_epilogue(const KernelArgs& a, const Tile& t, int m0, int c0, uint32_t taddr,
+                                                 WarpBlocks& blocks, const float* sbias) {
+    const JobArgs& j = a.job[0];
     const SoftmaxEpilogue& e = j.s;
-    const int row = m0 + lane;
+    const int row = m0 + blocks.lane;
     const int first = t.n0 + c0;
-    if (first >= j.n) return;
+    if (first >= j.n || m0 >= j.m) return;
     const int width = min(BN / 2, j.n - first);
     const int target = row < j.m ? e.target[row] - first : -1;
     float top = -INFINITY, logit = 0.0f;
@@ -305,18 +369,8 @@ __device__ __forceinline__ void softmax_epilogue(const JobArgs& j, const Tile& t
             v[i] = exp2f((__uint_as_float(r[i]) + sbias[c + i] - ref) * 1.4426950408889634f);
             sum[i & 3] += v[i];
         }
-        if (e.probs != nullptr && row < j.m) {
-            uint16_t* p = e.probs + (int64_t)row * e.probs_ld + first + c;
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (c + q * 8 < width) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        w[i] = prob16x2(v[q * 8 + 2 * i], v[q * 8 + 2 * i + 1]);
-                    *reinterpret_cast<uint4*>(p + q * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-        }
+        if (e.probs != nullptr)
+            blocks.store16(&a.to[0], first + c, m0, [&](int i) { return prob16x2(v[2 * i], v[2 * i + 1]); });
     }
     if (row < j.m) {
         if (target >= 0 && target < width) e.logit[row] = logit;
@@ -334,14 +388,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // the same offset in both CTAs: the dynamic segment starts at the same address in each
     uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
     uint8_t* ring = smem;
-    float* sbias_all = reinterpret_cast<float*>(ring + S * Cfg::kStageBytes);
-    uint16_t* stage_all = reinterpret_cast<uint16_t*>(sbias_all + kEpiWarps * (BN / 2));
-    uint64_t* bars = reinterpret_cast<uint64_t*>(stage_all + kEpiWarps * 32 * kStagePitch);
+    uint8_t* blocks_all = ring + S * Cfg::kStageBytes;  // a multiple of 1 KB, as each warp's part is
+    float* sbias_all = reinterpret_cast<float*>(blocks_all + kEpiWarps * kWarpBytes);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sbias_all + kEpiWarps * (BN / 2));
     uint64_t* full = bars;           // even CTA's: a stage has landed in both CTAs
     uint64_t* empty = bars + S;      // each CTA's: the products have read a stage
     uint64_t* tfull = bars + 2 * S;  // [2] each CTA's: a tile's sums are complete
     uint64_t* tempty = tfull + 2;    // [2] even CTA's: both CTAs have read them
-    uint64_t* done = tempty + 2;     // even CTA's: drain after a wait gave up
+    uint64_t* done = tempty + 2;     // even CTA's: the last products are complete
+    uint64_t* landed = done + 1;     // [kEpiWarps] a warp's residual block has arrived
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::kBarriers);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -358,6 +413,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             mbar_init(smem_u32(&tempty[i]), 2 * kEpiWarps);
         }
         mbar_init(smem_u32(done), 1);
+        for (int i = 0; i < kEpiWarps; ++i) mbar_init(smem_u32(&landed[i]), 1);
         fence_barrier_init();
     }
     if (warp == 1) {
@@ -458,13 +514,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         __syncwarp();
     } else {
         const int ew = warp - 2, quarter = warp & 3, half = ew >> 2;
-        uint16_t* stage = stage_all + ew * 32 * kStagePitch;
         float* sbias = sbias_all + ew * (BN / 2);
+        WarpBlocks blocks;
+        blocks.out = blocks_all + ew * kWarpBytes;
+        blocks.res = blocks.out + kOutBytes;
+        blocks.landed = &landed[ew];
+        blocks.lane = lane;
         const int c0 = half * (BN / 2);
         int tile = 0;
-        while (walk.next(&job, &unit)) {
+        bool ok = true;
+        while (ok && walk.next(&job, &unit)) {
             const JobArgs& j = a.job[job];
             const Tile t(j, unit, BN);
+            const int m0 = t.m0 + (int)rank * kRowsCta + quarter * 32;
+            // the residual's first block on its way before the sums are complete
+            if (EPI == kStore && j.e.res != nullptr && j.by_tma && m0 < j.m && t.n0 + c0 < j.n)
+                blocks.start_res(&a.tr, t.n0 + c0, m0);
             __syncwarp();
             for (int i = lane; i < BN / 2; i += 32) {
                 const int64_t col = t.n0 + c0 + i;
@@ -480,19 +545,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (!__all_sync(~0u, mbar_wait_cluster(smem_u32(&tfull[buf]), (tile >> 1) & 1, a.err, kErrWaitEpilogue)))
                 break;
             tc_fence_after();
-            const int m0 = t.m0 + (int)rank * kRowsCta + quarter * 32;
             const uint32_t taddr = tmem_base + buf * BN + c0 + ((uint32_t)quarter << 21);
             if constexpr (EPI == kSoftmax) {
-                softmax_epilogue<BN>(j, t, m0, c0, taddr, lane, sbias);
+                softmax_epilogue<BN>(a, t, m0, c0, taddr, blocks, sbias);
             } else {
                 const float alpha = j.e.count ? j.e.alpha / (float)max(*j.e.count, 1) : j.e.alpha;
-                epilogue<BN, DT>(j, t, m0, c0, taddr, lane, stage, sbias, alpha);
+                ok = epilogue<BN, DT>(a, job, t, m0, c0, taddr, blocks, sbias, alpha);
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&tempty[buf]), 0));
             ++tile;
         }
+        if (blocks.pending) mbar_wait(smem_u32(blocks.landed), blocks.parity, a.err, kErrWaitDrain);
+        if (lane == 0) bulk_wait_all();
+        __syncwarp();
     }
     // Neither CTA ends, or frees TMEM, while the other may still read its
     // shared memory or signal its barriers.
@@ -505,8 +572,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 // Sums the splits of a product and applies its epilogue.
 template <int DT>
-__global__ void __launch_bounds__(256) finish_kernel(const float* part, int splits, int64_t m, int64_t n,
-                                                     int64_t ld32, GemmEpilogue e) {
+__global__ void __launch_bounds__(256) finish_kernel(const float* part, int splits, int64_t m_pad, int64_t m,
+                                                     int64_t n, int64_t ld32, GemmEpilogue e) {
     using E = Elem<DT>;
     using T = typename E::T;
     const float alpha = e.count ? e.alpha / (float)max(*e.count, 1) : e.alpha;
@@ -514,7 +581,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const float* part, int spli
     for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * 256) {
         const int64_t i = at / n, c = at % n;
         float v = e.acc32 ? e.acc32[i * e.ld32 + c] : 0.0f;
-        for (int s = 0; s < splits; ++s) v += part[((int64_t)s * m + i) * ld32 + c];
+        for (int s = 0; s < splits; ++s) v += part[(s * m_pad + i) * ld32 + c];
         if (e.out32) {
             e.out32[i * e.ld32 + c] = v;
             continue;
@@ -536,7 +603,10 @@ __global__ void __launch_bounds__(256) pack_kernel(const uint16_t* in, int64_t l
             out[r * ld + c] = in[r * line + c * step];
 }
 
-bool encode(CUtensorMap* map, int dtype, const StagedOperand& s, int64_t rows, int64_t k, int tile_rows) {
+// A tensor map of a dense-enough matrix: `rows` lines of `inner` elements,
+// `ld` apart, in boxes of box_rows x box_inner.
+void encode(CUtensorMap* map, CUtensorMapDataType type, int elem, const void* base, int64_t inner, int64_t rows,
+            int64_t ld, int box_inner, int box_rows, CUtensorMapSwizzle swizzle) {
     static PFN_cuTensorMapEncodeTiled_v12000 enc = [] {
         void* p = nullptr;
         cudaDriverEntryPointQueryResult q;
@@ -545,15 +615,29 @@ bool encode(CUtensorMap* map, int dtype, const StagedOperand& s, int64_t rows, i
                    ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p)
                    : nullptr;
     }();
-    if (enc == nullptr) return false;
-    cuuint64_t dims[2] = {(cuuint64_t)(s.mn ? rows : k), (cuuint64_t)(s.mn ? k : rows)};
-    cuuint64_t strides[1] = {(cuuint64_t)s.ld * 2};
-    cuuint32_t box[2] = {64, (cuuint32_t)(s.mn ? kBK : tile_rows)};
+    if (enc == nullptr) fail(MG_E_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)(ld * elem)};
+    cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows};
     cuuint32_t one[2] = {1, 1};
-    return enc(map, dtype == MG_PREC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-               const_cast<void*>(s.data), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    if (enc(map, type, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        fail(MG_E_CUDA, "cuTensorMapEncodeTiled rejected a tensor map");
+}
+
+CUtensorMapDataType map_type(int dtype) {
+    return dtype == MG_PREC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+
+// An operand, in boxes of 64 contraction steps (128 bytes, or lines).
+void encode_operand(CUtensorMap* map, int dtype, const StagedOperand& s, int64_t rows, int64_t k, int tile_rows) {
+    encode(map, map_type(dtype), 2, s.data, s.mn ? rows : k, s.mn ? k : rows, s.ld, 64, s.mn ? kBK : tile_rows,
+           CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// A matrix that the epilogue moves in 32 x 32 blocks of 16-bit elements.
+void encode_blocks(CUtensorMap* map, int dtype, const void* base, int64_t m, int64_t n, int64_t ld) {
+    encode(map, map_type(dtype), 2, base, n, m, ld, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -593,13 +677,14 @@ void lay_out(JobArgs& j, const Job& g, int bn) {
     j.kb_split = j.kblocks;
     j.a_mn = g.a.mn;
     j.b_mn = g.b.mn;
+    j.m_pad = j.tiles_m * kRowsPair;
     need((int64_t)j.tiles_m * j.tiles_n < (int64_t(1) << 24), "too many tiles");
 }
 
 template <class Job>
 void encode_operands(KernelArgs& a, int i, int dtype, const Job& g, int bn) {
-    if (!encode(&a.ta[i], dtype, g.a, g.m, g.k, kRowsCta) || !encode(&a.tb[i], dtype, g.b, g.n, g.k, bn / 2))
-        fail(MG_E_CUDA, "cuTensorMapEncodeTiled rejected an operand's tensor map");
+    encode_operand(&a.ta[i], dtype, g.a, g.m, g.k, kRowsCta);
+    encode_operand(&a.tb[i], dtype, g.b, g.n, g.k, bn / 2);
 }
 
 // Narrow tiles where wide ones would leave pairs idle or mostly compute
@@ -666,8 +751,10 @@ void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, cudaStream
         const GemmJob& g = jobs[i];
         lay_out(j, g, bn);
         j.e = finish[i] = g.e;
-        j.vec = g.e.ld % 8 == 0 && g.n % 8 == 0 && aligned16(g.e.out) && aligned16(g.e.z) &&
-                (g.e.res == nullptr || (aligned16(g.e.res) && g.e.r_col == 1 && g.e.r_row % 8 == 0));
+        // what tensor maps ask of the outputs and the residual
+        j.by_tma = g.e.ld % 8 == 0 && aligned16(g.e.out) && aligned16(g.e.z) &&
+                   (g.e.res == nullptr || (aligned16(g.e.res) && g.e.r_col == 1 && g.e.r_row % 8 == 0 &&
+                                           g.e.r_row >= g.n && g.e.r_row < int64_t(1) << 38));
         const int64_t tiles = (int64_t)j.tiles_m * j.tiles_n;
         // Few tiles: their K steps are shared out over the idle pairs, at least 8 steps each.
         const int splits = tiles * 2 <= kPairs ? (int)std::min<int64_t>(kPairs / tiles, j.kblocks / 8) : 1;
@@ -676,14 +763,27 @@ void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, cudaStream
         if (j.splits > 1) {
             j.e = GemmEpilogue{};
             j.e.ld32 = up8(g.n);
-            j.e.out32 = w.take<float>((size_t)j.splits * g.m * j.e.ld32 * 4);
+            j.e.out32 = w.take<float>((size_t)j.splits * j.m_pad * j.e.ld32 * 4);
         }
         a.units[i] = (int)(tiles * j.splits);
         len[i] = j.kb_split + 4.0;  // a tile's epilogue is worth a few K steps
     }
     if (!go) return;
     w.require();
-    for (int i = 0; i < count; ++i) encode_operands(a, i, dtype, jobs[i], bn);
+    for (int i = 0; i < count; ++i) {
+        encode_operands(a, i, dtype, jobs[i], bn);
+        const JobArgs& j = a.job[i];
+        const GemmEpilogue& e = j.e;
+        if (e.out32 != nullptr)
+            encode(&a.to[i], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, e.out32, e.ld32, (int64_t)j.splits * j.m_pad, e.ld32,
+                   32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+        else if (j.by_tma)
+            encode_blocks(&a.to[i], dtype, e.out, j.m, j.n, e.ld);
+        if (!j.by_tma || e.out32 != nullptr) continue;
+        need(i == 0 || (e.z == nullptr && e.res == nullptr), "z and residual belong to a launch's first product");
+        if (e.z != nullptr) encode_blocks(&a.tz, dtype, e.z, j.m, j.n, e.ld);
+        if (e.res != nullptr) encode_blocks(&a.tr, dtype, e.res, j.m, j.n, e.r_row);
+    }
     a.head_start = count == 2 ? (int)(len[0] / len[1] + 0.5) : 0;
     launch<kStore>(a, bn, dtype, stream);
     for (int i = 0; i < count; ++i)
@@ -692,10 +792,10 @@ void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, cudaStream
             const unsigned grid = (unsigned)std::min<int64_t>((total + 255) / 256, 148 * 8);
             const float* part = a.job[i].e.out32;
             if (dtype == MG_PREC_BF16)
-                finish_kernel<MG_PREC_BF16><<<grid, 256, 0, stream>>>(part, a.job[i].splits, jobs[i].m, jobs[i].n,
+                finish_kernel<MG_PREC_BF16><<<grid, 256, 0, stream>>>(part, a.job[i].splits, a.job[i].m_pad, jobs[i].m, jobs[i].n,
                                                                       a.job[i].e.ld32, finish[i]);
             else
-                finish_kernel<MG_PREC_FP16><<<grid, 256, 0, stream>>>(part, a.job[i].splits, jobs[i].m, jobs[i].n,
+                finish_kernel<MG_PREC_FP16><<<grid, 256, 0, stream>>>(part, a.job[i].splits, a.job[i].m_pad, jobs[i].m, jobs[i].n,
                                                                       a.job[i].e.ld32, finish[i]);
             launched("finish_kernel");
         }
@@ -716,6 +816,7 @@ void gemm_softmax(int dtype, const SoftmaxJob& g, int block, cudaStream_t stream
     a.job[0].s = g.e;
     a.units[0] = a.job[0].tiles_m * a.job[0].tiles_n;
     encode_operands(a, 0, dtype, g, bn);
+    if (g.e.probs != nullptr) encode_blocks(&a.to[0], dtype, g.e.probs, g.m, g.e.probs_ld, g.e.probs_ld);
     launch<kSoftmax>(a, bn, dtype, stream);
 }
 

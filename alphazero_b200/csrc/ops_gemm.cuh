@@ -28,7 +28,9 @@ struct GemmEpilogue {
     int64_t r_row = 0, r_col = 0;
     void* out = nullptr;             // [m][n], row stride ld
     void* z = nullptr;               // [m][n], row stride ld
-    float* out32 = nullptr;          // acc + acc32 in fp32, row stride ld32 (a multiple of 8), and nothing else
+    // acc + acc32 in fp32, row stride ld32 (a multiple of 8), and nothing
+    // else; room for m rounded up to 256 rows
+    float* out32 = nullptr;
     const float* acc32 = nullptr;    // fp32 sums of earlier pieces, added to acc
     int64_t ld = 0, ld32 = 0;
     float res_scale = 0.0f;
@@ -96,11 +98,27 @@ inline StagedOperand transposed(StagedOperand s) {
 // One or two products in one launch (the one with more k first).
 void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, cudaStream_t stream);
 
+// Phi(z), the normal distribution function, and exp(-z^2 / 2): formula
+// 7.1.26 of Abramowitz and Stegun for erf(|z| / sqrt 2), which is within
+// 1.5e-7 and needs one exponential that GELU's slope shares.
+__device__ __forceinline__ float normal_cdf(float z, float* bell) {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+    float p = fmaf(1.061405429f, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    *bell = exp2f(z * z * -0.72134752044448170f);
+    const float tail = 0.5f * p * t * *bell;
+    return z < 0.0f ? tail : 1.0f - tail;
+}
+
 __device__ __forceinline__ float activate(float z, int act) {
+    float bell;
     switch (act) {
         case MG_ACT_RELU: return z < 0.0f ? 0.0f : z;  // NaN stays
-        case MG_ACT_SILU: return z / (1.0f + expf(-z));
-        case MG_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+        case MG_ACT_SILU: return __fdividef(z, 1.0f + __expf(-z));
+        case MG_ACT_GELU: return z * normal_cdf(z, &bell);
         default: return z;
     }
 }

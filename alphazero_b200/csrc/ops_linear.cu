@@ -12,12 +12,14 @@ __device__ __forceinline__ float slope(float z, int act) {
     switch (act) {
         case MG_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
         case MG_ACT_SILU: {
-            const float p = 1.0f / (1.0f + expf(-z));
+            const float p = __fdividef(1.0f, 1.0f + __expf(-z));
             return p * (1.0f + z * (1.0f - p));
         }
-        case MG_ACT_GELU:
-            return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) +
-                   z * expf(-0.5f * z * z) * 0.39894228040143268f;
+        case MG_ACT_GELU: {
+            float bell;
+            const float phi = normal_cdf(z, &bell);
+            return phi + z * bell * 0.39894228040143268f;
+        }
         default: return 1.0f;
     }
 }
