@@ -43,20 +43,20 @@ constexpr int kPairs = 74;             // of SMs on a B200 (148)
 constexpr int kGroup = 8;              // row tiles walked together (their B tiles stay in L2)
 constexpr int kStagePitch = 34;        // 16-bit elements per row staged without TMA (17 words: no bank conflicts)
 constexpr int kOutBytes = 4096;        // per epilogue warp: two 32 x 32 blocks of 16-bit, or one of fp32
-constexpr int kResBytes = 2048;        // a 32 x 32 block of the residual
-constexpr int kWarpBytes = kOutBytes + kResBytes;
+constexpr int kResBytes = 2048;        // a 32 x 32 block of the residual, of two
+constexpr int kWarpBytes = kOutBytes + 2 * kResBytes;
 
 template <int BN>
 struct Config {
-    static constexpr int kStages = BN == 256 ? 5 : 7;
+    static constexpr int kStages = BN == 256 ? 5 : 6;
     static constexpr uint32_t kABytes = kRowsCta * kBK * 2;
     static constexpr uint32_t kBBytes = BN / 2 * kBK * 2;
     static constexpr uint32_t kStageBytes = kABytes + kBBytes;
     static constexpr uint32_t kTmemCols = 2 * BN;
-    static constexpr int kBarriers = 2 * kStages + 5 + kEpiWarps;
-    // ring + per epilogue warp its blocks and a bias row + barriers + alignment slack
-    static constexpr int kSmem = kStages * kStageBytes + kEpiWarps * (kWarpBytes + BN / 2 * 4) + kBarriers * 8 +
-                                 16 + 1024;
+    static constexpr int kBarriers = 2 * kStages + 5 + 2 * kEpiWarps;
+    // ring + per epilogue warp its blocks and 16-bit bias + barriers + TMEM address
+    static constexpr int kSmem = kStages * kStageBytes + kEpiWarps * (kWarpBytes + BN / 2 * 2) + kBarriers * 8 + 16;
+    static_assert(kSmem <= 232448, "shared memory of an SM");
 };
 
 enum Epi : int { kStore, kSoftmax };
@@ -83,43 +83,73 @@ struct alignas(64) KernelArgs {
 
 // The units of a pair: job 0's round robin, then job 1's, handed out in the
 // order in which the pairs come free (pairs with one unit of job 0 fewer
-// start head_start units of job 1 earlier).
+// start head_start units of job 1 earlier).  Index i of job 0 and of job 1,
+// or -1 when the pair has no more of that job.
 struct UnitWalk {
-    int pairs, p, n0, n1, extra, ahead, c0, step = 0;
+    int pairs, p, n0, n1, extra, ahead;
     __device__ UnitWalk(const KernelArgs& a, int pair, int total) : pairs(total), p(pair) {
         n0 = a.units[0];
         n1 = a.units[1];
         extra = n0 % pairs;
         ahead = extra ? a.head_start : 0;
-        c0 = p < n0 ? (n0 - p + pairs - 1) / pairs : 0;
     }
-    __device__ bool next(int* job, int* unit) {
-        const int i = step++;
-        if (i < c0) {
-            *job = 0;
-            *unit = p + i * pairs;
-            return true;
+    __device__ __forceinline__ int unit(int job, int i) const {
+        if (job == 0) {
+            const int u = p + i * pairs;
+            return u < n0 ? u : -1;
         }
-        const int j = i - c0, early = pairs - extra;
-        int u;
-        if (p >= extra && j < ahead) u = j * early + (p - extra);
-        else if (p >= extra) u = ahead * early + (j - ahead) * pairs + p;
-        else u = ahead * early + j * pairs + p;
-        *job = 1;
-        *unit = u;
-        return u < n1;
+        const int early = pairs - extra;
+        int u = ahead * early + i * pairs + p;
+        if (p >= extra) u = i < ahead ? i * early + (p - extra) : u - ahead * pairs;
+        return u < n1 ? u : -1;
     }
 };
 
+// Where a job's units lie.  The job's sizes are read once into registers:
+// a kernel parameter under a variable index is a load, and so are they
+// after every asm statement that may touch memory.
+struct Tiling {
+    int tiles, tiles_m, per, full, splits, kb_split, kblocks;
+    float inv_tiles, inv_per, inv_full, inv_last;
+    __device__ explicit Tiling(const JobArgs& j) {
+        tiles_m = j.tiles_m;
+        tiles = j.tiles_m * j.tiles_n;
+        per = kGroup * j.tiles_n;
+        full = tiles_m / kGroup;  // groups of kGroup row tiles
+        splits = j.splits;
+        kb_split = j.kb_split;
+        kblocks = j.kblocks;
+        inv_tiles = 1.0f / tiles;
+        inv_per = 1.0f / per;
+        inv_full = 1.0f / kGroup;
+        inv_last = 1.0f / max(1, tiles_m % kGroup);
+    }
+};
+
+// n / d for 0 <= n < 2^24, with inv = 1 / d; the remainder stays in n.
+__device__ __forceinline__ int divide(int& n, int d, float inv) {
+    int q = (int)(__int2float_rn(n) * inv);
+    n -= q * d;
+    if (n < 0) {
+        n += d;
+        --q;
+    }
+    if (n >= d) {
+        n -= d;
+        ++q;
+    }
+    return q;
+}
+
 struct Tile {
     int m0, n0, kb0, kb1, split;
-    __device__ Tile(const JobArgs& j, int unit, int bn) {
-        const int tiles = j.tiles_m * j.tiles_n;
-        split = unit / tiles;
-        const int t = unit % tiles, per = kGroup * j.tiles_n;
-        const int first = t / per * kGroup, rows = min(kGroup, j.tiles_m - first);
-        m0 = (first + t % per % rows) * kRowsPair;
-        n0 = t % per / rows * bn;
+    __device__ __forceinline__ Tile(const Tiling& j, int unit, int bn) {
+        split = j.splits > 1 ? divide(unit, j.tiles, j.inv_tiles) : 0;
+        const int group = divide(unit, j.per, j.inv_per);
+        const bool last = group >= j.full;
+        const int column = divide(unit, last ? j.tiles_m - j.full * kGroup : kGroup, last ? j.inv_last : j.inv_full);
+        m0 = (group * kGroup + unit) * kRowsPair;
+        n0 = column * bn;
         kb0 = split * j.kb_split;
         kb1 = min(kb0 + j.kb_split, j.kblocks);
     }
@@ -149,12 +179,11 @@ __device__ __forceinline__ uint32_t swizzle128(int r, int q) { return r * 128 + 
 // An epilogue warp's shared memory, and which of its blocks are in use.
 struct WarpBlocks {
     uint8_t* out;      // [2][2048], or [4096]
-    uint8_t* res;
-    uint64_t* landed;  // the residual block has arrived
+    uint8_t* res;      // [2][2048]
+    uint64_t* landed;  // [2] a residual block has arrived
     int lane;
     int next = 0;      // out block to write
-    int parity = 0;
-    bool pending = false;  // a residual block is on its way
+    int started = 0, taken = 0;  // residual blocks
 
     // Writes v (a row per lane) to the next block and starts its store.
     template <class Words>
@@ -188,21 +217,25 @@ struct WarpBlocks {
             bulk_commit();
         }
     }
-    // The residual's block at (row, col): started, and (after a wait) read.
+    // Blocks of the residual in turn: started ahead, at most two, and (after
+    // a wait) read.
     __device__ __forceinline__ void start_res(const CUtensorMap* map, int col, int row) {
-        __syncwarp();  // every lane has read the last one
-        pending = true;
+        __syncwarp();  // every lane has read what the block held
         if (lane == 0) {
-            mbar_arrive_expect_tx(smem_u32(landed), kResBytes);
-            tma_load_2d(smem_u32(res), map, smem_u32(landed), col, row);
+            const uint32_t bar = smem_u32(&landed[started & 1]);
+            mbar_arrive_expect_tx(bar, kResBytes);
+            tma_load_2d(smem_u32(res + (started & 1) * kResBytes), map, bar, col, row);
         }
+        ++started;
     }
     __device__ __forceinline__ bool read_res(uint4 (&u)[4], int* err) {
-        const bool ok = __all_sync(~0u, mbar_wait(smem_u32(landed), parity, err, kErrWaitEpilogue));
-        parity ^= 1;
-        pending = false;
+        const int b = taken & 1;
+        const bool ok =
+            __all_sync(~0u, mbar_wait(smem_u32(&landed[b]), (taken >> 1) & 1, err, kErrWaitEpilogue));
+        ++taken;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) u[q] = *reinterpret_cast<const uint4*>(res + swizzle64(lane, q));
+        for (int q = 0; q < 4; ++q)
+            u[q] = *reinterpret_cast<const uint4*>(res + b * kResBytes + swizzle64(lane, q));
         return ok;
     }
 };
@@ -252,31 +285,69 @@ __device__ __forceinline__ void activate_all(float (&v)[32], int act) {
     }
 }
 
-// Columns [n0 + c0, + BN / 2) of rows [m0, + 32) of a finished tile.  False
+// v = v * alpha + bias of 32 columns.
+template <int DT>
+__device__ __forceinline__ void add_bias(float (&v)[32], float alpha, const uint16_t* sbias) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const uint4 u = *reinterpret_cast<const uint4*>(sbias + q * 8);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 b = unpack2<DT>(w[i]);
+            v[q * 8 + 2 * i] = fmaf(v[q * 8 + 2 * i], alpha, b.x);
+            v[q * 8 + 2 * i + 1] = fmaf(v[q * 8 + 2 * i + 1], alpha, b.y);
+        }
+    }
+}
+
+// What a warp's epilogue needs of a job, in registers.
+struct EpilogueJob {
+    int m, n, m_pad, act;
+    bool by_tma, has_z, has_res, has_acc32, has_out32;
+    float alpha, res_scale;
+    __device__ explicit EpilogueJob(const JobArgs& j) {
+        const GemmEpilogue& e = j.e;
+        m = j.m;
+        n = j.n;
+        m_pad = j.m_pad;
+        act = e.act;
+        by_tma = j.by_tma != 0;
+        has_z = e.z != nullptr;
+        has_res = e.res != nullptr;
+        has_acc32 = e.acc32 != nullptr;
+        has_out32 = e.out32 != nullptr;
+        alpha = e.count ? e.alpha / (float)max(*e.count, 1) : e.alpha;
+        res_scale = e.res_scale;
+    }
+};
+
+// Columns [n0 + c0, + BN / 2) of rows [m0, + 32) of a finished tile, whose
+// sums are given back by `release` as soon as they are in registers.  False
 // if a wait gave up.
-template <int BN, int DT>
-__device__ __forceinline__ bool epilogue(const KernelArgs& a, int job, const Tile& t, int m0, int c0, uint32_t taddr,
-                                         WarpBlocks& blocks, const float* sbias, float alpha) {
-    const JobArgs& j = a.job[job];
-    const GemmEpilogue& e = j.e;
+template <int BN, int DT, class Release>
+__device__ __forceinline__ bool epilogue(const KernelArgs& a, int job, const EpilogueJob& j, const Tile& t, int m0,
+                                         int c0, uint32_t taddr, WarpBlocks& blocks, const uint16_t* sbias,
+                                         Release release) {
+    const GemmEpilogue& e = a.job[job].e;
     const int rows = min(32, j.m - m0), lane = blocks.lane;
-    const bool res_tma = e.res != nullptr && j.by_tma;
+    const int width = rows > 0 ? min(BN / 2, j.n - t.n0 - c0) : 0;
+    if (width <= 0) release();
 #pragma unroll 1
-    for (int c = 0; c < BN / 2; c += 32) {
+    for (int c = 0; c < width; c += 32) {
         const int col = t.n0 + c0 + c;
-        const int cols = min(32, j.n - col);
-        if (cols <= 0 || rows <= 0) break;
         uint32_t r[32];
         tmem_ld_32cols(taddr + c, r);
         tmem_ld_wait();
+        if (c + 32 >= width) release();
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-        if (e.acc32 != nullptr && lane < rows) {
+        if (j.has_acc32 && lane < rows) {
             const float* p = e.acc32 + (int64_t)(m0 + lane) * e.ld32 + col;
 #pragma unroll
             for (int q = 0; q < 8; ++q)
-                if (q * 4 < cols) {
+                if (c + q * 4 < width) {
                     const float4 f = *reinterpret_cast<const float4*>(p + q * 4);
                     v[q * 4] += f.x;
                     v[q * 4 + 1] += f.y;
@@ -284,46 +355,46 @@ __device__ __forceinline__ bool epilogue(const KernelArgs& a, int job, const Til
                     v[q * 4 + 3] += f.w;
                 }
         }
-        if (e.out32 != nullptr) {
+        if (j.has_out32) {
             blocks.store32(&a.to[job], col, t.split * j.m_pad + m0, v);
             continue;
         }
+        add_bias<DT>(v, j.alpha, sbias + c);
+        const auto word = [&](int i) { return pack2<DT>(v[2 * i], v[2 * i + 1]); };
+        if (j.by_tma) {
+            if (j.has_z) blocks.store16(&a.tz, col, m0, word);
+            activate_all(v, j.act);
+            if (j.has_res) {
+                uint4 u[4];
+                if (!blocks.read_res(u, a.err)) return false;
+                if (c + 64 < width) blocks.start_res(&a.tr, col + 64, m0);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = v[i] * alpha + sbias[c + i];
-        if (e.z != nullptr) {
-            if (j.by_tma)
-                blocks.store16(&a.tz, col, m0, [&](int i) { return pack2<DT>(v[2 * i], v[2 * i + 1]); });
-            else
-                store_block<DT>(static_cast<uint16_t*>(e.z) + (int64_t)m0 * e.ld + col, e.ld, rows, cols, lane,
-                                reinterpret_cast<uint16_t*>(blocks.out), v);
-        }
-        activate_all(v, e.act);
-        if (res_tma) {
-            uint4 u[4];
-            if (!blocks.read_res(u, a.err)) return false;
-            if (c + 32 < BN / 2 && col + 32 < j.n) blocks.start_res(&a.tr, col + 32, m0);
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t w[4] = {u[q].x, u[q].y, u[q].z, u[q].w};
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const uint32_t w[4] = {u[q].x, u[q].y, u[q].z, u[q].w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 f = unpack2<DT>(w[i]);
-                    v[q * 8 + 2 * i] += e.res_scale * f.x;
-                    v[q * 8 + 2 * i + 1] += e.res_scale * f.y;
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 f = unpack2<DT>(w[i]);
+                        v[q * 8 + 2 * i] += j.res_scale * f.x;
+                        v[q * 8 + 2 * i + 1] += j.res_scale * f.y;
+                    }
                 }
             }
-        } else if (e.res != nullptr) {
+            blocks.store16(&a.to[job], col, m0, word);
+            continue;
+        }
+        const int cols = min(32, width - c);
+        uint16_t* stage = reinterpret_cast<uint16_t*>(blocks.out);
+        if (j.has_z)
+            store_block<DT>(static_cast<uint16_t*>(e.z) + (int64_t)m0 * e.ld + col, e.ld, rows, cols, lane, stage, v);
+        activate_all(v, j.act);
+        if (j.has_res) {
             float x[32];
             load_block<DT>(static_cast<const uint16_t*>(e.res) + m0 * e.r_row + col * e.r_col, e.r_row, e.r_col, rows,
-                           cols, lane, reinterpret_cast<uint16_t*>(blocks.out), x);
+                           cols, lane, stage, x);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] += e.res_scale * x[i];
+            for (int i = 0; i < 32; ++i) v[i] += j.res_scale * x[i];
         }
-        if (j.by_tma)
-            blocks.store16(&a.to[job], col, m0, [&](int i) { return pack2<DT>(v[2 * i], v[2 * i + 1]); });
-        else
-            store_block<DT>(static_cast<uint16_t*>(e.out) + (int64_t)m0 * e.ld + col, e.ld, rows, cols, lane,
-                            reinterpret_cast<uint16_t*>(blocks.out), v);
+        store_block<DT>(static_cast<uint16_t*>(e.out) + (int64_t)m0 * e.ld + col, e.ld, rows, cols, lane, stage, v);
     }
     return true;
 }
@@ -331,51 +402,62 @@ __device__ __forceinline__ bool epilogue(const KernelArgs& a, int job, const Til
 // The same columns and rows as softmax statistics.  A thread has its row's
 // block to itself, so the maximum and the sum need no exchange; the sums are
 // read from TMEM twice rather than held in BN / 2 registers.
-template <int BN>
-__device__ __forceinline__ void softmax_epilogue(const KernelArgs& a, const Tile& t, int m0, int c0, uint32_t taddr,
-                                                 WarpBlocks& blocks, const float* sbias) {
-    const JobArgs& j = a.job[0];
-    const SoftmaxEpilogue& e = j.s;
+template <int BN, int DT, class Release>
+__device__ __forceinline__ void softmax_epilogue(const KernelArgs& a, const SoftmaxEpilogue& e, int m, int n,
+                                                 const Tile& t, int m0, int c0, int target, uint32_t taddr,
+                                                 WarpBlocks& blocks, const uint16_t* sbias, Release release) {
     const int row = m0 + blocks.lane;
     const int first = t.n0 + c0;
-    if (first >= j.n || m0 >= j.m) return;
-    const int width = min(BN / 2, j.n - first);
-    const int target = row < j.m ? e.target[row] - first : -1;
-    float top = -INFINITY, logit = 0.0f;
+    const int width = m0 < m ? min(BN / 2, n - first) : 0;
+    if (width <= 0) {
+        release();
+        return;
+    }
+    target -= first;
+    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, logit = 0.0f;
 #pragma unroll 1
     for (int c = 0; c < width; c += 32) {
         uint32_t r[32];
         tmem_ld_32cols(taddr + c, r);
         tmem_ld_wait();
-        const bool here = target >= c && target < c + 32;
+        float l[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const float l = __uint_as_float(r[i]) + sbias[c + i];  // -inf past the last column
-            top = fmaxf(top, l);
-            if (here && target == c + i) logit = l;
+        for (int i = 0; i < 32; ++i) l[i] = __uint_as_float(r[i]);
+        add_bias<DT>(l, 1.0f, sbias + c);  // -inf past the last column
+#pragma unroll
+        for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], l[i]);
+        if (__any_sync(~0u, target >= c && target < c + 32)) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (target == c + i) logit = l[i];
         }
     }
-    const float ref = top == -INFINITY ? 0.0f : top;
+    const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    const float ref = most == -INFINITY ? 0.0f : most;
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
     for (int c = 0; c < width; c += 32) {
         uint32_t r[32];
         tmem_ld_32cols(taddr + c, r);
         tmem_ld_wait();
+        if (c + 32 >= width) release();
         float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+        add_bias<DT>(v, 1.0f, sbias + c);
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
             // the difference first: exact near the maximum, and in range for any finite logits
-            v[i] = exp2f((__uint_as_float(r[i]) + sbias[c + i] - ref) * 1.4426950408889634f);
+            v[i] = exp2f((v[i] - ref) * 1.4426950408889634f);
             sum[i & 3] += v[i];
         }
         if (e.probs != nullptr)
             blocks.store16(&a.to[0], first + c, m0, [&](int i) { return prob16x2(v[2 * i], v[2 * i + 1]); });
     }
-    if (row < j.m) {
+    if (row < m) {
         if (target >= 0 && target < width) e.logit[row] = logit;
         e.part[(int64_t)(first / (BN / 2)) * e.part_ld + row] =
-            make_float2(top, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+            make_float2(most, (sum[0] + sum[1]) + (sum[2] + sum[3]));
     }
 }
 
@@ -384,19 +466,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ KernelArgs a) {
     using Cfg = Config<BN>;
     constexpr int S = Cfg::kStages;
-    extern __shared__ uint8_t smem_raw[];
-    // the same offset in both CTAs: the dynamic segment starts at the same address in each
-    uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
-    uint8_t* ring = smem;
+    extern __shared__ __align__(1024) uint8_t ring[];  // at the same address in both CTAs
     uint8_t* blocks_all = ring + S * Cfg::kStageBytes;  // a multiple of 1 KB, as each warp's part is
-    float* sbias_all = reinterpret_cast<float*>(blocks_all + kEpiWarps * kWarpBytes);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sbias_all + kEpiWarps * (BN / 2));
+    uint16_t* bias_all = reinterpret_cast<uint16_t*>(blocks_all + kEpiWarps * kWarpBytes);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(bias_all + kEpiWarps * (BN / 2));
     uint64_t* full = bars;           // even CTA's: a stage has landed in both CTAs
     uint64_t* empty = bars + S;      // each CTA's: the products have read a stage
     uint64_t* tfull = bars + 2 * S;  // [2] each CTA's: a tile's sums are complete
     uint64_t* tempty = tfull + 2;    // [2] even CTA's: both CTAs have read them
     uint64_t* done = tempty + 2;     // even CTA's: the last products are complete
-    uint64_t* landed = done + 1;     // [kEpiWarps] a warp's residual block has arrived
+    uint64_t* landed = done + 1;     // [kEpiWarps][2] a warp's residual block has arrived
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::kBarriers);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -413,7 +492,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             mbar_init(smem_u32(&tempty[i]), 2 * kEpiWarps);
         }
         mbar_init(smem_u32(done), 1);
-        for (int i = 0; i < kEpiWarps; ++i) mbar_init(smem_u32(&landed[i]), 1);
+        for (int i = 0; i < 2 * kEpiWarps; ++i) mbar_init(smem_u32(&landed[i]), 1);
         fence_barrier_init();
     }
     if (warp == 1) {
@@ -426,138 +505,183 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
-    UnitWalk walk(a, pair, pairs);
-    int job, unit;
+    const UnitWalk walk(a, pair, pairs);
+    const int jobs = a.units[1] > 0 ? 2 : 1;
     if (warp == 0) {
-        if (lane == 0) {
-            int it = 0;
-            bool ok = true;
-            while (ok && walk.next(&job, &unit)) {
-                const JobArgs& j = a.job[job];
-                const Tile t(j, unit, BN);
+        // Control flow here and in the MMA warp is the whole warp's; one
+        // elected lane issues (elect_one).
+        int s = 0, round = 0;  // stage, and times around the ring
+        int64_t used = 0;
+        bool ok = true;
+        for (int job = 0; job < jobs && ok; ++job) {
+            const Tiling tiling(a.job[job]);
+            const bool a_mn = a.job[job].a_mn, b_mn = a.job[job].b_mn;
+            for (int i = 0, unit; ok && (unit = walk.unit(job, i)) >= 0; ++i) {
+                const Tile t(tiling, unit, BN);
                 const int am = t.m0 + (int)rank * kRowsCta, bn = t.n0 + (int)rank * (BN / 2);
-                for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
-                    const int s = it % S;
-                    if (!mbar_wait_cluster(smem_u32(&empty[s]), ((it / S) & 1) ^ 1, a.err, kErrWaitProducer)) {
+                for (int kb = t.kb0; kb < t.kb1; ++kb) {
+                    const uint32_t wait = smem_u32(&empty[s]);
+                    if (!mbar_wait_cluster_warp(wait, (round & 1) ^ 1, a.err, kErrWaitProducer)) {
                         ok = false;
                         break;
                     }
                     const uint32_t bar = map_to_rank(smem_u32(&full[s]), 0);
-                    if (rank == 0) mbar_arrive_expect_tx(smem_u32(&full[s]), 2 * Cfg::kStageBytes);
                     const uint32_t da = smem_u32(ring + s * Cfg::kStageBytes), db = da + Cfg::kABytes;
                     const int k0 = kb * kBK;
-                    if (j.a_mn) {
-                        tma_load_2d_pair(da, &a.ta[job], bar, am, k0);
-                        tma_load_2d_pair(da + 8192, &a.ta[job], bar, am + 64, k0);
-                    } else {
-                        tma_load_2d_pair(da, &a.ta[job], bar, k0, am);
+                    if (elect_one()) {
+                        if (rank == 0) mbar_arrive_expect_tx(smem_u32(&full[s]), 2 * Cfg::kStageBytes);
+                        if (a_mn) {
+                            tma_load_2d_pair(da, &a.ta[job], bar, am, k0);
+                            tma_load_2d_pair(da + 8192, &a.ta[job], bar, am + 64, k0);
+                        } else {
+                            tma_load_2d_pair(da, &a.ta[job], bar, k0, am);
+                        }
+                        if (b_mn) {
+                            tma_load_2d_pair(db, &a.tb[job], bar, bn, k0);
+                            if (BN == 256) tma_load_2d_pair(db + 8192, &a.tb[job], bar, bn + 64, k0);
+                        } else {
+                            tma_load_2d_pair(db, &a.tb[job], bar, k0, bn);
+                        }
                     }
-                    if (j.b_mn) {
-                        tma_load_2d_pair(db, &a.tb[job], bar, bn, k0);
-                        if (BN == 256) tma_load_2d_pair(db + 8192, &a.tb[job], bar, bn + 64, k0);
-                    } else {
-                        tma_load_2d_pair(db, &a.tb[job], bar, k0, bn);
+                    ++used;
+                    if (++s == S) {
+                        s = 0;
+                        ++round;
                     }
                 }
             }
-            // Every load has landed and every stage has been released (the
-            // release comes from the peer's commits) before this CTA ends.
-            for (int i = max(0, it - S); i < it; ++i) {
-                const int s = i % S;
-                if (rank == 0) mbar_wait_cluster(smem_u32(&full[s]), (i / S) & 1, a.err, kErrWaitDrain);
-                if (ok) mbar_wait_cluster(smem_u32(&empty[s]), (i / S) & 1, a.err, kErrWaitDrain);
-            }
         }
-        __syncwarp();
+        // Every load has landed and every stage has been released (the
+        // release comes from the peer's commits) before this CTA ends.
+        for (int i = 0; i < S && i < used; ++i) {
+            if (--s < 0) {
+                s = S - 1;
+                --round;
+            }
+            if (rank == 0) mbar_wait_cluster_warp(smem_u32(&full[s]), round & 1, a.err, kErrWaitDrain);
+            if (ok) mbar_wait_cluster_warp(smem_u32(&empty[s]), round & 1, a.err, kErrWaitDrain);
+        }
     } else if (warp == 1) {
-        if (rank == 0 && lane == 0) {
-            int it = 0, tile = 0;
+        if (rank == 0) {
+            int s = 0, round = 0, tile = 0;
             bool ok = true;
-            while (ok && walk.next(&job, &unit)) {
-                const JobArgs& j = a.job[job];
-                const Tile t(j, unit, BN);
-                const uint32_t idesc = idesc_f16(kRowsPair, BN, DT == MG_PREC_BF16) |
-                                       (j.a_mn ? kIdescAMn : 0) | (j.b_mn ? kIdescBMn : 0);
-                const uint64_t step_a = j.a_mn ? 2048 >> 4 : 32 >> 4, step_b = j.b_mn ? 2048 >> 4 : 32 >> 4;
-                const int buf = tile & 1;
-                if (!mbar_wait_cluster(smem_u32(&tempty[buf]), ((tile >> 1) & 1) ^ 1, a.err, kErrWaitMma)) break;
-                tc_fence_after();
-                const uint32_t acc = tmem_base + buf * BN;
-                for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
-                    const int s = it % S;
-                    if (!mbar_wait_cluster(smem_u32(&full[s]), (it / S) & 1, a.err, kErrWaitMma)) {
+            for (int job = 0; job < jobs && ok; ++job) {
+                const Tiling tiling(a.job[job]);
+                const bool a_mn = a.job[job].a_mn, b_mn = a.job[job].b_mn;
+                const uint32_t idesc = idesc_f16(kRowsPair, BN, DT == MG_PREC_BF16) | (a_mn ? kIdescAMn : 0) |
+                                       (b_mn ? kIdescBMn : 0);
+                const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, step_b = b_mn ? 2048 >> 4 : 32 >> 4;
+                const uint32_t ring_at = smem_u32(ring);
+                const uint64_t first_a = a_mn ? smem_desc_sw128_mn(ring_at) : smem_desc_sw128(ring_at);
+                const uint64_t first_b =
+                    b_mn ? smem_desc_sw128_mn(ring_at + Cfg::kABytes) : smem_desc_sw128(ring_at + Cfg::kABytes);
+                for (int i = 0, unit; ok && (unit = walk.unit(job, i)) >= 0; ++i) {
+                    const Tile t(tiling, unit, BN);
+                    const int buf = tile & 1;
+                    if (!mbar_wait_cluster_warp(smem_u32(&tempty[buf]), ((tile >> 1) & 1) ^ 1, a.err, kErrWaitMma)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t da = smem_u32(ring + s * Cfg::kStageBytes), db = da + Cfg::kABytes;
-                    uint64_t xa = j.a_mn ? smem_desc_sw128_mn(da) : smem_desc_sw128(da);
-                    uint64_t xb = j.b_mn ? smem_desc_sw128_mn(db) : smem_desc_sw128(db);
+                    const uint32_t acc = tmem_base + buf * BN;
+                    for (int kb = t.kb0; kb < t.kb1; ++kb) {
+                        if (!mbar_wait_cluster_warp(smem_u32(&full[s]), round & 1, a.err, kErrWaitMma)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint64_t xa = first_a + s * (Cfg::kStageBytes >> 4);
+                        const uint64_t xb = first_b + s * (Cfg::kStageBytes >> 4);
+                        if (elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < kBK / 16; ++kk) {
-                        mma_f16_pair(acc, xa, xb, idesc, kb > t.kb0 || kk > 0);
-                        xa += step_a;
-                        xb += step_b;
+                            for (int kk = 0; kk < kBK / 16; ++kk)
+                                mma_f16_pair(acc, xa + kk * step_a, xb + kk * step_b, idesc, kb > t.kb0 || kk > 0);
+                            mma_commit_pair(smem_u32(&empty[s]));
+                            if (kb + 1 == t.kb1) mma_commit_pair(smem_u32(&tfull[buf]));
+                        }
+                        if (++s == S) {
+                            s = 0;
+                            ++round;
+                        }
                     }
-                    mma_commit_pair(smem_u32(&empty[s]));
+                    ++tile;
                 }
-                if (!ok) break;
-                mma_commit_pair(smem_u32(&tfull[buf]));
-                ++tile;
             }
             // Products still in flight finish before TMEM is freed.
-            asm volatile(
-                "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(done))
-                : "memory");
-            mbar_wait_cluster(smem_u32(done), 0, a.err, kErrWaitDrain);
+            if (elect_one())
+                asm volatile(
+                    "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(done))
+                    : "memory");
+            mbar_wait_cluster_warp(smem_u32(done), 0, a.err, kErrWaitDrain);
         }
-        __syncwarp();
     } else {
         const int ew = warp - 2, quarter = warp & 3, half = ew >> 2;
-        float* sbias = sbias_all + ew * (BN / 2);
+        const int c0 = half * (BN / 2);
+        // the warp's own copy of its columns' bias: one shared by four warps would
+        // need a barrier, which a warp whose wait gave up would leave the others at
+        uint16_t* sbias = bias_all + ew * (BN / 2);
         WarpBlocks blocks;
         blocks.out = blocks_all + ew * kWarpBytes;
         blocks.res = blocks.out + kOutBytes;
-        blocks.landed = &landed[ew];
+        blocks.landed = &landed[2 * ew];
         blocks.lane = lane;
-        const int c0 = half * (BN / 2);
+        const uint32_t taddr0 = tmem_base + c0 + ((uint32_t)quarter << 21);
         int tile = 0;
         bool ok = true;
-        while (ok && walk.next(&job, &unit)) {
-            const JobArgs& j = a.job[job];
-            const Tile t(j, unit, BN);
-            const int m0 = t.m0 + (int)rank * kRowsCta + quarter * 32;
-            // the residual's first block on its way before the sums are complete
-            if (EPI == kStore && j.e.res != nullptr && j.by_tma && m0 < j.m && t.n0 + c0 < j.n)
-                blocks.start_res(&a.tr, t.n0 + c0, m0);
-            __syncwarp();
-            for (int i = lane; i < BN / 2; i += 32) {
-                const int64_t col = t.n0 + c0 + i;
-                const void* bias = EPI == kSoftmax ? j.s.bias : j.e.out32 == nullptr ? j.e.bias : nullptr;
-                float b = EPI == kSoftmax ? -INFINITY : 0.0f;
-                if (col < j.n)
-                    b = bias != nullptr ? Elem<DT>::get(static_cast<const typename Elem<DT>::T*>(bias)[col]) : 0.0f;
-                sbias[i] = b;
+        for (int job = 0; job < jobs && ok; ++job) {
+            const Tiling tiling(a.job[job]);
+            const EpilogueJob j(a.job[job]);
+            const SoftmaxEpilogue soft = a.job[0].s;
+            const void* bias = EPI == kSoftmax ? soft.bias : j.has_out32 ? nullptr : a.job[job].e.bias;
+            int bias_at = -1;  // first column of the tile whose bias is there
+            for (int i = 0, unit; ok && (unit = walk.unit(job, i)) >= 0; ++i) {
+                const Tile t(tiling, unit, BN);
+                const int m0 = t.m0 + (int)rank * kRowsCta + quarter * 32;
+                // what the tile needs besides its sums is on its way before they are complete
+                int target = -1;
+                if constexpr (EPI == kSoftmax) {
+                    if (m0 + lane < j.m) target = soft.target[m0 + lane];
+                } else if (j.has_res && j.by_tma && m0 < j.m) {
+                    const int col = t.n0 + c0;
+                    if (col < j.n) blocks.start_res(&a.tr, col, m0);
+                    if (BN / 2 > 32 && col + 32 < j.n) blocks.start_res(&a.tr, col + 32, m0);
+                }
+                if (t.n0 != bias_at) {
+                    bias_at = t.n0;
+                    __syncwarp();
+                    for (int b = lane; b < BN / 2; b += 32) {
+                        const int64_t col = t.n0 + c0 + b;
+                        // past the last column: nothing, or for the softmax a logit of -inf
+                        uint16_t v = EPI == kSoftmax && col >= j.n ? (DT == MG_PREC_BF16 ? 0xff80 : 0xfc00) : 0;
+                        if (bias != nullptr && col < j.n) v = static_cast<const uint16_t*>(bias)[col];
+                        sbias[b] = v;
+                    }
+                    __syncwarp();
+                }
+                const int buf = tile & 1;
+                // one answer for the warp, which goes on or stops together
+                if (!mbar_wait_cluster_warp(smem_u32(&tfull[buf]), (tile >> 1) & 1, a.err, kErrWaitEpilogue)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const auto release = [&] {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&tempty[buf]), 0));
+                };
+                if constexpr (EPI == kSoftmax)
+                    softmax_epilogue<BN, DT>(a, soft, j.m, j.n, t, m0, c0, target, taddr0 + buf * BN, blocks, sbias,
+                                         release);
+                else
+                    ok = epilogue<BN, DT>(a, job, j, t, m0, c0, taddr0 + buf * BN, blocks, sbias, release);
+                ++tile;
             }
-            __syncwarp();
-            const int buf = tile & 1;
-            // one answer for the warp, which goes on or stops together
-            if (!__all_sync(~0u, mbar_wait_cluster(smem_u32(&tfull[buf]), (tile >> 1) & 1, a.err, kErrWaitEpilogue)))
-                break;
-            tc_fence_after();
-            const uint32_t taddr = tmem_base + buf * BN + c0 + ((uint32_t)quarter << 21);
-            if constexpr (EPI == kSoftmax) {
-                softmax_epilogue<BN>(a, t, m0, c0, taddr, blocks, sbias);
-            } else {
-                const float alpha = j.e.count ? j.e.alpha / (float)max(*j.e.count, 1) : j.e.alpha;
-                ok = epilogue<BN, DT>(a, job, t, m0, c0, taddr, blocks, sbias, alpha);
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&tempty[buf]), 0));
-            ++tile;
         }
-        if (blocks.pending) mbar_wait(smem_u32(blocks.landed), blocks.parity, a.err, kErrWaitDrain);
+        while (blocks.taken < blocks.started) {  // only after a wait gave up
+            mbar_wait(smem_u32(&landed[2 * ew + (blocks.taken & 1)]), (blocks.taken >> 1) & 1, a.err, kErrWaitDrain);
+            ++blocks.taken;
+        }
         if (lane == 0) bulk_wait_all();
         __syncwarp();
     }

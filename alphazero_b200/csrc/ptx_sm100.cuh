@@ -370,6 +370,20 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     return r;
 }
 
+// True in one lane of a converged warp.  Code that issues TMA or tcgen05
+// instructions from warp-uniform control flow under this predicate keeps
+// their descriptors and addresses in uniform registers; from a branch on the
+// lane index each operand is moved there one instruction at a time.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+
 // Address in CTA `rank`'s shared memory of what `addr` is in this CTA's.
 __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
     uint32_t r;
@@ -412,6 +426,11 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
             return false;
         }
     }
+}
+
+// The same for a whole warp, with one answer.
+__device__ __forceinline__ bool mbar_wait_cluster_warp(uint32_t bar, uint32_t parity, int* err, int code) {
+    return __all_sync(~0u, mbar_wait_cluster(bar, parity, err, code));
 }
 
 // As tma_load_2d into this CTA's shared memory, counted on a barrier of
