@@ -10,14 +10,25 @@ namespace {
 __device__ int g_op_status;
 constexpr int kMaxDevices = 64;
 
+// 32 columns per block; 32 threads share a column's rows.
 template <int DT>
-__global__ void __launch_bounds__(256) add_rows_kernel(const float* sums, int64_t rows, int64_t cols, float alpha,
-                                                       const int* count, typename Elem<DT>::T* out) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= cols) return;
+__global__ void __launch_bounds__(1024) add_rows_kernel(const float* sums, int64_t rows, int64_t cols, float alpha,
+                                                        const int* count, typename Elem<DT>::T* out) {
+    __shared__ float part[32][33];
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+    griddep_launch_dependents();
+    griddep_wait();
     float s = 0.0f;
+    if (c < cols)
 #pragma unroll 8
-    for (int64_t r = 0; r < rows; ++r) s += sums[r * cols + c];
+        for (int64_t r = slice; r < rows; r += 32) s += sums[r * cols + c];
+    part[slice][lane] = s;
+    __syncthreads();
+    if (slice > 0 || c >= cols) return;
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s += part[i][lane];
     out[c] = Elem<DT>::put(s * (count ? alpha / (float)max(*count, 1) : alpha));
 }
 
@@ -29,15 +40,14 @@ std::string& last_op_error() {
 }
 
 void add_rows(int dtype, const float* sums, int64_t rows, int64_t cols, float alpha, const int* count,
-              void* out, cudaStream_t stream) {
-    const unsigned grid = (unsigned)((cols + 255) / 256);
+              void* out, Queue& q) {
+    const dim3 grid((unsigned)((cols + 31) / 32));
     if (dtype == MG_PREC_BF16)
-        add_rows_kernel<MG_PREC_BF16><<<grid, 256, 0, stream>>>(sums, rows, cols, alpha, count,
-                                                                static_cast<__nv_bfloat16*>(out));
+        q.launch("add_rows_kernel", add_rows_kernel<MG_PREC_BF16>, grid, 1024, 0, sums, rows, cols, alpha, count,
+                 static_cast<__nv_bfloat16*>(out));
     else
-        add_rows_kernel<MG_PREC_FP16><<<grid, 256, 0, stream>>>(sums, rows, cols, alpha, count,
-                                                                static_cast<__half*>(out));
-    launched("add_rows_kernel");
+        q.launch("add_rows_kernel", add_rows_kernel<MG_PREC_FP16>, grid, 1024, 0, sums, rows, cols, alpha, count,
+                 static_cast<__half*>(out));
 }
 
 int* op_status_word() {

@@ -10,6 +10,8 @@
 #include <cuda_runtime.h>
 #include <string>
 
+#include "ptx_sm100.cuh"
+
 namespace mgb {
 namespace ops {
 
@@ -58,28 +60,39 @@ inline void need(bool ok, const char* what) {
 inline void check(cudaError_t e, const char* where) {
     if (e != cudaSuccess) fail(MG_E_CUDA, std::string(where) + ": " + cudaGetErrorString(e));
 }
-inline void launched(const char* kernel) { check(cudaGetLastError(), kernel); }
 
-// Launches a kernel that may begin while the one before it in the stream is
-// finishing (programmatic dependent launch).  Such a kernel calls
-// griddep_wait() in every thread before it touches global memory, and so
-// does every kernel it can follow; the first kernel of a call is launched in
-// the ordinary way, after everything before it.
-template <class... P, class... A>
-void launch_next(const char* name, void (*kernel)(P...), dim3 grid, int block, int smem, cudaStream_t stream,
-                 A... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3((unsigned)block);
-    cfg.dynamicSmemBytes = (size_t)smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    check(cudaLaunchKernelEx(&cfg, kernel, P(args)...), name);
-}
+// The launches of one call, in order.  All but the first may begin while the
+// one before is finishing (programmatic dependent launch), so every kernel
+// that goes through here calls griddep_wait() in every thread before it
+// touches global memory; the first is launched in the ordinary way, after
+// everything the stream holds.
+class Queue {
+public:
+    explicit Queue(void* stream) : stream_(static_cast<cudaStream_t>(stream)) {}
+    template <class... P, class... A>
+    void launch(const char* name, void (*kernel)(P...), dim3 grid, int block, int smem, A... args) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3((unsigned)block);
+        cfg.dynamicSmemBytes = (size_t)smem;
+        cfg.stream = stream_;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = begun_ ? 1 : 0;
+        check(cudaLaunchKernelEx(&cfg, kernel, P(args)...), name);
+        begun_ = true;
+    }
+    void clear(void* p, size_t bytes) {
+        check(cudaMemsetAsync(p, 0, bytes, stream_), "cudaMemsetAsync");
+        begun_ = false;  // what follows a memset waits for it in the ordinary way
+    }
+
+private:
+    cudaStream_t stream_;
+    bool begun_ = false;
+};
 
 // Makes args->device current for one call.
 class OnDevice {
@@ -145,9 +158,9 @@ int guarded(F&& body) noexcept {
 int* op_status_word();
 
 // out[c] = alpha / max(*count, 1) * sum over `rows` rows of sums[r * cols + c],
-// in row order (count may be null: 1).
+// in a fixed order (count may be null: 1).
 void add_rows(int dtype, const float* sums, int64_t rows, int64_t cols, float alpha, const int* count,
-              void* out, cudaStream_t stream);
+              void* out, Queue& q);
 
 }  // namespace ops
 }  // namespace mgb

@@ -28,11 +28,15 @@ constexpr size_t kPieceBytes = size_t(1) << 30;
 template <int DT>
 constexpr float kDScale = DT == MG_PREC_FP16 ? 16384.0f : 1.0f;
 
-// target[i] (-1: not counted) and their number.
-__global__ void __launch_bounds__(1024) target_kernel(mg_cross_entropy_args a, int* target, int* count) {
+constexpr int kCountBlocks = 148;
+
+// target[i] (-1: not counted), and their number per block.
+__global__ void __launch_bounds__(1024) target_kernel(mg_cross_entropy_args a, int* target, int* counts) {
     __shared__ int part[32];
+    griddep_launch_dependents();
+    griddep_wait();
     int c = 0;
-    for (int64_t i = threadIdx.x; i < a.n; i += 1024) {
+    for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < a.n; i += (int64_t)gridDim.x * 1024) {
         const int t = (int)index_at(a.targets, a.target_bytes, i * a.target_stride, a.vocab);
         target[i] = t;
         c += t >= 0;
@@ -42,39 +46,51 @@ __global__ void __launch_bounds__(1024) target_kernel(mg_cross_entropy_args a, i
     __syncthreads();
     if (threadIdx.x < 32) {
         c = __reduce_add_sync(~0u, part[threadIdx.x]);
-        if (threadIdx.x == 0) *count = c;
+        if (threadIdx.x == 0) counts[blockIdx.x] = c;
     }
 }
 
-// logsumexp and loss of 32 rows per block: 32 threads share a row's blocks.
-// A row of -inf has lse -inf.
-__global__ void __launch_bounds__(1024)
+// (m, s) of a sum s exp(m) joined with another's.
+__device__ __forceinline__ void join(float& m, float& s, float2 p) {
+    const float top = fmaxf(m, p.x), ref = top == -INFINITY ? 0.0f : top;
+    s = s * exp2f((m - ref) * 1.4426950408889634f) + p.y * exp2f((p.x - ref) * 1.4426950408889634f);
+    m = top;
+}
+
+// logsumexp and loss per row; SLICES threads share a row's blocks.  A row of
+// -inf has lse -inf.  counts, if set: their sum goes to count.
+template <int SLICES>
+__global__ void __launch_bounds__(SLICES == 1 ? 128 : 1024)
     combine_kernel(int64_t rows, int blocks, const float2* part, int64_t part_ld, const int* target,
-                   const float* logit, float* lse, float* row_loss) {
-    __shared__ float2 mine[32][33];
-    const int64_t row = (int64_t)blockIdx.x * 32 + threadIdx.x % 32;
-    const int slice = threadIdx.x / 32;
+                   const float* logit, float* lse, float* row_loss, const int* counts, int count_blocks, int* count) {
+    griddep_launch_dependents();
+    griddep_wait();
+    if (counts != nullptr && blockIdx.x == 0 && threadIdx.x < 32) {
+        int c = 0;
+        for (int i = threadIdx.x; i < count_blocks; i += 32) c += counts[i];
+        c = __reduce_add_sync(~0u, c);
+        if (threadIdx.x == 0) *count = c;
+    }
+    constexpr int kRows = SLICES == 1 ? 128 : 32;
+    const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x % kRows;
+    const int slice = threadIdx.x / kRows;
     float m = -INFINITY, s = 0.0f;
     if (row < rows)
-        for (int b = slice; b < blocks; b += 32) {
-            const float2 p = part[(int64_t)b * part_ld + row];
-            const float top = fmaxf(m, p.x), ref = top == -INFINITY ? 0.0f : top;
-            s = s * exp2f((m - ref) * 1.4426950408889634f) + p.y * exp2f((p.x - ref) * 1.4426950408889634f);
-            m = top;
-        }
-    mine[slice][threadIdx.x % 32] = make_float2(m, s);
-    __syncthreads();
-    if (threadIdx.x >= 32 || row >= rows) return;
-    float top = -INFINITY, sum = 0.0f;
-    for (int i = 0; i < 32; ++i) top = fmaxf(top, mine[i][threadIdx.x].x);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    for (int i = 0; i < 32; ++i) {
-        const float2 p = mine[i][threadIdx.x];
-        sum += p.y * exp2f((p.x - ref) * 1.4426950408889634f);
+#pragma unroll 4
+        for (int b = slice; b < blocks; b += SLICES) join(m, s, part[(int64_t)b * part_ld + row]);
+    if constexpr (SLICES > 1) {
+        __shared__ float2 mine[SLICES][33];
+        mine[slice][threadIdx.x % 32] = make_float2(m, s);
+        __syncthreads();
+        if (slice > 0) return;
+        m = -INFINITY;
+        s = 0.0f;
+        for (int i = 0; i < SLICES; ++i) join(m, s, mine[i][threadIdx.x]);
     }
-    const float l = sum == 0.0f ? -INFINITY : ref + logf(sum);
+    if (row >= rows) return;
+    const float l = s == 0.0f ? -INFINITY : m + logf(s);
     lse[row] = l;
-    const float at = logit[row];
+    const float at = target[row] < 0 ? 0.0f : logit[row];
     row_loss[row] = target[row] < 0 ? 0.0f : at == -INFINITY ? INFINITY : l - at;
 }
 
@@ -93,6 +109,8 @@ __global__ void __launch_bounds__(256)
     const int64_t c = (int64_t)blockIdx.x * 256 + lane * 8;
     const int64_t r0 = (int64_t)blockIdx.y * rows_per_block, r1 = min(rows, r0 + rows_per_block);
     float sum[8] = {};
+    griddep_launch_dependents();
+    griddep_wait();
     if (c < vocab) {
         const float2* mine = part + c / block * part_ld;
 #pragma unroll 4
@@ -102,16 +120,22 @@ __global__ void __launch_bounds__(256)
             uint4* p = reinterpret_cast<uint4*>(probs + r * ld + c);
             const uint4 u = *p;
             const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-            const float f = l == -INFINITY ? 0.0f : exp2f((mine[r].x - l) * 1.4426950408889634f);
+            // a row that is not counted (whatever it holds) and one of -inf have no probabilities
+            float f = l == -INFINITY || t < 0 ? 0.0f : exp2f((mine[r].x - l) * 1.4426950408889634f);
+            f *= 0x1p112f;  // prob16_value's scale
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                v[i] = __uint_as_float(i & 1 ? w[i / 2] >> 16 << 11 : (w[i / 2] & 0xffffu) << 11) * f;
+            if (t >= c && t < c + 8)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (t == c + i) v[i] -= 1.0f;
             alignas(16) T d[8];
-            const int64_t hot = t < 0 ? -1 : t - c;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                float v = prob16_value(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu) * f;
-                if (hot == i) v -= 1.0f;
-                if (t < 0) v = 0.0f;
-                sum[i] += v;
-                d[i] = E::put(v * kDScale<DT>);
+                sum[i] += v[i];
+                d[i] = E::put(v[i] * kDScale<DT>);
             }
             *p = *reinterpret_cast<uint4*>(d);
         }
@@ -130,7 +154,9 @@ __global__ void __launch_bounds__(256)
 
 __global__ void __launch_bounds__(1024) loss_kernel(int64_t n, const float* row_loss, const int* count, float* loss) {
     __shared__ float part[1024];
+    griddep_wait();
     float s = 0.0f;
+#pragma unroll 8
     for (int64_t i = threadIdx.x; i < n; i += 1024) s += row_loss[i];
     part[threadIdx.x] = s;
     __syncthreads();
@@ -142,14 +168,14 @@ __global__ void __launch_bounds__(1024) loss_kernel(int64_t n, const float* row_
 }
 
 template <int DT>
-void run(const mg_cross_entropy_args& a, Workspace& w, bool go, cudaStream_t s) {
+void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
     using T = typename Elem<DT>::T;
     const bool grads = a.dw != nullptr;  // an empty dx may be null
     if (a.n == 0) {
         if (!go) return;
-        ops::check(cudaMemsetAsync(a.loss, 0, 4, s), "cudaMemsetAsync");
-        if (grads) ops::check(cudaMemsetAsync(a.dw, 0, (size_t)a.vocab * a.dim * 2, s), "cudaMemsetAsync");
-        if (a.db) ops::check(cudaMemsetAsync(a.db, 0, (size_t)a.vocab * 2, s), "cudaMemsetAsync");
+        q.clear(a.loss, 4);
+        if (grads) q.clear(a.dw, (size_t)a.vocab * a.dim * 2);
+        if (a.db) q.clear(a.db, (size_t)a.vocab * 2);
         return;
     }
     const int64_t ld = (a.vocab + 7) / 8 * 8;
@@ -161,25 +187,26 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, cudaStream_t s) 
     const int blocks = (int)((a.vocab + block - 1) / block);
 
     int* count = w.take<int>(4);
+    int* counts = w.take<int>(kCountBlocks * 4);
+    const int count_blocks = (int)std::min<int64_t>(kCountBlocks, (a.n + 1023) / 1024);
     int* target = w.take<int>((size_t)a.n * 4);
     float* logit = w.take<float>((size_t)piece * 4);
     float* lse = w.take<float>((size_t)piece * 4);
     float2* part = w.take<float2>((size_t)blocks * piece * 8);
     uint16_t* probs = grads ? w.take<uint16_t>((size_t)piece * ld * 2) : nullptr;
     const int64_t across = (a.vocab + 255) / 256;
-    const int64_t want = std::max<int64_t>(1, 148 * 16 / across);
+    const int64_t want = std::max<int64_t>(1, 148 * 4 / across);
     const int down_rows = (int)std::max<int64_t>(32, (piece + want - 1) / want);
     const int64_t down = (piece + down_rows - 1) / down_rows;  // of a whole piece
     float* sums = a.db ? w.take<float>((size_t)down * count_pieces * a.vocab * 4) : nullptr;
     const int64_t ld32 = (a.dim + 7) / 8 * 8;
     float* dw32 = grads && count_pieces > 1 ? w.take<float>((size_t)((a.vocab + 255) / 256 * 256) * ld32 * 4) : nullptr;
 
-    StagedOperand x = stage_operand(w, go, {a.x, a.x_row, a.x_col}, a.n, a.dim, s);
-    const StagedOperand weight = stage_operand(w, go, {a.weight, a.w_row, a.w_col}, a.vocab, a.dim, s);
+    StagedOperand x = stage_operand(w, go, {a.x, a.x_row, a.x_col}, a.n, a.dim, q);
+    const StagedOperand weight = stage_operand(w, go, {a.weight, a.w_row, a.w_col}, a.vocab, a.dim, q);
     if (go) {
         w.require();
-        target_kernel<<<1, 1024, 0, s>>>(a, target, count);
-        launched("target_kernel");
+        q.launch("target_kernel", target_kernel, dim3(count_blocks), 1024, 0, a, target, counts);
     }
     const float alpha = a.grad_scale / kDScale<DT>;
     int64_t sum_rows = 0;
@@ -203,18 +230,22 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, cudaStream_t s) 
             f.e.part_ld = piece;
             f.e.probs = probs;
             f.e.probs_ld = ld;
-            gemm_softmax(DT, f, block, s);
-            combine_kernel<<<(unsigned)((rows + 31) / 32), 1024, 0, s>>>(rows, blocks, part, piece, target + row0,
-                                                                       logit, lse, a.row_loss + row0);
-            launched("combine_kernel");
+            gemm_softmax(DT, f, block, q);
+            const int* sum_of = first ? counts : nullptr;
+            if (blocks <= 16)
+                q.launch("combine_kernel", combine_kernel<1>, dim3((unsigned)((rows + 127) / 128)), 128, 0, rows,
+                         blocks, part, piece, target + row0, logit, lse, a.row_loss + row0, sum_of, count_blocks,
+                         count);
+            else
+                q.launch("combine_kernel", combine_kernel<32>, dim3((unsigned)((rows + 31) / 32)), 1024, 0, rows,
+                         blocks, part, piece, target + row0, logit, lse, a.row_loss + row0, sum_of, count_blocks,
+                         count);
         }
         if (!grads) continue;
         const int64_t these = (rows + down_rows - 1) / down_rows;
         if (go) {
-            d_kernel<DT><<<dim3((unsigned)across, (unsigned)these), 256, 0, s>>>(
-                rows, a.vocab, block, probs, ld, part, piece, lse, target + row0, down_rows,
-                sums ? sums + sum_rows * a.vocab : nullptr);
-            launched("d_kernel");
+            q.launch("d_kernel", d_kernel<DT>, dim3((unsigned)across, (unsigned)these), 256, 0, rows, a.vocab, block,
+                     probs, ld, part, piece, lse, target + row0, down_rows, sums ? sums + sum_rows * a.vocab : nullptr);
         }
         sum_rows += these;
         StagedOperand d;
@@ -245,7 +276,7 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, cudaStream_t s) 
         jw.e.alpha = alpha;
         jw.e.count = count;
         Workspace again = w;  // every piece's scratch is the same
-        gemm(again, go, DT, jobs, 2, s);
+        gemm(again, go, DT, jobs, 2, q);
         if (go) continue;
         piece_scratch = std::max(piece_scratch, again.used() - w.used());
     }
@@ -253,9 +284,8 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, cudaStream_t s) 
         w.take(piece_scratch);
         return;
     }
-    if (a.db) add_rows(DT, sums, sum_rows, a.vocab, alpha * kDScale<DT>, count, a.db, s);
-    loss_kernel<<<1, 1024, 0, s>>>(a.n, a.row_loss, count, a.loss);
-    launched("loss_kernel");
+    if (a.db) add_rows(DT, sums, sum_rows, a.vocab, alpha * kDScale<DT>, count, a.db, q);
+    q.launch("loss_kernel", loss_kernel, dim3(1), 1024, 0, a.n, a.row_loss, count, a.loss);
 }
 
 void check(const mg_cross_entropy_args& a) {
@@ -273,9 +303,9 @@ void check(const mg_cross_entropy_args& a) {
     need(!grads || (a.db != nullptr) == (a.bias != nullptr), "db goes with a bias");
 }
 
-void cross_entropy(const mg_cross_entropy_args& a, Workspace& w, bool go, cudaStream_t s) {
-    if (a.dtype == MG_PREC_BF16) run<MG_PREC_BF16>(a, w, go, s);
-    else run<MG_PREC_FP16>(a, w, go, s);
+void cross_entropy(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
+    if (a.dtype == MG_PREC_BF16) run<MG_PREC_BF16>(a, w, go, q);
+    else run<MG_PREC_FP16>(a, w, go, q);
 }
 
 }  // namespace
@@ -289,7 +319,8 @@ extern "C" int mg_cross_entropy_workspace(const mg_cross_entropy_args* args, siz
         need(args != nullptr && bytes != nullptr, "args or bytes is null");
         check(*args);
         Workspace w;
-        cross_entropy(*args, w, false, nullptr);
+        Queue q(nullptr);
+        cross_entropy(*args, w, false, q);
         *bytes = w.used();
     });
 }
@@ -301,6 +332,7 @@ extern "C" int mg_cross_entropy(const mg_cross_entropy_args* args, void* workspa
         check(*args);
         OnDevice on(args->device);
         Workspace w(workspace, workspace_bytes);
-        cross_entropy(*args, w, true, static_cast<cudaStream_t>(stream));
+        Queue q(stream);
+        cross_entropy(*args, w, true, q);
     });
 }

@@ -14,7 +14,6 @@
 // over as many warps as its rows deserve, there are no atomics on sums, and
 // the result does not depend on the order in which blocks run.
 #include "ops_common.cuh"
-#include "ptx_sm100.cuh"
 
 #include <algorithm>
 
@@ -61,6 +60,7 @@ __global__ void __launch_bounds__(256) embed_kernel(mg_embed_args a, int64_t chu
     using T = typename E::T;
     using V = typename Bytes<B>::T;
     constexpr int N = B / (int)sizeof(T);
+    griddep_wait();
     const int lane = threadIdx.x & (lanes - 1);
     const int64_t c0 = (int64_t)blockIdx.y * (kPerLane * lanes) + lane;
     for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes; i < a.n;
@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(256) embed_kernel(mg_embed_args a, int64_t chu
 }
 
 template <int DT, int B>
-void embed_with(const mg_embed_args& a, cudaStream_t s) {
+void embed_with(const mg_embed_args& a, Queue& q) {
     const int64_t chunks = a.dim * elem_bytes(DT) / B;
     int lanes = 1;
     while (lanes < 32 && lanes < chunks) lanes *= 2;
@@ -93,19 +93,18 @@ void embed_with(const mg_embed_args& a, cudaStream_t s) {
     const dim3 grid((unsigned)std::min<int64_t>((a.n + rows_per_block - 1) / rows_per_block, 1 << 30),
                     (unsigned)segments);
     need(segments <= 65535, "dim is too large");
-    embed_kernel<DT, B><<<grid, 256, 0, s>>>(a, chunks, lanes);
-    launched("embed_kernel");
+    q.launch("embed_kernel", embed_kernel<DT, B>, grid, 256, 0, a, chunks, lanes);
 }
 
 template <int DT>
-void embed(const mg_embed_args& a, cudaStream_t s) {
+void embed(const mg_embed_args& a, Queue& q) {
     const int e = elem_bytes(DT);
     switch (widest(e, a.dim * e, a.table_row * e, 0, a.table, a.out)) {
-        case 16: return embed_with<DT, 16>(a, s);
-        case 8: return embed_with<DT, 8>(a, s);
-        case 4: return embed_with<DT, 4>(a, s);
+        case 16: return embed_with<DT, 16>(a, q);
+        case 8: return embed_with<DT, 8>(a, q);
+        case 4: return embed_with<DT, 4>(a, q);
         default:
-            if constexpr (DT != MG_PREC_FP32) embed_with<DT, 2>(a, s);
+            if constexpr (DT != MG_PREC_FP32) embed_with<DT, 2>(a, q);
     }
 }
 
@@ -503,14 +502,14 @@ __global__ void __launch_bounds__(256, 3) join_kernel(SumArgs a) {
 }
 
 template <int DT, bool VEC>
-void sum_rows(SumArgs a, cudaStream_t s) {
+void sum_rows(SumArgs a, Queue& q) {
     const int64_t sum_blocks = ((int64_t)a.windows * a.segments + 7) / 8;
     const int64_t zero_blocks = (a.vocab + 255) / 256, blocks = zero_blocks + sum_blocks;
     need(blocks < (int64_t(1) << 31) && a.segments <= 65535, "n times dim is too large");
-    launch_next("sum_kernel", sum_kernel<DT, VEC>, dim3((unsigned)blocks), 256, 0, s, a, zero_blocks);
+    q.launch("sum_kernel", sum_kernel<DT, VEC>, dim3((unsigned)blocks), 256, 0, a, zero_blocks);
     if (a.windows > 1)
-        launch_next("join_kernel", join_kernel<DT, VEC>,
-                    dim3((unsigned)((a.windows + 7) / 8), (unsigned)a.segments), 256, 0, s, a);
+        q.launch("join_kernel", join_kernel<DT, VEC>, dim3((unsigned)((a.windows + 7) / 8), (unsigned)a.segments), 256,
+                 0, a);
 }
 
 void plan_sort(SortArgs& a) {
@@ -523,7 +522,7 @@ void plan_sort(SortArgs& a) {
     a.blocks = (int)((a.n + a.steps * per_step - 1) / (a.steps * per_step));
 }
 
-void sort(SortArgs a, cudaStream_t s) {
+void sort(SortArgs a, Queue& q) {
     const int bins = 1 << a.bits, slices = std::max(1, kSortThreads / (bins / 4));
     const int most = kSortWarps * (4 << kMaxBits);
     check(cudaFuncSetAttribute(rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most),
@@ -531,22 +530,16 @@ void sort(SortArgs a, cudaStream_t s) {
     for (int pass = 0; pass < a.passes; ++pass) {
         a.in = a.pair[pass & 1];
         a.out = a.pair[(pass + 1) & 1];
-        if (pass == 0) {
-            rank_kernel<<<a.blocks, kSortThreads, kSortWarps * bins * 4, s>>>(a, pass);
-            launched("rank_kernel");
-        } else {
-            launch_next("rank_kernel", rank_kernel, dim3(a.blocks), kSortThreads, kSortWarps * bins * 4, s, a, pass);
-        }
-        launch_next("scatter_kernel", scatter_kernel, dim3(a.blocks), kSortThreads, slices * 2 * bins * 4, s, a,
-                    pass);
+        q.launch("rank_kernel", rank_kernel, dim3(a.blocks), kSortThreads, kSortWarps * bins * 4, a, pass);
+        q.launch("scatter_kernel", scatter_kernel, dim3(a.blocks), kSortThreads, slices * 2 * bins * 4, a, pass);
     }
 }
 
 template <int DT>
-void embed_backward(const mg_embed_backward_args& a, Workspace& w, bool go, cudaStream_t s) {
+void embed_backward(const mg_embed_backward_args& a, Workspace& w, bool go, Queue& q) {
     const int e = elem_bytes(DT);
     if (a.n == 0) {
-        if (go) check(cudaMemsetAsync(a.d_table, 0, (size_t)a.vocab * a.dim * e, s), "cudaMemsetAsync");
+        if (go) q.clear(a.d_table, (size_t)a.vocab * a.dim * e);
         return;
     }
     SortArgs sort_args{};
@@ -571,7 +564,7 @@ void embed_backward(const mg_embed_backward_args& a, Workspace& w, bool go, cuda
     sum.tail = w.take<float>((size_t)sum.windows * a.dim * 4);
     if (!go) return;
     w.require();
-    sort(sort_args, s);
+    sort(sort_args, q);
     sum.pair = sort_args.pair[sort_args.passes & 1];
     sum.grad = a.grad;
     sum.grad_row = a.grad_row;
@@ -579,14 +572,14 @@ void embed_backward(const mg_embed_backward_args& a, Workspace& w, bool go, cuda
     sum.vocab = a.vocab;
     sum.scale = a.scale;
     sum.d_table = a.d_table;
-    if (vec) sum_rows<DT, true>(sum, s);
-    else sum_rows<DT, false>(sum, s);
+    if (vec) sum_rows<DT, true>(sum, q);
+    else sum_rows<DT, false>(sum, q);
 }
 
-void embed_backward(const mg_embed_backward_args& a, Workspace& w, bool go, cudaStream_t s) {
-    if (a.dtype == MG_PREC_BF16) embed_backward<MG_PREC_BF16>(a, w, go, s);
-    else if (a.dtype == MG_PREC_FP16) embed_backward<MG_PREC_FP16>(a, w, go, s);
-    else embed_backward<MG_PREC_FP32>(a, w, go, s);
+void embed_backward(const mg_embed_backward_args& a, Workspace& w, bool go, Queue& q) {
+    if (a.dtype == MG_PREC_BF16) embed_backward<MG_PREC_BF16>(a, w, go, q);
+    else if (a.dtype == MG_PREC_FP16) embed_backward<MG_PREC_FP16>(a, w, go, q);
+    else embed_backward<MG_PREC_FP32>(a, w, go, q);
 }
 
 void check_tokens(const void* p, int bytes, int64_t stride, int64_t n) {
@@ -625,10 +618,10 @@ extern "C" int mg_embed(const mg_embed_args* args, void* stream) {
         check_args(*args);
         if (args->n == 0) return;
         OnDevice on(args->device);
-        auto s = static_cast<cudaStream_t>(stream);
-        if (args->dtype == MG_PREC_BF16) embed<MG_PREC_BF16>(*args, s);
-        else if (args->dtype == MG_PREC_FP16) embed<MG_PREC_FP16>(*args, s);
-        else embed<MG_PREC_FP32>(*args, s);
+        Queue q(stream);
+        if (args->dtype == MG_PREC_BF16) embed<MG_PREC_BF16>(*args, q);
+        else if (args->dtype == MG_PREC_FP16) embed<MG_PREC_FP16>(*args, q);
+        else embed<MG_PREC_FP32>(*args, q);
     });
 }
 
@@ -637,7 +630,8 @@ extern "C" int mg_embed_backward_workspace(const mg_embed_backward_args* args, s
         need(args != nullptr && bytes != nullptr, "args or bytes is null");
         check_args(*args);
         Workspace w;
-        embed_backward(*args, w, false, nullptr);
+        Queue q(nullptr);
+        embed_backward(*args, w, false, q);
         *bytes = w.used();
     });
 }
@@ -649,6 +643,7 @@ extern "C" int mg_embed_backward(const mg_embed_backward_args* args, void* works
         check_args(*args);
         OnDevice on(args->device);
         Workspace w(workspace, workspace_bytes);
-        embed_backward(*args, w, true, static_cast<cudaStream_t>(stream));
+        Queue q(stream);
+        embed_backward(*args, w, true, q);
     });
 }

@@ -24,7 +24,6 @@
 // The sums are double-buffered in TMEM: a tile's epilogue overlaps the next
 // tile's products.  Every wait is bounded (ptx_sm100.cuh).
 #include "ops_gemm.cuh"
-#include "ptx_sm100.cuh"
 
 #include <algorithm>
 #include <cmath>
@@ -247,8 +246,9 @@ __device__ __forceinline__ void load_block(const void* base, int64_t row, int64_
                                            uint16_t* stage, float (&v)[32]) {
     const uint16_t* p = static_cast<const uint16_t*>(base);
     __syncwarp();
-    for (int r = 0; r < rows; ++r)
-        if (lane < cols) stage[r * kStagePitch + lane] = p[r * row + lane * col];
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+        if (r < rows && lane < cols) stage[r * kStagePitch + lane] = p[r * row + lane * col];
     __syncwarp();
     const uint32_t* w = reinterpret_cast<const uint32_t*>(stage + lane * kStagePitch);
 #pragma unroll
@@ -268,8 +268,19 @@ __device__ __forceinline__ void store_block(void* base, int64_t row, int rows, i
 #pragma unroll
     for (int i = 0; i < 16; ++i) w[i] = pack2<DT>(v[2 * i], v[2 * i + 1]);
     __syncwarp();
-    for (int r = 0; r < rows; ++r)
-        if (lane < cols) p[r * row + lane] = stage[r * kStagePitch + lane];
+    if ((((uint32_t)row | (uint32_t)cols) & 1) == 0 && (reinterpret_cast<uintptr_t>(p) & 3) == 0) {
+        // two rows at a time, 4 bytes per lane
+        const int c = (lane & 15) * 2;
+#pragma unroll 8
+        for (int r = lane >> 4; r < 32; r += 2)
+            if (r < rows && c < cols)
+                *reinterpret_cast<uint32_t*>(p + r * row + c) =
+                    *reinterpret_cast<const uint32_t*>(stage + r * kStagePitch + c);
+        return;
+    }
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+        if (r < rows && lane < cols) p[r * row + lane] = stage[r * kStagePitch + lane];
 }
 
 __device__ __forceinline__ void activate_all(float (&v)[32], int act) {
@@ -504,6 +515,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    griddep_launch_dependents();
+    griddep_wait();
 
     const UnitWalk walk(a, pair, pairs);
     const int jobs = a.units[1] > 0 ? 2 : 1;
@@ -694,17 +707,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (warp == 1) tmem_dealloc_pair(tmem_base, Cfg::kTmemCols);
 }
 
-// Sums the splits of a product and applies its epilogue.
+// Sums the splits of a product and applies its epilogue; a row per
+// blockIdx.y.
 template <int DT>
-__global__ void __launch_bounds__(256) finish_kernel(const float* part, int splits, int64_t m_pad, int64_t m,
+__global__ void __launch_bounds__(128) finish_kernel(const float* part, int splits, int64_t m_pad, int64_t m,
                                                      int64_t n, int64_t ld32, GemmEpilogue e) {
     using E = Elem<DT>;
     using T = typename E::T;
+    griddep_launch_dependents();
+    griddep_wait();
     const float alpha = e.count ? e.alpha / (float)max(*e.count, 1) : e.alpha;
-    const int64_t total = m * n;
-    for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * 256) {
-        const int64_t i = at / n, c = at % n;
+    const int64_t c = (int64_t)blockIdx.x * 128 + threadIdx.x;
+    if (c >= n) return;
+    for (int64_t i = blockIdx.y; i < m; i += gridDim.y) {
         float v = e.acc32 ? e.acc32[i * e.ld32 + c] : 0.0f;
+#pragma unroll 8
         for (int s = 0; s < splits; ++s) v += part[(s * m_pad + i) * ld32 + c];
         if (e.out32) {
             e.out32[i * e.ld32 + c] = v;
@@ -719,12 +736,23 @@ __global__ void __launch_bounds__(256) finish_kernel(const float* part, int spli
     }
 }
 
-// Copies `rows` lines of `len` 16-bit elements (strides line, step) to lines of ld.
-__global__ void __launch_bounds__(256) pack_kernel(const uint16_t* in, int64_t line, int64_t step, int64_t rows,
+// Copies `lines` lines of `len` 16-bit elements (strides line, step) to lines
+// of ld; a warp per line and 256 columns, eight loads per lane in flight.
+__global__ void __launch_bounds__(256) pack_kernel(const uint16_t* in, int64_t line, int64_t step, int64_t lines,
                                                    int64_t len, int64_t ld, uint16_t* out) {
-    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y)
-        for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < len; c += (int64_t)gridDim.x * 256)
-            out[r * ld + c] = in[r * line + c * step];
+    griddep_launch_dependents();
+    griddep_wait();
+    const int64_t across = (len + 255) / 256, tasks = lines * across;
+    for (int64_t task = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); task < tasks; task += (int64_t)gridDim.x * 8) {
+        const int64_t r = task / across, c = task % across * 256 + (threadIdx.x & 31);
+        uint16_t v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c + 32 * i < len) v[i] = in[r * line + (c + 32 * i) * step];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c + 32 * i < len) out[r * ld + c + 32 * i] = v[i];
+    }
 }
 
 // A tensor map of a dense-enough matrix: `rows` lines of `inner` elements,
@@ -768,24 +796,23 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 int64_t up8(int64_t v) { return (v + 7) / 8 * 8; }
 
 template <int BN, int DT, int EPI>
-void launch_one(const KernelArgs& a, int pairs, cudaStream_t stream) {
+void launch_one(const KernelArgs& a, int pairs, Queue& q) {
     check(cudaFuncSetAttribute(gemm_kernel<BN, DT, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                Config<BN>::kSmem),
           "cudaFuncSetAttribute(gemm_kernel)");
-    gemm_kernel<BN, DT, EPI><<<2 * pairs, kThreads, Config<BN>::kSmem, stream>>>(a);
-    launched("gemm_kernel");
+    q.launch("gemm_kernel", gemm_kernel<BN, DT, EPI>, dim3(2 * pairs), kThreads, Config<BN>::kSmem, a);
 }
 
 template <int EPI>
-void launch(KernelArgs& a, int bn, int dtype, cudaStream_t stream) {
+void launch(KernelArgs& a, int bn, int dtype, Queue& q) {
     a.err = op_status_word();
     const int pairs = (int)std::min<int64_t>(kPairs, (int64_t)a.units[0] + a.units[1]);
     if (bn == 256) {
-        if (dtype == MG_PREC_BF16) launch_one<256, MG_PREC_BF16, EPI>(a, pairs, stream);
-        else launch_one<256, MG_PREC_FP16, EPI>(a, pairs, stream);
+        if (dtype == MG_PREC_BF16) launch_one<256, MG_PREC_BF16, EPI>(a, pairs, q);
+        else launch_one<256, MG_PREC_FP16, EPI>(a, pairs, q);
     } else {
-        if (dtype == MG_PREC_BF16) launch_one<128, MG_PREC_BF16, EPI>(a, pairs, stream);
-        else launch_one<128, MG_PREC_FP16, EPI>(a, pairs, stream);
+        if (dtype == MG_PREC_BF16) launch_one<128, MG_PREC_BF16, EPI>(a, pairs, q);
+        else launch_one<128, MG_PREC_FP16, EPI>(a, pairs, q);
     }
 }
 
@@ -833,7 +860,7 @@ int tile_columns(const Job* jobs, int count) {
 }  // namespace
 
 StagedOperand stage_operand(Workspace& w, bool go, const GemmOperand& op, int64_t rows, int64_t k,
-                            cudaStream_t stream) {
+                            Queue& q) {
     // a dimension of one element has no stride of its own
     const int64_t row = rows == 1 ? up8(std::max(k, op.row)) : op.row, col = k == 1 ? up8(std::max(rows, op.col)) : op.col;
     const int64_t top = int64_t(1) << 38;
@@ -856,15 +883,20 @@ StagedOperand stage_operand(Workspace& w, bool go, const GemmOperand& op, int64_
     s.data = out;
     if (go) {
         w.require();
-        const dim3 grid((unsigned)std::min<int64_t>((len + 255) / 256, 1024), (unsigned)std::min<int64_t>(lines, 65535));
-        pack_kernel<<<grid, 256, 0, stream>>>(static_cast<const uint16_t*>(op.data), s.mn ? op.col : op.row,
-                                              s.mn ? op.row : op.col, lines, len, s.ld, out);
-        launched("pack_kernel");
+        const int64_t tasks = lines * ((len + 255) / 256);
+        q.launch("pack_kernel", pack_kernel, dim3((unsigned)std::min<int64_t>((tasks + 7) / 8, 148 * 8)), 256, 0,
+                 static_cast<const uint16_t*>(op.data), s.mn ? op.col : op.row, s.mn ? op.row : op.col, lines, len,
+                 s.ld, out);
     }
     return s;
 }
 
-void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, cudaStream_t stream) {
+void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, Queue& q) {
+    if (count == 1 && jobs->m <= kSkinnyRows && !jobs->a.mn && !jobs->b.mn && jobs->e.out32 == nullptr &&
+        jobs->e.acc32 == nullptr) {
+        if (go) skinny(dtype, *jobs, q);
+        return;
+    }
     if (count == 2 && jobs[1].k > jobs[0].k) std::swap(jobs[0], jobs[1]);
     const int bn = tile_columns(jobs, count);
     KernelArgs a{};
@@ -909,23 +941,19 @@ void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, cudaStream
         if (e.res != nullptr) encode_blocks(&a.tr, dtype, e.res, j.m, j.n, e.r_row);
     }
     a.head_start = count == 2 ? (int)(len[0] / len[1] + 0.5) : 0;
-    launch<kStore>(a, bn, dtype, stream);
+    launch<kStore>(a, bn, dtype, q);
     for (int i = 0; i < count; ++i)
         if (a.job[i].splits > 1) {
-            const int64_t total = jobs[i].m * jobs[i].n;
-            const unsigned grid = (unsigned)std::min<int64_t>((total + 255) / 256, 148 * 8);
-            const float* part = a.job[i].e.out32;
-            if (dtype == MG_PREC_BF16)
-                finish_kernel<MG_PREC_BF16><<<grid, 256, 0, stream>>>(part, a.job[i].splits, a.job[i].m_pad, jobs[i].m, jobs[i].n,
-                                                                      a.job[i].e.ld32, finish[i]);
-            else
-                finish_kernel<MG_PREC_FP16><<<grid, 256, 0, stream>>>(part, a.job[i].splits, a.job[i].m_pad, jobs[i].m, jobs[i].n,
-                                                                      a.job[i].e.ld32, finish[i]);
-            launched("finish_kernel");
+            const int64_t m = jobs[i].m, n = jobs[i].n;
+            const dim3 grid((unsigned)((n + 127) / 128), (unsigned)std::min<int64_t>(m, 65535));
+            q.launch("finish_kernel",
+                     dtype == MG_PREC_BF16 ? finish_kernel<MG_PREC_BF16> : finish_kernel<MG_PREC_FP16>, grid, 128, 0,
+                     a.job[i].e.out32, a.job[i].splits, a.job[i].m_pad, m, n, a.job[i].e.ld32, finish[i]);
         }
 }
 
 int gemm_softmax_block(int64_t m, int64_t n) {
+    if (m <= kSkinnyRows) return 128;
     SoftmaxJob g;
     g.m = m;
     g.n = n;
@@ -933,7 +961,8 @@ int gemm_softmax_block(int64_t m, int64_t n) {
     return tile_columns(&g, 1) / 2;
 }
 
-void gemm_softmax(int dtype, const SoftmaxJob& g, int block, cudaStream_t stream) {
+void gemm_softmax(int dtype, const SoftmaxJob& g, int block, Queue& q) {
+    if (g.m <= kSkinnyRows && block == 128 && !g.a.mn && !g.b.mn) return skinny_softmax(dtype, g, q);
     const int bn = 2 * block;
     KernelArgs a{};
     lay_out(a.job[0], g, bn);
@@ -941,7 +970,7 @@ void gemm_softmax(int dtype, const SoftmaxJob& g, int block, cudaStream_t stream
     a.units[0] = a.job[0].tiles_m * a.job[0].tiles_n;
     encode_operands(a, 0, dtype, g, bn);
     if (g.e.probs != nullptr) encode_blocks(&a.to[0], dtype, g.e.probs, g.m, g.e.probs_ld, g.e.probs_ld);
-    launch<kSoftmax>(a, bn, dtype, stream);
+    launch<kSoftmax>(a, bn, dtype, q);
 }
 
 }  // namespace ops

@@ -45,6 +45,10 @@ struct GemmJob {
     GemmEpilogue e;
 };
 
+// Products of up to this many rows, both operands K-major, are bound by
+// reading B once: they take a kernel of their own (ops_skinny.cu).
+constexpr int kSkinnyRows = 16;
+
 // Softmax statistics of l = acc + bias instead of a product (the forward
 // half of the cross entropy).  A row's columns are taken in blocks of
 // `block` (gemm_softmax_block()); per block and row
@@ -67,7 +71,10 @@ struct SoftmaxJob {
 };
 int gemm_softmax_block(int64_t m, int64_t n);
 // `block`: gemm_softmax_block of the largest m that shares part's layout.
-void gemm_softmax(int dtype, const SoftmaxJob& job, int block, cudaStream_t stream);
+void gemm_softmax(int dtype, const SoftmaxJob& job, int block, Queue& q);
+
+void skinny(int dtype, const GemmJob& job, Queue& q);
+void skinny_softmax(int dtype, const SoftmaxJob& job, Queue& q);  // blocks of 128 columns
 
 // A number in [0, 1] in 16 bits: 4 bits of exponent and 12 of fraction, no
 // sign (relative error 2^-14 from 2^-14 up, absolute 2^-28 below).  A block's
@@ -88,7 +95,7 @@ __device__ __forceinline__ float prob16_value(uint32_t u) { return __uint_as_flo
 // Gives an operand of `rows` x k in a form the products read: itself where
 // it lies right, else a copy in the workspace (made now if `go`).
 StagedOperand stage_operand(Workspace& w, bool go, const GemmOperand& op, int64_t rows, int64_t k,
-                            cudaStream_t stream);
+                            Queue& q);
 // The same matrix with i and k exchanged.
 inline StagedOperand transposed(StagedOperand s) {
     s.mn = !s.mn;
@@ -96,7 +103,7 @@ inline StagedOperand transposed(StagedOperand s) {
 }
 
 // One or two products in one launch (the one with more k first).
-void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, cudaStream_t stream);
+void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, Queue& q);
 
 // Phi(z), the normal distribution function, and exp(-z^2 / 2): formula
 // 7.1.26 of Abramowitz and Stegun for erf(|z| / sqrt 2), which is within

@@ -40,6 +40,8 @@ __global__ void __launch_bounds__(256)
     const T* dy = static_cast<const T*>(a.grad);
     const T* z = static_cast<const T*>(a.z);
     float sum[V] = {};
+    griddep_launch_dependents();
+    griddep_wait();
     if (c < a.n)
         for (int64_t r = r0 + warp; r < r1; r += 8) {
             alignas(16) T dv[V], zv[V];
@@ -106,11 +108,11 @@ void check(const mg_linear_backward_args& a) {
          "a stride is negative");
 }
 
-void linear(const mg_linear_args& a, Workspace& w, bool go, cudaStream_t s) {
+void linear(const mg_linear_args& a, Workspace& w, bool go, Queue& q) {
     if (a.m == 0) return;
     GemmJob job;
-    job.a = stage_operand(w, go, {a.x, a.x_row, a.x_col}, a.m, a.k, s);
-    job.b = stage_operand(w, go, {a.weight, a.w_row, a.w_col}, a.n, a.k, s);
+    job.a = stage_operand(w, go, {a.x, a.x_row, a.x_col}, a.m, a.k, q);
+    job.b = stage_operand(w, go, {a.weight, a.w_row, a.w_col}, a.n, a.k, q);
     job.m = a.m;
     job.n = a.n;
     job.k = a.k;
@@ -123,16 +125,16 @@ void linear(const mg_linear_args& a, Workspace& w, bool go, cudaStream_t s) {
     job.e.ld = a.n;
     job.e.res_scale = a.residual_scale;
     job.e.act = a.activation;
-    gemm(w, go, a.dtype, &job, 1, s);
+    gemm(w, go, a.dtype, &job, 1, q);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-void linear_backward(const mg_linear_backward_args& a, Workspace& w, bool go, cudaStream_t s) {
+void linear_backward(const mg_linear_backward_args& a, Workspace& w, bool go, Queue& q) {
     if (a.m == 0) {
         if (!go) return;
-        if (a.dw) ops::check(cudaMemsetAsync(a.dw, 0, (size_t)a.n * a.k * 2, s), "cudaMemsetAsync");
-        if (a.db) ops::check(cudaMemsetAsync(a.db, 0, (size_t)a.n * 2, s), "cudaMemsetAsync");
+        if (a.dw) q.clear(a.dw, (size_t)a.n * a.k * 2);
+        if (a.db) q.clear(a.db, (size_t)a.n * 2);
         return;
     }
     const bool has_g = a.activation != MG_ACT_NONE;
@@ -142,8 +144,8 @@ void linear_backward(const mg_linear_backward_args& a, Workspace& w, bool go, cu
         const bool vec = a.n % 8 == 0 && aligned16(a.grad) && a.g_col == 1 && a.g_row % 8 == 0 &&
                          (!has_g || (aligned16(a.z) && a.z_col == 1 && a.z_row % 8 == 0));
         const int64_t across = (a.n + (vec ? 255 : 31)) / (vec ? 256 : 32);
-        // about eight blocks per SM, at least 32 rows each
-        const int64_t want = std::max<int64_t>(1, 148 * 8 / across);
+        // about four blocks per SM, at least 32 rows each
+        const int64_t want = std::max<int64_t>(1, 148 * 4 / across);
         const int rows = (int)std::max<int64_t>(32, (a.m + want - 1) / want);
         const int64_t down = (a.m + rows - 1) / rows;
         float* sums = a.db ? w.take<float>((size_t)down * a.n * 4) : nullptr;
@@ -151,24 +153,22 @@ void linear_backward(const mg_linear_backward_args& a, Workspace& w, bool go, cu
             w.require();
             const dim3 grid((unsigned)across, (unsigned)down);
             const bool bf = a.dtype == MG_PREC_BF16;
-            if (vec && bf) slope_kernel<MG_PREC_BF16, 8><<<grid, 256, 0, s>>>(a, g, ldg, rows, sums);
-            else if (vec) slope_kernel<MG_PREC_FP16, 8><<<grid, 256, 0, s>>>(a, g, ldg, rows, sums);
-            else if (bf) slope_kernel<MG_PREC_BF16, 1><<<grid, 256, 0, s>>>(a, g, ldg, rows, sums);
-            else slope_kernel<MG_PREC_FP16, 1><<<grid, 256, 0, s>>>(a, g, ldg, rows, sums);
-            launched("slope_kernel");
-            if (a.db) add_rows(a.dtype, sums, down, a.n, 1.0f, nullptr, a.db, s);
+            const auto kernel = vec ? (bf ? slope_kernel<MG_PREC_BF16, 8> : slope_kernel<MG_PREC_FP16, 8>)
+                                    : (bf ? slope_kernel<MG_PREC_BF16, 1> : slope_kernel<MG_PREC_FP16, 1>);
+            q.launch("slope_kernel", kernel, grid, 256, 0, a, g, ldg, rows, sums);
+            if (a.db) add_rows(a.dtype, sums, down, a.n, 1.0f, nullptr, a.db, q);
         }
     }
     StagedOperand gs;
     gs.data = g;
     gs.ld = ldg;
-    if (!has_g) gs = stage_operand(w, go, {a.grad, a.g_row, a.g_col}, a.m, a.n, s);
+    if (!has_g) gs = stage_operand(w, go, {a.grad, a.g_row, a.g_col}, a.m, a.n, q);
     GemmJob jobs[2];
     int count = 0;
     if (a.dx) {
         GemmJob& j = jobs[count++];
         j.a = gs;
-        j.b = stage_operand(w, go, {a.weight, a.w_col, a.w_row}, a.k, a.n, s);
+        j.b = stage_operand(w, go, {a.weight, a.w_col, a.w_row}, a.k, a.n, q);
         j.m = a.m;
         j.n = a.k;
         j.k = a.n;
@@ -178,14 +178,14 @@ void linear_backward(const mg_linear_backward_args& a, Workspace& w, bool go, cu
     if (a.dw) {
         GemmJob& j = jobs[count++];
         j.a = transposed(gs);
-        j.b = stage_operand(w, go, {a.x, a.x_col, a.x_row}, a.k, a.m, s);
+        j.b = stage_operand(w, go, {a.x, a.x_col, a.x_row}, a.k, a.m, q);
         j.m = a.n;
         j.n = a.k;
         j.k = a.m;
         j.e.out = a.dw;
         j.e.ld = a.k;
     }
-    if (count > 0) gemm(w, go, a.dtype, jobs, count, s);
+    if (count > 0) gemm(w, go, a.dtype, jobs, count, q);
 }
 
 }  // namespace
@@ -199,7 +199,8 @@ extern "C" int mg_linear_workspace(const mg_linear_args* args, size_t* bytes) {
         need(args != nullptr && bytes != nullptr, "args or bytes is null");
         check(*args);
         Workspace w;
-        linear(*args, w, false, nullptr);
+        Queue q(nullptr);
+        linear(*args, w, false, q);
         *bytes = w.used();
     });
 }
@@ -211,7 +212,8 @@ extern "C" int mg_linear(const mg_linear_args* args, void* workspace, size_t wor
         check(*args);
         OnDevice on(args->device);
         Workspace w(workspace, workspace_bytes);
-        linear(*args, w, true, static_cast<cudaStream_t>(stream));
+        Queue q(stream);
+        linear(*args, w, true, q);
     });
 }
 
@@ -220,7 +222,8 @@ extern "C" int mg_linear_backward_workspace(const mg_linear_backward_args* args,
         need(args != nullptr && bytes != nullptr, "args or bytes is null");
         check(*args);
         Workspace w;
-        linear_backward(*args, w, false, nullptr);
+        Queue q(nullptr);
+        linear_backward(*args, w, false, q);
         *bytes = w.used();
     });
 }
@@ -232,6 +235,7 @@ extern "C" int mg_linear_backward(const mg_linear_backward_args* args, void* wor
         check(*args);
         OnDevice on(args->device);
         Workspace w(workspace, workspace_bytes);
-        linear_backward(*args, w, true, static_cast<cudaStream_t>(stream));
+        Queue q(stream);
+        linear_backward(*args, w, true, q);
     });
 }

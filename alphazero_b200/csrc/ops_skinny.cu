@@ -1,0 +1,206 @@
+// Products of up to 16 rows: y = x W^T with few tokens, where the time is the
+// one read of W.
+//
+// W's rows are the M side of mma.sync.m16n8k16 and the tokens its N side, so
+// no work is padded beyond 8 tokens; the products are far from the limit of
+// even these instructions.  A contraction may run in any order as long as
+// both operands agree, so a lane takes 8 consecutive elements of a row in one
+// 16-byte load and lets them stand for the element pairs that the fragment
+// layout wants from two steps: W goes from memory to the tensor cores through
+// registers alone, with kAhead steps in flight.
+//
+// A warp has 16 rows of W; where W has too few rows to occupy the card, up to
+// eight warps share 16 rows, each with a part of K, and add up in shared
+// memory in a fixed order.  (On CTA pairs, tiles of 256 x BN with 13 rows in
+// use read W at half of the card's bandwidth: the tensor work is 16 times as
+// much.)
+#include "ops_gemm.cuh"
+
+#include <algorithm>
+#include <cmath>
+
+namespace mgb {
+namespace ops {
+namespace {
+
+constexpr int kAhead = 4;  // steps of 32 elements of K in flight
+
+struct SkinnyArgs {
+    const uint16_t* x;  // [m][k], row stride ldx
+    const uint16_t* w;  // [n][k], row stride ldw
+    int64_t ldx, ldw;
+    int m, n, k;
+    int share;   // warps per 16 rows
+    int k_part;  // of K per warp, a multiple of 32
+    GemmEpilogue e;
+    SoftmaxEpilogue s;
+};
+
+// 8 elements of a row from k on, zeros past its end.
+__device__ __forceinline__ uint4 load8(const uint16_t* row, int k, int end) {
+    if (k + 8 <= end) return __ldg(reinterpret_cast<const uint4*>(row + k));
+    uint32_t v[4] = {0, 0, 0, 0};
+    for (int i = 0; k + i < end; ++i) v[i / 2] |= (uint32_t)row[k + i] << (i & 1 ? 16 : 0);
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+template <int DT>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+    if constexpr (DT == MG_PREC_BF16)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// TILES: tokens in eights.  SOFTMAX: statistics of 128 columns per block
+// (share is 1), else the linear layer's epilogue.
+template <int DT, int TILES, bool SOFTMAX>
+__global__ void __launch_bounds__(256) skinny_kernel(SkinnyArgs a) {
+    using E = Elem<DT>;
+    using T = typename E::T;
+    constexpr int kTokens = 8 * TILES;
+    __shared__ float sums[128][kTokens + 1];  // [warp * 16 + row][token]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, t = lane & 3;
+    const int part = warp % a.share, rows = 128 / a.share;
+    const int n0 = blockIdx.x * rows;
+    griddep_launch_dependents();
+    griddep_wait();
+    {
+        const int row = n0 + warp / a.share * 16 + g;
+        const uint16_t* w0 = a.w + (int64_t)min(row, a.n - 1) * a.ldw;
+        const uint16_t* w1 = a.w + (int64_t)min(row + 8, a.n - 1) * a.ldw;
+        const uint16_t* x[TILES];
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) x[i] = a.x + (int64_t)min(8 * i + g, a.m - 1) * a.ldx;
+        const int begin = part * a.k_part, end = min(a.k, begin + a.k_part);
+        float c[TILES][4] = {};
+        for (int k0 = begin; k0 < end; k0 += 32 * kAhead) {
+            uint4 u0[kAhead], u1[kAhead], v[kAhead][TILES];
+#pragma unroll
+            for (int q = 0; q < kAhead; ++q) {
+                const int k = k0 + 32 * q + 8 * t;
+                u0[q] = load8(w0, k, end);
+                u1[q] = load8(w1, k, end);
+#pragma unroll
+                for (int i = 0; i < TILES; ++i) v[q][i] = load8(x[i], k, end);
+            }
+#pragma unroll
+            for (int q = 0; q < kAhead; ++q)
+#pragma unroll
+                for (int i = 0; i < TILES; ++i) {
+                    mma16816<DT>(c[i], u0[q].x, u1[q].x, u0[q].y, u1[q].y, v[q][i].x, v[q][i].y);
+                    mma16816<DT>(c[i], u0[q].z, u1[q].z, u0[q].w, u1[q].w, v[q][i].z, v[q][i].w);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+            sums[warp * 16 + g][8 * i + 2 * t] = c[i][0];
+            sums[warp * 16 + g][8 * i + 2 * t + 1] = c[i][1];
+            sums[warp * 16 + g + 8][8 * i + 2 * t] = c[i][2];
+            sums[warp * 16 + g + 8][8 * i + 2 * t + 1] = c[i][3];
+        }
+    }
+    __syncthreads();
+    if constexpr (SOFTMAX) {
+        const SoftmaxEpilogue& e = a.s;
+        // a warp per token, four columns per lane
+        for (int token = warp; token < a.m; token += 8) {
+            float l[4], top = -INFINITY;
+            const int target = e.target[token];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int col = n0 + lane * 4 + i;
+                l[i] = -INFINITY;
+                if (col < a.n)
+                    l[i] = sums[lane * 4 + i][token] + (e.bias ? E::get(static_cast<const T*>(e.bias)[col]) : 0.0f);
+                top = fmaxf(top, l[i]);
+                if (col == target) e.logit[token] = l[i];
+            }
+#pragma unroll
+            for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+            const float ref = top == -INFINITY ? 0.0f : top;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                l[i] = exp2f((l[i] - ref) * 1.4426950408889634f);
+                sum += l[i];
+            }
+#pragma unroll
+            for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
+            if (lane == 0) e.part[blockIdx.x * e.part_ld + token] = make_float2(top, sum);
+            // probs_ld is a multiple of 8, so four columns are inside or outside together
+            if (e.probs != nullptr && n0 + lane * 4 < e.probs_ld)
+                *reinterpret_cast<uint2*>(e.probs + token * e.probs_ld + n0 + lane * 4) =
+                    make_uint2(prob16x2(l[0], l[1]), prob16x2(l[2], l[3]));
+        }
+    } else {
+        const GemmEpilogue& e = a.e;
+        const float alpha = e.count ? e.alpha / (float)max(*e.count, 1) : e.alpha;
+        for (int i = threadIdx.x; i < rows * a.m; i += 256) {
+            const int r = i % rows, token = i / rows;
+            const int64_t col = n0 + r;
+            if (col >= a.n) continue;
+            float v = 0.0f;
+            for (int s = 0; s < a.share; ++s) v += sums[(r / 16 * a.share + s) * 16 + r % 16][token];
+            v *= alpha;
+            if (e.bias) v += E::get(static_cast<const T*>(e.bias)[col]);
+            if (e.z) static_cast<T*>(e.z)[token * e.ld + col] = E::put(v);
+            v = activate(v, e.act);
+            if (e.res) v += e.res_scale * E::get(static_cast<const T*>(e.res)[token * e.r_row + col * e.r_col]);
+            static_cast<T*>(e.out)[token * e.ld + col] = E::put(v);
+        }
+    }
+}
+
+template <class Job>
+SkinnyArgs lay_out(const Job& j) {
+    SkinnyArgs a{};
+    a.x = static_cast<const uint16_t*>(j.a.data);
+    a.w = static_cast<const uint16_t*>(j.b.data);
+    a.ldx = j.a.ld;
+    a.ldw = j.b.ld;
+    a.m = (int)j.m;
+    a.n = (int)j.n;
+    a.k = (int)j.k;
+    return a;
+}
+
+template <bool SOFTMAX>
+void launch(int dtype, SkinnyArgs& a, Queue& q) {
+    a.k_part = ((a.k + a.share - 1) / a.share + 31) / 32 * 32;
+    const int rows = 128 / a.share;
+    const dim3 grid((unsigned)((a.n + rows - 1) / rows));
+    const bool bf = dtype == MG_PREC_BF16;
+    const auto kernel = a.m <= 8 ? (bf ? skinny_kernel<MG_PREC_BF16, 1, SOFTMAX> : skinny_kernel<MG_PREC_FP16, 1, SOFTMAX>)
+                                 : (bf ? skinny_kernel<MG_PREC_BF16, 2, SOFTMAX> : skinny_kernel<MG_PREC_FP16, 2, SOFTMAX>);
+    q.launch("skinny_kernel", kernel, grid, 256, 0, a);
+}
+
+}  // namespace
+
+void skinny(int dtype, const GemmJob& j, Queue& q) {
+    SkinnyArgs a = lay_out(j);
+    a.e = j.e;
+    // warps enough to fill the card, each with at least one round of loads
+    a.share = 1;
+    while (a.share < 8 && (a.n + 15) / 16 * a.share < 148 * 24 && a.k > a.share * 32 * kAhead) a.share *= 2;
+    launch<false>(dtype, a, q);
+}
+
+void skinny_softmax(int dtype, const SoftmaxJob& j, Queue& q) {
+    SkinnyArgs a = lay_out(j);
+    a.s = j.e;
+    a.share = 1;
+    launch<true>(dtype, a, q);
+}
+
+}  // namespace ops
+}  // namespace mgb
