@@ -54,6 +54,7 @@ CUDA_SOURCES = [
     os.path.join(CSRC, "ops_api.cu"),
     os.path.join(CSRC, "ops_gemm.cu"),
     os.path.join(CSRC, "ops_skinny.cu"),
+    os.path.join(CSRC, "ops_post.cu"),
     os.path.join(CSRC, "ops_embed.cu"),
     os.path.join(CSRC, "ops_linear.cu"),
     os.path.join(CSRC, "ops_cross_entropy.cu"),

@@ -157,10 +157,5 @@ int guarded(F&& body) noexcept {
 // ptx_sm100.cuh from a wait that gave up) on the current device.
 int* op_status_word();
 
-// out[c] = alpha / max(*count, 1) * sum over `rows` rows of sums[r * cols + c],
-// in a fixed order (count may be null: 1).
-void add_rows(int dtype, const float* sums, int64_t rows, int64_t cols, float alpha, const int* count,
-              void* out, Queue& q);
-
 }  // namespace ops
 }  // namespace mgb

@@ -30,13 +30,16 @@ constexpr float kDScale = DT == MG_PREC_FP16 ? 16384.0f : 1.0f;
 
 constexpr int kCountBlocks = 148;
 
-// target[i] (-1: not counted), and their number per block.
-__global__ void __launch_bounds__(1024) target_kernel(mg_cross_entropy_args a, int* target, int* counts) {
+// target[i] (-1: not counted), and their number per block; blocks past
+// `blocks` copy operands.
+__global__ void __launch_bounds__(1024)
+    target_kernel(mg_cross_entropy_args a, int* target, int* counts, int blocks, Packs packs) {
     __shared__ int part[32];
     griddep_launch_dependents();
     griddep_wait();
+    if (blockIdx.x >= blocks) return pack_block(packs, blockIdx.x - blocks);
     int c = 0;
-    for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < a.n; i += (int64_t)gridDim.x * 1024) {
+    for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < a.n; i += (int64_t)blocks * 1024) {
         const int t = (int)index_at(a.targets, a.target_bytes, i * a.target_stride, a.vocab);
         target[i] = t;
         c += t >= 0;
@@ -57,41 +60,90 @@ __device__ __forceinline__ void join(float& m, float& s, float2 p) {
     m = top;
 }
 
-// logsumexp and loss per row; SLICES threads share a row's blocks.  A row of
-// -inf has lse -inf.  counts, if set: their sum goes to count.
-template <int SLICES>
-__global__ void __launch_bounds__(SLICES == 1 ? 128 : 1024)
+// logsumexp and loss per row, and the loss summed per block: a thread per row
+// where a row has few blocks of columns; with many, a warp per row, or where
+// there are few rows too, a block per row (lanes take the blocks in turn).
+// A row of -inf has lse -inf.  counts, if set: their sum goes to count.
+enum Combine : int { kThreadPerRow, kWarpPerRow, kBlockPerRow };
+constexpr int kFewBlocks = 16;
+
+template <Combine HOW>
+__global__ void __launch_bounds__(HOW == kThreadPerRow ? 128 : 1024)
     combine_kernel(int64_t rows, int blocks, const float2* part, int64_t part_ld, const int* target,
-                   const float* logit, float* lse, float* row_loss, const int* counts, int count_blocks, int* count) {
+                   const float* logit, float* lse, float* row_loss, float* loss_part, const int* counts,
+                   int count_blocks, int* count) {
+    constexpr bool FEW = HOW == kThreadPerRow;
+    __shared__ float2 tile[FEW ? 1 : 32][33];
+    __shared__ float losses[FEW ? 128 : 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     griddep_launch_dependents();
     griddep_wait();
-    if (counts != nullptr && blockIdx.x == 0 && threadIdx.x < 32) {
+    if (counts != nullptr && blockIdx.x == 0 && warp == 0) {
         int c = 0;
-        for (int i = threadIdx.x; i < count_blocks; i += 32) c += counts[i];
+        for (int i = lane; i < count_blocks; i += 32) c += counts[i];
         c = __reduce_add_sync(~0u, c);
-        if (threadIdx.x == 0) *count = c;
+        if (lane == 0) *count = c;
     }
-    constexpr int kRows = SLICES == 1 ? 128 : 32;
-    const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x % kRows;
-    const int slice = threadIdx.x / kRows;
+    constexpr int kRows = FEW ? 128 : HOW == kBlockPerRow ? 1 : 32;
+    const int64_t row0 = (int64_t)blockIdx.x * kRows;
+    const int64_t row = row0 + (FEW ? threadIdx.x : HOW == kBlockPerRow ? 0 : warp);
     float m = -INFINITY, s = 0.0f;
-    if (row < rows)
+    const auto join_lanes = [&] {
+        float top = m;
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+        s *= exp2f((m - (top == -INFINITY ? 0.0f : top)) * 1.4426950408889634f);
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) s += __shfl_xor_sync(~0u, s, d);
+        m = top;
+    };
+    if constexpr (FEW) {
+        if (row < rows)
 #pragma unroll 4
-        for (int b = slice; b < blocks; b += SLICES) join(m, s, part[(int64_t)b * part_ld + row]);
-    if constexpr (SLICES > 1) {
-        __shared__ float2 mine[SLICES][33];
-        mine[slice][threadIdx.x % 32] = make_float2(m, s);
+            for (int b = 0; b < blocks; ++b) join(m, s, part[(int64_t)b * part_ld + row]);
+    } else if constexpr (HOW == kBlockPerRow) {
+#pragma unroll 4
+        for (int b = threadIdx.x; b < blocks; b += 1024) join(m, s, part[(int64_t)b * part_ld + row]);
+        join_lanes();
+        tile[0][warp] = make_float2(m, s);
         __syncthreads();
-        if (slice > 0) return;
-        m = -INFINITY;
-        s = 0.0f;
-        for (int i = 0; i < SLICES; ++i) join(m, s, mine[i][threadIdx.x]);
+        m = tile[0][lane].x;
+        s = tile[0][lane].y;
+        join_lanes();
+    } else {
+        // 32 blocks x 32 rows at a time, read along the rows and turned round
+        for (int b0 = 0; b0 < blocks; b0 += 32) {
+            float2 p = make_float2(-INFINITY, 0.0f);
+            if (b0 + warp < blocks && row0 + lane < rows) p = part[(int64_t)(b0 + warp) * part_ld + row0 + lane];
+            tile[warp][lane] = p;
+            __syncthreads();
+            join(m, s, tile[lane][warp]);
+            __syncthreads();
+        }
+        join_lanes();
     }
-    if (row >= rows) return;
-    const float l = s == 0.0f ? -INFINITY : m + logf(s);
-    lse[row] = l;
-    const float at = target[row] < 0 ? 0.0f : logit[row];
-    row_loss[row] = target[row] < 0 ? 0.0f : at == -INFINITY ? INFINITY : l - at;
+    float loss = 0.0f;
+    if (row < rows) {
+        const float l = s == 0.0f ? -INFINITY : m + logf(s);
+        const float at = target[row] < 0 ? 0.0f : logit[row];
+        loss = target[row] < 0 ? 0.0f : at == -INFINITY ? INFINITY : l - at;
+        if (FEW || lane == 0) {  // (a block per row: every warp has the row, and writes the same)
+            lse[row] = l;
+            row_loss[row] = loss;
+        }
+    }
+    if constexpr (HOW == kBlockPerRow) {
+        if (threadIdx.x == 0) loss_part[blockIdx.x] = loss;
+        return;
+    }
+    losses[FEW ? threadIdx.x : warp] = loss;
+    __syncthreads();
+    if (warp > 0) return;
+    loss = 0.0f;
+    for (int i = lane; i < kRows; i += 32) loss += losses[i];
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) loss += __shfl_xor_sync(~0u, loss, d);
+    if (lane == 0) loss_part[blockIdx.x] = loss;
 }
 
 // probs (Prob16, per block of `block` columns) -> d = (softmax - onehot) in
@@ -152,21 +204,6 @@ __global__ void __launch_bounds__(256)
     sums[(int64_t)blockIdx.y * vocab + col] = s;
 }
 
-__global__ void __launch_bounds__(1024) loss_kernel(int64_t n, const float* row_loss, const int* count, float* loss) {
-    __shared__ float part[1024];
-    griddep_wait();
-    float s = 0.0f;
-#pragma unroll 8
-    for (int64_t i = threadIdx.x; i < n; i += 1024) s += row_loss[i];
-    part[threadIdx.x] = s;
-    __syncthreads();
-    for (int w = 512; w > 0; w /= 2) {
-        if (threadIdx.x < w) part[threadIdx.x] += part[threadIdx.x + w];
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) *loss = part[0] / (float)max(*count, 1);
-}
-
 template <int DT>
 void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
     using T = typename Elem<DT>::T;
@@ -183,7 +220,16 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
     const int64_t most = std::max<int64_t>(256, (int64_t)(kPieceBytes / 2) / ld / 256 * 256);
     const int64_t count_pieces = grads ? (a.n + most - 1) / most : 1;
     const int64_t piece = std::min(a.n, ((a.n + count_pieces - 1) / count_pieces + 255) / 256 * 256);
-    const int block = gemm_softmax_block(piece, a.vocab);
+    Packs packs;
+    StagedOperand x = stage_operand(w, packs, {a.x, a.x_row, a.x_col}, a.n, a.dim);
+    const StagedOperand weight = stage_operand(w, packs, {a.weight, a.w_row, a.w_col}, a.vocab, a.dim);
+    SoftmaxJob shape;
+    shape.a = x;
+    shape.b = weight;
+    shape.m = piece;
+    shape.n = a.vocab;
+    shape.k = a.dim;
+    const int block = gemm_softmax_block(shape);
     const int blocks = (int)((a.vocab + block - 1) / block);
 
     int* count = w.take<int>(4);
@@ -202,15 +248,18 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
     const int64_t ld32 = (a.dim + 7) / 8 * 8;
     float* dw32 = grads && count_pieces > 1 ? w.take<float>((size_t)((a.vocab + 255) / 256 * 256) * ld32 * 4) : nullptr;
 
-    StagedOperand x = stage_operand(w, go, {a.x, a.x_row, a.x_col}, a.n, a.dim, q);
-    const StagedOperand weight = stage_operand(w, go, {a.weight, a.w_row, a.w_col}, a.vocab, a.dim, q);
+    const Combine how = blocks <= kFewBlocks ? kThreadPerRow : piece <= 2 * 148 ? kBlockPerRow : kWarpPerRow;
+    const int64_t combine_rows = how == kThreadPerRow ? 128 : how == kBlockPerRow ? 1 : 32;
+    float* loss_part = w.take<float>((size_t)((piece + combine_rows - 1) / combine_rows * count_pieces) * 4);
     if (go) {
         w.require();
-        q.launch("target_kernel", target_kernel, dim3(count_blocks), 1024, 0, a, target, counts);
+        q.launch("target_kernel", target_kernel, dim3(count_blocks + packs.blocks()), 1024, 0, a, target, counts,
+                 count_blocks, packs);
     }
     const float alpha = a.grad_scale / kDScale<DT>;
-    int64_t sum_rows = 0;
+    int64_t sum_rows = 0, losses = 0;
     size_t piece_scratch = 0;
+    Post post;
     for (int64_t row0 = 0; row0 < a.n; row0 += piece) {
         const int64_t rows = std::min(piece, a.n - row0);
         const bool first = row0 == 0, last = row0 + rows == a.n;
@@ -232,14 +281,14 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
             f.e.probs_ld = ld;
             gemm_softmax(DT, f, block, q);
             const int* sum_of = first ? counts : nullptr;
-            if (blocks <= 16)
-                q.launch("combine_kernel", combine_kernel<1>, dim3((unsigned)((rows + 127) / 128)), 128, 0, rows,
-                         blocks, part, piece, target + row0, logit, lse, a.row_loss + row0, sum_of, count_blocks,
-                         count);
-            else
-                q.launch("combine_kernel", combine_kernel<32>, dim3((unsigned)((rows + 31) / 32)), 1024, 0, rows,
-                         blocks, part, piece, target + row0, logit, lse, a.row_loss + row0, sum_of, count_blocks,
-                         count);
+            const int64_t combine_blocks = (rows + combine_rows - 1) / combine_rows;
+            const auto kernel = how == kThreadPerRow  ? combine_kernel<kThreadPerRow>
+                                : how == kBlockPerRow ? combine_kernel<kBlockPerRow>
+                                                      : combine_kernel<kWarpPerRow>;
+            q.launch("combine_kernel", kernel, dim3((unsigned)combine_blocks), how == kThreadPerRow ? 128 : 1024, 0, rows,
+                     blocks, part, piece, target + row0, logit, lse, a.row_loss + row0, loss_part + losses, sum_of,
+                     count_blocks, count);
+            losses += combine_blocks;
         }
         if (!grads) continue;
         const int64_t these = (rows + down_rows - 1) / down_rows;
@@ -276,16 +325,20 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
         jw.e.alpha = alpha;
         jw.e.count = count;
         Workspace again = w;  // every piece's scratch is the same
-        gemm(again, go, DT, jobs, 2, q);
-        if (go) continue;
+        gemm(again, go, DT, jobs, 2, post, q);
+        if (go) {
+            if (!last) post.launch(DT, q);
+            continue;
+        }
         piece_scratch = std::max(piece_scratch, again.used() - w.used());
     }
     if (!go) {
         w.take(piece_scratch);
         return;
     }
-    if (a.db) add_rows(DT, sums, sum_rows, a.vocab, alpha * kDScale<DT>, count, a.db, q);
-    q.launch("loss_kernel", loss_kernel, dim3(1), 1024, 0, a.n, a.row_loss, count, a.loss);
+    if (a.db) post.add = AddRowsTask{sums, sum_rows, a.vocab, alpha * kDScale<DT>, count, a.db};
+    post.loss = LossTask{loss_part, losses, count, a.loss};
+    post.launch(DT, q);
 }
 
 void check(const mg_cross_entropy_args& a) {

@@ -410,9 +410,22 @@ __device__ __forceinline__ bool epilogue(const KernelArgs& a, int job, const Epi
     return true;
 }
 
-// The same columns and rows as softmax statistics.  A thread has its row's
-// block to itself, so the maximum and the sum need no exchange; the sums are
-// read from TMEM twice rather than held in BN / 2 registers.
+// As tmem_ld_32cols into floats.
+__device__ __forceinline__ void tmem_ld_32cols_to(uint32_t taddr, float* v) {
+    uint32_t r[32];
+    tmem_ld_32cols(taddr, r);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+// No use of v moves above this point (it is loaded asynchronously until the
+// wait before).
+__device__ __forceinline__ void pin(float (&v)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]));
+}
+
+// Softmax statistics of the same columns and rows.  A thread has its row's
+// block to itself, in registers, so the maximum and the sum need no exchange.
 template <int BN, int DT, class Release>
 __device__ __forceinline__ void softmax_epilogue(const KernelArgs& a, const SoftmaxEpilogue& e, int m, int n,
                                                  const Tile& t, int m0, int c0, int target, uint32_t taddr,
@@ -425,37 +438,35 @@ __device__ __forceinline__ void softmax_epilogue(const KernelArgs& a, const Soft
         return;
     }
     target -= first;
+    constexpr int W = BN / 2;
+    float l[W];
+#pragma unroll
+    for (int c = 0; c < W; c += 32)
+        if (c < width) tmem_ld_32cols_to(taddr + c, l + c);
+    tmem_ld_wait();
+    release();
     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, logit = 0.0f;
-#pragma unroll 1
-    for (int c = 0; c < width; c += 32) {
-        uint32_t r[32];
-        tmem_ld_32cols(taddr + c, r);
-        tmem_ld_wait();
-        float l[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) l[i] = __uint_as_float(r[i]);
-        add_bias<DT>(l, 1.0f, sbias + c);  // -inf past the last column
+    for (int c = 0; c < W; c += 32) {
+        if (c >= width) break;
+        float(&v)[32] = *reinterpret_cast<float(*)[32]>(l + c);
+        pin(v);
+        add_bias<DT>(v, 1.0f, sbias + c);  // -inf past the last column
 #pragma unroll
-        for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], l[i]);
+        for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], v[i]);
         if (__any_sync(~0u, target >= c && target < c + 32)) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-                if (target == c + i) logit = l[i];
+                if (target == c + i) logit = v[i];
         }
     }
     const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
     const float ref = most == -INFINITY ? 0.0f : most;
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1
-    for (int c = 0; c < width; c += 32) {
-        uint32_t r[32];
-        tmem_ld_32cols(taddr + c, r);
-        tmem_ld_wait();
-        if (c + 32 >= width) release();
-        float v[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-        add_bias<DT>(v, 1.0f, sbias + c);
+    for (int c = 0; c < W; c += 32) {
+        if (c >= width) break;
+        float(&v)[32] = *reinterpret_cast<float(*)[32]>(l + c);
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
             // the difference first: exact near the maximum, and in range for any finite logits
@@ -707,54 +718,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (warp == 1) tmem_dealloc_pair(tmem_base, Cfg::kTmemCols);
 }
 
-// Sums the splits of a product and applies its epilogue; a row per
-// blockIdx.y.
-template <int DT>
-__global__ void __launch_bounds__(128) finish_kernel(const float* part, int splits, int64_t m_pad, int64_t m,
-                                                     int64_t n, int64_t ld32, GemmEpilogue e) {
-    using E = Elem<DT>;
-    using T = typename E::T;
-    griddep_launch_dependents();
-    griddep_wait();
-    const float alpha = e.count ? e.alpha / (float)max(*e.count, 1) : e.alpha;
-    const int64_t c = (int64_t)blockIdx.x * 128 + threadIdx.x;
-    if (c >= n) return;
-    for (int64_t i = blockIdx.y; i < m; i += gridDim.y) {
-        float v = e.acc32 ? e.acc32[i * e.ld32 + c] : 0.0f;
-#pragma unroll 8
-        for (int s = 0; s < splits; ++s) v += part[(s * m_pad + i) * ld32 + c];
-        if (e.out32) {
-            e.out32[i * e.ld32 + c] = v;
-            continue;
-        }
-        v *= alpha;
-        if (e.bias) v += E::get(static_cast<const T*>(e.bias)[c]);
-        if (e.z) static_cast<T*>(e.z)[i * e.ld + c] = E::put(v);
-        v = activate(v, e.act);
-        if (e.res) v += e.res_scale * E::get(static_cast<const T*>(e.res)[i * e.r_row + c * e.r_col]);
-        static_cast<T*>(e.out)[i * e.ld + c] = E::put(v);
-    }
-}
-
-// Copies `lines` lines of `len` 16-bit elements (strides line, step) to lines
-// of ld; a warp per line and 256 columns, eight loads per lane in flight.
-__global__ void __launch_bounds__(256) pack_kernel(const uint16_t* in, int64_t line, int64_t step, int64_t lines,
-                                                   int64_t len, int64_t ld, uint16_t* out) {
-    griddep_launch_dependents();
-    griddep_wait();
-    const int64_t across = (len + 255) / 256, tasks = lines * across;
-    for (int64_t task = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); task < tasks; task += (int64_t)gridDim.x * 8) {
-        const int64_t r = task / across, c = task % across * 256 + (threadIdx.x & 31);
-        uint16_t v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (c + 32 * i < len) v[i] = in[r * line + (c + 32 * i) * step];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (c + 32 * i < len) out[r * ld + c + 32 * i] = v[i];
-    }
-}
-
 // A tensor map of a dense-enough matrix: `rows` lines of `inner` elements,
 // `ld` apart, in boxes of box_rows x box_inner.
 void encode(CUtensorMap* map, CUtensorMapDataType type, int elem, const void* base, int64_t inner, int64_t rows,
@@ -859,10 +822,10 @@ int tile_columns(const Job* jobs, int count) {
 
 }  // namespace
 
-StagedOperand stage_operand(Workspace& w, bool go, const GemmOperand& op, int64_t rows, int64_t k,
-                            Queue& q) {
+StagedOperand stage_operand(Workspace& w, Packs& packs, const GemmOperand& op, int64_t rows, int64_t k) {
     // a dimension of one element has no stride of its own
-    const int64_t row = rows == 1 ? up8(std::max(k, op.row)) : op.row, col = k == 1 ? up8(std::max(rows, op.col)) : op.col;
+    const int64_t row = rows == 1 ? up8(std::max(k, op.row)) : op.row;
+    const int64_t col = k == 1 ? up8(std::max(rows, op.col)) : op.col;
     const int64_t top = int64_t(1) << 38;
     StagedOperand s;
     s.data = op.data;
@@ -877,21 +840,20 @@ StagedOperand stage_operand(Workspace& w, bool go, const GemmOperand& op, int64_
     }
     // copied along the way it lies, so that reads and writes are both in order
     s.mn = op.row == 1 && op.col != 1;
-    const int64_t lines = s.mn ? k : rows, len = s.mn ? rows : k;
-    s.ld = up8(len);
-    uint16_t* out = w.take<uint16_t>((size_t)lines * s.ld * 2);
-    s.data = out;
-    if (go) {
-        w.require();
-        const int64_t tasks = lines * ((len + 255) / 256);
-        q.launch("pack_kernel", pack_kernel, dim3((unsigned)std::min<int64_t>((tasks + 7) / 8, 148 * 8)), 256, 0,
-                 static_cast<const uint16_t*>(op.data), s.mn ? op.col : op.row, s.mn ? op.row : op.col, lines, len,
-                 s.ld, out);
-    }
+    PackTask& t = packs.task[packs.count++];
+    t.lines = s.mn ? k : rows;
+    t.len = s.mn ? rows : k;
+    t.line = s.mn ? op.col : op.row;
+    t.step = s.mn ? op.row : op.col;
+    t.ld = s.ld = up8(t.len);
+    t.in = static_cast<const uint16_t*>(op.data);
+    t.out = w.take<uint16_t>((size_t)t.lines * t.ld * 2);
+    t.blocks = (int)std::min<int64_t>((t.lines * ((t.len + 255) / 256) + 7) / 8, 148 * 6);
+    s.data = t.out;
     return s;
 }
 
-void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, Queue& q) {
+void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, Post& post, Queue& q) {
     if (count == 1 && jobs->m <= kSkinnyRows && !jobs->a.mn && !jobs->b.mn && jobs->e.out32 == nullptr &&
         jobs->e.acc32 == nullptr) {
         if (go) skinny(dtype, *jobs, q);
@@ -943,26 +905,19 @@ void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, Queue& q) 
     a.head_start = count == 2 ? (int)(len[0] / len[1] + 0.5) : 0;
     launch<kStore>(a, bn, dtype, q);
     for (int i = 0; i < count; ++i)
-        if (a.job[i].splits > 1) {
-            const int64_t m = jobs[i].m, n = jobs[i].n;
-            const dim3 grid((unsigned)((n + 127) / 128), (unsigned)std::min<int64_t>(m, 65535));
-            q.launch("finish_kernel",
-                     dtype == MG_PREC_BF16 ? finish_kernel<MG_PREC_BF16> : finish_kernel<MG_PREC_FP16>, grid, 128, 0,
-                     a.job[i].e.out32, a.job[i].splits, a.job[i].m_pad, m, n, a.job[i].e.ld32, finish[i]);
-        }
+        if (a.job[i].splits > 1)
+            post.finish[post.finishes++] = FinishTask{a.job[i].e.out32,  a.job[i].splits, a.job[i].m_pad, jobs[i].m,
+                                                      jobs[i].n,         a.job[i].e.ld32, finish[i],      0};
 }
 
-int gemm_softmax_block(int64_t m, int64_t n) {
-    if (m <= kSkinnyRows) return 128;
-    SoftmaxJob g;
-    g.m = m;
-    g.n = n;
-    g.k = 1;
-    return tile_columns(&g, 1) / 2;
-}
+namespace {
+bool is_skinny(const SoftmaxJob& g) { return g.m <= kSkinnyRows && !g.a.mn && !g.b.mn; }
+}  // namespace
+
+int gemm_softmax_block(const SoftmaxJob& g) { return is_skinny(g) ? skinny_block(g.k) : tile_columns(&g, 1) / 2; }
 
 void gemm_softmax(int dtype, const SoftmaxJob& g, int block, Queue& q) {
-    if (g.m <= kSkinnyRows && block == 128 && !g.a.mn && !g.b.mn) return skinny_softmax(dtype, g, q);
+    if (is_skinny(g) && block == skinny_block(g.k)) return skinny_softmax(dtype, g, block, q);
     const int bn = 2 * block;
     KernelArgs a{};
     lay_out(a.job[0], g, bn);

@@ -69,12 +69,13 @@ struct SoftmaxJob {
     int64_t m = 0, n = 0, k = 0;
     SoftmaxEpilogue e;
 };
-int gemm_softmax_block(int64_t m, int64_t n);
-// `block`: gemm_softmax_block of the largest m that shares part's layout.
+int gemm_softmax_block(const SoftmaxJob& job);
+// `block`: gemm_softmax_block of the largest job that shares part's layout.
 void gemm_softmax(int dtype, const SoftmaxJob& job, int block, Queue& q);
 
 void skinny(int dtype, const GemmJob& job, Queue& q);
-void skinny_softmax(int dtype, const SoftmaxJob& job, Queue& q);  // blocks of 128 columns
+int skinny_block(int64_t k);  // columns per block of the statistics
+void skinny_softmax(int dtype, const SoftmaxJob& job, int block, Queue& q);
 
 // A number in [0, 1] in 16 bits: 4 bits of exponent and 12 of fraction, no
 // sign (relative error 2^-14 from 2^-14 up, absolute 2^-28 below).  A block's
@@ -92,18 +93,91 @@ __device__ __forceinline__ uint32_t prob16x2(float low, float high) {
 }
 __device__ __forceinline__ float prob16_value(uint32_t u) { return __uint_as_float(u << 11) * 0x1p112f; }
 
+// Copies of operands that do not lie right, made by blocks of the kernel that
+// comes first in a call (a launch of their own would cost as much as the
+// copy).  Lines of `len` elements (strides line, step) become lines of ld.
+struct PackTask {
+    const uint16_t* in;
+    uint16_t* out;
+    int64_t line, step, lines, len, ld;
+    int blocks;
+};
+struct Packs {
+    PackTask task[3];
+    int count = 0;
+    int blocks() const {
+        int n = 0;
+        for (int i = 0; i < count; ++i) n += task[i].blocks;
+        return n;
+    }
+    void launch(Queue& q) const;  // on their own, if there are any
+};
+
+// The share of block `block` (0 .. blocks() - 1): a warp per line and 256
+// columns, eight loads per lane in flight.
+__device__ __forceinline__ void pack_block(const Packs& packs, int block) {
+    int i = 0;
+    while (block >= packs.task[i].blocks) block -= packs.task[i++].blocks;
+    const PackTask& t = packs.task[i];
+    const int warps = blockDim.x >> 5;
+    const int64_t across = (t.len + 255) / 256, tasks = t.lines * across;
+    for (int64_t at = (int64_t)block * warps + (threadIdx.x >> 5); at < tasks; at += (int64_t)t.blocks * warps) {
+        const int64_t r = at / across, c = at % across * 256 + (threadIdx.x & 31);
+        const uint16_t* in = t.in + r * t.line;
+        uint16_t* out = t.out + r * t.ld;
+        uint16_t v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (c + 32 * k < t.len) v[k] = in[(c + 32 * k) * t.step];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (c + 32 * k < t.len) out[c + 32 * k] = v[k];
+    }
+}
+
+// What is left to do after the products of a call, in one launch: products
+// whose K was split are summed and given their epilogue, partial column sums
+// are added up, and the cross entropy's loss is.
+struct FinishTask {
+    const float* part;
+    int splits;
+    int64_t m_pad, m, n, ld32;
+    GemmEpilogue e;
+    int64_t blocks;
+};
+struct AddRowsTask {  // out[c] = alpha / max(*count, 1) * sum of `rows` rows of sums, in a fixed order
+    const float* sums;
+    int64_t rows, cols;
+    float alpha;
+    const int* count;
+    void* out;
+};
+struct LossTask {  // loss = sum of part[0 .. n) / max(*count, 1)
+    const float* part;
+    int64_t n;
+    const int* count;
+    float* loss;
+};
+struct Post {
+    FinishTask finish[2];
+    int finishes = 0;
+    AddRowsTask add{};   // out set: to do
+    LossTask loss{};     // loss set: to do
+    void launch(int dtype, Queue& q);  // if there is anything, which is then done
+};
+
 // Gives an operand of `rows` x k in a form the products read: itself where
-// it lies right, else a copy in the workspace (made now if `go`).
-StagedOperand stage_operand(Workspace& w, bool go, const GemmOperand& op, int64_t rows, int64_t k,
-                            Queue& q);
+// it lies right, else a copy in the workspace, to be made by `packs`.
+StagedOperand stage_operand(Workspace& w, Packs& packs, const GemmOperand& op, int64_t rows, int64_t k);
 // The same matrix with i and k exchanged.
 inline StagedOperand transposed(StagedOperand s) {
     s.mn = !s.mn;
     return s;
 }
 
-// One or two products in one launch (the one with more k first).
-void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, Queue& q);
+// One or two products in one launch (the one with more k first); `post` gets
+// what then remains to be done.
+void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, Post& post, Queue& q);
 
 // Phi(z), the normal distribution function, and exp(-z^2 / 2): formula
 // 7.1.26 of Abramowitz and Stegun for erf(|z| / sqrt 2), which is within

@@ -27,22 +27,27 @@ __device__ __forceinline__ float slope(float z, int act) {
 // g = grad * act'(z) (if g is set) and, per block of rows, the column sums of
 // grad * act'(z) before their rounding.  One pass; a thread has V adjacent
 // columns (V = 8: 16-byte accesses) of every eighth row of its block, the
-// eight sums of a column meet in shared memory.
+// eight sums of a column meet in shared memory.  Blocks past across * down
+// copy operands.
 template <int DT, int V>
 __global__ void __launch_bounds__(256)
-    slope_kernel(mg_linear_backward_args a, uint16_t* g, int64_t ldg, int rows_per_block, float* sums) {
+    slope_kernel(mg_linear_backward_args a, uint16_t* g, int64_t ldg, int rows_per_block, float* sums, int64_t across,
+                 int64_t down, Packs packs) {
     using E = Elem<DT>;
     using T = typename E::T;
     __shared__ float part[8][32 * V];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t c = (int64_t)blockIdx.x * (32 * V) + lane * V;
-    const int64_t r0 = (int64_t)blockIdx.y * rows_per_block, r1 = min(a.m, r0 + rows_per_block);
+    griddep_launch_dependents();
+    griddep_wait();
+    if (blockIdx.x >= across * down) return pack_block(packs, (int)(blockIdx.x - across * down));
+    const int64_t bx = blockIdx.x % across, by = blockIdx.x / across;
+    const int64_t c = bx * (32 * V) + lane * V;
+    const int64_t r0 = by * rows_per_block, r1 = min(a.m, r0 + rows_per_block);
     const T* dy = static_cast<const T*>(a.grad);
     const T* z = static_cast<const T*>(a.z);
     float sum[V] = {};
-    griddep_launch_dependents();
-    griddep_wait();
     if (c < a.n)
+#pragma unroll 2
         for (int64_t r = r0 + warp; r < r1; r += 8) {
             alignas(16) T dv[V], zv[V];
             if constexpr (V == 8) {
@@ -71,12 +76,12 @@ __global__ void __launch_bounds__(256)
     for (int i = 0; i < V; ++i) part[warp][lane * V + i] = sum[i];
     __syncthreads();
     for (int i = threadIdx.x; i < 32 * V; i += 256) {
-        const int64_t col = (int64_t)blockIdx.x * (32 * V) + i;
+        const int64_t col = bx * (32 * V) + i;
         if (col >= a.n) continue;
         float s = 0.0f;
 #pragma unroll
         for (int w = 0; w < 8; ++w) s += part[w][i];
-        sums[(int64_t)blockIdx.y * a.n + col] = s;
+        sums[by * a.n + col] = s;
     }
 }
 
@@ -110,9 +115,10 @@ void check(const mg_linear_backward_args& a) {
 
 void linear(const mg_linear_args& a, Workspace& w, bool go, Queue& q) {
     if (a.m == 0) return;
+    Packs packs;
     GemmJob job;
-    job.a = stage_operand(w, go, {a.x, a.x_row, a.x_col}, a.m, a.k, q);
-    job.b = stage_operand(w, go, {a.weight, a.w_row, a.w_col}, a.n, a.k, q);
+    job.a = stage_operand(w, packs, {a.x, a.x_row, a.x_col}, a.m, a.k);
+    job.b = stage_operand(w, packs, {a.weight, a.w_row, a.w_col}, a.n, a.k);
     job.m = a.m;
     job.n = a.n;
     job.k = a.k;
@@ -125,7 +131,13 @@ void linear(const mg_linear_args& a, Workspace& w, bool go, Queue& q) {
     job.e.ld = a.n;
     job.e.res_scale = a.residual_scale;
     job.e.act = a.activation;
-    gemm(w, go, a.dtype, &job, 1, q);
+    Post post;
+    if (go) {
+        w.require();
+        packs.launch(q);
+    }
+    gemm(w, go, a.dtype, &job, 1, post, q);
+    if (go) post.launch(a.dtype, q);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -137,9 +149,37 @@ void linear_backward(const mg_linear_backward_args& a, Workspace& w, bool go, Qu
         if (a.db) q.clear(a.db, (size_t)a.n * 2);
         return;
     }
+    Packs packs;
+    Post post;
+    GemmJob jobs[2];
+    int count = 0;
     const bool has_g = a.activation != MG_ACT_NONE;
     const int64_t ldg = (a.n + 7) / 8 * 8;
     uint16_t* g = has_g ? w.take<uint16_t>((size_t)a.m * ldg * 2) : nullptr;
+    StagedOperand gs;
+    gs.data = g;
+    gs.ld = ldg;
+    if (!has_g && (a.dx || a.dw)) gs = stage_operand(w, packs, {a.grad, a.g_row, a.g_col}, a.m, a.n);
+    if (a.dx) {
+        GemmJob& j = jobs[count++];
+        j.a = gs;
+        j.b = stage_operand(w, packs, {a.weight, a.w_col, a.w_row}, a.k, a.n);
+        j.m = a.m;
+        j.n = a.k;
+        j.k = a.n;
+        j.e.out = a.dx;
+        j.e.ld = a.k;
+    }
+    if (a.dw) {
+        GemmJob& j = jobs[count++];
+        j.a = transposed(gs);
+        j.b = stage_operand(w, packs, {a.x, a.x_col, a.x_row}, a.k, a.m);
+        j.m = a.n;
+        j.n = a.k;
+        j.k = a.m;
+        j.e.out = a.dw;
+        j.e.ld = a.k;
+    }
     if (a.db || has_g) {
         const bool vec = a.n % 8 == 0 && aligned16(a.grad) && a.g_col == 1 && a.g_row % 8 == 0 &&
                          (!has_g || (aligned16(a.z) && a.z_col == 1 && a.z_row % 8 == 0));
@@ -151,41 +191,21 @@ void linear_backward(const mg_linear_backward_args& a, Workspace& w, bool go, Qu
         float* sums = a.db ? w.take<float>((size_t)down * a.n * 4) : nullptr;
         if (go) {
             w.require();
-            const dim3 grid((unsigned)across, (unsigned)down);
+            const int64_t blocks = across * down + packs.blocks();
+            need(blocks < (int64_t(1) << 31), "too many blocks");
             const bool bf = a.dtype == MG_PREC_BF16;
             const auto kernel = vec ? (bf ? slope_kernel<MG_PREC_BF16, 8> : slope_kernel<MG_PREC_FP16, 8>)
                                     : (bf ? slope_kernel<MG_PREC_BF16, 1> : slope_kernel<MG_PREC_FP16, 1>);
-            q.launch("slope_kernel", kernel, grid, 256, 0, a, g, ldg, rows, sums);
-            if (a.db) add_rows(a.dtype, sums, down, a.n, 1.0f, nullptr, a.db, q);
+            q.launch("slope_kernel", kernel, dim3((unsigned)blocks), 256, 0, a, g, ldg, rows, sums, across, down,
+                     packs);
+            if (a.db) post.add = AddRowsTask{sums, down, a.n, 1.0f, nullptr, a.db};
         }
+    } else if (go) {
+        w.require();
+        packs.launch(q);
     }
-    StagedOperand gs;
-    gs.data = g;
-    gs.ld = ldg;
-    if (!has_g) gs = stage_operand(w, go, {a.grad, a.g_row, a.g_col}, a.m, a.n, q);
-    GemmJob jobs[2];
-    int count = 0;
-    if (a.dx) {
-        GemmJob& j = jobs[count++];
-        j.a = gs;
-        j.b = stage_operand(w, go, {a.weight, a.w_col, a.w_row}, a.k, a.n, q);
-        j.m = a.m;
-        j.n = a.k;
-        j.k = a.n;
-        j.e.out = a.dx;
-        j.e.ld = a.k;
-    }
-    if (a.dw) {
-        GemmJob& j = jobs[count++];
-        j.a = transposed(gs);
-        j.b = stage_operand(w, go, {a.x, a.x_col, a.x_row}, a.k, a.m, q);
-        j.m = a.n;
-        j.n = a.k;
-        j.k = a.m;
-        j.e.out = a.dw;
-        j.e.ld = a.k;
-    }
-    if (count > 0) gemm(w, go, a.dtype, jobs, count, q);
+    if (count > 0) gemm(w, go, a.dtype, jobs, count, post, q);
+    if (go) post.launch(a.dtype, q);
 }
 
 }  // namespace

@@ -7,12 +7,16 @@
 // both operands agree, so a lane takes 8 consecutive elements of a row in one
 // 16-byte load and lets them stand for the element pairs that the fragment
 // layout wants from two steps: W goes from memory to the tensor cores through
-// registers alone, with kAhead steps in flight.
+// registers alone, kAhead steps at a time.  (What bounds it besides memory is
+// the issue of instructions, about ten for a KB of W here.  A deeper queue
+// through shared memory by cp.async, with blocks that go on to further rows
+// without draining it, took 73 us for 13 tokens and 65536 rows of 2048 where
+// this takes 56; 45 for 8 tokens, 91% of the copy rate.)
 //
-// A warp has 16 rows of W; where W has too few rows to occupy the card, up to
-// eight warps share 16 rows, each with a part of K, and add up in shared
-// memory in a fixed order.  (On CTA pairs, tiles of 256 x BN with 13 rows in
-// use read W at half of the card's bandwidth: the tensor work is 16 times as
+// A warp has 16 rows of W; up to eight warps share 16 rows, each with a part
+// of K, and add up in shared memory in a fixed order: short blocks, so that
+// the card is full from the first wave to the last.  (On CTA pairs, tiles of
+// 256 x BN with 13 rows in use take 75 us: the tensor work is 16 times as
 // much.)
 #include "ops_gemm.cuh"
 
@@ -23,7 +27,6 @@ namespace mgb {
 namespace ops {
 namespace {
 
-constexpr int kAhead = 4;  // steps of 32 elements of K in flight
 
 struct SkinnyArgs {
     const uint16_t* x;  // [m][k], row stride ldx
@@ -38,9 +41,12 @@ struct SkinnyArgs {
 
 // 8 elements of a row from k on, zeros past its end.
 __device__ __forceinline__ uint4 load8(const uint16_t* row, int k, int end) {
+    if (k >= end) return make_uint4(0, 0, 0, 0);
     if (k + 8 <= end) return __ldg(reinterpret_cast<const uint4*>(row + k));
     uint32_t v[4] = {0, 0, 0, 0};
-    for (int i = 0; k + i < end; ++i) v[i / 2] |= (uint32_t)row[k + i] << (i & 1 ? 16 : 0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (k + i < end) v[i / 2] |= (uint32_t)row[k + i] << (i & 1 ? 16 : 0);
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
@@ -59,88 +65,50 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// TILES: tokens in eights.  SOFTMAX: statistics of 128 columns per block
-// (share is 1), else the linear layer's epilogue.
-template <int DT, int TILES, bool SOFTMAX>
-__global__ void __launch_bounds__(256) skinny_kernel(SkinnyArgs a) {
+// The epilogue of W's rows [n0, n0 + rows), whose parts are in `sums`.
+template <int DT, int TOKENS, bool SOFTMAX>
+__device__ __forceinline__ void finish(const SkinnyArgs& a, const float (&sums)[128][TOKENS + 1], int n0, int rows,
+                                       int group) {
     using E = Elem<DT>;
     using T = typename E::T;
-    constexpr int kTokens = 8 * TILES;
-    __shared__ float sums[128][kTokens + 1];  // [warp * 16 + row][token]
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int g = lane >> 2, t = lane & 3;
-    const int part = warp % a.share, rows = 128 / a.share;
-    const int n0 = blockIdx.x * rows;
-    griddep_launch_dependents();
-    griddep_wait();
-    {
-        const int row = n0 + warp / a.share * 16 + g;
-        const uint16_t* w0 = a.w + (int64_t)min(row, a.n - 1) * a.ldw;
-        const uint16_t* w1 = a.w + (int64_t)min(row + 8, a.n - 1) * a.ldw;
-        const uint16_t* x[TILES];
-#pragma unroll
-        for (int i = 0; i < TILES; ++i) x[i] = a.x + (int64_t)min(8 * i + g, a.m - 1) * a.ldx;
-        const int begin = part * a.k_part, end = min(a.k, begin + a.k_part);
-        float c[TILES][4] = {};
-        for (int k0 = begin; k0 < end; k0 += 32 * kAhead) {
-            uint4 u0[kAhead], u1[kAhead], v[kAhead][TILES];
-#pragma unroll
-            for (int q = 0; q < kAhead; ++q) {
-                const int k = k0 + 32 * q + 8 * t;
-                u0[q] = load8(w0, k, end);
-                u1[q] = load8(w1, k, end);
-#pragma unroll
-                for (int i = 0; i < TILES; ++i) v[q][i] = load8(x[i], k, end);
-            }
-#pragma unroll
-            for (int q = 0; q < kAhead; ++q)
-#pragma unroll
-                for (int i = 0; i < TILES; ++i) {
-                    mma16816<DT>(c[i], u0[q].x, u1[q].x, u0[q].y, u1[q].y, v[q][i].x, v[q][i].y);
-                    mma16816<DT>(c[i], u0[q].z, u1[q].z, u0[q].w, u1[q].w, v[q][i].z, v[q][i].w);
-                }
-        }
-#pragma unroll
-        for (int i = 0; i < TILES; ++i) {
-            sums[warp * 16 + g][8 * i + 2 * t] = c[i][0];
-            sums[warp * 16 + g][8 * i + 2 * t + 1] = c[i][1];
-            sums[warp * 16 + g + 8][8 * i + 2 * t] = c[i][2];
-            sums[warp * 16 + g + 8][8 * i + 2 * t + 1] = c[i][3];
-        }
-    }
-    __syncthreads();
+    const auto total = [&](int r, int token) {  // of row r of the block
+        float v = 0.0f;
+        for (int p = 0; p < a.share; ++p) v += sums[(r / 16 * a.share + p) * 16 + r % 16][token];
+        return v;
+    };
     if constexpr (SOFTMAX) {
         const SoftmaxEpilogue& e = a.s;
-        // a warp per token, four columns per lane
-        for (int token = warp; token < a.m; token += 8) {
-            float l[4], top = -INFINITY;
-            const int target = e.target[token];
+        // 256 / TOKENS lanes per token, each with every so many-th column
+        constexpr int kLanes = 256 / TOKENS, kEach = 128 / kLanes;
+        const int token = threadIdx.x / kLanes, first = threadIdx.x % kLanes;
+        const int target = token < a.m ? e.target[token] : -1;
+        float l[kEach], top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int col = n0 + lane * 4 + i;
-                l[i] = -INFINITY;
-                if (col < a.n)
-                    l[i] = sums[lane * 4 + i][token] + (e.bias ? E::get(static_cast<const T*>(e.bias)[col]) : 0.0f);
-                top = fmaxf(top, l[i]);
+        for (int i = 0; i < kEach; ++i) {
+            const int r = first + kLanes * i, col = n0 + r;
+            l[i] = -INFINITY;
+            if (r < rows && col < a.n) {
+                l[i] = total(r, token) + (e.bias ? E::get(static_cast<const T*>(e.bias)[col]) : 0.0f);
                 if (col == target) e.logit[token] = l[i];
             }
-#pragma unroll
-            for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-            const float ref = top == -INFINITY ? 0.0f : top;
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                l[i] = exp2f((l[i] - ref) * 1.4426950408889634f);
-                sum += l[i];
-            }
-#pragma unroll
-            for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
-            if (lane == 0) e.part[blockIdx.x * e.part_ld + token] = make_float2(top, sum);
-            // probs_ld is a multiple of 8, so four columns are inside or outside together
-            if (e.probs != nullptr && n0 + lane * 4 < e.probs_ld)
-                *reinterpret_cast<uint2*>(e.probs + token * e.probs_ld + n0 + lane * 4) =
-                    make_uint2(prob16x2(l[0], l[1]), prob16x2(l[2], l[3]));
+            top = fmaxf(top, l[i]);
         }
+#pragma unroll
+        for (int d = kLanes / 2; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int r = first + kLanes * i;
+            if (r >= rows) break;
+            l[i] = exp2f((l[i] - ref) * 1.4426950408889634f);
+            sum += l[i];
+            if (e.probs != nullptr && token < a.m && n0 + r < a.n)
+                e.probs[token * e.probs_ld + n0 + r] = (uint16_t)prob16(l[i]);
+        }
+#pragma unroll
+        for (int d = kLanes / 2; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
+        if (first == 0 && token < a.m) e.part[(int64_t)group * e.part_ld + token] = make_float2(top, sum);
     } else {
         const GemmEpilogue& e = a.e;
         const float alpha = e.count ? e.alpha / (float)max(*e.count, 1) : e.alpha;
@@ -148,9 +116,7 @@ __global__ void __launch_bounds__(256) skinny_kernel(SkinnyArgs a) {
             const int r = i % rows, token = i / rows;
             const int64_t col = n0 + r;
             if (col >= a.n) continue;
-            float v = 0.0f;
-            for (int s = 0; s < a.share; ++s) v += sums[(r / 16 * a.share + s) * 16 + r % 16][token];
-            v *= alpha;
+            float v = total(r, token) * alpha;
             if (e.bias) v += E::get(static_cast<const T*>(e.bias)[col]);
             if (e.z) static_cast<T*>(e.z)[token * e.ld + col] = E::put(v);
             v = activate(v, e.act);
@@ -158,6 +124,70 @@ __global__ void __launch_bounds__(256) skinny_kernel(SkinnyArgs a) {
             static_cast<T*>(e.out)[token * e.ld + col] = E::put(v);
         }
     }
+}
+
+// TILES: tokens in eights.  SOFTMAX: statistics of the block's columns, else
+// the linear layer's epilogue.
+template <int DT, int TILES, bool SOFTMAX>
+__global__ void __launch_bounds__(256, TILES == 1 ? 3 : 4) skinny_kernel(SkinnyArgs a) {
+    constexpr int kTokens = 8 * TILES;
+    constexpr int kAhead = TILES == 1 ? 4 : 2;  // steps of 32 elements of K in flight per warp
+    __shared__ float sums[128][kTokens + 1];  // [warp * 16 + row][token]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, t = lane & 3;
+    const int part = warp % a.share, rows = 128 / a.share;
+    const int n0 = blockIdx.x * rows;
+    griddep_launch_dependents();
+    griddep_wait();
+    const int row = n0 + warp / a.share * 16 + g;
+    const int begin = part * a.k_part, end = min(a.k, begin + a.k_part);
+    const uint16_t* w0 = a.w + (int64_t)min(row, a.n - 1) * a.ldw;
+    const uint16_t* w1 = a.w + (int64_t)min(row + 8, a.n - 1) * a.ldw;
+    const uint16_t* x[TILES];
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) x[i] = a.x + (int64_t)min(8 * i + g, a.m - 1) * a.ldx;
+    float c[TILES][4] = {};
+    const auto multiply = [&](const uint4 (&u0)[kAhead], const uint4 (&u1)[kAhead], const uint4 (&v)[kAhead][TILES]) {
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q)
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) {
+                mma16816<DT>(c[i], u0[q].x, u1[q].x, u0[q].y, u1[q].y, v[q][i].x, v[q][i].y);
+                mma16816<DT>(c[i], u0[q].z, u1[q].z, u0[q].w, u1[q].w, v[q][i].z, v[q][i].w);
+            }
+    };
+    int k = begin + 8 * t;
+    for (; k - 8 * t + 32 * kAhead <= end; k += 32 * kAhead) {
+        uint4 u0[kAhead], u1[kAhead], v[kAhead][TILES];
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {
+            u0[q] = __ldg(reinterpret_cast<const uint4*>(w0 + k + 32 * q));
+            u1[q] = __ldg(reinterpret_cast<const uint4*>(w1 + k + 32 * q));
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) v[q][i] = __ldg(reinterpret_cast<const uint4*>(x[i] + k + 32 * q));
+        }
+        multiply(u0, u1, v);
+    }
+    if (k - 8 * t < end) {
+        uint4 u0[kAhead], u1[kAhead], v[kAhead][TILES];
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {
+            u0[q] = load8(w0, k + 32 * q, end);
+            u1[q] = load8(w1, k + 32 * q, end);
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) v[q][i] = load8(x[i], k + 32 * q, end);
+        }
+        multiply(u0, u1, v);
+    }
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) {
+        sums[warp * 16 + g][8 * i + 2 * t] = c[i][0];
+        sums[warp * 16 + g][8 * i + 2 * t + 1] = c[i][1];
+        sums[warp * 16 + g + 8][8 * i + 2 * t] = c[i][2];
+        sums[warp * 16 + g + 8][8 * i + 2 * t + 1] = c[i][3];
+    }
+    __syncthreads();
+    finish<DT, kTokens, SOFTMAX>(a, sums, n0, rows, blockIdx.x);
 }
 
 template <class Job>
@@ -173,6 +203,13 @@ SkinnyArgs lay_out(const Job& j) {
     return a;
 }
 
+// Warps per 16 rows: as many as have at least four steps of K each.
+int share_of(int64_t k) {
+    int share = 1;
+    while (share < 8 && k > share * 128) share *= 2;
+    return share;
+}
+
 template <bool SOFTMAX>
 void launch(int dtype, SkinnyArgs& a, Queue& q) {
     a.k_part = ((a.k + a.share - 1) / a.share + 31) / 32 * 32;
@@ -186,19 +223,19 @@ void launch(int dtype, SkinnyArgs& a, Queue& q) {
 
 }  // namespace
 
+int skinny_block(int64_t k) { return 128 / share_of(k); }
+
 void skinny(int dtype, const GemmJob& j, Queue& q) {
     SkinnyArgs a = lay_out(j);
     a.e = j.e;
-    // warps enough to fill the card, each with at least one round of loads
-    a.share = 1;
-    while (a.share < 8 && (a.n + 15) / 16 * a.share < 148 * 24 && a.k > a.share * 32 * kAhead) a.share *= 2;
+    a.share = share_of(a.k);
     launch<false>(dtype, a, q);
 }
 
-void skinny_softmax(int dtype, const SoftmaxJob& j, Queue& q) {
+void skinny_softmax(int dtype, const SoftmaxJob& j, int block, Queue& q) {
     SkinnyArgs a = lay_out(j);
     a.s = j.e;
-    a.share = 1;
+    a.share = 128 / block;
     launch<true>(dtype, a, q);
 }
 
