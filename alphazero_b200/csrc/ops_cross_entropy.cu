@@ -2,7 +2,7 @@
 // (include/minigo_ops.h).
 //
 // Forward: the product's epilogue turns each tile of logits into a maximum
-// and a sum per row and block of 128 columns; the logits leave the chip in
+// and a sum per row and block of columns; the logits leave the chip in
 // no form.  combine_kernel joins the blocks of a row.
 //
 // With gradients each tile also leaves exp(l - its block's maximum) in 16

@@ -16,11 +16,13 @@
 //   warp 0     TMA producer (one thread), a ring of kStages K steps
 //   warp 1     TMEM; in the even CTA also the MMA issuer (one thread)
 //   warps 2-9  epilogue: warp w reads TMEM lanes 32 (w % 4) .. + 31 (a thread
-//              owns a row) and half of the columns, 32 at a time, through
+//              owns a row) and half of the columns, 64 at a time, through
 //              swizzled blocks of shared memory that TMA stores (and, for the
-//              residual, loads): a lane's own 16-byte stores to 32 rows at
-//              once cost 8.4 us for a 128 x 256 tile (184832 x 256 x 256:
-//              82 us)
+//              residual, loads a chunk ahead, past the end of a tile).  Short
+//              products are bound by these stores: the card writes 3.6 TB/s
+//              (torch's zero_), 5100 cycles for an SM's 128 x 256 sums, and an
+//              epilogue without a residual takes 5600; a lane's own 16-byte
+//              stores to 32 rows at once took 14000
 // The sums are double-buffered in TMEM: a tile's epilogue overlaps the next
 // tile's products.  Every wait is bounded (ptx_sm100.cuh).
 #include "ops_gemm.cuh"
@@ -41,9 +43,8 @@ constexpr int kThreads = 32 * (2 + kEpiWarps);
 constexpr int kPairs = 74;             // of SMs on a B200 (148)
 constexpr int kGroup = 8;              // row tiles walked together (their B tiles stay in L2)
 constexpr int kStagePitch = 34;        // 16-bit elements per row staged without TMA (17 words: no bank conflicts)
-constexpr int kOutBytes = 4096;        // per epilogue warp: two 32 x 32 blocks of 16-bit, or one of fp32
-constexpr int kResBytes = 2048;        // a 32 x 32 block of the residual, of two
-constexpr int kWarpBytes = kOutBytes + 2 * kResBytes;
+constexpr int kBlockBytes = 4096;      // 32 rows of 128 bytes: 64 columns of 16 bits or 32 of fp32
+constexpr int kWarpBytes = 2 * kBlockBytes;  // per epilogue warp
 
 template <int BN>
 struct Config {
@@ -52,9 +53,10 @@ struct Config {
     static constexpr uint32_t kBBytes = BN / 2 * kBK * 2;
     static constexpr uint32_t kStageBytes = kABytes + kBBytes;
     static constexpr uint32_t kTmemCols = 2 * BN;
+    static constexpr int kCols = BN / 2;  // of a tile per epilogue warp
     static constexpr int kBarriers = 2 * kStages + 5 + 2 * kEpiWarps;
     // ring + per epilogue warp its blocks and 16-bit bias + barriers + TMEM address
-    static constexpr int kSmem = kStages * kStageBytes + kEpiWarps * (kWarpBytes + BN / 2 * 2) + kBarriers * 8 + 16;
+    static constexpr int kSmem = kStages * kStageBytes + kEpiWarps * (kWarpBytes + kCols * 2) + kBarriers * 8 + 16;
     static_assert(kSmem <= 232448, "shared memory of an SM");
 };
 
@@ -170,71 +172,64 @@ __device__ __forceinline__ float2 unpack2(uint32_t u) {
     else return __half22float2(*reinterpret_cast<__half2*>(&u));
 }
 
-// Byte offset of 16-byte chunk q of row r in a block of 64-byte (128-byte)
-// rows as TMA swizzles it.
-__device__ __forceinline__ uint32_t swizzle64(int r, int q) { return r * 64 + ((q ^ (r >> 1 & 3)) << 4); }
+// Byte offset of 16-byte piece q of row r in a block of 128-byte rows as TMA
+// swizzles it.
 __device__ __forceinline__ uint32_t swizzle128(int r, int q) { return r * 128 + ((q ^ (r & 7)) << 4); }
 
-// An epilogue warp's shared memory, and which of its blocks are in use.
+// An epilogue warp's two blocks of shared memory, used in turn.  A residual
+// block lands where the result is then written: each lane replaces its own
+// row.
 struct WarpBlocks {
-    uint8_t* out;      // [2][2048], or [4096]
-    uint8_t* res;      // [2][2048]
+    uint8_t* blocks;   // [2][4096]
     uint64_t* landed;  // [2] a residual block has arrived
     int lane;
-    int next = 0;      // out block to write
-    int started = 0, taken = 0;  // residual blocks
+    int next = 0;        // block of the next chunk of columns
+    uint32_t phase = 0;  // bit b: parity of landed[b]
+    int flying = 0;      // residual blocks on their way
 
-    // Writes v (a row per lane) to the next block and starts its store.
-    template <class Words>
-    __device__ __forceinline__ void store16(const CUtensorMap* map, int col, int row, Words word) {
-        if (lane == 0) bulk_wait_read_n<1>();  // the store before last is done with this block
+    __device__ __forceinline__ uint8_t* at(int b) const { return blocks + b * kBlockBytes; }
+    // At most N of the warp's stores still read shared memory.
+    template <int N>
+    __device__ __forceinline__ void settle() {
+        if (lane == 0) bulk_wait_read_n<N>();
         __syncwarp();
-        uint8_t* p = out + next * 2048;
+    }
+    // Lane's 32 columns of 16 bits, the first (h = 0) or second half of block b.
+    template <class Words>
+    __device__ __forceinline__ void write16(int b, int h, Words word) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<uint4*>(p + swizzle64(lane, q)) =
+            *reinterpret_cast<uint4*>(at(b) + swizzle128(lane, 4 * h + q)) =
                 make_uint4(word(4 * q), word(4 * q + 1), word(4 * q + 2), word(4 * q + 3));
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-            tma_store_2d(map, smem_u32(p), col, row);
-            bulk_commit();
-        }
-        next ^= 1;
     }
-    __device__ __forceinline__ void store32(const CUtensorMap* map, int col, int row, const float (&v)[32]) {
-        if (lane == 0) bulk_wait_read_n<0>();
-        __syncwarp();
+    __device__ __forceinline__ void write32(int b, const float (&v)[32]) {
 #pragma unroll
         for (int q = 0; q < 8; ++q)
-            *reinterpret_cast<float4*>(out + swizzle128(lane, q)) =
+            *reinterpret_cast<float4*>(at(b) + swizzle128(lane, q)) =
                 make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+    }
+    // Starts the store of block b.
+    __device__ __forceinline__ void store(int b, const CUtensorMap* map, int col, int row) {
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-            tma_store_2d(map, smem_u32(out), col, row);
+            tma_store_2d(map, smem_u32(at(b)), col, row);
             bulk_commit();
         }
     }
-    // Blocks of the residual in turn: started ahead, at most two, and (after
-    // a wait) read.
-    __device__ __forceinline__ void start_res(const CUtensorMap* map, int col, int row) {
-        __syncwarp();  // every lane has read what the block held
+    // A chunk's residual into block b (settled), and the wait for it.
+    __device__ __forceinline__ void start_res(int b, const CUtensorMap* map, int col, int row) {
         if (lane == 0) {
-            const uint32_t bar = smem_u32(&landed[started & 1]);
-            mbar_arrive_expect_tx(bar, kResBytes);
-            tma_load_2d(smem_u32(res + (started & 1) * kResBytes), map, bar, col, row);
+            const uint32_t bar = smem_u32(&landed[b]);
+            mbar_arrive_expect_tx(bar, kBlockBytes);
+            tma_load_2d(smem_u32(at(b)), map, bar, col, row);
         }
-        ++started;
+        ++flying;
     }
-    __device__ __forceinline__ bool read_res(uint4 (&u)[4], int* err) {
-        const int b = taken & 1;
-        const bool ok =
-            __all_sync(~0u, mbar_wait(smem_u32(&landed[b]), (taken >> 1) & 1, err, kErrWaitEpilogue));
-        ++taken;
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            u[q] = *reinterpret_cast<const uint4*>(res + b * kResBytes + swizzle64(lane, q));
+    __device__ __forceinline__ bool wait_res(int b, int* err, int code) {
+        const bool ok = __all_sync(~0u, mbar_wait(smem_u32(&landed[b]), phase >> b & 1, err, code));
+        phase ^= 1u << b;
+        --flying;
         return ok;
     }
 };
@@ -333,20 +328,35 @@ struct EpilogueJob {
     }
 };
 
-// Columns [n0 + c0, + BN / 2) of rows [m0, + 32) of a finished tile, whose
+// Columns [n0 + c0, + kCols) of rows [m0, + 32) of a finished tile, whose
 // sums are given back by `release` as soon as they are in registers.  False
 // if a wait gave up.
+// The residual's block after the tile's last starts at column after_col (-1:
+// there is none) of row after_row.
 template <int BN, int DT, class Release>
 __device__ __forceinline__ bool epilogue(const KernelArgs& a, int job, const EpilogueJob& j, const Tile& t, int m0,
                                          int c0, uint32_t taddr, WarpBlocks& blocks, const uint16_t* sbias,
-                                         Release release) {
+                                         int after_col, int after_row, Release release) {
     const GemmEpilogue& e = a.job[job].e;
     const int rows = min(32, j.m - m0), lane = blocks.lane;
-    const int width = rows > 0 ? min(BN / 2, j.n - t.n0 - c0) : 0;
+    const int width = rows > 0 ? min(Config<BN>::kCols, j.n - t.n0 - c0) : 0;
     if (width <= 0) release();
 #pragma unroll 1
     for (int c = 0; c < width; c += 32) {
-        const int col = t.n0 + c0 + c;
+        const int col = t.n0 + c0 + c, h = c >> 5 & 1;
+        const bool ends = h == 1 || c + 32 >= width;  // of a chunk of 64 columns
+        if (j.by_tma && !j.has_out32 && h == 0) {
+            if (j.has_z) {
+                blocks.settle<0>();
+            } else if (j.has_res) {
+                if (!blocks.wait_res(blocks.next, a.err, kErrWaitEpilogue)) return false;
+                blocks.settle<0>();  // the chunk before's store, a chunk ago
+                if (c + 64 < width) blocks.start_res(blocks.next ^ 1, &a.tr, col + 64, m0);
+                else if (after_col >= 0) blocks.start_res(blocks.next ^ 1, &a.tr, after_col, after_row);
+            } else {
+                blocks.settle<1>();
+            }
+        }
         uint32_t r[32];
         tmem_ld_32cols(taddr + c, r);
         tmem_ld_wait();
@@ -367,18 +377,30 @@ __device__ __forceinline__ bool epilogue(const KernelArgs& a, int job, const Epi
                 }
         }
         if (j.has_out32) {
-            blocks.store32(&a.to[job], col, t.split * j.m_pad + m0, v);
+            blocks.settle<1>();
+            blocks.write32(blocks.next, v);
+            blocks.store(blocks.next, &a.to[job], col, t.split * j.m_pad + m0);
+            blocks.next ^= 1;
             continue;
         }
         add_bias<DT>(v, j.alpha, sbias + c);
-        const auto word = [&](int i) { return pack2<DT>(v[2 * i], v[2 * i + 1]); };
         if (j.by_tma) {
-            if (j.has_z) blocks.store16(&a.tz, col, m0, word);
+            const auto word = [&](int i) { return pack2<DT>(v[2 * i], v[2 * i + 1]); };
+            const int col64 = col - 32 * h;
+            if (j.has_z) blocks.write16(blocks.next ^ 1, h, word);
             activate_all(v, j.act);
             if (j.has_res) {
                 uint4 u[4];
-                if (!blocks.read_res(u, a.err)) return false;
-                if (c + 64 < width) blocks.start_res(&a.tr, col + 64, m0);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if (!j.has_z)
+                        u[q] = *reinterpret_cast<const uint4*>(blocks.at(blocks.next) + swizzle128(lane, 4 * h + q));
+                    else if (lane < rows && c + 8 * q < width)
+                        u[q] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(e.res) +
+                                                                    (int64_t)(m0 + lane) * e.r_row + col + 8 * q));
+                    else
+                        u[q] = make_uint4(0, 0, 0, 0);
+                }
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const uint32_t w[4] = {u[q].x, u[q].y, u[q].z, u[q].w};
@@ -390,11 +412,17 @@ __device__ __forceinline__ bool epilogue(const KernelArgs& a, int job, const Epi
                     }
                 }
             }
-            blocks.store16(&a.to[job], col, m0, word);
+            blocks.write16(blocks.next, h, word);
+            if (ends) {
+                if (j.has_z) blocks.store(blocks.next ^ 1, &a.tz, col64, m0);
+                blocks.store(blocks.next, &a.to[job], col64, m0);
+                blocks.next ^= 1;
+            }
             continue;
         }
+        blocks.settle<0>();
         const int cols = min(32, width - c);
-        uint16_t* stage = reinterpret_cast<uint16_t*>(blocks.out);
+        uint16_t* stage = reinterpret_cast<uint16_t*>(blocks.blocks);
         if (j.has_z)
             store_block<DT>(static_cast<uint16_t*>(e.z) + (int64_t)m0 * e.ld + col, e.ld, rows, cols, lane, stage, v);
         activate_all(v, j.act);
@@ -424,6 +452,13 @@ __device__ __forceinline__ void pin(float (&v)[32]) {
     for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]));
 }
 
+// 2^x; below 2^-126, 0.
+__device__ __forceinline__ float exp2_flush(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Softmax statistics of the same columns and rows.  A thread has its row's
 // block to itself, in registers, so the maximum and the sum need no exchange.
 template <int BN, int DT, class Release>
@@ -432,13 +467,13 @@ __device__ __forceinline__ void softmax_epilogue(const KernelArgs& a, const Soft
                                                  WarpBlocks& blocks, const uint16_t* sbias, Release release) {
     const int row = m0 + blocks.lane;
     const int first = t.n0 + c0;
-    const int width = m0 < m ? min(BN / 2, n - first) : 0;
+    constexpr int W = Config<BN>::kCols;
+    const int width = m0 < m ? min(W, n - first) : 0;
     if (width <= 0) {
         release();
         return;
     }
     target -= first;
-    constexpr int W = BN / 2;
     float l[W];
 #pragma unroll
     for (int c = 0; c < W; c += 32)
@@ -470,15 +505,22 @@ __device__ __forceinline__ void softmax_epilogue(const KernelArgs& a, const Soft
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
             // the difference first: exact near the maximum, and in range for any finite logits
-            v[i] = exp2f((v[i] - ref) * 1.4426950408889634f);
+            v[i] = exp2_flush((v[i] - ref) * 1.4426950408889634f);
             sum[i & 3] += v[i];
         }
-        if (e.probs != nullptr)
-            blocks.store16(&a.to[0], first + c, m0, [&](int i) { return prob16x2(v[2 * i], v[2 * i + 1]); });
+        if (e.probs != nullptr) {
+            const int h = c >> 5 & 1;
+            if (h == 0) blocks.settle<1>();
+            blocks.write16(blocks.next, h, [&](int i) { return prob16x2(v[2 * i], v[2 * i + 1]); });
+            if (h == 1 || c + 32 >= width) {
+                blocks.store(blocks.next, &a.to[0], first + c - 32 * h, m0);
+                blocks.next ^= 1;
+            }
+        }
     }
     if (row < m) {
         if (target >= 0 && target < width) e.logit[row] = logit;
-        e.part[(int64_t)(first / (BN / 2)) * e.part_ld + row] =
+        e.part[(int64_t)(first / W) * e.part_ld + row] =
             make_float2(most, (sum[0] + sum[1]) + (sum[2] + sum[3]));
     }
 }
@@ -491,7 +533,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     extern __shared__ __align__(1024) uint8_t ring[];  // at the same address in both CTAs
     uint8_t* blocks_all = ring + S * Cfg::kStageBytes;  // a multiple of 1 KB, as each warp's part is
     uint16_t* bias_all = reinterpret_cast<uint16_t*>(blocks_all + kEpiWarps * kWarpBytes);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(bias_all + kEpiWarps * (BN / 2));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(bias_all + kEpiWarps * Cfg::kCols);
     uint64_t* full = bars;           // even CTA's: a stage has landed in both CTAs
     uint64_t* empty = bars + S;      // each CTA's: the products have read a stage
     uint64_t* tfull = bars + 2 * S;  // [2] each CTA's: a tile's sums are complete
@@ -639,14 +681,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             mbar_wait_cluster_warp(smem_u32(done), 0, a.err, kErrWaitDrain);
         }
     } else {
-        const int ew = warp - 2, quarter = warp & 3, half = ew >> 2;
-        const int c0 = half * (BN / 2);
+        const int ew = warp - 2, quarter = warp & 3;
+        const int c0 = (ew >> 2) * Cfg::kCols;
         // the warp's own copy of its columns' bias: one shared by four warps would
         // need a barrier, which a warp whose wait gave up would leave the others at
-        uint16_t* sbias = bias_all + ew * (BN / 2);
+        uint16_t* sbias = bias_all + ew * Cfg::kCols;
         WarpBlocks blocks;
-        blocks.out = blocks_all + ew * kWarpBytes;
-        blocks.res = blocks.out + kOutBytes;
+        blocks.blocks = blocks_all + ew * kWarpBytes;
         blocks.landed = &landed[2 * ew];
         blocks.lane = lane;
         const uint32_t taddr0 = tmem_base + c0 + ((uint32_t)quarter << 21);
@@ -662,18 +703,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const Tile t(tiling, unit, BN);
                 const int m0 = t.m0 + (int)rank * kRowsCta + quarter * 32;
                 // what the tile needs besides its sums is on its way before they are complete
-                int target = -1;
+                int target = -1, after_col = -1, after_row = 0;
                 if constexpr (EPI == kSoftmax) {
                     if (m0 + lane < j.m) target = soft.target[m0 + lane];
-                } else if (j.has_res && j.by_tma && m0 < j.m) {
-                    const int col = t.n0 + c0;
-                    if (col < j.n) blocks.start_res(&a.tr, col, m0);
-                    if (BN / 2 > 32 && col + 32 < j.n) blocks.start_res(&a.tr, col + 32, m0);
+                } else if (j.has_res && j.by_tma && !j.has_z) {
+                    const auto mine = [&](const Tile& u, int* col, int* row) {
+                        *row = u.m0 + (int)rank * kRowsCta + quarter * 32;
+                        *col = u.n0 + c0;
+                        return *row < j.m && *col < j.n;
+                    };
+                    int col, row;
+                    if (blocks.flying == 0 && mine(t, &col, &row)) {
+                        blocks.settle<0>();
+                        blocks.start_res(blocks.next, &a.tr, col, row);
+                    }
+                    const int following = walk.unit(job, i + 1);
+                    after_col = -1;
+                    if (following >= 0 && mine(Tile(tiling, following, BN), &col, &row)) {
+                        after_col = col;
+                        after_row = row;
+                    }
                 }
                 if (t.n0 != bias_at) {
                     bias_at = t.n0;
                     __syncwarp();
-                    for (int b = lane; b < BN / 2; b += 32) {
+                    for (int b = lane; b < Cfg::kCols; b += 32) {
                         const int64_t col = t.n0 + c0 + b;
                         // past the last column: nothing, or for the softmax a logit of -inf
                         uint16_t v = EPI == kSoftmax && col >= j.n ? (DT == MG_PREC_BF16 ? 0xff80 : 0xfc00) : 0;
@@ -698,14 +752,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     softmax_epilogue<BN, DT>(a, soft, j.m, j.n, t, m0, c0, target, taddr0 + buf * BN, blocks, sbias,
                                          release);
                 else
-                    ok = epilogue<BN, DT>(a, job, j, t, m0, c0, taddr0 + buf * BN, blocks, sbias, release);
+                    ok = epilogue<BN, DT>(a, job, j, t, m0, c0, taddr0 + buf * BN, blocks, sbias, after_col, after_row,
+                                           release);
                 ++tile;
             }
         }
-        while (blocks.taken < blocks.started) {  // only after a wait gave up
-            mbar_wait(smem_u32(&landed[2 * ew + (blocks.taken & 1)]), (blocks.taken >> 1) & 1, a.err, kErrWaitDrain);
-            ++blocks.taken;
-        }
+        for (int b = blocks.next; blocks.flying > 0; b ^= 1)  // only after a wait gave up
+            blocks.wait_res(b, a.err, kErrWaitDrain);
         if (lane == 0) bulk_wait_all();
         __syncwarp();
     }
@@ -750,9 +803,9 @@ void encode_operand(CUtensorMap* map, int dtype, const StagedOperand& s, int64_t
            CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// A matrix that the epilogue moves in 32 x 32 blocks of 16-bit elements.
+// A matrix that the epilogue moves in blocks of 32 x 64 16-bit elements.
 void encode_blocks(CUtensorMap* map, int dtype, const void* base, int64_t m, int64_t n, int64_t ld) {
-    encode(map, map_type(dtype), 2, base, n, m, ld, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+    encode(map, map_type(dtype), 2, base, n, m, ld, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -197,7 +197,7 @@ __device__ __forceinline__ float normal_cdf(float z, float* bell) {
 __device__ __forceinline__ float activate(float z, int act) {
     float bell;
     switch (act) {
-        case MG_ACT_RELU: return z < 0.0f ? 0.0f : z;  // NaN stays
+        case MG_ACT_RELU: asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(z)); return z;  // NaN stays
         case MG_ACT_SILU: return __fdividef(z, 1.0f + __expf(-z));
         case MG_ACT_GELU: return z * normal_cdf(z, &bell);
         default: return z;
