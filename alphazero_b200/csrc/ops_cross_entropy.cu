@@ -61,8 +61,8 @@ __device__ __forceinline__ void join(float& m, float& s, float2 p) {
 }
 
 // logsumexp and loss per row, and the loss summed per block: a thread per row
-// where a row has few blocks of columns; with many, a warp per row, or where
-// there are few rows too, a block per row (lanes take the blocks in turn).
+// where a row has few blocks of columns; with many, 32 threads per row, or
+// where there are few rows too, a block per row.
 // A row of -inf has lse -inf.  counts, if set: their sum goes to count.
 enum Combine : int { kThreadPerRow, kWarpPerRow, kBlockPerRow };
 constexpr int kFewBlocks = 16;
@@ -111,15 +111,14 @@ __global__ void __launch_bounds__(HOW == kThreadPerRow ? 128 : 1024)
         s = tile[0][lane].y;
         join_lanes();
     } else {
-        // 32 blocks x 32 rows at a time, read along the rows and turned round
-        for (int b0 = 0; b0 < blocks; b0 += 32) {
-            float2 p = make_float2(-INFINITY, 0.0f);
-            if (b0 + warp < blocks && row0 + lane < rows) p = part[(int64_t)(b0 + warp) * part_ld + row0 + lane];
-            tile[warp][lane] = p;
-            __syncthreads();
-            join(m, s, tile[lane][warp]);
-            __syncthreads();
-        }
+        // read along the rows, a warp per block of columns in turn; then turned round
+        if (row0 + lane < rows)
+#pragma unroll 8
+            for (int b = warp; b < blocks; b += 32) join(m, s, part[(int64_t)b * part_ld + row0 + lane]);
+        tile[warp][lane] = make_float2(m, s);
+        __syncthreads();
+        m = tile[lane][warp].x;
+        s = tile[lane][warp].y;
         join_lanes();
     }
     float loss = 0.0f;
@@ -165,31 +164,44 @@ __global__ void __launch_bounds__(256)
     griddep_wait();
     if (c < vocab) {
         const float2* mine = part + c / block * part_ld;
-#pragma unroll 4
-        for (int64_t r = r0 + warp; r < r1; r += 8) {
-            const int t = target[r];
-            const float l = lse[r];
-            uint4* p = reinterpret_cast<uint4*>(probs + r * ld + c);
-            const uint4 u = *p;
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-            // a row that is not counted (whatever it holds) and one of -inf have no probabilities
-            float f = l == -INFINITY || t < 0 ? 0.0f : exp2f((mine[r].x - l) * 1.4426950408889634f);
-            f *= 0x1p112f;  // prob16_value's scale
-            float v[8];
+        // four rows at a time, their loads before the first store (which, for
+        // all that is known, might be to what they read)
+        constexpr int kRows = 4;
+        for (int64_t r = r0 + warp; r < r1; r += 8 * kRows) {
+            uint4 u[kRows];
+            int t[kRows];
+            float f[kRows], m[kRows];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                v[i] = __uint_as_float(i & 1 ? w[i / 2] >> 16 << 11 : (w[i / 2] & 0xffffu) << 11) * f;
-            if (t >= c && t < c + 8)
+            for (int q = 0; q < kRows; ++q) {
+                const int64_t row = min(r + 8 * q, r1 - 1);
+                u[q] = *reinterpret_cast<const uint4*>(probs + row * ld + c);
+                t[q] = target[row];
+                f[q] = lse[row];
+                m[q] = mine[row].x;
+            }
+#pragma unroll
+            for (int q = 0; q < kRows; ++q) {
+                if (r + 8 * q >= r1) break;
+                const uint32_t w[4] = {u[q].x, u[q].y, u[q].z, u[q].w};
+                // a row that is not counted (whatever it holds) and one of -inf have no probabilities
+                const float p = f[q] == -INFINITY || t[q] < 0 ? 0.0f : exp2f((m[q] - f[q]) * 1.4426950408889634f);
+                const float scale = p * 0x1p112f;  // prob16_value's
+                float v[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (t == c + i) v[i] -= 1.0f;
-            alignas(16) T d[8];
+                    v[i] = __uint_as_float(i & 1 ? w[i / 2] >> 16 << 11 : (w[i / 2] & 0xffffu) << 11) * scale;
+                if (t[q] >= c && t[q] < c + 8)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                sum[i] += v[i];
-                d[i] = E::put(v[i] * kDScale<DT>);
+                    for (int i = 0; i < 8; ++i)
+                        if (t[q] == c + i) v[i] -= 1.0f;
+                alignas(16) T d[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    sum[i] += v[i];
+                    d[i] = E::put(v[i] * kDScale<DT>);
+                }
+                *reinterpret_cast<uint4*>(probs + (r + 8 * q) * ld + c) = *reinterpret_cast<uint4*>(d);
             }
-            *p = *reinterpret_cast<uint4*>(d);
         }
     }
     if (sums == nullptr) return;
@@ -241,7 +253,7 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
     float2* part = w.take<float2>((size_t)blocks * piece * 8);
     uint16_t* probs = grads ? w.take<uint16_t>((size_t)piece * ld * 2) : nullptr;
     const int64_t across = (a.vocab + 255) / 256;
-    const int64_t want = std::max<int64_t>(1, 148 * 4 / across);
+    const int64_t want = std::max<int64_t>(1, 148 * 8 / across);
     const int down_rows = (int)std::max<int64_t>(32, (piece + want - 1) / want);
     const int64_t down = (piece + down_rows - 1) / down_rows;  // of a whole piece
     float* sums = a.db ? w.take<float>((size_t)down * count_pieces * a.vocab * 4) : nullptr;

@@ -227,7 +227,7 @@ struct WarpBlocks {
         ++flying;
     }
     __device__ __forceinline__ bool wait_res(int b, int* err, int code) {
-        const bool ok = __all_sync(~0u, mbar_wait(smem_u32(&landed[b]), phase >> b & 1, err, code));
+        const bool ok = mbar_wait_warp(smem_u32(&landed[b]), phase >> b & 1, err, code);
         phase ^= 1u << b;
         --flying;
         return ok;
@@ -452,13 +452,6 @@ __device__ __forceinline__ void pin(float (&v)[32]) {
     for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]));
 }
 
-// 2^x; below 2^-126, 0.
-__device__ __forceinline__ float exp2_flush(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // Softmax statistics of the same columns and rows.  A thread has its row's
 // block to itself, in registers, so the maximum and the sum need no exchange.
 template <int BN, int DT, class Release>
@@ -587,7 +580,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int am = t.m0 + (int)rank * kRowsCta, bn = t.n0 + (int)rank * (BN / 2);
                 for (int kb = t.kb0; kb < t.kb1; ++kb) {
                     const uint32_t wait = smem_u32(&empty[s]);
-                    if (!mbar_wait_cluster_warp(wait, (round & 1) ^ 1, a.err, kErrWaitProducer)) {
+                    if (!mbar_wait_warp(wait, (round & 1) ^ 1, a.err, kErrWaitProducer)) {
                         ok = false;
                         break;
                     }
@@ -624,8 +617,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 s = S - 1;
                 --round;
             }
-            if (rank == 0) mbar_wait_cluster_warp(smem_u32(&full[s]), round & 1, a.err, kErrWaitDrain);
-            if (ok) mbar_wait_cluster_warp(smem_u32(&empty[s]), round & 1, a.err, kErrWaitDrain);
+            if (rank == 0) mbar_wait_warp(smem_u32(&full[s]), round & 1, a.err, kErrWaitDrain);
+            if (ok) mbar_wait_warp(smem_u32(&empty[s]), round & 1, a.err, kErrWaitDrain);
         }
     } else if (warp == 1) {
         if (rank == 0) {
@@ -644,14 +637,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 for (int i = 0, unit; ok && (unit = walk.unit(job, i)) >= 0; ++i) {
                     const Tile t(tiling, unit, BN);
                     const int buf = tile & 1;
-                    if (!mbar_wait_cluster_warp(smem_u32(&tempty[buf]), ((tile >> 1) & 1) ^ 1, a.err, kErrWaitMma)) {
+                    if (!mbar_wait_warp(smem_u32(&tempty[buf]), ((tile >> 1) & 1) ^ 1, a.err, kErrWaitMma)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
                     const uint32_t acc = tmem_base + buf * BN;
                     for (int kb = t.kb0; kb < t.kb1; ++kb) {
-                        if (!mbar_wait_cluster_warp(smem_u32(&full[s]), round & 1, a.err, kErrWaitMma)) {
+                        if (!mbar_wait_warp(smem_u32(&full[s]), round & 1, a.err, kErrWaitMma)) {
                             ok = false;
                             break;
                         }
@@ -678,7 +671,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 asm volatile(
                     "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(done))
                     : "memory");
-            mbar_wait_cluster_warp(smem_u32(done), 0, a.err, kErrWaitDrain);
+            mbar_wait_warp(smem_u32(done), 0, a.err, kErrWaitDrain);
         }
     } else {
         const int ew = warp - 2, quarter = warp & 3;
@@ -738,7 +731,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
                 const int buf = tile & 1;
                 // one answer for the warp, which goes on or stops together
-                if (!mbar_wait_cluster_warp(smem_u32(&tfull[buf]), (tile >> 1) & 1, a.err, kErrWaitEpilogue)) {
+                if (!mbar_wait_warp(smem_u32(&tfull[buf]), (tile >> 1) & 1, a.err, kErrWaitEpilogue)) {
                     ok = false;
                     break;
                 }

@@ -179,26 +179,40 @@ inline StagedOperand transposed(StagedOperand s) {
 // what then remains to be done.
 void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, Post& post, Queue& q);
 
+// 2^x; below 2^-126, 0.
+__device__ __forceinline__ float exp2_flush(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 1 / x to a unit or two in the last place, for 1 <= x (0 at infinity).
+__device__ __forceinline__ float reciprocal(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Phi(z), the normal distribution function, and exp(-z^2 / 2): formula
 // 7.1.26 of Abramowitz and Stegun for erf(|z| / sqrt 2), which is within
 // 1.5e-7 and needs one exponential that GELU's slope shares.
 __device__ __forceinline__ float normal_cdf(float z, float* bell) {
-    const float x = fabsf(z) * 0.70710678118654752f;
-    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
-    float p = fmaf(1.061405429f, t, -1.453152027f);
-    p = fmaf(p, t, 1.421413741f);
-    p = fmaf(p, t, -0.284496736f);
-    p = fmaf(p, t, 0.254829592f);
-    *bell = exp2f(z * z * -0.72134752044448170f);
-    const float tail = 0.5f * p * t * *bell;
+    const float t = reciprocal(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.0f));
+    float p = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+    p = fmaf(p, t, 0.5f * 1.421413741f);
+    p = fmaf(p, t, 0.5f * -0.284496736f);
+    p = fmaf(p, t, 0.5f * 0.254829592f);
+    *bell = exp2_flush(z * -0.72134752044448170f * z);
+    const float tail = p * t * *bell;
     return z < 0.0f ? tail : 1.0f - tail;
 }
+// 1 / (1 + exp(-z)).
+__device__ __forceinline__ float logistic(float z) { return reciprocal(1.0f + exp2_flush(z * -1.4426950408889634f)); }
 
 __device__ __forceinline__ float activate(float z, int act) {
     float bell;
     switch (act) {
         case MG_ACT_RELU: asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(z)); return z;  // NaN stays
-        case MG_ACT_SILU: return __fdividef(z, 1.0f + __expf(-z));
+        case MG_ACT_SILU: return z * logistic(z);
         case MG_ACT_GELU: return z * normal_cdf(z, &bell);
         default: return z;
     }

@@ -12,7 +12,7 @@ __device__ __forceinline__ float slope(float z, int act) {
     switch (act) {
         case MG_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
         case MG_ACT_SILU: {
-            const float p = __fdividef(1.0f, 1.0f + __expf(-z));
+            const float p = logistic(z);
             return p * (1.0f + z * (1.0f - p));
         }
         case MG_ACT_GELU: {

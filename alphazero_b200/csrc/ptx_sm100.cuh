@@ -398,39 +398,16 @@ __device__ __forceinline__ void cluster_sync() {
 }
 
 // Arrives on a barrier of any CTA of the cluster (a map_to_rank address).
+// Ordered after this thread's accesses at CTA scope only: for signals about
+// tensor memory, whose accesses tcgen05.wait and tcgen05.fence order.  (At
+// cluster scope it waits for the thread's global stores, about 1000 cycles.)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
-// mbar_wait for phases that another CTA of the cluster arrives on.
-__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, int* err, int code) {
-    if (mbar_try_wait_cluster(bar, parity)) return true;
-    const uint64_t t0 = global_timer_ns();
-    while (true) {
-        for (int i = 0; i < 32; ++i)
-            if (mbar_try_wait_cluster(bar, parity)) return true;
-        if (global_timer_ns() - t0 > kWaitLimitNs) {
-            atomicCAS(err, 0, code);
-            return false;
-        }
-    }
-}
-
-// The same for a whole warp, with one answer.
-__device__ __forceinline__ bool mbar_wait_cluster_warp(uint32_t bar, uint32_t parity, int* err, int code) {
-    return __all_sync(~0u, mbar_wait_cluster(bar, parity, err, code));
+// mbar_wait for a whole warp, with one answer.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, int* err, int code) {
+    return __all_sync(~0u, mbar_wait(bar, parity, err, code));
 }
 
 // As tma_load_2d into this CTA's shared memory, counted on a barrier of
