@@ -147,17 +147,20 @@ __global__ void __launch_bounds__(HOW == kThreadPerRow ? 128 : 1024)
 
 // probs (Prob16, per block of `block` columns) -> d = (softmax - onehot) in
 // place, and its column sums before rounding per block of rows.  A thread
-// has 8 adjacent columns of every eighth row; the factor from the block's
-// maximum to the row's logsumexp is one exp per thread and row.
+// has 8 adjacent columns; `wide` of the block's eight warps lie side by side
+// (up to 4 KB of a row at once: with one, 512 bytes, the same work ran at two
+// thirds of the speed), the others take further rows.  The factor from the
+// block's maximum to the row's logsumexp is one exp per thread and row.
 template <int DT>
 __global__ void __launch_bounds__(256)
     d_kernel(int64_t rows, int64_t vocab, int block, uint16_t* probs, int64_t ld, const float2* part,
-             int64_t part_ld, const float* lse, const int* target, int rows_per_block, float* sums) {
+             int64_t part_ld, const float* lse, const int* target, int wide, int rows_per_block, float* sums) {
     using E = Elem<DT>;
     using T = typename E::T;
     __shared__ float acc[8][256];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t c = (int64_t)blockIdx.x * 256 + lane * 8;
+    const int deep = 8 / wide, down = warp / wide;
+    const int64_t c = ((int64_t)blockIdx.x * wide + warp % wide) * 256 + lane * 8;
     const int64_t r0 = (int64_t)blockIdx.y * rows_per_block, r1 = min(rows, r0 + rows_per_block);
     float sum[8] = {};
     griddep_launch_dependents();
@@ -167,13 +170,13 @@ __global__ void __launch_bounds__(256)
         // four rows at a time, their loads before the first store (which, for
         // all that is known, might be to what they read)
         constexpr int kRows = 4;
-        for (int64_t r = r0 + warp; r < r1; r += 8 * kRows) {
+        for (int64_t r = r0 + down; r < r1; r += deep * kRows) {
             uint4 u[kRows];
             int t[kRows];
             float f[kRows], m[kRows];
 #pragma unroll
             for (int q = 0; q < kRows; ++q) {
-                const int64_t row = min(r + 8 * q, r1 - 1);
+                const int64_t row = min(r + deep * q, r1 - 1);
                 u[q] = *reinterpret_cast<const uint4*>(probs + row * ld + c);
                 t[q] = target[row];
                 f[q] = lse[row];
@@ -181,7 +184,7 @@ __global__ void __launch_bounds__(256)
             }
 #pragma unroll
             for (int q = 0; q < kRows; ++q) {
-                if (r + 8 * q >= r1) break;
+                if (r + deep * q >= r1) break;
                 const uint32_t w[4] = {u[q].x, u[q].y, u[q].z, u[q].w};
                 // a row that is not counted (whatever it holds) and one of -inf have no probabilities
                 const float p = f[q] == -INFINITY || t[q] < 0 ? 0.0f : exp2f((m[q] - f[q]) * 1.4426950408889634f);
@@ -200,7 +203,7 @@ __global__ void __launch_bounds__(256)
                     sum[i] += v[i];
                     d[i] = E::put(v[i] * kDScale<DT>);
                 }
-                *reinterpret_cast<uint4*>(probs + (r + 8 * q) * ld + c) = *reinterpret_cast<uint4*>(d);
+                *reinterpret_cast<uint4*>(probs + (r + deep * q) * ld + c) = *reinterpret_cast<uint4*>(d);
             }
         }
     }
@@ -208,12 +211,13 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[warp][lane * 8 + i] = sum[i];
     __syncthreads();
-    const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (col >= vocab) return;
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s += acc[i][threadIdx.x];
-    sums[(int64_t)blockIdx.y * vocab + col] = s;
+    for (int i = threadIdx.x; i < wide * 256; i += 256) {
+        const int64_t col = (int64_t)blockIdx.x * wide * 256 + i;
+        if (col >= vocab) break;
+        float s = 0.0f;
+        for (int w = i / 256; w < 8; w += wide) s += acc[w][i % 256];
+        sums[(int64_t)blockIdx.y * vocab + col] = s;
+    }
 }
 
 template <int DT>
@@ -252,9 +256,12 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
     float* lse = w.take<float>((size_t)piece * 4);
     float2* part = w.take<float2>((size_t)blocks * piece * 8);
     uint16_t* probs = grads ? w.take<uint16_t>((size_t)piece * ld * 2) : nullptr;
-    const int64_t across = (a.vocab + 255) / 256;
+    int wide = 1;
+    while (wide < 8 && wide * 256 < a.vocab) wide *= 2;
+    const int64_t across = (a.vocab + 256 * wide - 1) / (256 * wide);
+    // up to eight blocks per SM, at least sixteen rows per warp and block
     const int64_t want = std::max<int64_t>(1, 148 * 8 / across);
-    const int down_rows = (int)std::max<int64_t>(32, (piece + want - 1) / want);
+    const int down_rows = (int)std::max<int64_t>(128 / wide, (piece + want - 1) / want);
     const int64_t down = (piece + down_rows - 1) / down_rows;  // of a whole piece
     float* sums = a.db ? w.take<float>((size_t)down * count_pieces * a.vocab * 4) : nullptr;
     const int64_t ld32 = (a.dim + 7) / 8 * 8;
@@ -306,7 +313,7 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
         const int64_t these = (rows + down_rows - 1) / down_rows;
         if (go) {
             q.launch("d_kernel", d_kernel<DT>, dim3((unsigned)across, (unsigned)these), 256, 0, rows, a.vocab, block,
-                     probs, ld, part, piece, lse, target + row0, down_rows, sums ? sums + sum_rows * a.vocab : nullptr);
+                     probs, ld, part, piece, lse, target + row0, wide, down_rows, sums ? sums + sum_rows * a.vocab : nullptr);
         }
         sum_rows += these;
         StagedOperand d;

@@ -366,15 +366,13 @@ __device__ __forceinline__ bool epilogue(const KernelArgs& a, int job, const Epi
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
         if (j.has_acc32 && lane < rows) {
             const float* p = e.acc32 + (int64_t)(m0 + lane) * e.ld32 + col;
+            uint32_t u[32];
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-                if (c + q * 4 < width) {
-                    const float4 f = *reinterpret_cast<const float4*>(p + q * 4);
-                    v[q * 4] += f.x;
-                    v[q * 4 + 1] += f.y;
-                    v[q * 4 + 2] += f.z;
-                    v[q * 4 + 3] += f.w;
-                }
+            for (int q = 0; q < 4; ++q)  // ld32 is a multiple of 8
+                if (c + q * 8 < width) ld_once_v8(p + q * 8, u + q * 8);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (c + i / 8 * 8 < width) v[i] += __uint_as_float(u[i]);
         }
         if (j.has_out32) {
             blocks.settle<1>();

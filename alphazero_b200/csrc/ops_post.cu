@@ -66,21 +66,26 @@ __device__ __forceinline__ void finish_block(const FinishTask& t, int64_t block,
     }
 }
 
-// 32 columns; 32 threads share a column's rows.
+// `slices` threads share a column: one where there are few rows, up to 32.
+__host__ __device__ inline int add_rows_slices(int64_t rows) { return rows <= 16 ? 1 : rows <= 256 ? 8 : 32; }
+
 template <int DT>
 __device__ __forceinline__ void add_rows_block(const AddRowsTask& t, int64_t block, float* shared) {
-    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
-    const int64_t c = block * 32 + lane;
+    const int slices = add_rows_slices(t.rows), columns = kPostThreads / slices;
+    const int slice = threadIdx.x / columns, lane = threadIdx.x % columns;
+    const int64_t c = block * columns + lane;
     float s = 0.0f;
     if (c < t.cols)
 #pragma unroll 8
-        for (int64_t r = slice; r < t.rows; r += 32) s += t.sums[r * t.cols + c];
-    shared[slice * 33 + lane] = s;
-    __syncthreads();
+        for (int64_t r = slice; r < t.rows; r += slices) s += t.sums[r * t.cols + c];
+    if (slices > 1) {
+        shared[threadIdx.x] = s;
+        __syncthreads();
+        s = 0.0f;
+        if (slice == 0)
+            for (int i = 0; i < slices; ++i) s += shared[i * columns + lane];
+    }
     if (slice > 0 || c >= t.cols) return;
-    s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) s += shared[i * 33 + lane];
     static_cast<typename Elem<DT>::T*>(t.out)[c] =
         Elem<DT>::put(s * (t.count ? t.alpha / (float)max(*t.count, 1) : t.alpha));
 }
@@ -131,7 +136,10 @@ void Post::launch(int dtype, Queue& q) {
         blocks += t.blocks;
     }
     if (loss.loss != nullptr) ++blocks;
-    if (add.out != nullptr) blocks += (add.cols + 31) / 32;
+    if (add.out != nullptr) {
+        const int columns = kPostThreads / add_rows_slices(add.rows);
+        blocks += (add.cols + columns - 1) / columns;
+    }
     if (blocks > 0) {
         need(blocks < (int64_t(1) << 31), "too many blocks");
         q.launch("post_kernel", dtype == MG_PREC_BF16 ? post_kernel<MG_PREC_BF16> : post_kernel<MG_PREC_FP16>,

@@ -225,6 +225,14 @@ __device__ __forceinline__ void ld_cg_v8(const void* p, uint32_t* r) {
                  : "l"(p));
 }
 
+// The same for data that is read once: no place in L1, the first to go in L2.
+__device__ __forceinline__ void ld_once_v8(const void* p, uint32_t* r) {
+    asm volatile("ld.global.L1::no_allocate.L2::evict_first.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                   "=r"(r[6]), "=r"(r[7])
+                 : "l"(p));
+}
+
 // Waits until every committed bulk store has finished reading shared memory.
 __device__ __forceinline__ void bulk_wait_read() {
     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
