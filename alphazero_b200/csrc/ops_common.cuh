@@ -47,6 +47,31 @@ __device__ __forceinline__ int64_t index_at(const void* p, int bytes, int64_t i,
     return t >= 0 && t < limit ? t : -1;
 }
 
+// Eight 16-bit elements from p on, which is element `at` of memory that holds
+// elements [0, span); what lies past it comes back as anything.  16 bytes at
+// any alignment by 32-bit loads, as far as those stay inside.
+__device__ __forceinline__ uint4 load8_unaligned(const uint16_t* p, int64_t at, int64_t span) {
+    const bool odd = (reinterpret_cast<uintptr_t>(p) & 2) != 0;
+    uint32_t w[5];
+    if (at >= odd && at + 8 + odd <= span) {
+        const uint32_t* q = reinterpret_cast<const uint32_t*>(p - odd);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __ldg(q + i);
+        w[4] = odd ? __ldg(q + 4) : 0;
+    } else {
+        uint32_t h[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = at + i < span ? p[i] : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = odd ? __byte_perm(i ? h[2 * i - 1] : 0, h[2 * i], 0x5410)
+                                              : __byte_perm(h[2 * i], h[2 * i + 1], 0x5410);
+        w[4] = h[7];
+    }
+    if (!odd) return make_uint4(w[0], w[1], w[2], w[3]);
+    return make_uint4(__byte_perm(w[0], w[1], 0x5432), __byte_perm(w[1], w[2], 0x5432),
+                      __byte_perm(w[2], w[3], 0x5432), __byte_perm(w[3], w[4], 0x5432));
+}
+
 // ---- host side ----
 
 struct OpFailure {

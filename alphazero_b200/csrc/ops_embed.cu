@@ -1,9 +1,8 @@
 // Embedding lookup with scaling and its gradient (include/minigo_ops.h).
 // Both are bound by memory: each moves n rows of dim elements once.
 //
-// Lookup: a group of lanes per row, up to four independent loads of up to 16
-// bytes per lane; rows longer than that are cut into segments on the grid's
-// other axis, so that a few long rows still fill the card.
+// Lookup: a warp (or 8 lanes) per row, pieces of up to 16 bytes, four of them
+// in flight per lane.
 //
 // Gradient: the tokens are sorted (stable, so equal tokens stay in order of
 // position), then cut into windows of equal length whatever the tokens are.
@@ -51,49 +50,55 @@ int widest(int elem, int64_t row_bytes, int64_t stride_a, int64_t stride_b, cons
 
 // ---- lookup ----
 
-constexpr int kPerLane = 4;  // vectors of a segment that a lane holds
+constexpr int kPerLane = 4;  // pieces of B bytes that a lane has in flight
 
-// `lanes` (a power of two up to 32) per row and segment; chunks = vectors per row.
-template <int DT, int B>
-__global__ void __launch_bounds__(256) embed_kernel(mg_embed_args a, int64_t chunks, int lanes) {
+// LANES lanes per row; pieces = row in pieces of B bytes.  Rows that are not
+// whole 16-byte pieces are bound by the issue of instructions, so offsets are
+// 32-bit and known when compiled, and a piece is one compare, one load, its
+// products and one store.
+template <int DT, int B, int LANES>
+__global__ void __launch_bounds__(256) embed_kernel(mg_embed_args a, int pieces) {
     using E = Elem<DT>;
     using T = typename E::T;
     using V = typename Bytes<B>::T;
     constexpr int N = B / (int)sizeof(T);
     griddep_wait();
-    const int lane = threadIdx.x & (lanes - 1);
-    const int64_t c0 = (int64_t)blockIdx.y * (kPerLane * lanes) + lane;
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes; i < a.n;
-         i += (int64_t)gridDim.x * 256 / lanes) {
+    const int lane = threadIdx.x & (LANES - 1);
+    const float scale = a.scale;
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES; i < a.n;
+         i += (int64_t)gridDim.x * 256 / LANES) {
         const int64_t t = index_at(a.tokens, a.token_bytes, i * a.token_stride, a.vocab);
-        const V* row = reinterpret_cast<const V*>(static_cast<const T*>(a.table) + t * a.table_row);
+        const V* row = reinterpret_cast<const V*>(static_cast<const T*>(a.table) + max(t, (int64_t)0) * a.table_row);
         V* out = reinterpret_cast<V*>(static_cast<T*>(a.out) + i * a.dim);
-        alignas(16) V v[kPerLane];
+        for (int c = blockIdx.y * (kPerLane * LANES) + lane; c < pieces; c += gridDim.y * (kPerLane * LANES)) {
+            const int left = pieces - c;
+            alignas(16) V v[kPerLane];
 #pragma unroll
-        for (int q = 0; q < kPerLane; ++q)
-            if (c0 + q * lanes < chunks && t >= 0) v[q] = __ldg(row + c0 + q * lanes);
+            for (int q = 0; q < kPerLane; ++q)
+                if (q * LANES < left) v[q] = __ldg(row + c + q * LANES);
 #pragma unroll
-        for (int q = 0; q < kPerLane; ++q) {
-            if (c0 + q * lanes >= chunks) continue;
-            alignas(16) T e[N];
-            *reinterpret_cast<V*>(e) = v[q];
+            for (int q = 0; q < kPerLane; ++q) {
+                alignas(16) T e[N];
+                *reinterpret_cast<V*>(e) = v[q];
 #pragma unroll
-            for (int j = 0; j < N; ++j) e[j] = E::put(t < 0 ? 0.0f : E::get(e[j]) * a.scale);
-            out[c0 + q * lanes] = *reinterpret_cast<V*>(e);
+                for (int j = 0; j < N; ++j) e[j] = E::put(t < 0 ? 0.0f : E::get(e[j]) * scale);
+                if (q * LANES < left) out[c + q * LANES] = *reinterpret_cast<V*>(e);
+            }
         }
     }
 }
 
 template <int DT, int B>
 void embed_with(const mg_embed_args& a, Queue& q) {
-    const int64_t chunks = a.dim * elem_bytes(DT) / B;
-    int lanes = 1;
-    while (lanes < 32 && lanes < chunks) lanes *= 2;
-    const int64_t rows_per_block = 256 / lanes, segments = (chunks + kPerLane * lanes - 1) / (kPerLane * lanes);
-    const dim3 grid((unsigned)std::min<int64_t>((a.n + rows_per_block - 1) / rows_per_block, 1 << 30),
-                    (unsigned)segments);
-    need(segments <= 65535, "dim is too large");
-    q.launch("embed_kernel", embed_kernel<DT, B>, grid, 256, 0, a, chunks, lanes);
+    const int64_t pieces = a.dim * elem_bytes(DT) / B;
+    need(pieces < (int64_t(1) << 31), "dim is too large");
+    const bool narrow = pieces <= 8 * kPerLane;
+    const int64_t rows = narrow ? 32 : 8, blocks = (a.n + rows - 1) / rows;
+    // a few long rows are cut up to fill the card
+    const int64_t segments = (pieces + 32 * kPerLane - 1) / (32 * kPerLane);
+    const int64_t cuts = narrow ? 1 : std::clamp<int64_t>(148 * 8 / blocks, 1, std::min<int64_t>(segments, 65535));
+    q.launch("embed_kernel", narrow ? embed_kernel<DT, B, 8> : embed_kernel<DT, B, 32>,
+             dim3((unsigned)std::min<int64_t>(blocks, 1 << 30), (unsigned)cuts), 256, 0, a, (int)pieces);
 }
 
 template <int DT>
@@ -284,43 +289,40 @@ struct SumArgs {
     float* tail;  // [windows][dim] sums of one that begins here and goes on
 };
 
-// Columns of a segment that a lane has: N adjacent ones with 16-byte
-// accesses, otherwise N of them 32 apart.
-template <int DT, bool VEC>
+// Columns of a segment that a lane has: N (16 bytes), in accesses of B bytes
+// that lie 32 lanes apart.
+template <int DT, int B>
 struct Columns {
     using E = Elem<DT>;
     using T = typename E::T;
+    using V = typename Bytes<B>::T;
     static constexpr int N = 16 / (int)sizeof(T);
+    static constexpr int kEach = B / (int)sizeof(T);  // columns of an access
     static constexpr int kSegment = 32 * N;
     int64_t c0, dim;
-    __device__ Columns(int64_t segment, int64_t dim) : c0(segment * kSegment + (VEC ? N : 1) * (threadIdx.x & 31)), dim(dim) {}
-    __device__ __forceinline__ int64_t col(int i) const { return c0 + (VEC ? i : 32 * i); }
+    __device__ Columns(int64_t segment, int64_t dim)
+        : c0(segment * kSegment + kEach * (threadIdx.x & 31)), dim(dim) {}
+    __device__ __forceinline__ int64_t col(int i) const { return c0 + i / kEach * (32 * kEach) + i % kEach; }
     __device__ __forceinline__ void load(const T* row, T (&v)[N]) const {
-        if constexpr (VEC) {
-            if (c0 < dim) *reinterpret_cast<uint4*>(v) = __ldg(reinterpret_cast<const uint4*>(row + c0));
-        } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (col(i) < dim) v[i] = row[col(i)];
-        }
+        for (int i = 0; i < N; i += kEach)
+            if (col(i) < dim) *reinterpret_cast<V*>(v + i) = __ldg(reinterpret_cast<const V*>(row + col(i)));
     }
     __device__ __forceinline__ void store(T* row, const float (&s)[N], float scale) const {
         alignas(16) T v[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = E::put(s[i] * scale);
-        if constexpr (VEC) {
-            if (c0 < dim) *reinterpret_cast<uint4*>(row + c0) = *reinterpret_cast<uint4*>(v);
-        } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (col(i) < dim) row[col(i)] = v[i];
-        }
+        for (int i = 0; i < N; i += kEach)
+            if (col(i) < dim) *reinterpret_cast<V*>(row + col(i)) = *reinterpret_cast<V*>(v + i);
     }
+    // fp32 scratch, whose rows are dim long: 16-byte accesses where rows allow
+    static constexpr int kWide = B == 16 ? 4 : 1;
     __device__ __forceinline__ void load32(const float* row, float (&s)[N]) const {
 #pragma unroll
-        for (int i = 0; i < N; i += VEC ? 4 : 1)
+        for (int i = 0; i < N; i += kWide)
             if (col(i) < dim) {
-                if constexpr (VEC) {
+                if constexpr (kWide == 4) {
                     const float4 f = *reinterpret_cast<const float4*>(row + col(i));
                     s[i] = f.x, s[i + 1] = f.y, s[i + 2] = f.z, s[i + 3] = f.w;
                 } else {
@@ -330,9 +332,9 @@ struct Columns {
     }
     __device__ __forceinline__ void store32(float* row, const float (&s)[N]) const {
 #pragma unroll
-        for (int i = 0; i < N; i += VEC ? 4 : 1)
+        for (int i = 0; i < N; i += kWide)
             if (col(i) < dim) {
-                if constexpr (VEC)
+                if constexpr (kWide == 4)
                     *reinterpret_cast<float4*>(row + col(i)) = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
                 else
                     row[col(i)] = s[i];
@@ -353,12 +355,25 @@ __device__ __forceinline__ int lower_bound(const uint2* pair, int n, uint32_t v)
     return lo;
 }
 
-// The first zero_blocks blocks write zeros to the rows, of 256 entries each,
-// that no token names (first, so that their searches overlap the sums); the
-// others sum the windows, a warp per window and segment.
-template <int DT, bool VEC>
-__global__ void __launch_bounds__(256, 3) sum_kernel(SumArgs a, int64_t zero_blocks) {
-    using C = Columns<DT, VEC>;
+// Zeros to a row of any alignment.
+template <int DT>
+__device__ __forceinline__ void zero_row(typename Elem<DT>::T* row, int64_t dim, int lane) {
+    using T = typename Elem<DT>::T;
+    constexpr int N = 16 / (int)sizeof(T);
+    const int64_t head = min(dim, (int64_t)((-reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T)));
+    const int64_t body = (dim - head) / N, tail = head + body * N;
+    if (lane < head) row[lane] = Elem<DT>::put(0.0f);
+    uint4* p = reinterpret_cast<uint4*>(row + head);
+    for (int64_t i = lane; i < body; i += 32) p[i] = make_uint4(0, 0, 0, 0);
+    if (tail + lane < dim) row[tail + lane] = Elem<DT>::put(0.0f);
+}
+
+// The first zero_blocks blocks write zeros to the rows, of zero_rows entries
+// each, that no token names (first, so that their searches overlap the
+// sums); the others sum the windows, a warp per window and segment.
+template <int DT, int B>
+__global__ void __launch_bounds__(256, 3) sum_kernel(SumArgs a, int64_t zero_blocks, int zero_rows) {
+    using C = Columns<DT, B>;
     using T = typename C::T;
     constexpr int N = C::N;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -366,19 +381,16 @@ __global__ void __launch_bounds__(256, 3) sum_kernel(SumArgs a, int64_t zero_blo
     griddep_wait();
     if (blockIdx.x < zero_blocks) {
         __shared__ bool empty[256];
-        const int64_t v0 = (int64_t)blockIdx.x * 256, v = v0 + threadIdx.x;
+        const int64_t v0 = (int64_t)blockIdx.x * zero_rows, v = v0 + threadIdx.x;
         bool none = false;
-        if (v < a.vocab) {
+        if (threadIdx.x < zero_rows && v < a.vocab) {
             const int at = lower_bound(a.pair, a.n, (uint32_t)v);
             none = at == a.n || a.pair[at].x != (uint32_t)v;
         }
         empty[threadIdx.x] = none;
         __syncthreads();
-        const float zero[N] = {};
-        for (int r = warp; r < 256; r += 8)
-            if (empty[r])
-                for (int64_t s = 0; s < a.segments; ++s)
-                    C(s, a.dim).store(static_cast<T*>(a.d_table) + (v0 + r) * a.dim, zero, 1.0f);
+        for (int r = warp; r < zero_rows; r += 8)
+            if (empty[r]) zero_row<DT>(static_cast<T*>(a.d_table) + (v0 + r) * a.dim, a.dim, lane);
         return;
     }
     const int64_t task = (blockIdx.x - zero_blocks) * 8 + warp;
@@ -429,9 +441,9 @@ __global__ void __launch_bounds__(256, 3) sum_kernel(SumArgs a, int64_t zero_blo
 // Adds the parts of the runs that begin in windows 8 blockIdx.x .. + 7 and
 // go past their end.  A run of up to 32 windows more is its warp's own work;
 // for a longer one the block's warps take equal stretches of its windows.
-template <int DT, bool VEC>
+template <int DT, int B>
 __global__ void __launch_bounds__(256, 3) join_kernel(SumArgs a) {
-    using C = Columns<DT, VEC>;
+    using C = Columns<DT, B>;
     using T = typename C::T;
     constexpr int N = C::N;
     __shared__ float part[8][32][N + 1];
@@ -501,14 +513,16 @@ __global__ void __launch_bounds__(256, 3) join_kernel(SumArgs a) {
     }
 }
 
-template <int DT, bool VEC>
+template <int DT, int B>
 void sum_rows(SumArgs a, Queue& q) {
     const int64_t sum_blocks = ((int64_t)a.windows * a.segments + 7) / 8;
-    const int64_t zero_blocks = (a.vocab + 255) / 256, blocks = zero_blocks + sum_blocks;
+    // as many blocks for the empty rows as fill the card, up to 256 rows each
+    const int zero_rows = (int)std::clamp<int64_t>(a.vocab / (148 * 4) / 8 * 8, 8, 256);
+    const int64_t zero_blocks = (a.vocab + zero_rows - 1) / zero_rows, blocks = zero_blocks + sum_blocks;
     need(blocks < (int64_t(1) << 31) && a.segments <= 65535, "n times dim is too large");
-    q.launch("sum_kernel", sum_kernel<DT, VEC>, dim3((unsigned)blocks), 256, 0, a, zero_blocks);
+    q.launch("sum_kernel", sum_kernel<DT, B>, dim3((unsigned)blocks), 256, 0, a, zero_blocks, zero_rows);
     if (a.windows > 1)
-        q.launch("join_kernel", join_kernel<DT, VEC>, dim3((unsigned)((a.windows + 7) / 8), (unsigned)a.segments), 256,
+        q.launch("join_kernel", join_kernel<DT, B>, dim3((unsigned)((a.windows + 7) / 8), (unsigned)a.segments), 256,
                  0, a);
 }
 
@@ -552,7 +566,6 @@ void embed_backward(const mg_embed_backward_args& a, Workspace& w, bool go, Queu
     for (int i = 0; i < 2; ++i) sort_args.pair[i] = w.take<uint2>((size_t)a.n * 8);
     sort_args.place = w.take<uint32_t>((size_t)a.n * 4);
     sort_args.counts = w.take<uint32_t>((size_t)sort_args.blocks * 4 << sort_args.bits);
-    const bool vec = widest(e, a.dim * e, a.grad_row * e, 0, a.grad, a.d_table) == 16;
     SumArgs sum{};
     sum.n = (int)a.n;
     const int segment = 32 * 16 / e;
@@ -572,8 +585,13 @@ void embed_backward(const mg_embed_backward_args& a, Workspace& w, bool go, Queu
     sum.vocab = a.vocab;
     sum.scale = a.scale;
     sum.d_table = a.d_table;
-    if (vec) sum_rows<DT, true>(sum, q);
-    else sum_rows<DT, false>(sum, q);
+    switch (widest(e, a.dim * e, a.grad_row * e, 0, a.grad, a.d_table)) {
+        case 16: return sum_rows<DT, 16>(sum, q);
+        case 8: return sum_rows<DT, 8>(sum, q);
+        case 4: return sum_rows<DT, 4>(sum, q);
+        default:
+            if constexpr (DT != MG_PREC_FP32) sum_rows<DT, 2>(sum, q);
+    }
 }
 
 void embed_backward(const mg_embed_backward_args& a, Workspace& w, bool go, Queue& q) {

@@ -42,7 +42,6 @@ constexpr int kEpiWarps = 8;
 constexpr int kThreads = 32 * (2 + kEpiWarps);
 constexpr int kPairs = 74;             // of SMs on a B200 (148)
 constexpr int kGroup = 8;              // row tiles walked together (their B tiles stay in L2)
-constexpr int kStagePitch = 34;        // 16-bit elements per row staged without TMA (17 words: no bank conflicts)
 constexpr int kBlockBytes = 4096;      // 32 rows of 128 bytes: 64 columns of 16 bits or 32 of fp32
 constexpr int kWarpBytes = 2 * kBlockBytes;  // per epilogue warp
 
@@ -234,48 +233,59 @@ struct WarpBlocks {
     }
 };
 
-// The same blocks for matrices that no tensor map describes (any strides and
-// alignment): a row at a time, coalesced, through a staging block.
-template <int DT>
-__device__ __forceinline__ void load_block(const void* base, int64_t row, int64_t col, int rows, int cols, int lane,
-                                           uint16_t* stage, float (&v)[32]) {
-    const uint16_t* p = static_cast<const uint16_t*>(base);
+// A block from or to a matrix that no tensor map describes (any strides and
+// alignment): a row at a time, so that the warp's accesses are in order.
+__device__ __forceinline__ void load_rows(uint8_t* block, const uint16_t* p, int64_t row, int64_t col, int rows,
+                                          int cols, int lane) {
     __syncwarp();
 #pragma unroll 8
     for (int r = 0; r < 32; ++r)
-        if (r < rows && lane < cols) stage[r * kStagePitch + lane] = p[r * row + lane * col];
-    __syncwarp();
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(stage + lane * kStagePitch);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const float2 f = unpack2<DT>(w[i]);
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-    }
+        for (int k = 0; k < 2; ++k) {
+            const int c = lane + 32 * k;
+            if (r < rows && c < cols)
+                *reinterpret_cast<uint16_t*>(block + swizzle128(r, c >> 3) + (c & 7) * 2) = p[r * row + c * col];
+        }
+    __syncwarp();
 }
 
-template <int DT>
-__device__ __forceinline__ void store_block(void* base, int64_t row, int rows, int cols, int lane, uint16_t* stage,
-                                            const float (&v)[32]) {
-    uint16_t* p = static_cast<uint16_t*>(base);
-    __syncwarp();
-    uint32_t* w = reinterpret_cast<uint32_t*>(stage + lane * kStagePitch);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = pack2<DT>(v[2 * i], v[2 * i + 1]);
-    __syncwarp();
-    if ((((uint32_t)row | (uint32_t)cols) & 1) == 0 && (reinterpret_cast<uintptr_t>(p) & 3) == 0) {
-        // two rows at a time, 4 bytes per lane
-        const int c = (lane & 15) * 2;
-#pragma unroll 8
-        for (int r = lane >> 4; r < 32; r += 2)
-            if (r < rows && c < cols)
-                *reinterpret_cast<uint32_t*>(p + r * row + c) =
-                    *reinterpret_cast<const uint32_t*>(stage + r * kStagePitch + c);
+// Two elements per lane; rows that begin off a 4-byte boundary are shifted by
+// one element between the lanes, and their first and last go on their own.
+__device__ __forceinline__ void store_row(uint16_t* q, uint32_t w, bool odd, int cols, int lane) {
+    const int c = 2 * lane;
+    if (!odd) {
+        if (c + 1 < cols) *reinterpret_cast<uint32_t*>(q + c) = w;
+        else if (c < cols) q[c] = (uint16_t)w;
         return;
     }
-#pragma unroll 8
-    for (int r = 0; r < 32; ++r)
-        if (r < rows && lane < cols) p[r * row + lane] = stage[r * kStagePitch + lane];
+    const uint32_t up = __byte_perm(w, __shfl_down_sync(~0u, w, 1), 0x5432);  // elements c + 1, c + 2
+    if (c + 2 < cols) *reinterpret_cast<uint32_t*>(q + c + 1) = up;
+    // of an even number of columns the last one's place is its lane's second
+    const bool last = c + 2 == cols;
+    if (lane == 0 || last) q[last && lane > 0 ? c + 1 : 0] = (uint16_t)(last && lane > 0 ? w >> 16 : w);
+    if (lane == 0 && last) q[1] = (uint16_t)(w >> 16);
+}
+
+__device__ __forceinline__ void store_rows(const uint8_t* block, uint16_t* p, int64_t row, int rows, int cols,
+                                           int lane) {
+    __syncwarp();
+    const bool odd = (reinterpret_cast<uintptr_t>(p) & 2) != 0, turns = (row & 1) != 0;  // from row to row
+    const uint32_t at = smem_u32(block) + (lane & 3) * 4;
+    const auto word = [&](int r) {
+        uint32_t w;
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at + swizzle128(r, lane >> 2)));
+        return w;
+    };
+    if (rows == 32 && cols == 64) {
+#pragma unroll 4
+        for (int r = 0; r < 32; r += 2, p += 2 * row) {
+            const uint32_t w0 = word(r), w1 = word(r + 1);
+            store_row(p, w0, odd, 64, lane);
+            store_row(p + row, w1, odd != turns, 64, lane);
+        }
+        return;
+    }
+    for (int r = 0; r < rows; ++r, p += row) store_row(p, word(r), odd != (turns && (r & 1)), cols, lane);
 }
 
 __device__ __forceinline__ void activate_all(float (&v)[32], int act) {
@@ -345,8 +355,14 @@ __device__ __forceinline__ bool epilogue(const KernelArgs& a, int job, const Epi
     for (int c = 0; c < width; c += 32) {
         const int col = t.n0 + c0 + c, h = c >> 5 & 1;
         const bool ends = h == 1 || c + 32 >= width;  // of a chunk of 64 columns
-        if (j.by_tma && !j.has_out32 && h == 0) {
-            if (j.has_z) {
+        const int cols = min(64, width - c);
+        if (!j.has_out32 && h == 0) {
+            if (!j.by_tma) {
+                blocks.settle<0>();
+                if (j.has_res)
+                    load_rows(blocks.at(blocks.next), static_cast<const uint16_t*>(e.res) + m0 * e.r_row + col * e.r_col,
+                              e.r_row, e.r_col, rows, cols, lane);
+            } else if (j.has_z) {
                 blocks.settle<0>();
             } else if (j.has_res) {
                 if (!blocks.wait_res(blocks.next, a.err, kErrWaitEpilogue)) return false;
@@ -382,56 +398,45 @@ __device__ __forceinline__ bool epilogue(const KernelArgs& a, int job, const Epi
             continue;
         }
         add_bias<DT>(v, j.alpha, sbias + c);
-        if (j.by_tma) {
-            const auto word = [&](int i) { return pack2<DT>(v[2 * i], v[2 * i + 1]); };
-            const int col64 = col - 32 * h;
-            if (j.has_z) blocks.write16(blocks.next ^ 1, h, word);
-            activate_all(v, j.act);
-            if (j.has_res) {
-                uint4 u[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    if (!j.has_z)
-                        u[q] = *reinterpret_cast<const uint4*>(blocks.at(blocks.next) + swizzle128(lane, 4 * h + q));
-                    else if (lane < rows && c + 8 * q < width)
-                        u[q] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(e.res) +
-                                                                    (int64_t)(m0 + lane) * e.r_row + col + 8 * q));
-                    else
-                        u[q] = make_uint4(0, 0, 0, 0);
-                }
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const uint32_t w[4] = {u[q].x, u[q].y, u[q].z, u[q].w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 f = unpack2<DT>(w[i]);
-                        v[q * 8 + 2 * i] += j.res_scale * f.x;
-                        v[q * 8 + 2 * i + 1] += j.res_scale * f.y;
-                    }
-                }
-            }
-            blocks.write16(blocks.next, h, word);
-            if (ends) {
-                if (j.has_z) blocks.store(blocks.next ^ 1, &a.tz, col64, m0);
-                blocks.store(blocks.next, &a.to[job], col64, m0);
-                blocks.next ^= 1;
-            }
-            continue;
-        }
-        blocks.settle<0>();
-        const int cols = min(32, width - c);
-        uint16_t* stage = reinterpret_cast<uint16_t*>(blocks.blocks);
-        if (j.has_z)
-            store_block<DT>(static_cast<uint16_t*>(e.z) + (int64_t)m0 * e.ld + col, e.ld, rows, cols, lane, stage, v);
+        const auto word = [&](int i) { return pack2<DT>(v[2 * i], v[2 * i + 1]); };
+        const int col64 = col - 32 * h;
+        if (j.has_z) blocks.write16(blocks.next ^ 1, h, word);
         activate_all(v, j.act);
         if (j.has_res) {
-            float x[32];
-            load_block<DT>(static_cast<const uint16_t*>(e.res) + m0 * e.r_row + col * e.r_col, e.r_row, e.r_col, rows,
-                           cols, lane, stage, x);
+            uint4 u[4];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] += j.res_scale * x[i];
+            for (int q = 0; q < 4; ++q) {
+                if (!(j.has_z && j.by_tma))
+                    u[q] = *reinterpret_cast<const uint4*>(blocks.at(blocks.next) + swizzle128(lane, 4 * h + q));
+                else if (lane < rows && c + 8 * q < width)
+                    u[q] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(e.res) +
+                                                                (int64_t)(m0 + lane) * e.r_row + col + 8 * q));
+                else
+                    u[q] = make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t w[4] = {u[q].x, u[q].y, u[q].z, u[q].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = unpack2<DT>(w[i]);
+                    v[q * 8 + 2 * i] += j.res_scale * f.x;
+                    v[q * 8 + 2 * i + 1] += j.res_scale * f.y;
+                }
+            }
         }
-        store_block<DT>(static_cast<uint16_t*>(e.out) + (int64_t)m0 * e.ld + col, e.ld, rows, cols, lane, stage, v);
+        blocks.write16(blocks.next, h, word);
+        if (!ends) continue;
+        if (j.by_tma) {
+            if (j.has_z) blocks.store(blocks.next ^ 1, &a.tz, col64, m0);
+            blocks.store(blocks.next, &a.to[job], col64, m0);
+        } else {
+            const int64_t at = (int64_t)m0 * e.ld + col64;
+            const int stored = min(64, width - (c - 32 * h));
+            if (j.has_z) store_rows(blocks.at(blocks.next ^ 1), static_cast<uint16_t*>(e.z) + at, e.ld, rows, stored, lane);
+            store_rows(blocks.at(blocks.next), static_cast<uint16_t*>(e.out) + at, e.ld, rows, stored, lane);
+        }
+        blocks.next ^= 1;
     }
     return true;
 }
@@ -892,7 +897,7 @@ StagedOperand stage_operand(Workspace& w, Packs& packs, const GemmOperand& op, i
     t.ld = s.ld = up8(t.len);
     t.in = static_cast<const uint16_t*>(op.data);
     t.out = w.take<uint16_t>((size_t)t.lines * t.ld * 2);
-    t.blocks = (int)std::min<int64_t>((t.lines * ((t.len + 255) / 256) + 7) / 8, 148 * 6);
+    t.blocks = (int)std::min<int64_t>((t.lines * ((t.len + 511) / 512) + 7) / 8, 148 * 6);
     s.data = t.out;
     return s;
 }

@@ -113,25 +113,37 @@ struct Packs {
     void launch(Queue& q) const;  // on their own, if there are any
 };
 
-// The share of block `block` (0 .. blocks() - 1): a warp per line and 256
-// columns, eight loads per lane in flight.
+// The share of block `block` (0 .. blocks() - 1): a warp per line and 512
+// columns, 16 bytes per lane and store.
 __device__ __forceinline__ void pack_block(const Packs& packs, int block) {
     int i = 0;
     while (block >= packs.task[i].blocks) block -= packs.task[i++].blocks;
     const PackTask& t = packs.task[i];
     const int warps = blockDim.x >> 5;
-    const int64_t across = (t.len + 255) / 256, tasks = t.lines * across;
+    const int64_t across = (t.len + 511) / 512, tasks = t.lines * across;
+    const int64_t line = t.line, len = t.len, step = t.step, ld = t.ld, span = (t.lines - 1) * line + len;
+    const uint16_t* const in = t.in;
+    uint16_t* const out = t.out;
     for (int64_t at = (int64_t)block * warps + (threadIdx.x >> 5); at < tasks; at += (int64_t)t.blocks * warps) {
-        const int64_t r = at / across, c = at % across * 256 + (threadIdx.x & 31);
-        const uint16_t* in = t.in + r * t.line;
-        uint16_t* out = t.out + r * t.ld;
-        uint16_t v[8];
+        const int64_t r = at / across, c = at % across * 512 + (threadIdx.x & 31) * 8;
+        uint4 v[2];
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (c + 32 * k < t.len) v[k] = in[(c + 32 * k) * t.step];
+        for (int k = 0; k < 2; ++k) {
+            const int64_t col = c + 256 * k;
+            if (col >= len) continue;
+            if (step == 1) {
+                v[k] = load8_unaligned(in + r * line + col, r * line + col, span);
+            } else {
+                uint32_t h[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (c + 32 * k < t.len) out[c + 32 * k] = v[k];
+                for (int e = 0; e < 8; ++e) h[e] = col + e < len ? in[r * line + (col + e) * step] : 0;
+                v[k] = make_uint4(__byte_perm(h[0], h[1], 0x5410), __byte_perm(h[2], h[3], 0x5410),
+                                  __byte_perm(h[4], h[5], 0x5410), __byte_perm(h[6], h[7], 0x5410));
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (c + 256 * k < len) *reinterpret_cast<uint4*>(out + r * ld + c + 256 * k) = v[k];
     }
 }
 
