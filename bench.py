@@ -322,8 +322,13 @@ def run_reference(args, wl):
 
     sd = weights.make_state_dict(board, filters, blocks, seed=0, variant="init")
     # the reference's own src/game.cpp generates the positions (bit-identical
-    # to the product's generator; the reference arm maps no product library)
-    x = oracle.ref_random_positions(board, batch, 1000, max_moves)
+    # to the product's generator; the reference arm maps no product library
+    # where a reference tree was there to build it from)
+    if oracle.ref_available():
+        x = oracle.ref_random_positions(board, batch, 1000, max_moves)
+    else:
+        from alphazero_b200 import host_lib
+        x = host_lib.random_positions(board, batch, 1000, max_moves)
     threads = os.cpu_count() or 1
     orc = oracle.EigenOracle(sd)
     t0 = time.perf_counter()
