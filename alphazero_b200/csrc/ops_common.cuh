@@ -47,6 +47,19 @@ __device__ __forceinline__ int64_t index_at(const void* p, int bytes, int64_t i,
     return t >= 0 && t < limit ? t : -1;
 }
 
+// Targets (or any indices) as the caller keeps them.
+struct Indices {
+    const void* data = nullptr;
+    int64_t stride = 0, limit = 0;
+    int bytes = 8;
+    __device__ __forceinline__ int at(int64_t i) const { return (int)index_at(data, bytes, i * stride, limit); }
+    Indices from(int64_t first) const {
+        Indices r = *this;
+        r.data = static_cast<const char*>(data) + first * stride * bytes;
+        return r;
+    }
+};
+
 // Eight 16-bit elements from p on, which is element `at` of memory that holds
 // elements [0, span); what lies past it comes back as anything.  16 bytes at
 // any alignment by 32-bit loads, as far as those stay inside.

@@ -28,29 +28,23 @@ constexpr size_t kPieceBytes = size_t(1) << 30;
 template <int DT>
 constexpr float kDScale = DT == MG_PREC_FP16 ? 16384.0f : 1.0f;
 
+// The number of counted rows, per block: only where there are several pieces
+// (else combine_kernel counts).
 constexpr int kCountBlocks = 148;
 
-// target[i] (-1: not counted), and their number per block; blocks past
-// `blocks` copy operands.
-__global__ void __launch_bounds__(1024)
-    target_kernel(mg_cross_entropy_args a, int* target, int* counts, int blocks, Packs packs) {
-    __shared__ int part[32];
+__global__ void __launch_bounds__(1024) count_kernel(Indices target, int64_t n, int* counts) {
     griddep_launch_dependents();
     griddep_wait();
-    if (blockIdx.x >= blocks) return pack_block(packs, blockIdx.x - blocks);
     int c = 0;
-    for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < a.n; i += (int64_t)blocks * 1024) {
-        const int t = (int)index_at(a.targets, a.target_bytes, i * a.target_stride, a.vocab);
-        target[i] = t;
-        c += t >= 0;
-    }
+    for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 1024)
+        c += target.at(i) >= 0;
     c = __reduce_add_sync(~0u, c);
+    __shared__ int part[32];
     if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = c;
     __syncthreads();
-    if (threadIdx.x < 32) {
-        c = __reduce_add_sync(~0u, part[threadIdx.x]);
-        if (threadIdx.x == 0) counts[blockIdx.x] = c;
-    }
+    if (threadIdx.x >= 32) return;
+    c = __reduce_add_sync(~0u, part[threadIdx.x]);
+    if (threadIdx.x == 0) counts[blockIdx.x] = c;
 }
 
 // (m, s) of a sum s exp(m) joined with another's.
@@ -63,27 +57,20 @@ __device__ __forceinline__ void join(float& m, float& s, float2 p) {
 // logsumexp and loss per row, and the loss summed per block: a thread per row
 // where a row has few blocks of columns; with many, 32 threads per row, or
 // where there are few rows too, a block per row.
-// A row of -inf has lse -inf.  counts, if set: their sum goes to count.
+// A row of -inf has lse -inf.  counts, if set: the counted rows per block.
 enum Combine : int { kThreadPerRow, kWarpPerRow, kBlockPerRow };
 constexpr int kFewBlocks = 16;
 
 template <Combine HOW>
 __global__ void __launch_bounds__(HOW == kThreadPerRow ? 128 : 1024)
-    combine_kernel(int64_t rows, int blocks, const float2* part, int64_t part_ld, const int* target,
-                   const float* logit, float* lse, float* row_loss, float* loss_part, const int* counts,
-                   int count_blocks, int* count) {
+    combine_kernel(int64_t rows, int blocks, const float2* part, int64_t part_ld, Indices target,
+                   const float* logit, float* lse, float* row_loss, float* loss_part, int* counts) {
     constexpr bool FEW = HOW == kThreadPerRow;
     __shared__ float2 tile[FEW ? 1 : 32][33];
     __shared__ float losses[FEW ? 128 : 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     griddep_launch_dependents();
     griddep_wait();
-    if (counts != nullptr && blockIdx.x == 0 && warp == 0) {
-        int c = 0;
-        for (int i = lane; i < count_blocks; i += 32) c += counts[i];
-        c = __reduce_add_sync(~0u, c);
-        if (lane == 0) *count = c;
-    }
     constexpr int kRows = FEW ? 128 : HOW == kBlockPerRow ? 1 : 32;
     const int64_t row0 = (int64_t)blockIdx.x * kRows;
     const int64_t row = row0 + (FEW ? threadIdx.x : HOW == kBlockPerRow ? 0 : warp);
@@ -122,27 +109,35 @@ __global__ void __launch_bounds__(HOW == kThreadPerRow ? 128 : 1024)
         join_lanes();
     }
     float loss = 0.0f;
+    bool counted = false;
     if (row < rows) {
         const float l = s == 0.0f ? -INFINITY : m + logf(s);
-        const float at = target[row] < 0 ? 0.0f : logit[row];
-        loss = target[row] < 0 ? 0.0f : at == -INFINITY ? INFINITY : l - at;
+        counted = target.at(row) >= 0;
+        const float at = counted ? logit[row] : 0.0f;
+        if (counted) loss = at == -INFINITY ? INFINITY : l - at;
         if (FEW || lane == 0) {  // (a block per row: every warp has the row, and writes the same)
             lse[row] = l;
             row_loss[row] = loss;
         }
     }
     if constexpr (HOW == kBlockPerRow) {
-        if (threadIdx.x == 0) loss_part[blockIdx.x] = loss;
+        if (threadIdx.x == 0) {
+            loss_part[blockIdx.x] = loss;
+            if (counts) counts[blockIdx.x] = counted;
+        }
         return;
     }
     losses[FEW ? threadIdx.x : warp] = loss;
-    __syncthreads();
+    const int all = __syncthreads_count(counted) / (FEW ? 1 : 32);
     if (warp > 0) return;
     loss = 0.0f;
     for (int i = lane; i < kRows; i += 32) loss += losses[i];
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) loss += __shfl_xor_sync(~0u, loss, d);
-    if (lane == 0) loss_part[blockIdx.x] = loss;
+    if (lane == 0) {
+        loss_part[blockIdx.x] = loss;
+        if (counts) counts[blockIdx.x] = all;
+    }
 }
 
 // probs (Prob16, per block of `block` columns) -> d = (softmax - onehot) in
@@ -151,34 +146,46 @@ __global__ void __launch_bounds__(HOW == kThreadPerRow ? 128 : 1024)
 // (up to 4 KB of a row at once: with one, 512 bytes, the same work ran at two
 // thirds of the speed), the others take further rows.  The factor from the
 // block's maximum to the row's logsumexp is one exp per thread and row.
+// Block 0 also adds up counts, if set, to count.
 template <int DT>
 __global__ void __launch_bounds__(256)
-    d_kernel(int64_t rows, int64_t vocab, int block, uint16_t* probs, int64_t ld, const float2* part,
-             int64_t part_ld, const float* lse, const int* target, int wide, int rows_per_block, float* sums) {
+    d_kernel(int rows, int64_t vocab, int block, uint16_t* probs, int64_t ld, const float2* part, int64_t part_ld,
+             const float* lse, Indices target, int wide, int rows_per_block, float* sums, const int* counts,
+             int64_t counts_n, int* count) {
     using E = Elem<DT>;
     using T = typename E::T;
     __shared__ float acc[8][256];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int deep = 8 / wide, down = warp / wide;
     const int64_t c = ((int64_t)blockIdx.x * wide + warp % wide) * 256 + lane * 8;
-    const int64_t r0 = (int64_t)blockIdx.y * rows_per_block, r1 = min(rows, r0 + rows_per_block);
+    const int r0 = blockIdx.y * rows_per_block, r1 = min(rows, r0 + rows_per_block);
     float sum[8] = {};
     griddep_launch_dependents();
     griddep_wait();
+    if (counts != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && warp == 0) {
+        int n = 0;
+        for (int64_t i = lane; i < counts_n; i += 32) n += counts[i];
+        n = __reduce_add_sync(~0u, n);
+        if (lane == 0) *count = n;
+    }
     if (c < vocab) {
         const float2* mine = part + c / block * part_ld;
+        const int64_t step = deep * ld;
+        uint16_t* p = probs + (int64_t)(r0 + down) * ld + c;
+        const int column = (int)c;
         // four rows at a time, their loads before the first store (which, for
         // all that is known, might be to what they read)
         constexpr int kRows = 4;
-        for (int64_t r = r0 + down; r < r1; r += deep * kRows) {
+        for (int r = r0 + down; r < r1; r += deep * kRows, p += kRows * step) {
             uint4 u[kRows];
             int t[kRows];
             float f[kRows], m[kRows];
 #pragma unroll
             for (int q = 0; q < kRows; ++q) {
-                const int64_t row = min(r + deep * q, r1 - 1);
-                u[q] = *reinterpret_cast<const uint4*>(probs + row * ld + c);
-                t[q] = target[row];
+                const int row = r + deep * q;
+                if (row >= r1) continue;
+                u[q] = *reinterpret_cast<const uint4*>(p + q * step);
+                t[q] = target.at(row);
                 f[q] = lse[row];
                 m[q] = mine[row].x;
             }
@@ -187,23 +194,26 @@ __global__ void __launch_bounds__(256)
                 if (r + deep * q >= r1) break;
                 const uint32_t w[4] = {u[q].x, u[q].y, u[q].z, u[q].w};
                 // a row that is not counted (whatever it holds) and one of -inf have no probabilities
-                const float p = f[q] == -INFINITY || t[q] < 0 ? 0.0f : exp2f((m[q] - f[q]) * 1.4426950408889634f);
-                const float scale = p * 0x1p112f;  // prob16_value's
+                float scale = exp2_flush((m[q] - f[q]) * 1.4426950408889634f) * 0x1p112f;  // prob16_value's
+                if (f[q] == -INFINITY || t[q] < 0) scale = 0.0f;
                 float v[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    v[i] = __uint_as_float(i & 1 ? w[i / 2] >> 16 << 11 : (w[i / 2] & 0xffffu) << 11) * scale;
-                if (t[q] >= c && t[q] < c + 8)
+                for (int i = 0; i < 4; ++i) {
+                    v[2 * i] = __uint_as_float((w[i] << 11) & 0x07fff800u) * scale;
+                    v[2 * i + 1] = __uint_as_float((w[i] >> 5) & 0x07fff800u) * scale;
+                }
+                const uint32_t hot = (uint32_t)(t[q] - column);
+                if (hot < 8 && t[q] >= 0)
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        if (t[q] == c + i) v[i] -= 1.0f;
+                        if (hot == i) v[i] -= 1.0f;
+                if (sums != nullptr)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sum[i] += v[i];
                 alignas(16) T d[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    sum[i] += v[i];
-                    d[i] = E::put(v[i] * kDScale<DT>);
-                }
-                *reinterpret_cast<uint4*>(probs + (r + deep * q) * ld + c) = *reinterpret_cast<uint4*>(d);
+                for (int i = 0; i < 8; ++i) d[i] = E::put(v[i] * kDScale<DT>);
+                *reinterpret_cast<uint4*>(p + q * step) = *reinterpret_cast<uint4*>(d);
             }
         }
     }
@@ -249,9 +259,11 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
     const int blocks = (int)((a.vocab + block - 1) / block);
 
     int* count = w.take<int>(4);
-    int* counts = w.take<int>(kCountBlocks * 4);
-    const int count_blocks = (int)std::min<int64_t>(kCountBlocks, (a.n + 1023) / 1024);
-    int* target = w.take<int>((size_t)a.n * 4);
+    Indices target;
+    target.data = a.targets;
+    target.bytes = a.target_bytes;
+    target.stride = a.target_stride;
+    target.limit = a.vocab;
     float* logit = w.take<float>((size_t)piece * 4);
     float* lse = w.take<float>((size_t)piece * 4);
     float2* part = w.take<float2>((size_t)blocks * piece * 8);
@@ -270,10 +282,14 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
     const Combine how = blocks <= kFewBlocks ? kThreadPerRow : piece <= 2 * 148 ? kBlockPerRow : kWarpPerRow;
     const int64_t combine_rows = how == kThreadPerRow ? 128 : how == kBlockPerRow ? 1 : 32;
     float* loss_part = w.take<float>((size_t)((piece + combine_rows - 1) / combine_rows * count_pieces) * 4);
+    const bool apart = count_pieces > 1;  // rows counted by a kernel of their own
+    const int64_t counts_n = apart ? std::min<int64_t>(kCountBlocks, (a.n + 1023) / 1024)
+                                   : (piece + combine_rows - 1) / combine_rows;
+    int* counts = w.take<int>((size_t)counts_n * 4);
     if (go) {
         w.require();
-        q.launch("target_kernel", target_kernel, dim3(count_blocks + packs.blocks()), 1024, 0, a, target, counts,
-                 count_blocks, packs);
+        packs.launch(q);
+        if (apart) q.launch("count_kernel", count_kernel, dim3((unsigned)counts_n), 1024, 0, target, a.n, counts);
     }
     const float alpha = a.grad_scale / kDScale<DT>;
     int64_t sum_rows = 0, losses = 0;
@@ -292,28 +308,28 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
             f.n = a.vocab;
             f.k = a.dim;
             f.e.bias = a.bias;
-            f.e.target = target + row0;
+            f.e.target = target.from(row0);
             f.e.logit = logit;
             f.e.part = part;
             f.e.part_ld = piece;
             f.e.probs = probs;
             f.e.probs_ld = ld;
             gemm_softmax(DT, f, block, q);
-            const int* sum_of = first ? counts : nullptr;
             const int64_t combine_blocks = (rows + combine_rows - 1) / combine_rows;
             const auto kernel = how == kThreadPerRow  ? combine_kernel<kThreadPerRow>
                                 : how == kBlockPerRow ? combine_kernel<kBlockPerRow>
                                                       : combine_kernel<kWarpPerRow>;
             q.launch("combine_kernel", kernel, dim3((unsigned)combine_blocks), how == kThreadPerRow ? 128 : 1024, 0, rows,
-                     blocks, part, piece, target + row0, logit, lse, a.row_loss + row0, loss_part + losses, sum_of,
-                     count_blocks, count);
+                     blocks, part, piece, target.from(row0), logit, lse, a.row_loss + row0, loss_part + losses,
+                     apart ? nullptr : counts);
             losses += combine_blocks;
         }
         if (!grads) continue;
         const int64_t these = (rows + down_rows - 1) / down_rows;
         if (go) {
-            q.launch("d_kernel", d_kernel<DT>, dim3((unsigned)across, (unsigned)these), 256, 0, rows, a.vocab, block,
-                     probs, ld, part, piece, lse, target + row0, wide, down_rows, sums ? sums + sum_rows * a.vocab : nullptr);
+            q.launch("d_kernel", d_kernel<DT>, dim3((unsigned)across, (unsigned)these), 256, 0, (int)rows, a.vocab, block,
+                     probs, ld, part, piece, lse, target.from(row0), wide, down_rows,
+                     sums ? sums + sum_rows * a.vocab : nullptr, first ? counts : nullptr, counts_n, count);
         }
         sum_rows += these;
         StagedOperand d;
@@ -356,7 +372,7 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
         return;
     }
     if (a.db) post.add = AddRowsTask{sums, sum_rows, a.vocab, alpha * kDScale<DT>, count, a.db};
-    post.loss = LossTask{loss_part, losses, count, a.loss};
+    post.loss = LossTask{loss_part, losses, counts, counts_n, a.loss};
     post.launch(DT, q);
 }
 

@@ -701,7 +701,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 // what the tile needs besides its sums is on its way before they are complete
                 int target = -1, after_col = -1, after_row = 0;
                 if constexpr (EPI == kSoftmax) {
-                    if (m0 + lane < j.m) target = soft.target[m0 + lane];
+                    if (m0 + lane < j.m) target = soft.target.at(m0 + lane);
                 } else if (j.has_res && j.by_tma && !j.has_z) {
                     const auto mine = [&](const Tile& u, int* col, int* row) {
                         *row = u.m0 + (int)rank * kRowsCta + quarter * 32;
@@ -913,27 +913,33 @@ void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, Post& post
     KernelArgs a{};
     GemmEpilogue finish[2];
     double len[2] = {0, 0};
+    int64_t share = 0;  // K steps per pair, a tile's epilogue counted as 8
+    for (int i = 0; i < count; ++i) {
+        lay_out(a.job[i], jobs[i], bn);
+        share += (int64_t)a.job[i].tiles_m * a.job[i].tiles_n * std::max(8, a.job[i].kblocks);
+    }
+    share = (share + kPairs - 1) / kPairs;
     for (int i = 0; i < count; ++i) {
         JobArgs& j = a.job[i];
         const GemmJob& g = jobs[i];
-        lay_out(j, g, bn);
         j.e = finish[i] = g.e;
         // what tensor maps ask of the outputs and the residual
         j.by_tma = g.e.ld % 8 == 0 && aligned16(g.e.out) && aligned16(g.e.z) &&
                    (g.e.res == nullptr || (aligned16(g.e.res) && g.e.r_col == 1 && g.e.r_row % 8 == 0 &&
                                            g.e.r_row >= g.n && g.e.r_row < int64_t(1) << 38));
         const int64_t tiles = (int64_t)j.tiles_m * j.tiles_n;
-        // Few tiles: their K steps are shared out over the idle pairs, at least 8 steps each.
-        const int splits = tiles * 2 <= kPairs ? (int)std::min<int64_t>(kPairs / tiles, j.kblocks / 8) : 1;
-        j.kb_split = (j.kblocks + std::max(splits, 1) - 1) / std::max(splits, 1);
+        // Few tiles: their K steps are shared out, in units about as long as a pair's share
+        // of all the work (of no fewer than 8 steps, which an epilogue's time is worth).
+        if (tiles * 2 <= kPairs) j.kb_split = (int)std::min<int64_t>(j.kblocks, std::max<int64_t>(8, share));
         j.splits = (j.kblocks + j.kb_split - 1) / j.kb_split;
+        j.kb_split = (j.kblocks + j.splits - 1) / j.splits;
         if (j.splits > 1) {
             j.e = GemmEpilogue{};
             j.e.ld32 = up8(g.n);
             j.e.out32 = w.take<float>((size_t)j.splits * j.m_pad * j.e.ld32 * 4);
         }
         a.units[i] = (int)(tiles * j.splits);
-        len[i] = j.kb_split + 4.0;  // a tile's epilogue is worth a few K steps
+        len[i] = std::max(8, j.kb_split);
     }
     if (!go) return;
     w.require();

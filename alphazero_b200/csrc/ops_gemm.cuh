@@ -57,7 +57,7 @@ constexpr int kSkinnyRows = 16;
 // probs is set, probs[row * probs_ld + col] = exp(l - max) as a Prob16.
 struct SoftmaxEpilogue {
     const void* bias = nullptr;       // [n]
-    const int* target = nullptr;      // [m], -1 for none
+    Indices target;                   // [m]
     float* logit = nullptr;           // [m]
     float2* part = nullptr;
     int64_t part_ld = 0;
@@ -164,10 +164,11 @@ struct AddRowsTask {  // out[c] = alpha / max(*count, 1) * sum of `rows` rows of
     const int* count;
     void* out;
 };
-struct LossTask {  // loss = sum of part[0 .. n) / max(*count, 1)
+struct LossTask {  // loss = sum of part[0 .. n) / max(sum of counts[0 .. counts_n), 1)
     const float* part;
     int64_t n;
-    const int* count;
+    const int* counts;
+    int64_t counts_n;
     float* loss;
 };
 struct Post {

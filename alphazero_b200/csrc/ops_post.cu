@@ -90,17 +90,24 @@ __device__ __forceinline__ void add_rows_block(const AddRowsTask& t, int64_t blo
         Elem<DT>::put(s * (t.count ? t.alpha / (float)max(*t.count, 1) : t.alpha));
 }
 
-__device__ __forceinline__ void loss_block(const LossTask& t, float* shared) {
+__device__ __forceinline__ void loss_block(const LossTask& t, float2* shared) {
     float s = 0.0f;
+    int c = 0;
 #pragma unroll 4
     for (int64_t i = threadIdx.x; i < t.n; i += kPostThreads) s += t.part[i];
-    shared[threadIdx.x] = s;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < t.counts_n; i += kPostThreads) c += t.counts[i];
+    shared[threadIdx.x] = make_float2(s, __int_as_float(c));
     __syncthreads();
     for (int w = kPostThreads / 2; w > 0; w /= 2) {
-        if (threadIdx.x < w) shared[threadIdx.x] += shared[threadIdx.x + w];
+        if (threadIdx.x < w) {
+            const float2 x = shared[threadIdx.x], y = shared[threadIdx.x + w];
+            shared[threadIdx.x] =
+                make_float2(x.x + y.x, __int_as_float(__float_as_int(x.y) + __float_as_int(y.y)));
+        }
         __syncthreads();
     }
-    if (threadIdx.x == 0) *t.loss = shared[0] / (float)max(*t.count, 1);
+    if (threadIdx.x == 0) *t.loss = shared[0].x / (float)max(__float_as_int(shared[0].y), 1);
 }
 
 template <int DT>
@@ -115,7 +122,7 @@ __global__ void __launch_bounds__(kPostThreads) post_kernel(Post p) {
         block -= p.finish[i].blocks;
     }
     if (p.loss.loss != nullptr) {
-        if (block == 0) return loss_block(p.loss, reinterpret_cast<float*>(shared));
+        if (block == 0) return loss_block(p.loss, reinterpret_cast<float2*>(shared));
         --block;
     }
     if (p.add.out != nullptr) add_rows_block<DT>(p.add, block, reinterpret_cast<float*>(shared));

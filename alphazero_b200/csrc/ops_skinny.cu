@@ -81,7 +81,7 @@ __device__ __forceinline__ void finish(const SkinnyArgs& a, const float (&sums)[
         // 256 / TOKENS lanes per token, each with every so many-th column
         constexpr int kLanes = 256 / TOKENS, kEach = 128 / kLanes;
         const int token = threadIdx.x / kLanes, first = threadIdx.x % kLanes;
-        const int target = token < a.m ? e.target[token] : -1;
+        const int target = token < a.m ? e.target.at(token) : -1;
         float l[kEach], top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
@@ -129,9 +129,9 @@ __device__ __forceinline__ void finish(const SkinnyArgs& a, const float (&sums)[
 // TILES: tokens in eights.  SOFTMAX: statistics of the block's columns, else
 // the linear layer's epilogue.
 template <int DT, int TILES, bool SOFTMAX>
-__global__ void __launch_bounds__(256, TILES == 1 ? 3 : 4) skinny_kernel(SkinnyArgs a) {
+__global__ void __launch_bounds__(256, 3) skinny_kernel(SkinnyArgs a) {
     constexpr int kTokens = 8 * TILES;
-    constexpr int kAhead = TILES == 1 ? 4 : 2;  // steps of 32 elements of K in flight per warp
+    constexpr int kAhead = 4;  // steps of 32 elements of K whose W is in flight per warp
     __shared__ float sums[128][kTokens + 1];  // [warp * 16 + row][token]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
@@ -147,37 +147,28 @@ __global__ void __launch_bounds__(256, TILES == 1 ? 3 : 4) skinny_kernel(SkinnyA
 #pragma unroll
     for (int i = 0; i < TILES; ++i) x[i] = a.x + (int64_t)min(8 * i + g, a.m - 1) * a.ldx;
     float c[TILES][4] = {};
-    const auto multiply = [&](const uint4 (&u0)[kAhead], const uint4 (&u1)[kAhead], const uint4 (&v)[kAhead][TILES]) {
-#pragma unroll
-        for (int q = 0; q < kAhead; ++q)
-#pragma unroll
-            for (int i = 0; i < TILES; ++i) {
-                mma16816<DT>(c[i], u0[q].x, u1[q].x, u0[q].y, u1[q].y, v[q][i].x, v[q][i].y);
-                mma16816<DT>(c[i], u0[q].z, u1[q].z, u0[q].w, u1[q].w, v[q][i].z, v[q][i].w);
-            }
+    const auto multiply = [&](int i, uint4 u0, uint4 u1, uint4 v) {
+        mma16816<DT>(c[i], u0.x, u1.x, u0.y, u1.y, v.x, v.y);
+        mma16816<DT>(c[i], u0.z, u1.z, u0.w, u1.w, v.z, v.w);
     };
     int k = begin + 8 * t;
     for (; k - 8 * t + 32 * kAhead <= end; k += 32 * kAhead) {
-        uint4 u0[kAhead], u1[kAhead], v[kAhead][TILES];
+        uint4 u0[kAhead], u1[kAhead];
 #pragma unroll
         for (int q = 0; q < kAhead; ++q) {
             u0[q] = __ldg(reinterpret_cast<const uint4*>(w0 + k + 32 * q));
             u1[q] = __ldg(reinterpret_cast<const uint4*>(w1 + k + 32 * q));
-#pragma unroll
-            for (int i = 0; i < TILES; ++i) v[q][i] = __ldg(reinterpret_cast<const uint4*>(x[i] + k + 32 * q));
         }
-        multiply(u0, u1, v);
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q)
+#pragma unroll
+            for (int i = 0; i < TILES; ++i)
+                multiply(i, u0[q], u1[q], __ldg(reinterpret_cast<const uint4*>(x[i] + k + 32 * q)));
     }
-    if (k - 8 * t < end) {
-        uint4 u0[kAhead], u1[kAhead], v[kAhead][TILES];
+    for (; k - 8 * t < end; k += 32) {
+        const uint4 u0 = load8(w0, k, end), u1 = load8(w1, k, end);
 #pragma unroll
-        for (int q = 0; q < kAhead; ++q) {
-            u0[q] = load8(w0, k + 32 * q, end);
-            u1[q] = load8(w1, k + 32 * q, end);
-#pragma unroll
-            for (int i = 0; i < TILES; ++i) v[q][i] = load8(x[i], k + 32 * q, end);
-        }
-        multiply(u0, u1, v);
+        for (int i = 0; i < TILES; ++i) multiply(i, u0, u1, load8(x[i], k, end));
     }
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
