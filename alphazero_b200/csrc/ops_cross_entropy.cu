@@ -24,10 +24,6 @@ namespace {
 // the fp32 sums of dw a trip through memory.
 constexpr size_t kPieceBytes = size_t(1) << 30;
 
-// d is kept times 2^14 in fp16, so that small probabilities keep their bits.
-template <int DT>
-constexpr float kDScale = DT == MG_PREC_FP16 ? 16384.0f : 1.0f;
-
 // The number of counted rows, per block: only where there are several pieces
 // (else combine_kernel counts).
 constexpr int kCountBlocks = 148;
@@ -255,18 +251,19 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
     shape.m = piece;
     shape.n = a.vocab;
     shape.k = a.dim;
+    const bool rows_whole = gemm_rows_pays(shape);
     const int block = gemm_softmax_block(shape);
     const int blocks = (int)((a.vocab + block - 1) / block);
 
-    int* count = w.take<int>(4);
     Indices target;
     target.data = a.targets;
     target.bytes = a.target_bytes;
     target.stride = a.target_stride;
     target.limit = a.vocab;
-    float* logit = w.take<float>((size_t)piece * 4);
-    float* lse = w.take<float>((size_t)piece * 4);
-    float2* part = w.take<float2>((size_t)blocks * piece * 8);
+    const size_t per_row = rows_whole ? 0 : (size_t)piece * 4;
+    float* logit = w.take<float>(per_row);
+    float* lse = w.take<float>(per_row);
+    float2* part = w.take<float2>(blocks * 2 * per_row);
     uint16_t* probs = grads ? w.take<uint16_t>((size_t)piece * ld * 2) : nullptr;
     int wide = 1;
     while (wide < 8 && wide * 256 < a.vocab) wide *= 2;
@@ -274,18 +271,21 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
     // up to eight blocks per SM, at least sixteen rows per warp and block
     const int64_t want = std::max<int64_t>(1, 148 * 8 / across);
     const int down_rows = (int)std::max<int64_t>(128 / wide, (piece + want - 1) / want);
-    const int64_t down = (piece + down_rows - 1) / down_rows;  // of a whole piece
+    const int ctas = gemm_rows_ctas(piece);
+    const int64_t down = rows_whole ? ctas : (piece + down_rows - 1) / down_rows;  // of a whole piece
     float* sums = a.db ? w.take<float>((size_t)down * count_pieces * a.vocab * 4) : nullptr;
     const int64_t ld32 = (a.dim + 7) / 8 * 8;
     float* dw32 = grads && count_pieces > 1 ? w.take<float>((size_t)((a.vocab + 255) / 256 * 256) * ld32 * 4) : nullptr;
 
     const Combine how = blocks <= kFewBlocks ? kThreadPerRow : piece <= 2 * 148 ? kBlockPerRow : kWarpPerRow;
     const int64_t combine_rows = how == kThreadPerRow ? 128 : how == kBlockPerRow ? 1 : 32;
-    float* loss_part = w.take<float>((size_t)((piece + combine_rows - 1) / combine_rows * count_pieces) * 4);
+    const int64_t parts = rows_whole ? ctas : (piece + combine_rows - 1) / combine_rows;  // of a piece's loss
+    float* loss_part = w.take<float>((size_t)(parts * count_pieces) * 4);
     const bool apart = count_pieces > 1;  // rows counted by a kernel of their own
-    const int64_t counts_n = apart ? std::min<int64_t>(kCountBlocks, (a.n + 1023) / 1024)
-                                   : (piece + combine_rows - 1) / combine_rows;
+    const int counts_n = (int)(apart ? std::min<int64_t>(kCountBlocks, (a.n + 1023) / 1024) : parts);
     int* counts = w.take<int>((size_t)counts_n * 4);
+    int* total = w.take<int>(4);
+    const Count count = rows_whole ? Count{counts, counts_n} : Count{total, 1};
     if (go) {
         w.require();
         packs.launch(q);
@@ -300,7 +300,24 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
         const bool first = row0 == 0, last = row0 + rows == a.n;
         StagedOperand xp = x;  // row0 is a multiple of 256: still aligned
         xp.data = static_cast<const uint16_t*>(x.data) + row0 * (x.mn ? 1 : x.ld);
-        if (go) {
+        if (go && rows_whole) {
+            RowsJob f;
+            f.a = xp;
+            f.b = weight;
+            f.m = rows;
+            f.n = a.vocab;
+            f.k = a.dim;
+            f.e.bias = a.bias;
+            f.e.target = target.from(row0);
+            f.e.row_loss = a.row_loss + row0;
+            f.e.loss = loss_part + losses;
+            f.e.counts = apart ? nullptr : counts;
+            f.e.d = probs;
+            f.e.ld = ld;
+            f.e.sums = sums ? sums + sum_rows * a.vocab : nullptr;
+            gemm_rows(DT, f, q);
+            losses += gemm_rows_ctas(rows);
+        } else if (go) {
             SoftmaxJob f;
             f.a = xp;
             f.b = weight;
@@ -325,11 +342,11 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
             losses += combine_blocks;
         }
         if (!grads) continue;
-        const int64_t these = (rows + down_rows - 1) / down_rows;
-        if (go) {
+        const int64_t these = rows_whole ? gemm_rows_ctas(rows) : (rows + down_rows - 1) / down_rows;
+        if (go && !rows_whole) {
             q.launch("d_kernel", d_kernel<DT>, dim3((unsigned)across, (unsigned)these), 256, 0, (int)rows, a.vocab, block,
                      probs, ld, part, piece, lse, target.from(row0), wide, down_rows,
-                     sums ? sums + sum_rows * a.vocab : nullptr, first ? counts : nullptr, counts_n, count);
+                     sums ? sums + sum_rows * a.vocab : nullptr, first ? counts : nullptr, (int64_t)counts_n, total);
         }
         sum_rows += these;
         StagedOperand d;

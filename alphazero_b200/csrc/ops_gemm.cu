@@ -38,28 +38,45 @@ namespace {
 constexpr int kRowsCta = 128;          // rows of a tile per CTA
 constexpr int kRowsPair = 256;
 constexpr int kBK = 64;                // K elements per stage
-constexpr int kEpiWarps = 8;
-constexpr int kThreads = 32 * (2 + kEpiWarps);
 constexpr int kPairs = 74;             // of SMs on a B200 (148)
 constexpr int kGroup = 8;              // row tiles walked together (their B tiles stay in L2)
 constexpr int kBlockBytes = 4096;      // 32 rows of 128 bytes: 64 columns of 16 bits or 32 of fp32
 constexpr int kWarpBytes = 2 * kBlockBytes;  // per epilogue warp
 
+enum Epi : int { kStore, kSoftmax, kRows };
+
 template <int BN>
 struct Config {
+    static constexpr int kEpiWarps = 8;
     static constexpr int kStages = BN == 256 ? 5 : 6;
     static constexpr uint32_t kABytes = kRowsCta * kBK * 2;
     static constexpr uint32_t kBBytes = BN / 2 * kBK * 2;
     static constexpr uint32_t kStageBytes = kABytes + kBBytes;
-    static constexpr uint32_t kTmemCols = 2 * BN;
     static constexpr int kCols = BN / 2;  // of a tile per epilogue warp
-    static constexpr int kBarriers = 2 * kStages + 5 + 2 * kEpiWarps;
+    static constexpr int kBarriers = 2 * kStages + 9 + 2 * kEpiWarps;
     // ring + per epilogue warp its blocks and 16-bit bias + barriers + TMEM address
     static constexpr int kSmem = kStages * kStageBytes + kEpiWarps * (kWarpBytes + kCols * 2) + kBarriers * 8 + 16;
     static_assert(kSmem <= 232448, "shared memory of an SM");
 };
 
-enum Epi : int { kStore, kSoftmax };
+// kRows has 16 epilogue warps (its time is theirs: with eight, two per
+// scheduler, it took 28 us instead of RROWS for 32768 rows of 256 and 362
+// columns), a stage less and more shared memory of their own: per warp two
+// blocks of 32 x 32 16-bit elements and, in 32 bits, the bias, sums and counts
+// of its columns (32 of every 128), per CTA the exchange of row statistics
+// ([2][4][128] float2), the barriers for that and each warp's loss and count.
+template <int EPI>
+constexpr int kEpiWarps = EPI == kRows ? 16 : 8;
+template <int EPI>
+constexpr int kThreads = 32 * (2 + kEpiWarps<EPI>);
+constexpr int kRowsColumnsWarp = kRowsColumns / 4;
+constexpr int kRowsStages = Config<128>::kStages - 1;
+constexpr int kRowsBlock = 2048;
+constexpr int kRowsWarpBytes = 2 * kRowsBlock + kRowsColumnsWarp * 12;
+constexpr int kRowsStats = 2 * 4 * kRowsCta * 8;
+constexpr int kRowsSmem = kRowsStages * Config<128>::kStageBytes + kEpiWarps<kRows> * (kRowsWarpBytes + 16) + kRowsStats +
+                          Config<128>::kBarriers * 8 + 16;
+static_assert(kRowsSmem <= 232448, "shared memory of an SM");
 
 struct JobArgs {
     int m, n, kblocks;
@@ -67,8 +84,10 @@ struct JobArgs {
     int a_mn, b_mn;
     int by_tma;  // outputs, z and residual go through their tensor maps
     int m_pad;   // rows of out32 per split
+    int across;  // kRows: column tiles of a unit
     GemmEpilogue e;
     SoftmaxEpilogue s;
+    RowsEpilogue r;
 };
 
 struct alignas(64) KernelArgs {
@@ -322,7 +341,7 @@ struct EpilogueJob {
     int m, n, m_pad, act;
     bool by_tma, has_z, has_res, has_acc32, has_out32;
     float alpha, res_scale;
-    __device__ explicit EpilogueJob(const JobArgs& j) {
+    __device__ EpilogueJob(const JobArgs& j, int lane) {
         const GemmEpilogue& e = j.e;
         m = j.m;
         n = j.n;
@@ -333,7 +352,7 @@ struct EpilogueJob {
         has_res = e.res != nullptr;
         has_acc32 = e.acc32 != nullptr;
         has_out32 = e.out32 != nullptr;
-        alpha = e.count ? e.alpha / (float)max(*e.count, 1) : e.alpha;
+        alpha = scaled_alpha(e.alpha, e.count, lane);
         res_scale = e.res_scale;
     }
 };
@@ -521,22 +540,224 @@ __device__ __forceinline__ void softmax_epilogue(const KernelArgs& a, const Soft
     }
 }
 
+// Two fp32 numbers side by side: sums and products of both are one instruction.
+struct Two {
+    uint64_t u;
+    __device__ __forceinline__ explicit Two(uint64_t bits) : u(bits) {}
+    __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(u) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ void get(float& a, float& b) const {
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(u));
+    }
+};
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.u) : "l"(b.u));
+    return a;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.u) : "l"(b.u));
+    return a;
+}
+__device__ __forceinline__ Two mul_add(Two a, Two b, Two c) {
+    asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(a.u) : "l"(b.u), "l"(c.u));
+    return a;
+}
+
+// Sum over the warp's lanes of v[i], to lane i: each step halves the columns
+// that a lane still has and doubles the rows in their sums.
+__device__ __forceinline__ float sum_lanes(float (&v)[32], int lane) {
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) {
+        const bool up = (lane & d) != 0;
+#pragma unroll
+        for (int i = 0; i < d; ++i) {
+            const float keep = up ? v[i + d] : v[i], give = up ? v[i] : v[i + d];
+            v[i] = keep + __shfl_xor_sync(~0u, give, d);
+        }
+    }
+    return v[0];
+}
+
+// v[at], at in [0, 32), by halves.
+__device__ __forceinline__ float pick(const float (&v)[32], uint32_t at) {
+    float t[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t[i] = at & 16 ? v[i + 16] : v[i];
+#pragma unroll
+    for (int d = 8; d > 0; d /= 2)
+#pragma unroll
+        for (int i = 0; i < d; ++i) t[i] = at & d ? t[i + d] : t[i];
+    return t[0];
+}
+
+// What an epilogue warp of kRows keeps in shared memory for its columns
+// (32 of every 128), and adds up over its units.
+struct RowsWarp {
+    uint8_t* blocks;  // [2][kRowsBlock]
+    float* bias;      // [kRowsColumnsWarp] -inf past the last column
+    float* columns;   // [kRowsColumnsWarp] sums of the probabilities of counted rows
+    int* targets;     // [kRowsColumnsWarp] how many rows' target the column is
+    int next = 0;     // block
+    float loss = 0.0f;
+    int counted = 0;
+};
+
+// A unit of kRows: 32 rows from m0 on, of which this warp has columns
+// share * 32 .. + 31 of every 128; the others are three warps' with which it
+// exchanges maximum and sum.  The sums of products are read from TMEM
+// twice, since a row of them has no room in registers and an exponential
+// costs no more than keeping one in fewer bits would.  The loops stay rolled:
+// written out, each instruction would be fetched once or twice in all, and
+// warps waited for that most (with eight warps, 34 us instead of 28).  wait(t) and release(t): column tile t's sums are complete, are
+// no longer needed.
+template <int DT, class Wait, class Release, class Exchange, class Address>
+__device__ __forceinline__ bool rows_epilogue(const KernelArgs& a, const RowsEpilogue& e, int m, int n, int across,
+                                              int m0, int share, int target, int lane, RowsWarp& own,
+                                              Wait wait, Release release, Exchange exchange, Address address) {
+    constexpr float kLog2e = 1.4426950408889634f;
+    const int row = m0 + lane, first = share * 32;
+    if (m0 >= m) {
+        for (int t = 0; t < across; ++t) {
+            if (!wait(t)) return false;
+            release(t);
+        }
+        return true;
+    }
+    // logits of 32 columns
+    const auto load = [&](int t, float(&v)[32]) {
+        tmem_ld_32cols_to(address(t), v);
+        const float4* bias = reinterpret_cast<const float4*>(own.bias + t * 32);
+        tmem_ld_wait();
+        pin(v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 b = bias[i];
+            (Two(v[4 * i], v[4 * i + 1]) + Two(b.x, b.y)).get(v[4 * i], v[4 * i + 1]);
+            (Two(v[4 * i + 2], v[4 * i + 3]) + Two(b.z, b.w)).get(v[4 * i + 2], v[4 * i + 3]);
+        }
+    };
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll 1
+    for (int t = 0; t < across; ++t) {
+        if (!wait(t)) return false;
+        if (t * 128 + first >= n) continue;
+        float v[32];
+        load(t, v);
+        float most[4] = {top, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            asm("max.f32 %0, %0, %1, %2;" : "+f"(most[i & 3]) : "f"(v[2 * i]), "f"(v[2 * i + 1]));
+        const float next = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+        const float ref = next == -INFINITY ? 0.0f : next;
+        Two part[2] = {Two(0.0f, 0.0f), Two(0.0f, 0.0f)};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float x, y;
+            ((Two(v[2 * i], v[2 * i + 1]) + Two(-ref, -ref)) * Two(kLog2e, kLog2e)).get(x, y);
+            part[i & 1] = part[i & 1] + Two(exp2_flush(x), exp2_flush(y));
+        }
+        float x, y;
+        (part[0] + part[1]).get(x, y);
+        sum = sum * exp2_flush((top - ref) * kLog2e) + (x + y);
+        top = next;
+    }
+    float2 all[4];
+    if (!exchange(make_float2(top, sum), all)) return false;
+    top = fmaxf(fmaxf(all[0].x, all[1].x), fmaxf(all[2].x, all[3].x));
+    const float ref = top == -INFINITY ? 0.0f : top;
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += all[i].y * exp2_flush((all[i].x - ref) * kLog2e);
+    const float shift = sum == 0.0f ? 0.0f : -log2f(sum);  // no sum: every logit is -inf
+    const bool grads = e.d != nullptr, live = target >= 0, all_live = __all_sync(~0u, live);
+    float logit = 0.0f;
+#pragma unroll 1
+    for (int t = 0; t < across; ++t) {
+        const int col = t * 128 + first;
+        const uint32_t hot = (uint32_t)(target - col);
+        const bool any = __any_sync(~0u, hot < 32);
+        if (col >= n || (!grads && !any)) {
+            release(t);
+            continue;
+        }
+        float v[32];
+        load(t, v);
+        release(t);
+        if (any) {
+            const float at = pick(v, hot);
+            if (hot < 32) logit = at;
+        }
+        if (!grads) continue;
+        // softmax as one exponential, whose argument is exact near the maximum
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float x, y;
+            mul_add(Two(v[2 * i], v[2 * i + 1]) + Two(-ref, -ref), Two(kLog2e, kLog2e), Two(shift, shift)).get(x, y);
+            v[2 * i] = exp2_flush(x);
+            v[2 * i + 1] = exp2_flush(y);
+        }
+        if (!all_live)  // a row that is not counted, whatever it holds
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = live ? v[i] : 0.0f;
+        // 64 bytes per row, as TMA swizzles them
+        uint8_t* block = own.blocks + own.next * kRowsBlock + lane * 64;
+        const auto place = [&](int q) { return block + ((q ^ (lane >> 1 & 3)) << 4); };
+        if (lane == 0) bulk_wait_read_n<1>();
+        __syncwarp();
+        const auto word = [&](int i) { return pack2<DT>(v[2 * i] * kDScale<DT>, v[2 * i + 1] * kDScale<DT>); };
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint4*>(place(q)) = make_uint4(word(4 * q), word(4 * q + 1), word(4 * q + 2), word(4 * q + 3));
+        if (hot < 32) {
+            using E = Elem<DT>;
+            const float d = exp2_flush(fmaf(logit - ref, kLog2e, shift)) - 1.0f;
+            reinterpret_cast<typename E::T*>(place(hot >> 3))[hot & 7] = E::put(d * kDScale<DT>);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            tma_store_2d(&a.to[0], smem_u32(block), col, m0);
+            bulk_commit();
+        }
+        own.next ^= 1;
+        if (e.sums != nullptr) own.columns[t * 32 + lane] += sum_lanes(v, lane);
+    }
+    if (row >= m) return true;
+    if (live && (target & 96) == first) {
+        const float loss = logit == -INFINITY ? INFINITY : (top - logit) + logf(sum);
+        e.row_loss[row] = loss;
+        own.loss += loss;
+        ++own.counted;
+        atomicAdd(&own.targets[target / 128 * 32 + target % 32], 1);
+    } else if (!live && share == 0) {
+        e.row_loss[row] = 0.0f;
+    }
+    return true;
+}
+
 template <int BN, int DT, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<EPI>, 1)
     gemm_kernel(const __grid_constant__ KernelArgs a) {
     using Cfg = Config<BN>;
-    constexpr int S = Cfg::kStages;
+    constexpr int S = EPI == kRows ? kRowsStages : Cfg::kStages;
     extern __shared__ __align__(1024) uint8_t ring[];  // at the same address in both CTAs
+    constexpr int EW = kEpiWarps<EPI>;
+    constexpr int kWarp = EPI == kRows ? kRowsWarpBytes : kWarpBytes + Cfg::kCols * 2;  // of blocks, then the rest
+    constexpr int kBlocks = EPI == kRows ? 2 * kRowsBlock : kWarpBytes;
+    constexpr int kBufs = EPI == kRows ? 4 : 2;         // of BN columns of TMEM
     uint8_t* blocks_all = ring + S * Cfg::kStageBytes;  // a multiple of 1 KB, as each warp's part is
-    uint16_t* bias_all = reinterpret_cast<uint16_t*>(blocks_all + kEpiWarps * kWarpBytes);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(bias_all + kEpiWarps * Cfg::kCols);
+    uint8_t* own_all = blocks_all + EW * kBlocks;       // per warp its 16-bit bias, or a RowsWarp's columns
+    float2* stats = reinterpret_cast<float2*>(own_all + EW * (kWarp - kBlocks));  // kRows: [2][4][kRowsCta]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(stats + (EPI == kRows ? kRowsStats / 8 : 0));
     uint64_t* full = bars;           // even CTA's: a stage has landed in both CTAs
     uint64_t* empty = bars + S;      // each CTA's: the products have read a stage
-    uint64_t* tfull = bars + 2 * S;  // [2] each CTA's: a tile's sums are complete
-    uint64_t* tempty = tfull + 2;    // [2] even CTA's: both CTAs have read them
-    uint64_t* done = tempty + 2;     // even CTA's: the last products are complete
-    uint64_t* landed = done + 1;     // [kEpiWarps][2] a warp's residual block has arrived
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::kBarriers);
+    uint64_t* tfull = bars + 2 * S;  // [kBufs] each CTA's: a tile's sums are complete
+    uint64_t* tempty = tfull + 4;    // [kBufs] even CTA's: both CTAs have read them
+    uint64_t* done = tempty + 4;     // even CTA's: the last products are complete
+    uint64_t* landed = done + 1;     // [EW][2] a warp's residual block has arrived
+    uint64_t* told = bars + Cfg::kBarriers;  // kRows: [EW] the warps of its rows have left their statistics
+    float* loss_all = reinterpret_cast<float*>(told + (EPI == kRows ? EW : 0));  // kRows: [EW]
+    int* count_all = reinterpret_cast<int*>(loss_all + (EPI == kRows ? EW : 0));  // kRows: [EW]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(count_all + (EPI == kRows ? EW : 0));
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
@@ -547,16 +768,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             mbar_init(smem_u32(&full[s]), 1);
             mbar_init(smem_u32(&empty[s]), 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kBufs; ++i) {
             mbar_init(smem_u32(&tfull[i]), 1);
-            mbar_init(smem_u32(&tempty[i]), 2 * kEpiWarps);
+            mbar_init(smem_u32(&tempty[i]), 2 * EW);
         }
         mbar_init(smem_u32(done), 1);
-        for (int i = 0; i < 2 * kEpiWarps; ++i) mbar_init(smem_u32(&landed[i]), 1);
+        for (int i = 0; EPI != kRows && i < 2 * EW; ++i) mbar_init(smem_u32(&landed[i]), 1);
+        for (int i = 0; EPI == kRows && i < EW; ++i) mbar_init(smem_u32(&told[i]), 4);
         fence_barrier_init();
     }
     if (warp == 1) {
-        tmem_alloc_pair(smem_u32(tmem_slot), Cfg::kTmemCols);
+        tmem_alloc_pair(smem_u32(tmem_slot), kBufs * BN);
         tmem_relinquish_pair();
     }
     tc_fence_before();
@@ -580,8 +802,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const bool a_mn = a.job[job].a_mn, b_mn = a.job[job].b_mn;
             for (int i = 0, unit; ok && (unit = walk.unit(job, i)) >= 0; ++i) {
                 const Tile t(tiling, unit, BN);
-                const int am = t.m0 + (int)rank * kRowsCta, bn = t.n0 + (int)rank * (BN / 2);
-                for (int kb = t.kb0; kb < t.kb1; ++kb) {
+                const int am = t.m0 + (int)rank * kRowsCta;
+                int bn = t.n0 + (int)rank * (BN / 2), kb = t.kb0;
+                const int steps = (t.kb1 - t.kb0) * (EPI == kRows ? a.job[0].across : 1);
+                for (int step = 0; step < steps; ++step, ++kb) {
+                    if (EPI == kRows && kb == t.kb1) {
+                        kb = t.kb0;
+                        bn += BN;
+                    }
                     const uint32_t wait = smem_u32(&empty[s]);
                     if (!mbar_wait_warp(wait, (round & 1) ^ 1, a.err, kErrWaitProducer)) {
                         ok = false;
@@ -639,34 +867,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     b_mn ? smem_desc_sw128_mn(ring_at + Cfg::kABytes) : smem_desc_sw128(ring_at + Cfg::kABytes);
                 for (int i = 0, unit; ok && (unit = walk.unit(job, i)) >= 0; ++i) {
                     const Tile t(tiling, unit, BN);
-                    const int buf = tile & 1;
-                    if (!mbar_wait_warp(smem_u32(&tempty[buf]), ((tile >> 1) & 1) ^ 1, a.err, kErrWaitMma)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t acc = tmem_base + buf * BN;
-                    for (int kb = t.kb0; kb < t.kb1; ++kb) {
-                        if (!mbar_wait_warp(smem_u32(&full[s]), round & 1, a.err, kErrWaitMma)) {
+                    const int tiles = EPI == kRows ? a.job[0].across : 1;
+                    for (int x = 0; x < tiles && ok; ++x) {
+                        const int buf = tile % kBufs;
+                        if (!mbar_wait_warp(smem_u32(&tempty[buf]), ((tile / kBufs) & 1) ^ 1, a.err, kErrWaitMma)) {
                             ok = false;
                             break;
                         }
                         tc_fence_after();
-                        const uint64_t xa = first_a + s * (Cfg::kStageBytes >> 4);
-                        const uint64_t xb = first_b + s * (Cfg::kStageBytes >> 4);
-                        if (elect_one()) {
+                        const uint32_t acc = tmem_base + buf * BN;
+                        for (int kb = t.kb0; kb < t.kb1; ++kb) {
+                            if (!mbar_wait_warp(smem_u32(&full[s]), round & 1, a.err, kErrWaitMma)) {
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
+                            const uint64_t xa = first_a + s * (Cfg::kStageBytes >> 4);
+                            const uint64_t xb = first_b + s * (Cfg::kStageBytes >> 4);
+                            if (elect_one()) {
 #pragma unroll
-                            for (int kk = 0; kk < kBK / 16; ++kk)
-                                mma_f16_pair(acc, xa + kk * step_a, xb + kk * step_b, idesc, kb > t.kb0 || kk > 0);
-                            mma_commit_pair(smem_u32(&empty[s]));
-                            if (kb + 1 == t.kb1) mma_commit_pair(smem_u32(&tfull[buf]));
+                                for (int kk = 0; kk < kBK / 16; ++kk)
+                                    mma_f16_pair(acc, xa + kk * step_a, xb + kk * step_b, idesc, kb > t.kb0 || kk > 0);
+                                mma_commit_pair(smem_u32(&empty[s]));
+                                if (kb + 1 == t.kb1) mma_commit_pair(smem_u32(&tfull[buf]));
+                            }
+                            if (++s == S) {
+                                s = 0;
+                                ++round;
+                            }
                         }
-                        if (++s == S) {
-                            s = 0;
-                            ++round;
-                        }
+                        ++tile;
                     }
-                    ++tile;
                 }
             }
             // Products still in flight finish before TMEM is freed.
@@ -681,17 +912,76 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int c0 = (ew >> 2) * Cfg::kCols;
         // the warp's own copy of its columns' bias: one shared by four warps would
         // need a barrier, which a warp whose wait gave up would leave the others at
-        uint16_t* sbias = bias_all + ew * Cfg::kCols;
+        uint16_t* sbias = reinterpret_cast<uint16_t*>(own_all + ew * (kWarp - kBlocks));
         WarpBlocks blocks;
-        blocks.blocks = blocks_all + ew * kWarpBytes;
+        blocks.blocks = blocks_all + ew * kBlocks;
         blocks.landed = &landed[2 * ew];
         blocks.lane = lane;
         const uint32_t taddr0 = tmem_base + c0 + ((uint32_t)quarter << 21);
         int tile = 0;
         bool ok = true;
-        for (int job = 0; job < jobs && ok; ++job) {
+        if constexpr (EPI == kRows) {
+            const JobArgs& job = a.job[0];
+            const RowsEpilogue e = job.r;
+            const Tiling tiling(job);
+            const int m = job.m, n = job.n, across = job.across, share = ew >> 2;
+            RowsWarp own;
+            own.blocks = blocks.blocks;
+            own.bias = reinterpret_cast<float*>(sbias);
+            own.columns = own.bias + kRowsColumnsWarp;
+            own.targets = reinterpret_cast<int*>(own.columns + kRowsColumnsWarp);
+            for (int t = 0; t < across; ++t) {
+                const int col = t * 128 + share * 32 + lane;
+                float v = col < n ? 0.0f : -INFINITY;
+                if (e.bias != nullptr && col < n) v = Elem<DT>::get(static_cast<const typename Elem<DT>::T*>(e.bias)[col]);
+                own.bias[t * 32 + lane] = v;
+                own.columns[t * 32 + lane] = 0.0f;
+                own.targets[t * 32 + lane] = 0;
+            }
+            __syncwarp();
+            for (int i = 0, unit; ok && (unit = walk.unit(0, i)) >= 0; ++i) {
+                const int m0 = Tile(tiling, unit, BN).m0 + (int)rank * kRowsCta + quarter * 32;
+                const int target = m0 + lane < m ? (int)e.target.at(m0 + lane) : -1;
+                const auto wait = [&](int t) {
+                    const int at = tile + t;
+                    const bool there =
+                        mbar_wait_warp(smem_u32(&tfull[at % kBufs]), at / kBufs & 1, a.err, kErrWaitEpilogue);
+                    tc_fence_after();
+                    return there;
+                };
+                const auto release = [&](int t) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&tempty[(tile + t) % kBufs]), 0));
+                };
+                // The statistics lie in buffers by turns: the other warps, which are at most
+                // a unit behind, may still read the last ones.
+                const auto exchange = [&](float2 mine, float2(&all)[4]) {
+                    float2* at = stats + (i & 1) * 4 * kRowsCta + quarter * 32 + lane;
+                    at[share * kRowsCta] = mine;
+                    __syncwarp();
+                    if (lane < 4) mbar_arrive(smem_u32(&told[lane * 4 + (ew & 3)]));
+                    if (!mbar_wait_warp(smem_u32(&told[ew]), i & 1, a.err, kErrWaitEpilogue)) return false;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) all[k] = at[k * kRowsCta];
+                    return true;
+                };
+                const auto address = [&](int t) {
+                    return tmem_base + (tile + t) % kBufs * BN + share * 32 + ((uint32_t)quarter << 21);
+                };
+                ok = rows_epilogue<DT>(a, e, m, n, across, m0, share, target, lane, own, wait, release, exchange, address);
+                tile += across;
+            }
+#pragma unroll
+            for (int d = 16; d > 0; d /= 2) own.loss += __shfl_xor_sync(~0u, own.loss, d);
+            own.counted = __reduce_add_sync(~0u, own.counted);
+            if (lane == 0) {
+                loss_all[ew] = own.loss;
+                count_all[ew] = own.counted;
+            }
+        } else for (int job = 0; job < jobs && ok; ++job) {
             const Tiling tiling(a.job[job]);
-            const EpilogueJob j(a.job[job]);
+            const EpilogueJob j(a.job[job], lane);
             const SoftmaxEpilogue soft = a.job[0].s;
             const void* bias = EPI == kSoftmax ? soft.bias : j.has_out32 ? nullptr : a.job[job].e.bias;
             int bias_at = -1;  // first column of the tile whose bias is there
@@ -762,9 +1052,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // shared memory or signal its barriers.
     tc_fence_before();
     __syncthreads();
+    if constexpr (EPI == kRows) {
+        // what the CTA's warps have added up, joined in a fixed order
+        const RowsEpilogue& e = a.job[0].r;
+        if (threadIdx.x == 0) {
+            float loss = 0.0f;
+            int count = 0;
+            for (int i = 0; i < EW; ++i) {
+                loss += loss_all[i];
+                count += count_all[i];
+            }
+            e.loss[blockIdx.x] = loss;
+            if (e.counts != nullptr) e.counts[blockIdx.x] = count;
+        }
+        const int n = a.job[0].n;
+        if (e.sums != nullptr && threadIdx.x < n) {
+            const int c = threadIdx.x, at = c / 128 * 32 + c % 32;
+            float sum = 0.0f;
+            int targets = 0;
+            for (int i = 0; i < 4; ++i) {
+                const float* columns = reinterpret_cast<const float*>(own_all + (c / 32 % 4 * 4 + i) * (kWarp - kBlocks)) +
+                                       kRowsColumnsWarp;
+                sum += columns[at];
+                targets += reinterpret_cast<const int*>(columns + kRowsColumnsWarp)[at];
+            }
+            e.sums[(int64_t)blockIdx.x * n + c] = sum - (float)targets;
+        }
+    }
     cluster_sync();
     tc_fence_after();
-    if (warp == 1) tmem_dealloc_pair(tmem_base, Cfg::kTmemCols);
+    if (warp == 1) tmem_dealloc_pair(tmem_base, kBufs * BN);
 }
 
 // A tensor map of a dense-enough matrix: `rows` lines of `inner` elements,
@@ -812,7 +1129,16 @@ void launch_one(const KernelArgs& a, int pairs, Queue& q) {
     check(cudaFuncSetAttribute(gemm_kernel<BN, DT, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                Config<BN>::kSmem),
           "cudaFuncSetAttribute(gemm_kernel)");
-    q.launch("gemm_kernel", gemm_kernel<BN, DT, EPI>, dim3(2 * pairs), kThreads, Config<BN>::kSmem, a);
+    q.launch("gemm_kernel", gemm_kernel<BN, DT, EPI>, dim3(2 * pairs), kThreads<EPI>, Config<BN>::kSmem, a);
+}
+
+void launch_rows(KernelArgs& a, int dtype, Queue& q) {
+    a.err = op_status_word();
+    const int pairs = std::min(kPairs, a.units[0]);
+    const auto kernel = dtype == MG_PREC_BF16 ? gemm_kernel<128, MG_PREC_BF16, kRows> : gemm_kernel<128, MG_PREC_FP16, kRows>;
+    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem),
+          "cudaFuncSetAttribute(gemm_kernel)");
+    q.launch("gemm_kernel", kernel, dim3(2 * pairs), kThreads<kRows>, kRowsSmem, a);
 }
 
 template <int EPI>
@@ -904,7 +1230,7 @@ StagedOperand stage_operand(Workspace& w, Packs& packs, const GemmOperand& op, i
 
 void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, Post& post, Queue& q) {
     if (count == 1 && jobs->m <= kSkinnyRows && !jobs->a.mn && !jobs->b.mn && jobs->e.out32 == nullptr &&
-        jobs->e.acc32 == nullptr) {
+        jobs->e.acc32 == nullptr && jobs->e.count.parts == nullptr) {
         if (go) skinny(dtype, *jobs, q);
         return;
     }
@@ -981,6 +1307,30 @@ void gemm_softmax(int dtype, const SoftmaxJob& g, int block, Queue& q) {
     encode_operands(a, 0, dtype, g, bn);
     if (g.e.probs != nullptr) encode_blocks(&a.to[0], dtype, g.e.probs, g.m, g.e.probs_ld, g.e.probs_ld);
     launch<kSoftmax>(a, bn, dtype, q);
+}
+
+bool gemm_rows_pays(const SoftmaxJob& g) {
+    if (g.n > kRowsColumns || is_skinny(g)) return false;
+    const int64_t down = (g.m + kRowsPair - 1) / kRowsPair, across = (g.n + 127) / 128, steps = (g.k + kBK - 1) / kBK;
+    const int64_t whole = (down + kPairs - 1) / kPairs * across * steps;
+    const int64_t tiles = (down * across + kPairs - 1) / kPairs * steps;
+    return whole <= tiles + 40;
+}
+
+int gemm_rows_ctas(int64_t m) { return (int)std::min<int64_t>(kPairs, (m + kRowsPair - 1) / kRowsPair) * 2; }
+
+void gemm_rows(int dtype, const RowsJob& g, Queue& q) {
+    KernelArgs a{};
+    JobArgs& j = a.job[0];
+    lay_out(j, g, 128);
+    j.across = j.tiles_n;
+    j.tiles_n = 1;
+    j.r = g.e;
+    a.units[0] = j.tiles_m;
+    encode_operands(a, 0, dtype, g, 128);
+    if (g.e.d != nullptr)
+        encode(&a.to[0], map_type(dtype), 2, g.e.d, g.e.ld, g.m, g.e.ld, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+    launch_rows(a, dtype, q);
 }
 
 }  // namespace ops

@@ -21,6 +21,19 @@ struct StagedOperand {
     bool mn = false;
 };
 
+// A number that earlier kernels left in n parts.
+struct Count {
+    const int* parts = nullptr;
+    int n = 0;
+};
+// Its sum, to every lane of the calling warp.
+__device__ __forceinline__ int count_total(const Count& c, int lane) {
+    int s = 0;
+#pragma unroll 4
+    for (int i = lane; i < c.n; i += 32) s += c.parts[i];
+    return __reduce_add_sync(~0u, s);
+}
+
 // z = alpha * acc + bias; out = act(z) + res_scale * res, both 16-bit.
 struct GemmEpilogue {
     const void* bias = nullptr;      // [n]
@@ -36,8 +49,12 @@ struct GemmEpilogue {
     float res_scale = 0.0f;
     int act = MG_ACT_NONE;
     float alpha = 1.0f;
-    const int* count = nullptr;      // alpha is divided by max(*count, 1)
+    Count count;                     // if set, alpha is divided by max(count, 1)
 };
+// To be called by whole warps.
+__device__ __forceinline__ float scaled_alpha(float alpha, const Count& count, int lane) {
+    return count.parts != nullptr ? alpha / (float)max(count_total(count, lane), 1) : alpha;
+}
 
 struct GemmJob {
     StagedOperand a, b;
@@ -69,9 +86,38 @@ struct SoftmaxJob {
     int64_t m = 0, n = 0, k = 0;
     SoftmaxEpilogue e;
 };
+// d is kept times 2^14 in fp16, so that small probabilities keep their bits.
+template <int DT>
+constexpr float kDScale = DT == MG_PREC_FP16 ? 16384.0f : 1.0f;
+
 int gemm_softmax_block(const SoftmaxJob& job);
 // `block`: gemm_softmax_block of the largest job that shares part's layout.
 void gemm_softmax(int dtype, const SoftmaxJob& job, int block, Queue& q);
+
+// The same, whole rows at a time, where n is small: the sums of 256 rows and
+// up to kRowsColumns columns stay in TMEM until the rows' softmax is known,
+// which then leaves the chip as d = (softmax - onehot) * kDScale.  Each of
+// the gemm_rows_ctas(m) CTAs also leaves its rows' summed loss, how many of
+// them are counted and the column sums of d / kDScale before its rounding.
+constexpr int kRowsColumns = 512;
+struct RowsEpilogue {
+    const void* bias = nullptr;    // [n]
+    Indices target;                // [m]
+    float* row_loss = nullptr;     // [m]
+    float* loss = nullptr;         // [ctas]
+    int* counts = nullptr;         // [ctas], or null
+    uint16_t* d = nullptr;         // [m][n], row stride ld; null: no gradient
+    int64_t ld = 0;                // a multiple of 8
+    float* sums = nullptr;         // [ctas][n], or null
+};
+struct RowsJob {
+    StagedOperand a, b;
+    int64_t m = 0, n = 0, k = 0;
+    RowsEpilogue e;
+};
+bool gemm_rows_pays(const SoftmaxJob& job);
+int gemm_rows_ctas(int64_t m);
+void gemm_rows(int dtype, const RowsJob& job, Queue& q);
 
 void skinny(int dtype, const GemmJob& job, Queue& q);
 int skinny_block(int64_t k);  // columns per block of the statistics
@@ -157,11 +203,11 @@ struct FinishTask {
     GemmEpilogue e;
     int64_t blocks;
 };
-struct AddRowsTask {  // out[c] = alpha / max(*count, 1) * sum of `rows` rows of sums, in a fixed order
+struct AddRowsTask {  // out[c] = alpha / max(count, 1) * sum of `rows` rows of sums, in a fixed order
     const float* sums;
     int64_t rows, cols;
     float alpha;
-    const int* count;
+    Count count;
     void* out;
 };
 struct LossTask {  // loss = sum of part[0 .. n) / max(sum of counts[0 .. counts_n), 1)

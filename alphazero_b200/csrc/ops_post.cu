@@ -29,6 +29,7 @@ __device__ __forceinline__ void finish_block(const FinishTask& t, int64_t block,
     const int64_t across = (t.n + 127) / 128;
     const int64_t i = block / across * rows + warp / slices, c = block % across * 128 + lane * 4;
     const int slice = warp % slices;
+    const float alpha = scaled_alpha(e.alpha, e.count, lane);
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const bool in = i < t.m && c < t.n;
     if (in)
@@ -47,7 +48,6 @@ __device__ __forceinline__ void finish_block(const FinishTask& t, int64_t block,
         }
     }
     if (!in) return;
-    const float alpha = e.count ? e.alpha / (float)max(*e.count, 1) : e.alpha;
     float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -74,6 +74,7 @@ __device__ __forceinline__ void add_rows_block(const AddRowsTask& t, int64_t blo
     const int slices = add_rows_slices(t.rows), columns = kPostThreads / slices;
     const int slice = threadIdx.x / columns, lane = threadIdx.x % columns;
     const int64_t c = block * columns + lane;
+    const float alpha = scaled_alpha(t.alpha, t.count, threadIdx.x & 31);
     float s = 0.0f;
     if (c < t.cols)
 #pragma unroll 8
@@ -86,8 +87,7 @@ __device__ __forceinline__ void add_rows_block(const AddRowsTask& t, int64_t blo
             for (int i = 0; i < slices; ++i) s += shared[i * columns + lane];
     }
     if (slice > 0 || c >= t.cols) return;
-    static_cast<typename Elem<DT>::T*>(t.out)[c] =
-        Elem<DT>::put(s * (t.count ? t.alpha / (float)max(*t.count, 1) : t.alpha));
+    static_cast<typename Elem<DT>::T*>(t.out)[c] = Elem<DT>::put(s * alpha);
 }
 
 __device__ __forceinline__ void loss_block(const LossTask& t, float2* shared) {

@@ -27,7 +27,6 @@ namespace mgb {
 namespace ops {
 namespace {
 
-
 struct SkinnyArgs {
     const uint16_t* x;  // [m][k], row stride ldx
     const uint16_t* w;  // [n][k], row stride ldw
@@ -111,7 +110,7 @@ __device__ __forceinline__ void finish(const SkinnyArgs& a, const float (&sums)[
         if (first == 0 && token < a.m) e.part[(int64_t)group * e.part_ld + token] = make_float2(top, sum);
     } else {
         const GemmEpilogue& e = a.e;
-        const float alpha = e.count ? e.alpha / (float)max(*e.count, 1) : e.alpha;
+        const float alpha = e.alpha;
         for (int i = threadIdx.x; i < rows * a.m; i += 256) {
             const int r = i % rows, token = i / rows;
             const int64_t col = n0 + r;

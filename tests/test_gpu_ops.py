@@ -293,6 +293,32 @@ def test_cross_entropy(dtype, bias, n, vocab, dim):
     check_cross_entropy(x, w, integers(n, -1, vocab + 1), b, 512.0 if dtype == torch.float16 else 1.0)
 
 
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("n,vocab,dim", [(17, 1, 64), (100, 64, 70), (255, 65, 8), (256, 82, 256), (258, 128, 64),
+                                         (700, 170, 128), (1030, 256, 33), (513, 257, 64), (300, 362, 4000),
+                                         (40, 384, 64), (333, 385, 72), (129, 448, 128), (600, 512, 64),
+                                         (31, 513, 64), (19500, 362, 64), (40000, 82, 40)])
+def test_cross_entropy_few_classes(bias, n, vocab, dim):
+    x, w = make(n, dim), make(vocab, dim, seed=1, scale=2 * dim ** -0.5)
+    b = make(vocab, seed=2) if bias else None
+    check_cross_entropy(x, w, integers(n, -1, vocab + 1), b)
+
+
+@pytest.mark.parametrize("low", [-INF, -3.0e38])
+def test_cross_entropy_few_classes_banned(low):
+    n, vocab = 200, 450
+    x, w, b = make(n, 64), make(vocab, 64, seed=1, scale=0.3), make(vocab, seed=2)
+    b[64:450] = low  # whole halves of a row among them
+    t = integers(n, 0, 64)
+    got = check_cross_entropy(x, w, t, b)
+    assert not got[3][64:].any() and not got[4][64:].any()
+    b[:] = low
+    got = check_cross_entropy(x, w, t, b)
+    if low == -INF:
+        assert (got[1] == INF).all()
+    assert torch.isfinite(got[2]).all() and torch.isfinite(got[3]).all()
+
+
 @pytest.mark.parametrize("how", ["transposed", "offset", "spread"])
 def test_cross_entropy_layouts(how):
     x, w, b = make(150, 72), make(390, 72, seed=1, scale=0.2), make(390, seed=2)
