@@ -3,7 +3,9 @@
 //
 // Forward: the product's epilogue turns each tile of logits into a maximum
 // and a sum per row and block of columns; the logits leave the chip in
-// no form.  combine_kernel joins the blocks of a row.
+// no form.  combine_kernel joins the blocks of a row.  Where there are few
+// columns (kRowsColumns) the product's launch has whole rows, and leaves their
+// losses and d itself.
 //
 // With gradients each tile also leaves exp(l - its block's maximum) in 16
 // bits (Prob16, ops_gemm.cuh), for a piece of the rows at a time.  Once a
@@ -251,7 +253,7 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
     shape.m = piece;
     shape.n = a.vocab;
     shape.k = a.dim;
-    const bool rows_whole = gemm_rows_pays(shape);
+    const bool rows_whole = gemm_rows_pays(shape, grads);
     const int block = gemm_softmax_block(shape);
     const int blocks = (int)((a.vocab + block - 1) / block);
 

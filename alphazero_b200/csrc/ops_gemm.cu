@@ -60,7 +60,7 @@ struct Config {
 };
 
 // kRows has 16 epilogue warps (its time is theirs: with eight, two per
-// scheduler, it took 28 us instead of RROWS for 32768 rows of 256 and 362
+// scheduler, it took 28 us instead of 25 for 32768 rows of 256 and 362
 // columns), a stage less and more shared memory of their own: per warp two
 // blocks of 32 x 32 16-bit elements and, in 32 bits, the bias, sums and counts
 // of its columns (32 of every 128), per CTA the exchange of row statistics
@@ -1309,12 +1309,19 @@ void gemm_softmax(int dtype, const SoftmaxJob& g, int block, Queue& q) {
     launch<kSoftmax>(a, bn, dtype, q);
 }
 
-bool gemm_rows_pays(const SoftmaxJob& g) {
+// A pair takes a unit's column tiles one after another, which other pairs
+// would share where rows are few; it saves the joining launch, with gradients
+// also the pass over the probabilities.  Measured in us (this way, by tiles;
+// 362 classes) for rows x dim, with the K steps more on a pair's way:
+// gradients 32768 x 256 (0) 49, 63; 256 x 256 (8) 23, 27; 4096 x 1024 (32)
+// 38.5, 39.  Loss alone 32768 x 256 (0) 18, 23; 256 x 256 (8) 12.3, 10.8;
+// 4096 x 1024 (32) 20, 14.
+bool gemm_rows_pays(const SoftmaxJob& g, bool grads) {
     if (g.n > kRowsColumns || is_skinny(g)) return false;
     const int64_t down = (g.m + kRowsPair - 1) / kRowsPair, across = (g.n + 127) / 128, steps = (g.k + kBK - 1) / kBK;
     const int64_t whole = (down + kPairs - 1) / kPairs * across * steps;
     const int64_t tiles = (down * across + kPairs - 1) / kPairs * steps;
-    return whole <= tiles + 40;
+    return whole <= tiles + (grads ? 32 : 4);
 }
 
 int gemm_rows_ctas(int64_t m) { return (int)std::min<int64_t>(kPairs, (m + kRowsPair - 1) / kRowsPair) * 2; }

@@ -115,7 +115,7 @@ struct RowsJob {
     int64_t m = 0, n = 0, k = 0;
     RowsEpilogue e;
 };
-bool gemm_rows_pays(const SoftmaxJob& job);
+bool gemm_rows_pays(const SoftmaxJob& job, bool grads);
 int gemm_rows_ctas(int64_t m);
 void gemm_rows(int dtype, const RowsJob& job, Queue& q);
 

@@ -49,6 +49,15 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, int k, int end) {
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
+// Of W, which is read once: no place in L1, where x stays.
+__device__ __forceinline__ uint4 load_once(const uint16_t* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+
 template <int DT>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
@@ -155,8 +164,8 @@ __global__ void __launch_bounds__(256, 3) skinny_kernel(SkinnyArgs a) {
         uint4 u0[kAhead], u1[kAhead];
 #pragma unroll
         for (int q = 0; q < kAhead; ++q) {
-            u0[q] = __ldg(reinterpret_cast<const uint4*>(w0 + k + 32 * q));
-            u1[q] = __ldg(reinterpret_cast<const uint4*>(w1 + k + 32 * q));
+            u0[q] = load_once(w0 + k + 32 * q);
+            u1[q] = load_once(w1 + k + 32 * q);
         }
 #pragma unroll
         for (int q = 0; q < kAhead; ++q)
