@@ -1,7 +1,8 @@
 """Builds the package's native libraries in-tree (alphazero_b200/lib/).
 
   libminigo_cuda.so  CUDA kernels for sm_100a + engine + C ABI
-                     (include/minigo_cuda.h); nvcc, static cudart.
+                     (include/minigo_cuda.h, and include/minigo_ops.h for the
+                     training operators); nvcc, static cudart.
   libminigo_host.so  CPU-only helpers (include/minigo_host.h): position
                      generator and ONNX reader; g++.
   libminigo_evaluator.so  CudaEngine / GpuEvaluator / ShardedEvaluator

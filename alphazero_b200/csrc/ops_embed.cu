@@ -659,8 +659,8 @@ void check_args(const mg_embed_args& a) {
 
 void check_args(const mg_embed_backward_args& a) {
     need(a.n >= 0 && a.vocab >= 1 && a.dim >= 1, "sizes: n >= 0, vocab >= 1, dim >= 1");
-    need(a.n < (int64_t(1) << 31) && a.vocab < (int64_t(1) << 31) && a.dim < (int64_t(1) << 30),
-         "n and vocab must be below 2^31, dim below 2^30");
+    need(a.n < (int64_t(1) << 31) - 1024 && a.vocab < (int64_t(1) << 31) && a.dim < (int64_t(1) << 30),
+         "n must be below 2^31 - 1024, vocab below 2^31, dim below 2^30");
     need(a.dtype >= MG_PREC_BF16 && a.dtype <= MG_PREC_FP32, "dtype is not an MG_PREC_* value");
     check_tokens(a.tokens, a.token_bytes, a.token_stride, a.n);
     need(a.grad_row >= 0, "grad_row is negative");

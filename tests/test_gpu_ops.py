@@ -115,6 +115,27 @@ def test_embed_backward(dtype, kind, n, vocab, dim):
     assert torch.equal(got, ops.embed_backward(g, t, vocab, scale))  # no order of blocks in the result
 
 
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("kind", sorted(TOKENS))
+@pytest.mark.parametrize("n,vocab,dim", [(17, 1023, 65), (2000, 82, 130), (9000, 362, 64), (33000, 31, 3),
+                                         (70001, 170, 258), (40000, 1000, 33), (12000, 1, 70), (1200000, 82, 40)])
+def test_embed_backward_few_entries(dtype, kind, n, vocab, dim):
+    test_embed_backward(dtype, kind, n, vocab, dim)
+
+
+@pytest.mark.parametrize("n,vocab,dim", [(5000, 82, 48), (9000, 362, 7), (20000, 1100, 72)])
+def test_embed_backward_alignment(n, vocab, dim):
+    t = integers(n, -1, vocab)
+    g = make(n, dim, dtype=torch.float16)
+    want = ops.embed_backward(g, t, vocab)
+    for how in ("transposed", "offset", "spread"):
+        assert torch.equal(ops.embed_backward(laid(g, how), t, vocab), want)
+    assert torch.equal(ops.embed_backward(g, t.int(), vocab), want)
+    wide = torch.zeros(n, 2, dtype=torch.int64, device="cuda")
+    wide[:, 0] = t
+    assert torch.equal(ops.embed_backward(g, wide[:, 0], vocab), want)
+
+
 def test_embed_backward_layouts():
     t = integers(240, -1, 41)
     g = make(240, 48, dtype=torch.float32)
