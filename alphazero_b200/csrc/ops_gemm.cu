@@ -35,6 +35,13 @@ namespace mgb {
 namespace ops {
 namespace {
 
+// Where sums end in 32 bits (the losses), K steps that the tensor cores add up
+// on their own.  They cut off what does not fit a sum, so a chain of products
+// comes out too small by about 1e-9 of itself for each of its elements; sums
+// of such chains are rounded to nearest.  Losses of 2000 rows of 4096, 8000
+// classes: off by 6e-7 of themselves as one chain, 1.5e-7 by 16 steps, 8e-8 by
+// 8; 4096 rows of 2048, 65536 classes take 700, 702 and 723 us.
+constexpr int kChain = 16;
 constexpr int kRowsCta = 128;          // rows of a tile per CTA
 constexpr int kRowsPair = 256;
 constexpr int kBK = 64;                // K elements per stage
@@ -85,6 +92,7 @@ struct JobArgs {
     int by_tma;  // outputs, z and residual go through their tensor maps
     int m_pad;   // rows of out32 per split
     int across;  // kRows: column tiles of a unit
+    int chain;   // kSoftmax: K steps whose products add up in TMEM
     GemmEpilogue e;
     SoftmaxEpilogue s;
     RowsEpilogue r;
@@ -476,31 +484,47 @@ __device__ __forceinline__ void pin(float (&v)[32]) {
 
 // Softmax statistics of the same columns and rows.  A thread has its row's
 // block to itself, in registers, so the maximum and the sum need no exchange.
-template <int BN, int DT, class Release>
-__device__ __forceinline__ void softmax_epilogue(const KernelArgs& a, const SoftmaxEpilogue& e, int m, int n,
-                                                 const Tile& t, int m0, int c0, int target, uint32_t taddr,
-                                                 WarpBlocks& blocks, const uint16_t* sbias, Release release) {
+// The tile's sums come in `parts`, which are added here.
+template <int BN, int DT, class Wait, class Release, class Address>
+__device__ __forceinline__ bool softmax_epilogue(const KernelArgs& a, const SoftmaxEpilogue& e, int m, int n,
+                                                 const Tile& t, int m0, int c0, int target, WarpBlocks& blocks,
+                                                 const uint16_t* sbias, int parts, Wait wait, Release release,
+                                                 Address address) {
     const int row = m0 + blocks.lane;
     const int first = t.n0 + c0;
     constexpr int W = Config<BN>::kCols;
     const int width = m0 < m ? min(W, n - first) : 0;
-    if (width <= 0) {
-        release();
-        return;
-    }
     target -= first;
     float l[W];
+    for (int p = 0; p < parts; ++p) {
+        if (!wait(p)) return false;
+        const uint32_t taddr = address(p);
+        if (p == 0) {
 #pragma unroll
-    for (int c = 0; c < W; c += 32)
-        if (c < width) tmem_ld_32cols_to(taddr + c, l + c);
-    tmem_ld_wait();
-    release();
+            for (int c = 0; c < W; c += 32)
+                if (c < width) tmem_ld_32cols_to(taddr + c, l + c);
+            tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < W; c += 32) pin(*reinterpret_cast<float(*)[32]>(l + c));
+        } else {
+#pragma unroll
+            for (int c = 0; c < W; c += 16) {
+                if (c >= width) break;
+                uint32_t r[16];
+                tmem_ld_16cols(taddr + c, r);
+                tmem_ld_wait(r);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) l[c + i] += __uint_as_float(r[i]);
+            }
+        }
+        release(p);
+    }
+    if (width <= 0) return true;
     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, logit = 0.0f;
 #pragma unroll
     for (int c = 0; c < W; c += 32) {
         if (c >= width) break;
         float(&v)[32] = *reinterpret_cast<float(*)[32]>(l + c);
-        pin(v);
         add_bias<DT>(v, 1.0f, sbias + c);  // -inf past the last column
 #pragma unroll
         for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], v[i]);
@@ -538,6 +562,7 @@ __device__ __forceinline__ void softmax_epilogue(const KernelArgs& a, const Soft
         e.part[(int64_t)(first / W) * e.part_ld + row] =
             make_float2(most, (sum[0] + sum[1]) + (sum[2] + sum[3]));
     }
+    return true;
 }
 
 // Two fp32 numbers side by side: sums and products of both are one instruction.
@@ -867,8 +892,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<EPI>, 1)
                     b_mn ? smem_desc_sw128_mn(ring_at + Cfg::kABytes) : smem_desc_sw128(ring_at + Cfg::kABytes);
                 for (int i = 0, unit; ok && (unit = walk.unit(job, i)) >= 0; ++i) {
                     const Tile t(tiling, unit, BN);
-                    const int tiles = EPI == kRows ? a.job[0].across : 1;
-                    for (int x = 0; x < tiles && ok; ++x) {
+                    // kRows: a part per column tile; kSoftmax: per stretch of K
+                    const int chain = EPI == kSoftmax ? a.job[0].chain : t.kb1 - t.kb0;
+                    const int parts = EPI == kRows ? a.job[0].across : EPI == kSoftmax ? (t.kb1 + chain - 1) / chain : 1;
+                    for (int x = 0; x < parts && ok; ++x) {
+                        const int kb0 = EPI == kSoftmax ? x * chain : t.kb0, kb1 = min(t.kb1, kb0 + chain);
                         const int buf = tile % kBufs;
                         if (!mbar_wait_warp(smem_u32(&tempty[buf]), ((tile / kBufs) & 1) ^ 1, a.err, kErrWaitMma)) {
                             ok = false;
@@ -876,7 +904,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<EPI>, 1)
                         }
                         tc_fence_after();
                         const uint32_t acc = tmem_base + buf * BN;
-                        for (int kb = t.kb0; kb < t.kb1; ++kb) {
+                        for (int kb = kb0; kb < kb1; ++kb) {
                             if (!mbar_wait_warp(smem_u32(&full[s]), round & 1, a.err, kErrWaitMma)) {
                                 ok = false;
                                 break;
@@ -887,9 +915,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<EPI>, 1)
                             if (elect_one()) {
 #pragma unroll
                                 for (int kk = 0; kk < kBK / 16; ++kk)
-                                    mma_f16_pair(acc, xa + kk * step_a, xb + kk * step_b, idesc, kb > t.kb0 || kk > 0);
+                                    mma_f16_pair(acc, xa + kk * step_a, xb + kk * step_b, idesc, kb > kb0 || kk > 0);
                                 mma_commit_pair(smem_u32(&empty[s]));
-                                if (kb + 1 == t.kb1) mma_commit_pair(smem_u32(&tfull[buf]));
+                                if (kb + 1 == kb1) mma_commit_pair(smem_u32(&tfull[buf]));
                             }
                             if (++s == S) {
                                 s = 0;
@@ -1022,25 +1050,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<EPI>, 1)
                     }
                     __syncwarp();
                 }
-                const int buf = tile & 1;
                 // one answer for the warp, which goes on or stops together
-                if (!mbar_wait_warp(smem_u32(&tfull[buf]), (tile >> 1) & 1, a.err, kErrWaitEpilogue)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const auto release = [&] {
+                const auto wait = [&](int p) {
+                    const int at = tile + p;
+                    const bool there = mbar_wait_warp(smem_u32(&tfull[at & 1]), at >> 1 & 1, a.err, kErrWaitEpilogue);
+                    tc_fence_after();
+                    return there;
+                };
+                const auto release = [&](int p) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&tempty[buf]), 0));
+                    if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&tempty[(tile + p) & 1]), 0));
                 };
-                if constexpr (EPI == kSoftmax)
-                    softmax_epilogue<BN, DT>(a, soft, j.m, j.n, t, m0, c0, target, taddr0 + buf * BN, blocks, sbias,
-                                         release);
-                else
-                    ok = epilogue<BN, DT>(a, job, j, t, m0, c0, taddr0 + buf * BN, blocks, sbias, after_col, after_row,
-                                           release);
-                ++tile;
+                if constexpr (EPI == kSoftmax) {
+                    const int parts = (t.kb1 + a.job[0].chain - 1) / a.job[0].chain;
+                    ok = softmax_epilogue<BN, DT>(a, soft, j.m, j.n, t, m0, c0, target, blocks, sbias, parts, wait, release,
+                                                  [&](int p) { return taddr0 + ((tile + p) & 1) * BN; });
+                    tile += parts;
+                } else {
+                    if (!wait(0)) {
+                        ok = false;
+                        break;
+                    }
+                    ok = epilogue<BN, DT>(a, job, j, t, m0, c0, taddr0 + (tile & 1) * BN, blocks, sbias, after_col, after_row,
+                                          [&] { release(0); });
+                    ++tile;
+                }
             }
         }
         for (int b = blocks.next; blocks.flying > 0; b ^= 1)  // only after a wait gave up
@@ -1304,6 +1339,7 @@ void gemm_softmax(int dtype, const SoftmaxJob& g, int block, Queue& q) {
     lay_out(a.job[0], g, bn);
     a.job[0].s = g.e;
     a.units[0] = a.job[0].tiles_m * a.job[0].tiles_n;
+    a.job[0].chain = kChain;
     encode_operands(a, 0, dtype, g, bn);
     if (g.e.probs != nullptr) encode_blocks(&a.to[0], dtype, g.e.probs, g.m, g.e.probs_ld, g.e.probs_ld);
     launch<kSoftmax>(a, bn, dtype, q);
@@ -1317,7 +1353,8 @@ void gemm_softmax(int dtype, const SoftmaxJob& g, int block, Queue& q) {
 // 38.5, 39.  Loss alone 32768 x 256 (0) 18, 23; 256 x 256 (8) 12.3, 10.8;
 // 4096 x 1024 (32) 20, 14.
 bool gemm_rows_pays(const SoftmaxJob& g, bool grads) {
-    if (g.n > kRowsColumns || is_skinny(g)) return false;
+    // (chains of products are not cut up there)
+    if (g.n > kRowsColumns || g.k > kChain * kBK || is_skinny(g)) return false;
     const int64_t down = (g.m + kRowsPair - 1) / kRowsPair, across = (g.n + 127) / 128, steps = (g.k + kBK - 1) / kBK;
     const int64_t whole = (down + kPairs - 1) / kPairs * across * steps;
     const int64_t tiles = (down * across + kPairs - 1) / kPairs * steps;
