@@ -122,7 +122,7 @@ void embed(const mg_embed_args& a, Queue& q) {
 // earlier blocks and moves the tokens.  The moves are scattered 8-byte
 // writes, which one SM does at about one a clock: so the sort uses up to 148
 // blocks rather than one cluster (16 CTAs: 22 us a digit for 65536 tokens,
-// where these two take 7).
+// where these two take 13).
 
 constexpr int kSortWarps = 16;
 constexpr int kSortThreads = 32 * kSortWarps;
@@ -612,8 +612,11 @@ void embed_backward(const mg_embed_backward_args& a, Workspace& w, bool go, Queu
     sum.n = (int)a.n;
     const int segment = 32 * 16 / e;
     sum.segments = (a.dim + segment - 1) / segment;
-    // windows long enough that few runs cross them, short enough for 24 warps on each SM at once
-    sum.window = (int)std::clamp<int64_t>((a.n * sum.segments / (148 * 24) + 7) / 8 * 8, 16, 128);
+    // Windows long enough that few runs cross them, and as many as the card's warps (24 on
+    // each SM) can take in equal rounds: 128 tokens at most and a last round of a few blocks
+    // made it 109 us instead of 96 for 100003 tokens of 1000, 73 instead of 60 for 30000 of 2048.
+    const int64_t warps = 148 * 24, work = a.n * sum.segments, rounds = (work + warps * 256 - 1) / (warps * 256);
+    sum.window = (int)std::max<int64_t>(16, ((work + warps * rounds - 1) / (warps * rounds) + 7) / 8 * 8);
     sum.windows = (int)((a.n + sum.window - 1) / sum.window);
     sum.head = w.take<float>((size_t)sum.windows * a.dim * 4);
     sum.tail = w.take<float>((size_t)sum.windows * a.dim * 4);
