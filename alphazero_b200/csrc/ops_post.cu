@@ -1,5 +1,8 @@
 // The small launches around the products: copies of operands before them,
-// sums after them (ops_gemm.cuh).
+// sums after them (ops_gemm.cuh).  What remains after a call's products is one
+// launch, since each costs a few us whatever it does (4 for a loss alone, 9
+// with 16 splits of a 362 x 256 product and 148 rows of column sums, of which
+// most is the latency of its loads).
 #include "ops_gemm.cuh"
 
 #include <algorithm>

@@ -7,11 +7,13 @@
 // both operands agree, so a lane takes 8 consecutive elements of a row in one
 // 16-byte load and lets them stand for the element pairs that the fragment
 // layout wants from two steps: W goes from memory to the tensor cores through
-// registers alone, kAhead steps at a time.  (What bounds it besides memory is
-// the issue of instructions, about ten for a KB of W here.  A deeper queue
-// through shared memory by cp.async, with blocks that go on to further rows
-// without draining it, took 73 us for 13 tokens and 65536 rows of 2048 where
-// this takes 56; 45 for 8 tokens, 91% of the copy rate.)
+// registers alone, kAhead steps at a time, past L1, where x stays.  65536 rows
+// of 2048: 41 us for one token, 43 for 8 (95% of the copy rate), 53 for 13,
+// where x's loads are as many as W's and warps wait for both.  (For 13 tokens
+// a queue through shared memory by cp.async, with blocks that go on to further
+// rows without draining it, took 73 us; steps loaded one by one as others are
+// used up, 72; 32 rows per warp, which halve x's loads, 54, but 64 instead of
+// 56 for 16384 rows of 8192.)
 //
 // A warp has 16 rows of W; up to eight warps share 16 rows, each with a part
 // of K, and add up in shared memory in a fixed order: short blocks, so that
