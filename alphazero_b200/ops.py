@@ -10,7 +10,7 @@ ValueError (wrong shapes or values) or TypeError (wrong types or devices);
 failures of the library raise RuntimeError.  There is no CPU fallback.
 
 ``embedding``, ``linear_layer`` and ``cross_entropy_loss`` are the same
-operators for torch's autograd.  The reference trains with torch on its own
+operators for torch's autograd (first derivatives; a second one raises).  The reference trains with torch on its own
 (scripts/train.py) and has no counterpart.
 """
 from __future__ import annotations
@@ -19,6 +19,7 @@ import ctypes
 import struct
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import engine
 
@@ -331,6 +332,7 @@ class _Embedding(torch.autograd.Function):
         return embed(tokens, table, scale)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         (tokens,) = ctx.saved_tensors
         return None, embed_backward(grad, tokens, ctx.vocab, ctx.scale), None
@@ -348,6 +350,7 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         x, weight, z = ctx.saved_tensors
         dx, dw, db = linear_backward(grad, x, weight, z, ctx.activation, ctx.has_bias)
@@ -366,6 +369,7 @@ class _CrossEntropy(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         factor = grad / ctx.grad_scale
         dx, dw, db = (None if t is None else (t * factor).to(t.dtype) for t in ctx.saved_tensors)

@@ -407,6 +407,20 @@ def test_cross_entropy_in_several_pieces():
     check_cross_entropy(x, w, integers(n, -5, vocab), b)
 
 
+def test_cross_entropy_few_classes_in_several_pieces():
+    n, vocab, dim = 1060000, 510, 8
+    x, w, b = make(n, dim), make(vocab, dim, seed=1, scale=0.5), make(vocab, seed=2)
+    check_cross_entropy(x, w, integers(n, -1, vocab), b)
+
+
+def test_autograd_once():
+    x, w = make(20, 64).requires_grad_(), make(40, 64, seed=1, scale=0.2).requires_grad_()
+    y = ops.linear_layer(x, w, activation="gelu")
+    (d,) = torch.autograd.grad(y.float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(d.float().sum(), w)
+
+
 def test_cross_entropy_gradient_by_differences():
     n, vocab, dim = 60, 100, 32
     x, w, b = (make(n, dim, dtype=torch.float16), make(vocab, dim, dtype=torch.float16, seed=1, scale=0.3),
