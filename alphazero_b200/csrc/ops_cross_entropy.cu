@@ -52,6 +52,70 @@ __device__ __forceinline__ void join(float& m, float& s, float2 p) {
     m = top;
 }
 
+// The same of the warp's lanes.
+__device__ __forceinline__ void join_lanes(float& m, float& s) {
+    float top = m;
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+    s *= exp2f((m - (top == -INFINITY ? 0.0f : top)) * 1.4426950408889634f);
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) s += __shfl_xor_sync(~0u, s, d);
+    m = top;
+}
+
+// A row's loss, given that it is counted.
+__device__ __forceinline__ float loss_of(float m, float s, float at) {
+    const float lse = s == 0.0f ? -INFINITY : m + logf(s);
+    return at == -INFINITY ? INFINITY : lse - at;
+}
+
+// A few rows without gradients: their losses and the mean in one launch, by a
+// cluster whose CTAs have two rows each and leave their losses with the first.
+// Bound by latency: 7.6 us for 13 rows of 4096 blocks of columns, where a block per
+// row and another launch for the mean took 8.8 and the step between them.
+constexpr int kFewRows = 16;
+
+__global__ void __cluster_dims__(kFewRows / 2, 1, 1) __launch_bounds__(1024)
+    few_rows_kernel(int rows, int blocks, const float2* part, int64_t part_ld, Indices target, const float* logit,
+                    float* row_loss, float* loss) {
+    __shared__ float2 sums[32];
+    __shared__ float2 losses[kFewRows];  // the first CTA's: a row's loss and 1, or zeros
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = warp >> 4;
+    const int rank = (int)cluster_rank(), row = rank + half * (kFewRows / 2);
+    griddep_launch_dependents();
+    cluster_sync();  // all CTAs have begun: their shared memory can be written
+    griddep_wait();
+    float m = -INFINITY, s = 0.0f;
+    if (row < rows)
+#pragma unroll 8
+        for (int b = threadIdx.x & 511; b < blocks; b += 512) join(m, s, part[(int64_t)b * part_ld + row]);
+    join_lanes(m, s);
+    if (lane == 0) sums[warp] = make_float2(m, s);
+    __syncthreads();
+    if ((warp & 15) == 0) {
+        const float2 p = lane < 16 ? sums[half * 16 + lane] : make_float2(-INFINITY, 0.0f);
+        m = p.x;
+        s = p.y;
+        join_lanes(m, s);
+        if (lane == 0) {
+            const bool counted = row < rows && target.at(row) >= 0;
+            const float l = counted ? loss_of(m, s, logit[row]) : 0.0f;
+            if (row < rows) row_loss[row] = l;
+            asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(map_to_rank(smem_u32(&losses[row]), 0)), "f"(l),
+                         "f"(counted ? 1.0f : 0.0f)
+                         : "memory");
+        }
+    }
+    cluster_sync();
+    if (rank > 0 || threadIdx.x > 0) return;
+    float all = 0.0f, count = 0.0f;
+    for (int r = 0; r < rows; ++r) {
+        all += losses[r].x;
+        count += losses[r].y;
+    }
+    *loss = all / fmaxf(count, 1.0f);
+}
+
 // Bound by latency: 5 us for 13 rows of 4096 blocks of columns, 13 for 4096
 // rows of 513.
 // logsumexp and loss per row, and the loss summed per block: a thread per row
@@ -75,15 +139,6 @@ __global__ void __launch_bounds__(HOW == kThreadPerRow ? 128 : 1024)
     const int64_t row0 = (int64_t)blockIdx.x * kRows;
     const int64_t row = row0 + (FEW ? threadIdx.x : HOW == kBlockPerRow ? 0 : warp);
     float m = -INFINITY, s = 0.0f;
-    const auto join_lanes = [&] {
-        float top = m;
-#pragma unroll
-        for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-        s *= exp2f((m - (top == -INFINITY ? 0.0f : top)) * 1.4426950408889634f);
-#pragma unroll
-        for (int d = 16; d > 0; d /= 2) s += __shfl_xor_sync(~0u, s, d);
-        m = top;
-    };
     if constexpr (FEW) {
         if (row < rows)
 #pragma unroll 4
@@ -91,12 +146,12 @@ __global__ void __launch_bounds__(HOW == kThreadPerRow ? 128 : 1024)
     } else if constexpr (HOW == kBlockPerRow) {
 #pragma unroll 4
         for (int b = threadIdx.x; b < blocks; b += 1024) join(m, s, part[(int64_t)b * part_ld + row]);
-        join_lanes();
+        join_lanes(m, s);
         tile[0][warp] = make_float2(m, s);
         __syncthreads();
         m = tile[0][lane].x;
         s = tile[0][lane].y;
-        join_lanes();
+        join_lanes(m, s);
     } else {
         // read along the rows, a warp per block of columns in turn; then turned round
         if (row0 + lane < rows)
@@ -106,15 +161,14 @@ __global__ void __launch_bounds__(HOW == kThreadPerRow ? 128 : 1024)
         __syncthreads();
         m = tile[lane][warp].x;
         s = tile[lane][warp].y;
-        join_lanes();
+        join_lanes(m, s);
     }
     float loss = 0.0f;
     bool counted = false;
     if (row < rows) {
         const float l = s == 0.0f ? -INFINITY : m + logf(s);
         counted = target.at(row) >= 0;
-        const float at = counted ? logit[row] : 0.0f;
-        if (counted) loss = at == -INFINITY ? INFINITY : l - at;
+        if (counted) loss = loss_of(m, s, logit[row]);
         if (FEW || lane == 0) {  // (a block per row: every warp has the row, and writes the same)
             lse[row] = l;
             row_loss[row] = loss;
@@ -257,6 +311,7 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
     shape.n = a.vocab;
     shape.k = a.dim;
     const bool rows_whole = gemm_rows_pays(shape, grads);
+    const bool few = !grads && !rows_whole && a.n <= kFewRows;
     const int block = gemm_softmax_block(shape);
     const int blocks = (int)((a.vocab + block - 1) / block);
 
@@ -337,6 +392,11 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
             f.e.probs = probs;
             f.e.probs_ld = ld;
             gemm_softmax(DT, f, block, q);
+            if (few) {
+                q.launch("few_rows_kernel", few_rows_kernel, dim3(kFewRows / 2), 1024, 0, (int)rows, blocks, part, piece, target,
+                         logit, a.row_loss, a.loss);
+                return;
+            }
             const int64_t combine_blocks = (rows + combine_rows - 1) / combine_rows;
             const auto kernel = how == kThreadPerRow  ? combine_kernel<kThreadPerRow>
                                 : how == kBlockPerRow ? combine_kernel<kBlockPerRow>
