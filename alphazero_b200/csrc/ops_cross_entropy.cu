@@ -106,6 +106,7 @@ __global__ void __cluster_dims__(kFewRows / 2, 1, 1) __launch_bounds__(1024)
                          : "memory");
         }
     }
+    __syncwarp();
     cluster_sync();
     if (rank > 0 || threadIdx.x > 0) return;
     float all = 0.0f, count = 0.0f;
@@ -312,8 +313,8 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
     shape.k = a.dim;
     const bool rows_whole = gemm_rows_pays(shape, grads);
     const bool few = !grads && !rows_whole && a.n <= kFewRows;
-    const int block = gemm_softmax_block(shape);
-    const int blocks = (int)((a.vocab + block - 1) / block);
+    const SoftmaxBlocks cut = gemm_softmax_blocks(shape, grads);
+    const int block = cut.columns, blocks = cut.count;
 
     Indices target;
     target.data = a.targets;
@@ -459,9 +460,9 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
 }
 
 void check(const mg_cross_entropy_args& a) {
-    const int64_t top = int64_t(1) << 31;
+    const int64_t top = (int64_t(1) << 31) - 1024;  // whole tiles still count in 32 bits
     need(a.n >= 0 && a.vocab >= 1 && a.dim >= 1, "sizes: n >= 0, vocab >= 1, dim >= 1");
-    need(a.n < top && a.vocab < top && a.dim < top, "n, vocab and dim must be below 2^31");
+    need(a.n < top && a.vocab < top && a.dim < top, "n, vocab and dim must be below 2^31 - 1024");
     need(a.dtype == MG_PREC_BF16 || a.dtype == MG_PREC_FP16, "dtype must be MG_PREC_BF16 or MG_PREC_FP16");
     need(a.target_bytes == 8 || a.target_bytes == 4, "targets are int64 or int32 (target_bytes 8 or 4)");
     need(a.target_stride >= 0 && a.x_row >= 0 && a.x_col >= 0 && a.w_row >= 0 && a.w_col >= 0,

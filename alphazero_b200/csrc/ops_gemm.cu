@@ -1152,11 +1152,15 @@ CUtensorMapDataType map_type(int dtype) {
     return dtype == MG_PREC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
 }
 
+}  // namespace
+
 // An operand, in boxes of 64 contraction steps (128 bytes, or lines).
 void encode_operand(CUtensorMap* map, int dtype, const StagedOperand& s, int64_t rows, int64_t k, int tile_rows) {
     encode(map, map_type(dtype), 2, s.data, s.mn ? rows : k, s.mn ? k : rows, s.ld, 64, s.mn ? kBK : tile_rows,
            CU_TENSOR_MAP_SWIZZLE_128B);
 }
+
+namespace {
 
 // A matrix that the epilogue moves in blocks of 32 x 64 16-bit elements.
 void encode_blocks(CUtensorMap* map, int dtype, const void* base, int64_t m, int64_t n, int64_t ld) {
@@ -1337,11 +1341,16 @@ namespace {
 bool is_skinny(const SoftmaxJob& g) { return g.m <= kSkinnyRows && !g.a.mn && !g.b.mn; }
 }  // namespace
 
-int gemm_softmax_block(const SoftmaxJob& g) { return is_skinny(g) ? skinny_block(g.k) : tile_columns(&g, 1) / 2; }
+SoftmaxBlocks gemm_softmax_blocks(const SoftmaxJob& g, bool even) {
+    if (is_skinny(g)) return skinny_blocks(g.m, g.n, g.k, even);
+    const int columns = tile_columns(&g, 1) / 2;
+    return {columns, (int)((g.n + columns - 1) / columns)};
+}
 
-void gemm_softmax(int dtype, const SoftmaxJob& g, int block, Queue& q) {
-    if (is_skinny(g) && block == skinny_block(g.k)) return skinny_softmax(dtype, g, block, q);
-    const int bn = 2 * block;
+void gemm_softmax(int dtype, const SoftmaxJob& g, int columns, Queue& q) {
+    if (is_skinny(g) && (columns == 0 || columns == skinny_blocks(g.m, g.n, g.k, true).columns))
+        return skinny_softmax(dtype, g, columns, q);
+    const int bn = 2 * columns;
     KernelArgs a{};
     lay_out(a.job[0], g, bn);
     a.job[0].s = g.e;

@@ -67,8 +67,8 @@ struct GemmJob {
 constexpr int kSkinnyRows = 16;
 
 // Softmax statistics of l = acc + bias instead of a product (the forward
-// half of the cross entropy).  A row's columns are taken in blocks of
-// `block` (gemm_softmax_block()); per block and row
+// half of the cross entropy).  A row's columns are taken in blocks
+// (gemm_softmax_blocks()); per block and row
 //   part[block * part_ld + row] = (max, sum of exp(l - max)),
 // (-inf, 0) for a block of -inf; logit[row] = l at the row's target; and, if
 // probs is set, probs[row * probs_ld + col] = exp(l - max) as a Prob16.
@@ -90,9 +90,15 @@ struct SoftmaxJob {
 template <int DT>
 constexpr float kDScale = DT == MG_PREC_FP16 ? 16384.0f : 1.0f;
 
-int gemm_softmax_block(const SoftmaxJob& job);
-// `block`: gemm_softmax_block of the largest job that shares part's layout.
-void gemm_softmax(int dtype, const SoftmaxJob& job, int block, Queue& q);
+struct SoftmaxBlocks {
+    int columns;  // of each, or 0: some number (not to be used with probs)
+    int count;
+};
+// The blocks of the largest job that shares part's layout; even: all have
+// the same number of columns.
+SoftmaxBlocks gemm_softmax_blocks(const SoftmaxJob& job, bool even);
+// `columns` of those.
+void gemm_softmax(int dtype, const SoftmaxJob& job, int columns, Queue& q);
 
 // The same, whole rows at a time, where n is small: the sums of 256 rows and
 // up to kRowsColumns columns stay in TMEM until the rows' softmax is known,
@@ -120,8 +126,12 @@ int gemm_rows_ctas(int64_t m);
 void gemm_rows(int dtype, const RowsJob& job, Queue& q);
 
 void skinny(int dtype, const GemmJob& job, Queue& q);
-int skinny_block(int64_t k);  // columns per block of the statistics
+SoftmaxBlocks skinny_blocks(int64_t m, int64_t n, int64_t k, bool even);
 void skinny_softmax(int dtype, const SoftmaxJob& job, int block, Queue& q);
+
+// The tensor map of an operand of rows x k, in boxes of tile_rows (at most 64
+// where it lies along its rows) x 64.
+void encode_operand(CUtensorMap* map, int dtype, const StagedOperand& s, int64_t rows, int64_t k, int tile_rows);
 
 // A number in [0, 1] in 16 bits: 4 bits of exponent and 12 of fraction, no
 // sign (relative error 2^-14 from 2^-14 up, absolute 2^-28 below).  A block's

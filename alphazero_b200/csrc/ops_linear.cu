@@ -87,9 +87,9 @@ __global__ void __launch_bounds__(256)
 }
 
 void check_sizes(int64_t m, int64_t n, int64_t k) {
-    const int64_t top = int64_t(1) << 31;
+    const int64_t top = (int64_t(1) << 31) - 1024;  // whole tiles still count in 32 bits
     need(m >= 0 && n >= 1 && k >= 1, "sizes: m >= 0, n >= 1, k >= 1");
-    need(m < top && n < top && k < top, "m, n and k must be below 2^31");
+    need(m < top && n < top && k < top, "m, n and k must be below 2^31 - 1024");
 }
 
 void check(const mg_linear_args& a) {

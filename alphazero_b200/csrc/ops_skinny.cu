@@ -222,11 +222,235 @@ void launch(int dtype, SkinnyArgs& a, Queue& q) {
     q.launch("skinny_kernel", kernel, grid, 256, 0, a);
 }
 
+// ---- nine to sixteen tokens, many rows of W ----
+//
+// W's rows are the M side of tcgen05.mma (128 per tile) and the tokens its N
+// side; both come to shared memory by TMA, so that neither L1 nor the issue of
+// loads limits the one read of W: up to kStages steps of it are on their way
+// per SM.  A thread of the four epilogue warps has a row of W and all tokens;
+// tiles alternate between two sets of 16 columns of TMEM.  Tiles have as many
+// rows as give every SM the same number of them (an SM reads about 65 GB/s
+// alone, so a last round on some is no faster than one on all); what the
+// other rows of the products hold is not used.  STREAMTIME
+
+constexpr int kTileRows = 128, kTileTokens = 16, kStepK = 64, kStages = 11;
+constexpr uint32_t kWBytes = kTileRows * kStepK * 2, kXBytes = kTileTokens * kStepK * 2, kStageBytes = kWBytes + kXBytes;
+constexpr int kStreamThreads = 32 * 6;
+constexpr int kStreamSmem = kStages * kStageBytes + (2 * kStages + 5) * 8 + 16;
+
+struct alignas(64) StreamArgs {
+    CUtensorMap tw, tx;
+    int m, n, steps, tiles;
+    int rows;    // of W per tile, up to kTileRows
+    int groups;  // of 32 columns or fewer, SOFTMAX
+    GemmEpilogue e;
+    SoftmaxEpilogue s;
+    int* err;
+};
+
+// The lane's row of W is column `col`, past the warp's part if it is not
+// below `end`; v: its sums, per token.
+template <int DT, bool SOFTMAX>
+__device__ __forceinline__ void stream_epilogue(const StreamArgs& a, float (&v)[kTileTokens], int col, int end,
+                                                int group, int target, int lane) {
+    using E = Elem<DT>;
+    using T = typename E::T;
+    if constexpr (SOFTMAX) {
+        const SoftmaxEpilogue& e = a.s;
+        const float bias = e.bias != nullptr && col < end ? E::get(static_cast<const T*>(e.bias)[col]) : 0.0f;
+        float2 mine = make_float2(-INFINITY, 0.0f);  // lane i: token i's
+#pragma unroll
+        for (int t = 0; t < kTileTokens; ++t) {
+            if (t >= a.m) break;
+            const float l = col < end ? v[t] + bias : -INFINITY;
+            if (col == __shfl_sync(~0u, target, t) && col < end) e.logit[t] = l;
+            float top = l;
+#pragma unroll
+            for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+            const float p = exp2f((l - (top == -INFINITY ? 0.0f : top)) * 1.4426950408889634f);
+            if (e.probs != nullptr && col < end) e.probs[t * e.probs_ld + col] = (uint16_t)prob16(p);
+            float sum = p;
+#pragma unroll
+            for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
+            if (lane == t) mine = make_float2(top, sum);
+        }
+        if (lane < a.m && group < a.groups) e.part[(int64_t)group * e.part_ld + lane] = mine;
+    } else {
+        const GemmEpilogue& e = a.e;
+        if (col >= end) return;
+        const float bias = e.bias != nullptr ? E::get(static_cast<const T*>(e.bias)[col]) : 0.0f;
+#pragma unroll
+        for (int t = 0; t < kTileTokens; ++t) {
+            if (t >= a.m) break;
+            float y = v[t] * e.alpha + bias;
+            if (e.z) static_cast<T*>(e.z)[t * e.ld + col] = E::put(y);
+            y = activate(y, e.act);
+            if (e.res) y += e.res_scale * E::get(static_cast<const T*>(e.res)[t * e.r_row + col * e.r_col]);
+            static_cast<T*>(e.out)[t * e.ld + col] = E::put(y);
+        }
+    }
+}
+
+template <int DT, bool SOFTMAX>
+__global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_constant__ StreamArgs a) {
+    extern __shared__ __align__(1024) uint8_t ring[];
+    uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages * kStageBytes);  // a stage has landed
+    uint64_t* empty = full + kStages;                                            // its products are complete
+    uint64_t* tfull = empty + kStages;                                           // [2] a tile's sums are complete
+    uint64_t* tempty = tfull + 2;                                                // [2] they have been read
+    uint64_t* done = tempty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(smem_u32(&full[s]), 1);
+            mbar_init(smem_u32(&empty[s]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&tfull[i]), 1);
+            mbar_init(smem_u32(&tempty[i]), 4);
+        }
+        mbar_init(smem_u32(done), 1);
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(tmem_slot), 2 * kTileTokens);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    griddep_launch_dependents();
+    griddep_wait();
+
+    if (warp == 0) {
+        int s = 0, round = 0;
+        int64_t used = 0;
+        bool ok = true;
+        for (int tile = blockIdx.x; ok && tile < a.tiles; tile += gridDim.x)
+            for (int k = 0; k < a.steps; ++k) {
+                if (!mbar_wait_warp(smem_u32(&empty[s]), (round & 1) ^ 1, a.err, kErrWaitProducer)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t at = smem_u32(ring + s * kStageBytes), bar = smem_u32(&full[s]);
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(bar, a.rows * kStepK * 2 + kXBytes);
+                    tma_load_2d(at, &a.tw, bar, k * kStepK, tile * a.rows);
+                    tma_load_2d(at + kWBytes, &a.tx, bar, k * kStepK, 0);
+                }
+                ++used;
+                if (++s == kStages) {
+                    s = 0;
+                    ++round;
+                }
+            }
+        // every load has landed before this CTA ends
+        for (int i = 0; i < kStages && i < used; ++i) {
+            if (--s < 0) {
+                s = kStages - 1;
+                --round;
+            }
+            mbar_wait_warp(smem_u32(&full[s]), round & 1, a.err, kErrWaitDrain);
+        }
+    } else if (warp == 1) {
+        constexpr uint32_t idesc = idesc_f16(kTileRows, kTileTokens, DT == MG_PREC_BF16);
+        const uint64_t w0 = smem_desc_sw128(smem_u32(ring)), x0 = smem_desc_sw128(smem_u32(ring) + kWBytes);
+        int s = 0, round = 0, count = 0;
+        bool ok = true;
+        for (int tile = blockIdx.x; ok && tile < a.tiles; tile += gridDim.x, ++count) {
+            const int buf = count & 1;
+            if (!mbar_wait_warp(smem_u32(&tempty[buf]), ((count >> 1) & 1) ^ 1, a.err, kErrWaitMma)) break;
+            tc_fence_after();
+            for (int k = 0; k < a.steps; ++k) {
+                if (!mbar_wait_warp(smem_u32(&full[s]), round & 1, a.err, kErrWaitMma)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint64_t w = w0 + s * (kStageBytes >> 4), x = x0 + s * (kStageBytes >> 4);
+                if (elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < kStepK / 16; ++kk)
+                        mma_f16(tmem_base + buf * kTileTokens, w + kk * 2, x + kk * 2, idesc, k > 0 || kk > 0);
+                    mma_commit(smem_u32(&empty[s]));
+                    if (k + 1 == a.steps) mma_commit(smem_u32(&tfull[buf]));
+                }
+                if (++s == kStages) {
+                    s = 0;
+                    ++round;
+                }
+            }
+        }
+        // products still in flight finish before TMEM is freed
+        if (elect_one()) mma_commit(smem_u32(done));
+        mbar_wait_warp(smem_u32(done), 0, a.err, kErrWaitDrain);
+    } else {
+        const int quarter = warp & 3, parts = (a.rows + 31) / 32;  // of a tile, a warp each
+        const int target = SOFTMAX && lane < a.m ? a.s.target.at(lane) : -1;
+        int count = 0;
+        for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++count) {
+            const int buf = count & 1;
+            if (!mbar_wait_warp(smem_u32(&tfull[buf]), (count >> 1) & 1, a.err, kErrWaitEpilogue)) break;
+            tc_fence_after();
+            uint32_t r[kTileTokens];
+            tmem_ld_16cols(tmem_base + buf * kTileTokens + ((uint32_t)quarter << 21), r);
+            tmem_ld_wait(r);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&tempty[buf]));
+            float v[kTileTokens];
+#pragma unroll
+            for (int t = 0; t < kTileTokens; ++t) v[t] = __uint_as_float(r[t]);
+            const int first = tile * a.rows + quarter * 32, end = min(a.n, (tile + 1) * a.rows);
+            if (quarter < parts) stream_epilogue<DT, SOFTMAX>(a, v, first + lane, end, tile * parts + quarter, target, lane);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tmem_base, 2 * kTileTokens);
+}
+
+// Rows of W per tile: as many as give each SM as many tiles.
+int stream_rows(int64_t n) {
+    const int64_t rounds = (n + 148 * kTileRows - 1) / (148 * kTileRows);
+    return (int)((n + 148 * rounds - 1) / (148 * rounds));
+}
+bool streams(int64_t m, int64_t n) { return m > 8 && n >= 2048; }
+
+template <bool SOFTMAX, class Job>
+void stream(int dtype, const Job& j, int rows, StreamArgs& a, Queue& q) {
+    a.rows = rows;
+    encode_operand(&a.tw, dtype, j.b, j.n, j.k, rows);
+    encode_operand(&a.tx, dtype, j.a, j.m, j.k, kTileTokens);
+    a.m = (int)j.m;
+    a.n = (int)j.n;
+    a.steps = (int)((j.k + kStepK - 1) / kStepK);
+    a.tiles = (int)((j.n + rows - 1) / rows);
+    a.err = op_status_word();
+    const auto kernel = dtype == MG_PREC_BF16 ? stream_kernel<MG_PREC_BF16, SOFTMAX> : stream_kernel<MG_PREC_FP16, SOFTMAX>;
+    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamSmem),
+          "cudaFuncSetAttribute(stream_kernel)");
+    q.launch("stream_kernel", kernel, dim3((unsigned)std::min(a.tiles, 148)), kStreamThreads, kStreamSmem, a);
+}
+
 }  // namespace
 
-int skinny_block(int64_t k) { return 128 / share_of(k); }
+SoftmaxBlocks skinny_blocks(int64_t m, int64_t n, int64_t k, bool even) {
+    if (!streams(m, n)) return {128 / share_of(k), (int)((n * share_of(k) + 127) / 128)};
+    if (even) return {32, (int)((n + 31) / 32)};
+    const int rows = stream_rows(n);
+    return {0, (int)((n + rows - 1) / rows) * ((rows + 31) / 32)};
+}
 
 void skinny(int dtype, const GemmJob& j, Queue& q) {
+    if (streams(j.m, j.n)) {
+        StreamArgs s{};
+        s.e = j.e;
+        return stream<false>(dtype, j, stream_rows(j.n), s, q);
+    }
     SkinnyArgs a = lay_out(j);
     a.e = j.e;
     a.share = share_of(a.k);
@@ -234,9 +458,15 @@ void skinny(int dtype, const GemmJob& j, Queue& q) {
 }
 
 void skinny_softmax(int dtype, const SoftmaxJob& j, int block, Queue& q) {
+    if (streams(j.m, j.n)) {
+        StreamArgs s{};
+        s.s = j.e;
+        s.groups = skinny_blocks(j.m, j.n, j.k, block > 0).count;
+        return stream<true>(dtype, j, block > 0 ? kTileRows : stream_rows(j.n), s, q);
+    }
     SkinnyArgs a = lay_out(j);
     a.s = j.e;
-    a.share = 128 / block;
+    a.share = share_of(a.k);
     launch<true>(dtype, a, q);
 }
 

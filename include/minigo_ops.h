@@ -150,7 +150,8 @@ int mg_linear_backward(const mg_linear_backward_args* args, void* workspace, siz
  * of d over rows; rows that are not counted give nothing.  d is rounded to
  * the operands' type once.  FP16 gradients are small: give a grad_scale
  * that keeps them in range.  All three gradients, or none, except that db
- * is NULL without a bias.  n may be 0; vocab and dim may not.  vocab < 2^31. */
+ * is NULL without a bias.  n may be 0; vocab and dim may not.  n, vocab and dim
+ * are below 2^31 - 1024. */
 typedef struct mg_cross_entropy_args {
     const void* x;
     const void* weight;

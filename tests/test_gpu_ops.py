@@ -186,6 +186,13 @@ def test_linear(dtype, name, m, n, k):
         ref.within(z, want_z, off_z)
 
 
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("name", sorted(ops.ACTIVATIONS))
+@pytest.mark.parametrize("m,n,k", [(9, 2050, 64), (13, 5001, 72), (16, 20000, 136), (12, 40000, 7), (10, 19072, 1500)])
+def test_linear_few_tokens(dtype, name, m, n, k):
+    test_linear(dtype, name, m, n, k)
+
+
 @pytest.mark.parametrize("m", [1, 40, 300])
 @pytest.mark.parametrize("how", ["transposed", "offset", "spread"])
 def test_linear_layouts(m, how):
@@ -323,6 +330,15 @@ def test_cross_entropy_few_classes(bias, n, vocab, dim):
     x, w = make(n, dim), make(vocab, dim, seed=1, scale=2 * dim ** -0.5)
     b = make(vocab, seed=2) if bias else None
     check_cross_entropy(x, w, integers(n, -1, vocab + 1), b)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("n,vocab,dim", [(16, 20003, 264), (9, 2048, 64), (10, 2049, 65), (12, 19001, 1030)])
+def test_cross_entropy_few_rows(dtype, n, vocab, dim):
+    x, w = make(n, dim, dtype=dtype), make(vocab, dim, dtype=dtype, seed=1, scale=2 * dim ** -0.5)
+    b = make(vocab, dtype=dtype, seed=2)
+    b[vocab // 2:vocab // 2 + 200] = -INF
+    check_cross_entropy(x, w, integers(n, -1, vocab // 2), b, 512.0 if dtype == torch.float16 else 1.0)
 
 
 @pytest.mark.parametrize("low", [-INF, -3.0e38])
