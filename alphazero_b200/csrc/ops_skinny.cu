@@ -228,13 +228,18 @@ void launch(int dtype, SkinnyArgs& a, Queue& q) {
 // side; both come to shared memory by TMA, so that neither L1 nor the issue of
 // loads limits the one read of W: up to kStages steps of it are on their way
 // per SM.  A thread of the four epilogue warps has a row of W and all tokens;
-// tiles alternate between two sets of 16 columns of TMEM.  Tiles have as many
+// tiles alternate between two halves of the TMEM.  Tiles have as many
 // rows as give every SM the same number of them (an SM reads about 65 GB/s
 // alone, so a last round on some is no faster than one on all); what the
-// other rows of the products hold is not used.  STREAMTIME
+// other rows of the products hold is not used.  CTAs begin at different steps
+// of k, so that they do not all ask for the same piece of x.  65536 rows of
+// 2048 and 13 tokens: 46 us, 90% of the rate of a plain copy.
 
-constexpr int kTileRows = 128, kTileTokens = 16, kStepK = 64, kStages = 11;
-constexpr uint32_t kWBytes = kTileRows * kStepK * 2, kXBytes = kTileTokens * kStepK * 2, kStageBytes = kWBytes + kXBytes;
+constexpr int kTileRows = 128, kTileTokens = 16, kStepK = 64, kChunks = 2, kStages = 5;  // a stage has kChunks of kStepK
+constexpr uint32_t kWBytes = kTileRows * kStepK * 2, kXBytes = kTileTokens * kStepK * 2, kStageBytes = kChunks * (kWBytes + kXBytes);
+// A stage's eight products each add to sums of their own: the tensor cores cut
+// their running sums, so long chains come out too small (ops_gemm.cu).
+constexpr int kSums = kChunks * kStepK / 16;
 constexpr int kStreamThreads = 32 * 6;
 constexpr int kStreamSmem = kStages * kStageBytes + (2 * kStages + 5) * 8 + 16;
 
@@ -314,7 +319,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
         fence_barrier_init();
     }
     if (warp == 1) {
-        tmem_alloc(smem_u32(tmem_slot), 2 * kTileTokens);
+        tmem_alloc(smem_u32(tmem_slot), 2 * kSums * kTileTokens);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -335,10 +340,14 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
                     break;
                 }
                 const uint32_t at = smem_u32(ring + s * kStageBytes), bar = smem_u32(&full[s]);
+                const int from = (k + (int)blockIdx.x) % a.steps * kChunks;
                 if (elect_one()) {
-                    mbar_arrive_expect_tx(bar, a.rows * kStepK * 2 + kXBytes);
-                    tma_load_2d(at, &a.tw, bar, k * kStepK, tile * a.rows);
-                    tma_load_2d(at + kWBytes, &a.tx, bar, k * kStepK, 0);
+                    mbar_arrive_expect_tx(bar, kChunks * (a.rows * kStepK * 2 + kXBytes));
+#pragma unroll
+                    for (int i = 0; i < kChunks; ++i) {
+                        tma_load_2d(at + i * kWBytes, &a.tw, bar, (from + i) * kStepK, tile * a.rows);
+                        tma_load_2d(at + kChunks * kWBytes + i * kXBytes, &a.tx, bar, (from + i) * kStepK, 0);
+                    }
                 }
                 ++used;
                 if (++s == kStages) {
@@ -356,7 +365,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
         }
     } else if (warp == 1) {
         constexpr uint32_t idesc = idesc_f16(kTileRows, kTileTokens, DT == MG_PREC_BF16);
-        const uint64_t w0 = smem_desc_sw128(smem_u32(ring)), x0 = smem_desc_sw128(smem_u32(ring) + kWBytes);
+        const uint64_t w0 = smem_desc_sw128(smem_u32(ring)), x0 = smem_desc_sw128(smem_u32(ring) + kChunks * kWBytes);
         int s = 0, round = 0, count = 0;
         bool ok = true;
         for (int tile = blockIdx.x; ok && tile < a.tiles; tile += gridDim.x, ++count) {
@@ -372,8 +381,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
                 const uint64_t w = w0 + s * (kStageBytes >> 4), x = x0 + s * (kStageBytes >> 4);
                 if (elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < kStepK / 16; ++kk)
-                        mma_f16(tmem_base + buf * kTileTokens, w + kk * 2, x + kk * 2, idesc, k > 0 || kk > 0);
+                    for (int kk = 0; kk < kSums; ++kk)
+                        mma_f16(tmem_base + (buf * kSums + kk) * kTileTokens, w + kk / 4 * (kWBytes >> 4) + kk % 4 * 2,
+                                x + kk / 4 * (kXBytes >> 4) + kk % 4 * 2, idesc, k > 0);
                     mma_commit(smem_u32(&empty[s]));
                     if (k + 1 == a.steps) mma_commit(smem_u32(&tfull[buf]));
                 }
@@ -394,15 +404,18 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
             const int buf = count & 1;
             if (!mbar_wait_warp(smem_u32(&tfull[buf]), (count >> 1) & 1, a.err, kErrWaitEpilogue)) break;
             tc_fence_after();
-            uint32_t r[kTileTokens];
-            tmem_ld_16cols(tmem_base + buf * kTileTokens + ((uint32_t)quarter << 21), r);
-            tmem_ld_wait(r);
+            float v[kTileTokens] = {};
+#pragma unroll
+            for (int i = 0; i < kSums; ++i) {
+                uint32_t r[kTileTokens];
+                tmem_ld_16cols(tmem_base + (buf * kSums + i) * kTileTokens + ((uint32_t)quarter << 21), r);
+                tmem_ld_wait(r);
+#pragma unroll
+                for (int t = 0; t < kTileTokens; ++t) v[t] += __uint_as_float(r[t]);
+            }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&tempty[buf]));
-            float v[kTileTokens];
-#pragma unroll
-            for (int t = 0; t < kTileTokens; ++t) v[t] = __uint_as_float(r[t]);
             const int first = tile * a.rows + quarter * 32, end = min(a.n, (tile + 1) * a.rows);
             if (quarter < parts) stream_epilogue<DT, SOFTMAX>(a, v, first + lane, end, tile * parts + quarter, target, lane);
         }
@@ -410,7 +423,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) stream_kernel(const __grid_
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 1) tmem_dealloc(tmem_base, 2 * kTileTokens);
+    if (warp == 1) tmem_dealloc(tmem_base, 2 * kSums * kTileTokens);
 }
 
 // Rows of W per tile: as many as give each SM as many tiles.
@@ -418,7 +431,12 @@ int stream_rows(int64_t n) {
     const int64_t rounds = (n + 148 * kTileRows - 1) / (148 * kTileRows);
     return (int)((n + 148 * rounds - 1) / (148 * rounds));
 }
-bool streams(int64_t m, int64_t n) { return m > 8 && n >= 2048; }
+// In us, this way and by the kernel above, 9 and 16 tokens, rows of W x k:
+// 65536 x 2048 46 and 48, 54 and 56; 16384 x 8192 46 and 47, 57 and 58; 131072
+// x 1000 50 and 51, 74 and 83; 19072 x 2048 17 and 18, 17 and 18; 8192 x 2048
+// 10 and 11, 11 and 11; 16384 x 512 7 and 8, 8 and 8; 4096 x 4096 15 and 16, 10
+// and 10 (tiles of few rows: a step's latency).
+bool streams(int64_t m, int64_t n, int64_t k) { return m > 8 && n >= 148 * 64 && n * k >= int64_t(1) << 25; }
 
 template <bool SOFTMAX, class Job>
 void stream(int dtype, const Job& j, int rows, StreamArgs& a, Queue& q) {
@@ -427,7 +445,7 @@ void stream(int dtype, const Job& j, int rows, StreamArgs& a, Queue& q) {
     encode_operand(&a.tx, dtype, j.a, j.m, j.k, kTileTokens);
     a.m = (int)j.m;
     a.n = (int)j.n;
-    a.steps = (int)((j.k + kStepK - 1) / kStepK);
+    a.steps = (int)((j.k + kChunks * kStepK - 1) / (kChunks * kStepK));
     a.tiles = (int)((j.n + rows - 1) / rows);
     a.err = op_status_word();
     const auto kernel = dtype == MG_PREC_BF16 ? stream_kernel<MG_PREC_BF16, SOFTMAX> : stream_kernel<MG_PREC_FP16, SOFTMAX>;
@@ -439,14 +457,14 @@ void stream(int dtype, const Job& j, int rows, StreamArgs& a, Queue& q) {
 }  // namespace
 
 SoftmaxBlocks skinny_blocks(int64_t m, int64_t n, int64_t k, bool even) {
-    if (!streams(m, n)) return {128 / share_of(k), (int)((n * share_of(k) + 127) / 128)};
+    if (!streams(m, n, k)) return {128 / share_of(k), (int)((n * share_of(k) + 127) / 128)};
     if (even) return {32, (int)((n + 31) / 32)};
     const int rows = stream_rows(n);
     return {0, (int)((n + rows - 1) / rows) * ((rows + 31) / 32)};
 }
 
 void skinny(int dtype, const GemmJob& j, Queue& q) {
-    if (streams(j.m, j.n)) {
+    if (streams(j.m, j.n, j.k)) {
         StreamArgs s{};
         s.e = j.e;
         return stream<false>(dtype, j, stream_rows(j.n), s, q);
@@ -458,7 +476,7 @@ void skinny(int dtype, const GemmJob& j, Queue& q) {
 }
 
 void skinny_softmax(int dtype, const SoftmaxJob& j, int block, Queue& q) {
-    if (streams(j.m, j.n)) {
+    if (streams(j.m, j.n, j.k)) {
         StreamArgs s{};
         s.s = j.e;
         s.groups = skinny_blocks(j.m, j.n, j.k, block > 0).count;

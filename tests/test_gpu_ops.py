@@ -188,7 +188,8 @@ def test_linear(dtype, name, m, n, k):
 
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("name", sorted(ops.ACTIVATIONS))
-@pytest.mark.parametrize("m,n,k", [(9, 2050, 64), (13, 5001, 72), (16, 20000, 136), (12, 40000, 7), (10, 19072, 1500)])
+@pytest.mark.parametrize("m,n,k", [(9, 2050, 64), (13, 5001, 72), (16, 20000, 136), (12, 40000, 7), (10, 19072, 1500),
+                                   (16, 20003, 1736), (9, 65537, 520), (12, 9472, 3545), (13, 33000, 1024)])
 def test_linear_few_tokens(dtype, name, m, n, k):
     test_linear(dtype, name, m, n, k)
 
@@ -333,7 +334,8 @@ def test_cross_entropy_few_classes(bias, n, vocab, dim):
 
 
 @pytest.mark.parametrize("dtype", HALF)
-@pytest.mark.parametrize("n,vocab,dim", [(16, 20003, 264), (9, 2048, 64), (10, 2049, 65), (12, 19001, 1030)])
+@pytest.mark.parametrize("n,vocab,dim", [(16, 20003, 264), (9, 2048, 64), (10, 2049, 65), (12, 19001, 1030), (16, 20003, 1736),
+                                         (11, 65537, 520)])
 def test_cross_entropy_few_rows(dtype, n, vocab, dim):
     x, w = make(n, dim, dtype=dtype), make(vocab, dim, dtype=dtype, seed=1, scale=2 * dim ** -0.5)
     b = make(vocab, dtype=dtype, seed=2)
