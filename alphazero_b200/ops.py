@@ -65,14 +65,15 @@ _stream = torch._C._cuda_getCurrentRawStream
 
 
 def _call(name: str, args: bytes, like, device: int) -> None:
-    L = lib()
+    L = _LIB or lib()
     need = ctypes.c_size_t()
     code = getattr(L, name + "_workspace")(args, ctypes.byref(need))
     if code:
         _raise(code)
+    size = need.value
     # torch's allocator orders the block's reuse after this stream's work
-    w = like.new_empty(need.value, dtype=torch.uint8) if need.value else None
-    code = getattr(L, name)(args, w.data_ptr() if w is not None else None, need.value, _stream(device))
+    w = like.new_empty(size, dtype=torch.uint8) if size else None
+    code = getattr(L, name)(args, w.data_ptr() if size else None, size, _stream(device))
     if code:
         _raise(code)
 
@@ -91,11 +92,11 @@ def synchronize(device=None) -> None:
 
 def _on_gpu(t, name: str) -> int:
     """The index of the tensor's device."""
+    if isinstance(t, torch.Tensor) and t.is_cuda:
+        return t.get_device()
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor, not {type(t).__name__}")
-    if not t.is_cuda:
-        raise TypeError(f"{name} must be a CUDA tensor (it is on {t.device})")
-    return t.get_device()
+    raise TypeError(f"{name} must be a CUDA tensor (it is on {t.device})")
 
 
 def _same(t, name: str, like, what: str, device: int) -> None:
@@ -125,21 +126,22 @@ def _indices(t, name: str, like, device: int) -> int:
 def _flat(t):
     """t as a vector, and its stride."""
     v = t if t.dim() == 1 else t.reshape(-1)
-    return v, v.stride(0)
+    return v, v.stride()[0]
 
 
 def _matrix(t, name: str, cols=None):
     """t [..., cols] as [rows, cols]; a copy only where the leading
     dimensions cannot be one."""
-    if t.dim() < 1:
+    shape = t.shape
+    if not shape:
         raise ValueError(f"{name} must have at least one dimension")
-    if cols is not None and t.shape[-1] != cols:
-        raise ValueError(f"{name} has {t.shape[-1]} columns, expected {cols}")
-    if t.dim() == 2:
+    if cols is not None and shape[-1] != cols:
+        raise ValueError(f"{name} has {shape[-1]} columns, expected {cols}")
+    if len(shape) == 2:
         return t
-    if t.shape[-1] == 0:
+    if shape[-1] == 0:
         raise ValueError(f"{name} has no columns")
-    return t.reshape(-1, t.shape[-1])
+    return t.reshape(-1, shape[-1])
 
 
 def _weight(t, name: str, like, what: str, device: int) -> None:
@@ -157,7 +159,7 @@ def _vector(t, name: str, n: int, like, what: str, device: int):
 
 def _rows(t):
     """t with unit column stride."""
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+    return t if t.stride()[1] == 1 or t.shape[1] == 1 else t.contiguous()
 
 
 def _ptr(t) -> int:
@@ -184,10 +186,14 @@ def embed(tokens, table, scale: float = 1.0):
         raise ValueError(f"table must be a matrix, not {tuple(table.shape)}")
     vocab, dim = table.shape
     t, t_stride = _flat(tokens)
-    table = _rows(table)
-    out = table.new_empty((*tokens.shape, dim))
-    code = lib().mg_embed(_EMBED.pack(t.data_ptr(), table.data_ptr(), out.data_ptr(), t.shape[0], vocab,
-                                      dim, t_stride, table.stride(0), scale, dt, tb, d), _stream(d))
+    row, column = table.stride()
+    if column != 1 and dim != 1:
+        table = table.contiguous()
+        row = dim
+    n = t.numel()
+    out = table.new_empty((n, dim) if t is tokens else (*tokens.shape, dim))
+    code = (_LIB or lib()).mg_embed(_EMBED.pack(t.data_ptr(), table.data_ptr(), out.data_ptr(), n, vocab,
+                                                dim, t_stride, row, scale, dt, tb, d), _stream(d))
     if code:
         _raise(code)
     return out
@@ -227,7 +233,7 @@ def linear(x, weight, bias=None, residual=None, activation: str = "none",
     n, k = weight.shape
     x2 = _matrix(x, "x", k)
     b = None if bias is None else _vector(bias, "bias", n, x, "x", d)
-    shape = (*x.shape[:-1], n)
+    shape = (x2.shape[0], n) if x2 is x else (*x.shape[:-1], n)
     r, r_row, r_col = None, 0, 0
     if residual is not None:
         _same(residual, "residual", x, "x", d)
