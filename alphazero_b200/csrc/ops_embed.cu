@@ -233,11 +233,20 @@ __global__ void __launch_bounds__(kSortThreads) scatter_kernel(SortArgs a, int p
     if (threadIdx.x < slices * quads) {
         const int quad = threadIdx.x % quads, slice = threadIdx.x / quads;
         uint4 before = make_uint4(0, 0, 0, 0), all = before;
-#pragma unroll 8
-        for (int b = slice; b < a.blocks; b += slices) {
-            const uint4 c = *reinterpret_cast<const uint4*>(a.counts + (int64_t)b * bins + quad * 4);
-            all.x += c.x, all.y += c.y, all.z += c.z, all.w += c.w;
-            if (b < blockIdx.x) before.x += c.x, before.y += c.y, before.z += c.z, before.w += c.w;
+        for (int b0 = slice; b0 < a.blocks; b0 += 8 * slices) {  // eight loads at once, whatever is left
+            uint4 c[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const int b = b0 + q * slices;
+                c[q] = b < a.blocks ? *reinterpret_cast<const uint4*>(a.counts + (int64_t)b * bins + quad * 4)
+                                    : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                all.x += c[q].x, all.y += c[q].y, all.z += c[q].z, all.w += c[q].w;
+                if (b0 + q * slices < blockIdx.x)
+                    before.x += c[q].x, before.y += c[q].y, before.z += c[q].z, before.w += c[q].w;
+            }
         }
         *reinterpret_cast<uint4*>(rows + (slice * 2) * bins + quad * 4) = before;
         *reinterpret_cast<uint4*>(rows + (slice * 2 + 1) * bins + quad * 4) = all;
@@ -271,11 +280,18 @@ __global__ void __launch_bounds__(kSortThreads) scatter_kernel(SortArgs a, int p
     }
     const int64_t begin = (int64_t)blockIdx.x * a.steps * kSortThreads;
     const int64_t end = min((int64_t)a.n, begin + (int64_t)a.steps * kSortThreads);
-#pragma unroll 4
-    for (int64_t i = begin + threadIdx.x; i < end; i += kSortThreads) {
-        uint32_t pos;
-        const uint32_t k = sort_key(a, pass, i, &pos);
-        a.out[rows[k >> shift & (bins - 1)] + a.place[i]] = make_uint2(k, pos);
+    for (int64_t i0 = begin + threadIdx.x; i0 < end; i0 += kBatch * kSortThreads) {
+        uint32_t k[kBatch], pos[kBatch], place[kBatch];
+#pragma unroll
+        for (int q = 0; q < kBatch; ++q) {
+            const int64_t i = i0 + q * kSortThreads;
+            if (i >= end) continue;
+            k[q] = sort_key(a, pass, i, &pos[q]);
+            place[q] = a.place[i];
+        }
+#pragma unroll
+        for (int q = 0; q < kBatch; ++q)
+            if (i0 + q * kSortThreads < end) a.out[rows[k[q] >> shift & (bins - 1)] + place[q]] = make_uint2(k[q], pos[q]);
     }
 }
 
