@@ -13,9 +13,9 @@
 // window order.  So a token that makes up a tenth of the batch is spread
 // over as many warps as its rows deserve, there are no atomics on sums, and
 // the result does not depend on the order in which blocks run.  100003 rows of
-// 1000 bf16 into 65536 entries: two digits' sort 28 us, bound by the latency
-// of its four launches; the sums 65 us, 5.1 TB/s of rows read and entries
-// written; the join 7 us.
+// 1000 bf16 into 65536 entries: two digits' sort 26 us, bound by the latency
+// of its four launches; the sums 66 us, 5 TB/s of rows read and entries
+// written; the join 6 us.
 #include "ops_common.cuh"
 
 #include <algorithm>
@@ -126,7 +126,7 @@ void embed(const mg_embed_args& a, Queue& q) {
 // earlier blocks and moves the tokens.  The moves are scattered 8-byte
 // writes, which one SM does at about one a clock: so the sort uses up to 148
 // blocks rather than one cluster (16 CTAs: 22 us a digit for 65536 tokens,
-// where these two take 13).
+// where these two take 12).
 
 constexpr int kSortWarps = 16;
 constexpr int kSortThreads = 32 * kSortWarps;
