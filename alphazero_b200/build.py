@@ -70,6 +70,7 @@ CUDA_HEADERS = [
     os.path.join(HOST, "onnx_reader.h"),
     os.path.join(CSRC, "ops_common.cuh"),
     os.path.join(CSRC, "ops_gemm.cuh"),
+    os.path.join(CSRC, "sorted_search.cuh"),
     os.path.join(INCLUDE, "minigo_cuda.h"),
     os.path.join(INCLUDE, "minigo_ops.h"),
 ]

@@ -17,6 +17,7 @@
 // of its four launches; the sums 66 us, 5 TB/s of rows read and entries
 // written; the join 6 us.
 #include "ops_common.cuh"
+#include "sorted_search.cuh"
 
 #include <algorithm>
 
@@ -399,16 +400,11 @@ struct Columns {
 
 constexpr int kAhead = 8;  // rows in flight per warp
 
-// First place in the sorted tokens whose token is at least v.
-__device__ __forceinline__ int lower_bound(const uint2* pair, int n, uint32_t v) {
-    int lo = 0, hi = n;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (pair[mid].x < v) lo = mid + 1;
-        else hi = mid;
-    }
-    return lo;
-}
+// The sorted tokens, for lower_bound.
+struct SortedTokens {
+    const uint2* pair;
+    __device__ __forceinline__ uint32_t operator()(int i) const { return pair[i].x; }
+};
 
 // Zeros to a row of any alignment.
 template <int DT>
@@ -439,7 +435,7 @@ __global__ void __launch_bounds__(256, 3) sum_kernel(SumArgs a, int64_t zero_blo
         const int64_t v0 = (int64_t)blockIdx.x * zero_rows, v = v0 + threadIdx.x;
         bool none = false;
         if (threadIdx.x < zero_rows && v < a.vocab) {
-            const int at = lower_bound(a.pair, a.n, (uint32_t)v);
+            const int at = lower_bound(SortedTokens{a.pair}, a.n, (uint32_t)v);
             none = at == a.n || a.pair[at].x != (uint32_t)v;
         }
         empty[threadIdx.x] = none;
