@@ -95,6 +95,11 @@ struct OpFailure {
 inline void need(bool ok, const char* what) {
     if (!ok) fail(MG_E_ARG, what);
 }
+// Kernels read and write whole elements.
+inline void need_aligned(const void* p, int bytes, const char* name) {
+    if (reinterpret_cast<uintptr_t>(p) % bytes != 0)
+        fail(MG_E_ARG, std::string(name) + " is not aligned to its elements");
+}
 inline void check(cudaError_t e, const char* where) {
     if (e != cudaSuccess) fail(MG_E_CUDA, std::string(where) + ": " + cudaGetErrorString(e));
 }

@@ -472,6 +472,15 @@ void check(const mg_cross_entropy_args& a) {
     const bool grads = a.dx || a.dw || a.db;
     need(!grads || (a.dw && (a.n == 0 || a.dx)), "gradients: give both dx and dw, or neither (and no db)");
     need(!grads || (a.db != nullptr) == (a.bias != nullptr), "db goes with a bias");
+    need_aligned(a.x, 2, "x");
+    need_aligned(a.weight, 2, "weight");
+    need_aligned(a.bias, 2, "bias");
+    need_aligned(a.targets, a.target_bytes, "targets");
+    need_aligned(a.loss, 4, "loss");
+    need_aligned(a.row_loss, 4, "row_loss");
+    need_aligned(a.dx, 2, "dx");
+    need_aligned(a.dw, 2, "dw");
+    need_aligned(a.db, 2, "db");
 }
 
 void cross_entropy(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {

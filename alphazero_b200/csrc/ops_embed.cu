@@ -665,6 +665,7 @@ void check_tokens(const void* p, int bytes, int64_t stride, int64_t n) {
     need(bytes == 8 || bytes == 4, "tokens are int64 or int32 (token_bytes 8 or 4)");
     need(n == 0 || p != nullptr, "tokens is null");
     need(stride >= 0, "token_stride is negative");
+    need_aligned(p, bytes, "tokens");
 }
 
 void check_args(const mg_embed_args& a) {
@@ -674,6 +675,8 @@ void check_args(const mg_embed_args& a) {
     check_tokens(a.tokens, a.token_bytes, a.token_stride, a.n);
     need(a.table_row >= 0, "table_row is negative");
     need(a.n == 0 || (a.table != nullptr && a.out != nullptr), "table or out is null");
+    need_aligned(a.table, elem_bytes(a.dtype), "table");
+    need_aligned(a.out, elem_bytes(a.dtype), "out");
 }
 
 void check_args(const mg_embed_backward_args& a) {
@@ -684,6 +687,8 @@ void check_args(const mg_embed_backward_args& a) {
     check_tokens(a.tokens, a.token_bytes, a.token_stride, a.n);
     need(a.grad_row >= 0, "grad_row is negative");
     need(a.d_table != nullptr && (a.n == 0 || a.grad != nullptr), "grad or d_table is null");
+    need_aligned(a.grad, elem_bytes(a.dtype), "grad");
+    need_aligned(a.d_table, elem_bytes(a.dtype), "d_table");
 }
 
 }  // namespace

@@ -99,6 +99,12 @@ void check(const mg_linear_args& a) {
     need(a.m == 0 || (a.x && a.weight && a.y), "x, weight or y is null");
     need(a.x_row >= 0 && a.x_col >= 0 && a.w_row >= 0 && a.w_col >= 0 && a.r_row >= 0 && a.r_col >= 0,
          "a stride is negative");
+    need_aligned(a.x, 2, "x");
+    need_aligned(a.weight, 2, "weight");
+    need_aligned(a.bias, 2, "bias");
+    need_aligned(a.residual, 2, "residual");
+    need_aligned(a.y, 2, "y");
+    need_aligned(a.z, 2, "z");
 }
 
 void check(const mg_linear_backward_args& a) {
@@ -112,6 +118,13 @@ void check(const mg_linear_backward_args& a) {
     need(a.g_row >= 0 && a.g_col >= 0 && a.x_row >= 0 && a.x_col >= 0 && a.w_row >= 0 &&
              a.w_col >= 0 && a.z_row >= 0 && a.z_col >= 0,
          "a stride is negative");
+    need_aligned(a.grad, 2, "grad");
+    need_aligned(a.x, 2, "x");
+    need_aligned(a.weight, 2, "weight");
+    need_aligned(a.z, 2, "z");
+    need_aligned(a.dx, 2, "dx");
+    need_aligned(a.dw, 2, "dw");
+    need_aligned(a.db, 2, "db");
 }
 
 void linear(const mg_linear_args& a, Workspace& w, bool go, Queue& q) {

@@ -28,6 +28,7 @@
  * strides (a column stride of 1 with a row stride that is a multiple of 8
  * and a 16-byte aligned base is read in place; the transposed form too;
  * others are first copied to the workspace).  Outputs are dense row-major.
+ * Every pointer is aligned to its elements.
  */
 #ifndef MINIGO_OPS_H
 #define MINIGO_OPS_H
