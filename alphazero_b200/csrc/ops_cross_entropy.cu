@@ -202,12 +202,13 @@ __global__ void __launch_bounds__(HOW == kThreadPerRow ? 128 : 1024)
 // half longer), the others take further rows.  The factor from the
 // block's maximum to the row's logsumexp is one exp per thread and row.
 // Bound by memory: 4096 x 65544 take 213 us, 5 TB/s read and written.
-// Block 0 also adds up counts, if set, to count.
+// Block 0 also adds up counts, if set, to count; each step of rows has a block
+// that looks for rows whose x would reach dw through d = 0 (CleanRows).
 template <int DT>
 __global__ void __launch_bounds__(256)
     d_kernel(int rows, int64_t vocab, int block, uint16_t* probs, int64_t ld, const float2* part, int64_t part_ld,
              const float* lse, Indices target, int wide, int rows_per_block, float* sums, const int* counts,
-             int64_t counts_n, int* count) {
+             int64_t counts_n, int* count, CleanRows clean) {
     using E = Elem<DT>;
     using T = typename E::T;
     __shared__ float acc[8][256];
@@ -224,6 +225,12 @@ __global__ void __launch_bounds__(256)
         n = __reduce_add_sync(~0u, n);
         if (lane == 0) *count = n;
     }
+    const int steps = (rows + kStepRows - 1) / kStepRows, step0 = blockIdx.y * gridDim.x + blockIdx.x;
+    const auto is_bad = [&](int g) {
+        const int row = g * kStepRows + threadIdx.x;
+        return threadIdx.x < kStepRows && row < rows && !isfinite(lse[row]) && target.at(row) < 0;
+    };
+    const bool bad = step0 < steps && is_bad(step0);  // its loads are ahead of the others
     if (c < vocab) {
         const float2* mine = part + c / block * part_ld;
         const int64_t step = deep * ld;
@@ -272,6 +279,11 @@ __global__ void __launch_bounds__(256)
                 *reinterpret_cast<uint4*>(p + q * step) = *reinterpret_cast<uint4*>(d);
             }
         }
+    }
+    for (int g = step0; g < steps; g += gridDim.x * gridDim.y) {
+        const bool any = __syncthreads_or(g == step0 ? bad : is_bad(g));
+        if (threadIdx.x == 0) clean.use[g] = any;
+        if (any) clean_step(clean, g, rows, target, threadIdx.x, 256);
     }
     if (sums == nullptr) return;
 #pragma unroll
@@ -326,6 +338,20 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
     float* lse = w.take<float>(per_row);
     float2* part = w.take<float2>(blocks * 2 * per_row);
     uint16_t* probs = grads ? w.take<uint16_t>((size_t)piece * ld * 2) : nullptr;
+    // a copy of x as x lies, of which few steps are ever written
+    StagedOperand other = x;
+    other.ld = ((x.mn ? piece : a.dim) + 7) / 8 * 8;
+    CleanRows clean;
+    if (grads) {
+        clean.clean = w.take<uint16_t>((size_t)(x.mn ? a.dim : piece) * other.ld * 2);
+        clean.use = w.take<uint16_t>((size_t)(piece + 255) / 256 * (256 / kStepRows) * 2);
+    }
+    other.data = clean.clean;
+    clean.row = x.mn ? 1 : x.ld;
+    clean.col = x.mn ? x.ld : 1;
+    clean.clean_row = x.mn ? 1 : other.ld;
+    clean.clean_col = x.mn ? other.ld : 1;
+    clean.dim = a.dim;
     int wide = 1;
     while (wide < 8 && wide * 256 < a.vocab) wide *= 2;
     const int64_t across = (a.vocab + 256 * wide - 1) / (256 * wide);
@@ -361,6 +387,7 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
         const bool first = row0 == 0, last = row0 + rows == a.n;
         StagedOperand xp = x;  // row0 is a multiple of 256: still aligned
         xp.data = static_cast<const uint16_t*>(x.data) + row0 * (x.mn ? 1 : x.ld);
+        clean.x = static_cast<const uint16_t*>(xp.data);
         if (go && rows_whole) {
             RowsJob f;
             f.a = xp;
@@ -376,6 +403,7 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
             f.e.d = probs;
             f.e.ld = ld;
             f.e.sums = sums ? sums + sum_rows * a.vocab : nullptr;
+            f.e.clean = clean;
             gemm_rows(DT, f, q);
             losses += gemm_rows_ctas(rows);
         } else if (go) {
@@ -412,7 +440,7 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
         if (go && !rows_whole) {
             q.launch("d_kernel", d_kernel<DT>, dim3((unsigned)across, (unsigned)these), 256, 0, (int)rows, a.vocab, block,
                      probs, ld, part, piece, lse, target.from(row0), wide, down_rows,
-                     sums ? sums + sum_rows * a.vocab : nullptr, first ? counts : nullptr, (int64_t)counts_n, total);
+                     sums ? sums + sum_rows * a.vocab : nullptr, first ? counts : nullptr, (int64_t)counts_n, total, clean);
         }
         sum_rows += these;
         StagedOperand d;
@@ -432,6 +460,8 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
         GemmJob& jw = jobs[1];
         jw.a = transposed(d);
         jw.b = transposed(xp);
+        jw.use_other = clean.use;
+        jw.b_other = transposed(other);
         jw.m = a.vocab;
         jw.n = a.dim;
         jw.k = rows;

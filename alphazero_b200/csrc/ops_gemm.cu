@@ -51,7 +51,7 @@ namespace {
 constexpr int kChain = 16;
 constexpr int kRowsCta = 128;          // rows of a tile per CTA
 constexpr int kRowsPair = 256;
-constexpr int kBK = 64;                // K elements per stage
+constexpr int kBK = kStepRows;         // K elements per stage
 constexpr int kPairs = 74;             // of SMs on a B200 (148)
 constexpr int kGroup = 8;              // row tiles walked together (their B tiles stay in L2)
 constexpr int kBlockBytes = 4096;      // 32 rows of 128 bytes: 64 columns of 16 bits or 32 of fp32
@@ -100,6 +100,7 @@ struct JobArgs {
     int m_pad;   // rows of out32 per split
     int across;  // kRows: column tiles of a unit
     int chain;   // kSoftmax: K steps whose products add up in TMEM
+    const uint16_t* use_other;  // GemmJob's
     GemmEpilogue e;
     SoftmaxEpilogue s;
     RowsEpilogue r;
@@ -109,6 +110,7 @@ struct alignas(64) KernelArgs {
     CUtensorMap ta[2], tb[2];
     CUtensorMap to[2];   // out, out32 or probs
     CUtensorMap tz, tr;  // z and residual of job 0
+    CUtensorMap tb_other;  // of the job with use_other
     JobArgs job[2];
     int units[2];
     int head_start;  // units of job 1 that a pair does while others finish their last unit of job 0
@@ -652,6 +654,7 @@ __device__ __forceinline__ bool rows_epilogue(const KernelArgs& a, const RowsEpi
             if (!wait(t)) return false;
             release(t);
         }
+        if (e.d != nullptr && share == 0 && lane == 0) reinterpret_cast<uint8_t*>(e.clean.use)[m0 / 32] = 0;
         return true;
     }
     // logits of 32 columns
@@ -753,6 +756,13 @@ __device__ __forceinline__ bool rows_epilogue(const KernelArgs& a, const RowsEpi
         own.next ^= 1;
         if (e.sums != nullptr) own.columns[t * 32 + lane] += sum_lanes(v, lane);
     }
+    if (grads && share == 0) {
+        const bool bad = row < m && !live && !(sum > 0.0f && sum < INFINITY);
+        const bool any = __any_sync(~0u, bad);
+        if (lane == 0) reinterpret_cast<uint8_t*>(e.clean.use)[m0 / 32] = any;
+        // (two warps may copy a step, and then write the same)
+        if (any) clean_step(e.clean, m0 / kStepRows, m, e.target, lane, 32);
+    }
     if (row >= m) return true;
     if (live && (target & 96) == first) {
         const float loss = logit == -INFINITY ? INFINITY : (top - logit) + logf(sum);
@@ -832,8 +842,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<EPI>, 1)
         for (int job = 0; job < jobs && ok; ++job) {
             const Tiling tiling(a.job[job]);
             const bool a_mn = a.job[job].a_mn, b_mn = a.job[job].b_mn;
+            const uint16_t* use_other = EPI == kStore ? a.job[job].use_other : nullptr;
             for (int i = 0, unit; ok && (unit = walk.unit(job, i)) >= 0; ++i) {
                 const Tile t(tiling, unit, BN);
+                uint32_t other = 0;  // the next 32 steps that b_other has
                 const int am = t.m0 + (int)rank * kRowsCta;
                 int bn = t.n0 + (int)rank * (BN / 2), kb = t.kb0;
                 const int steps = (t.kb1 - t.kb0) * (EPI == kRows ? a.job[0].across : 1);
@@ -841,6 +853,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<EPI>, 1)
                     if (EPI == kRows && kb == t.kb1) {
                         kb = t.kb0;
                         bn += BN;
+                    }
+                    const CUtensorMap* tb = &a.tb[job];
+                    if (use_other != nullptr) {
+                        if (step % 32 == 0)
+                            other = __ballot_sync(~0u, kb + lane < t.kb1 && use_other[kb + lane] != 0);
+                        if (other >> step % 32 & 1) tb = &a.tb_other;
                     }
                     const uint32_t wait = smem_u32(&empty[s]);
                     if (!mbar_wait_warp(wait, (round & 1) ^ 1, a.err, kErrWaitProducer)) {
@@ -859,10 +877,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<EPI>, 1)
                             tma_load_2d_pair(da, &a.ta[job], bar, k0, am);
                         }
                         if (b_mn) {
-                            tma_load_2d_pair(db, &a.tb[job], bar, bn, k0);
-                            if (BN == 256) tma_load_2d_pair(db + 8192, &a.tb[job], bar, bn + 64, k0);
+                            tma_load_2d_pair(db, tb, bar, bn, k0);
+                            if (BN == 256) tma_load_2d_pair(db + 8192, tb, bar, bn + 64, k0);
                         } else {
-                            tma_load_2d_pair(db, &a.tb[job], bar, k0, bn);
+                            tma_load_2d_pair(db, tb, bar, k0, bn);
                         }
                     }
                     ++used;
@@ -1222,6 +1240,13 @@ void encode_operands(KernelArgs& a, int i, int dtype, const Job& g, int bn) {
     encode_operand(&a.tb[i], dtype, g.b, g.n, g.k, bn / 2);
 }
 
+void encode_other(KernelArgs& a, int i, int dtype, const GemmJob& g, int bn) {
+    need(i == 0 || a.job[0].use_other == nullptr, "one product of a launch reads steps from elsewhere");
+    need(g.b_other.mn == g.b.mn, "both copies of an operand lie the same way");
+    a.job[i].use_other = g.use_other;
+    encode_operand(&a.tb_other, dtype, g.b_other, g.n, g.k, bn / 2);
+}
+
 // Narrow tiles where wide ones would leave pairs idle or mostly compute
 // padding; a narrow tile costs more than half a wide one, since it reads A
 // as often.
@@ -1276,7 +1301,7 @@ StagedOperand stage_operand(Workspace& w, Packs& packs, const GemmOperand& op, i
 
 void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, Post& post, Queue& q) {
     if (count == 1 && jobs->m <= kSkinnyRows && !jobs->a.mn && !jobs->b.mn && jobs->e.out32 == nullptr &&
-        jobs->e.acc32 == nullptr && jobs->e.count.parts == nullptr) {
+        jobs->e.acc32 == nullptr && jobs->e.count.parts == nullptr && jobs->use_other == nullptr) {
         if (go) skinny(dtype, *jobs, q);
         return;
     }
@@ -1317,6 +1342,7 @@ void gemm(Workspace& w, bool go, int dtype, GemmJob* jobs, int count, Post& post
     w.require();
     for (int i = 0; i < count; ++i) {
         encode_operands(a, i, dtype, jobs[i], bn);
+        if (jobs[i].use_other != nullptr) encode_other(a, i, dtype, jobs[i], bn);
         const JobArgs& j = a.job[i];
         const GemmEpilogue& e = j.e;
         if (e.out32 != nullptr)

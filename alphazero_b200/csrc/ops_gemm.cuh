@@ -56,11 +56,46 @@ __device__ __forceinline__ float scaled_alpha(float alpha, const Count& count, i
     return count.parts != nullptr ? alpha / (float)max(count_total(count, lane), 1) : alpha;
 }
 
+// Steps of 64 elements of the contraction, in which a product may take an
+// operand from somewhere else.
+constexpr int kStepRows = 64;
+
 struct GemmJob {
     StagedOperand a, b;
     int64_t m = 0, n = 0, k = 0;
     GemmEpilogue e;
+    // If set, per step of k: whether it is to be read from b_other, a matrix
+    // like b, instead.
+    const uint16_t* use_other = nullptr;
+    StagedOperand b_other;
 };
+
+// Rows of x that are not counted have d = 0, which leaves them out of
+// dw = d^T x unless they hold an infinity or NaN.  The kernel that knows
+// the rows' softmax sees such a row by its logits (one that is not finite
+// makes every logit an infinity or NaN, so the row's sum of exponentials is
+// NaN or zero) and copies its step of rows with zeros in place of the rows
+// that are not counted; dw's product reads that step from the copy.
+struct CleanRows {
+    const uint16_t* x = nullptr;
+    int64_t row = 0, col = 0;
+    uint16_t* clean = nullptr;
+    int64_t clean_row = 0, clean_col = 0;
+    uint16_t* use = nullptr;  // [steps], or as bytes per 32 rows: not zero where the copy is to be read
+    int64_t dim = 0;
+};
+
+// One step's copy, by `count` threads.
+__device__ __forceinline__ void clean_step(const CleanRows& c, int step, int rows, const Indices& target, int thread,
+                                           int count) {
+    const bool along = c.col == 1;  // rows of x
+#pragma unroll 1
+    for (int64_t e = thread; e < kStepRows * c.dim; e += count) {
+        const int64_t i = (int64_t)step * kStepRows + (along ? e / c.dim : e % kStepRows);
+        const int64_t j = along ? e % c.dim : e / kStepRows;
+        if (i < rows) c.clean[i * c.clean_row + j * c.clean_col] = target.at(i) >= 0 ? c.x[i * c.row + j * c.col] : 0;
+    }
+}
 
 // Products of up to this many rows, both operands K-major, are bound by
 // reading B once: they take a kernel of their own (ops_skinny.cu).
@@ -115,6 +150,7 @@ struct RowsEpilogue {
     uint16_t* d = nullptr;         // [m][n], row stride ld; null: no gradient
     int64_t ld = 0;                // a multiple of 8
     float* sums = nullptr;         // [ctas][n], or null
+    CleanRows clean;               // with d
 };
 struct RowsJob {
     StagedOperand a, b;
