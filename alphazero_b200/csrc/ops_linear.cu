@@ -8,9 +8,9 @@ namespace mgb {
 namespace ops {
 namespace {
 
+// act'(z) of the smooth ones.
 __device__ __forceinline__ float slope(float z, int act) {
     switch (act) {
-        case MG_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
         case MG_ACT_SILU: {
             const float p = logistic(z);
             return p * (1.0f + z * (1.0f - p));
@@ -22,6 +22,12 @@ __device__ __forceinline__ float slope(float z, int act) {
         }
         default: return 1.0f;
     }
+}
+
+// A ReLU that is shut lets nothing through, an infinity or NaN neither.
+__device__ __forceinline__ float times_slope(float v, float z, int act) {
+    if (act == MG_ACT_RELU) return z > 0.0f ? v : 0.0f;
+    return v * slope(z, act);
 }
 
 // g = grad * act'(z) (if g is set) and, per block of rows, the column sums of
@@ -62,7 +68,7 @@ __global__ void __launch_bounds__(256)
             for (int i = 0; i < V; ++i) {
                 float v = E::get(dv[i]);
                 if (g) {
-                    v *= slope(E::get(zv[i]), a.activation);
+                    v = times_slope(v, E::get(zv[i]), a.activation);
                     dv[i] = E::put(v);
                 }
                 sum[i] += v;

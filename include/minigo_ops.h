@@ -116,8 +116,8 @@ int mg_linear(const mg_linear_args* args, void* workspace, size_t workspace_byte
  * g = grad * act'(z), rounded to the operands' type (unless there is no
  * activation); dx = g weight [m][k], dw = g^T x [n][k], db = sum of g over
  * rows [n] or NULL.  dx and dw may be NULL to leave them out.  act' of RELU
- * is 0 at z = 0.  The residual's gradient is residual_scale * grad and
- * needs no kernel. */
+ * is 0 at z = 0, and where it is 0 so is g, whatever grad holds.  The
+ * residual's gradient is residual_scale * grad and needs no kernel. */
 typedef struct mg_linear_backward_args {
     const void* grad;
     const void* x;

@@ -79,3 +79,52 @@ def test_counted_rows_keep_their_nan():
         assert torch.isnan(loss) and torch.isnan(rows[7]) and torch.isnan(dx[7]).all()
         assert torch.isnan(dw).all() and torch.isnan(db).all()  # d of row 7 is NaN in every class
         assert not dx[out].any() and not rows[out].any()
+
+
+# ---- gradients of the linear layer and of the embedding ----
+
+@pytest.mark.parametrize("n", [40, 37])  # by eight columns, one by one
+@pytest.mark.parametrize("value", [INF, -INF, math.nan])
+def test_a_shut_relu_lets_nothing_through(n, value):
+    m, k = 70, 24
+    g, x, w, z = make(m, n), make(m, k, seed=1), make(n, k, seed=2), make(m, n, seed=3)
+    z[5, 3], z[6, 4], z[7, 9] = -1.0, 0.0, -INF
+    want = ops.linear_backward(g, x, w, z, "relu")
+    bad = g.clone()
+    for i, j in ((5, 3), (6, 4), (7, 9)):
+        bad[i, j] = value
+    for a, b in zip(ops.linear_backward(bad, x, w, z, "relu"), want):
+        assert torch.equal(a, b) and torch.isfinite(a).all()
+
+
+@pytest.mark.parametrize("name", ["none", "relu", "silu", "gelu"])
+def test_linear_backward_keeps_odd_values_to_their_places(name):
+    m, n, k = 70, 40, 24
+    g, x, w, z = make(m, n), make(m, k, seed=1), make(n, k, seed=2), make(m, n, seed=3).abs()
+    good = ops.linear_backward(g, x, w, z, name)
+    bad = g.clone()
+    bad[9, 11] = math.nan
+    dx, dw, db = ops.linear_backward(bad, x, w, z, name)
+    rows, cols = torch.arange(m, device="cuda") != 9, torch.arange(n, device="cuda") != 11
+    assert torch.equal(dx[rows], good[0][rows]) and torch.isnan(dx[9]).all()
+    assert torch.equal(dw[cols], good[1][cols]) and torch.isnan(dw[11]).all()
+    assert torch.equal(db[cols], good[2][cols]) and torch.isnan(db[11])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("n", [50, 5000])
+def test_embed_backward_keeps_odd_values_to_their_entries(dtype, n):
+    vocab, dim = 82, 40
+    t = integers(n, 0, vocab - 2)
+    t[::7], t[1::7] = -1, vocab
+    g = make(n, dim, dtype=dtype)
+    good = ops.embed_backward(g, t, vocab)
+    bad = g.clone()
+    bad[::7], bad[1::7] = math.nan, INF  # padding
+    assert torch.equal(ops.embed_backward(bad, t, vocab), good)
+    bad[2, 3], bad[3, 4] = math.nan, -INF
+    d = ops.embed_backward(bad, t, vocab)
+    hit = torch.zeros(vocab, dim, dtype=torch.bool, device="cuda")
+    hit[t[2], 3] = hit[t[3], 4] = True
+    assert torch.isnan(d[t[2], 3]) and not torch.isfinite(d[t[3], 4])
+    assert torch.equal(d[~hit], good[~hit])
