@@ -360,7 +360,8 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
     const int down_rows = (int)std::max<int64_t>(128 / wide, (piece + want - 1) / want);
     const int ctas = gemm_rows_ctas(piece);
     const int64_t down = rows_whole ? ctas : (piece + down_rows - 1) / down_rows;  // of a whole piece
-    float* sums = a.db ? w.take<float>((size_t)down * count_pieces * a.vocab * 4) : nullptr;
+    float* sums = a.db ? w.take<float>((size_t)down * a.vocab * 4) : nullptr;
+    float* db32 = a.db && count_pieces > 1 ? w.take<float>((size_t)a.vocab * 4) : nullptr;  // of earlier pieces
     const int64_t ld32 = (a.dim + 7) / 8 * 8;
     float* dw32 = grads && count_pieces > 1 ? w.take<float>((size_t)((a.vocab + 255) / 256 * 256) * ld32 * 4) : nullptr;
 
@@ -379,7 +380,7 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
         if (apart) q.launch("count_kernel", count_kernel, dim3((unsigned)counts_n), 1024, 0, target, a.n, counts);
     }
     const float alpha = a.grad_scale / kDScale<DT>;
-    int64_t sum_rows = 0, losses = 0;
+    int64_t losses = 0;
     size_t piece_scratch = 0;
     Post post;
     for (int64_t row0 = 0; row0 < a.n; row0 += piece) {
@@ -402,7 +403,7 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
             f.e.counts = apart ? nullptr : counts;
             f.e.d = probs;
             f.e.ld = ld;
-            f.e.sums = sums ? sums + sum_rows * a.vocab : nullptr;
+            f.e.sums = sums;
             f.e.clean = clean;
             gemm_rows(DT, f, q);
             losses += gemm_rows_ctas(rows);
@@ -440,9 +441,8 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
         if (go && !rows_whole) {
             q.launch("d_kernel", d_kernel<DT>, dim3((unsigned)across, (unsigned)these), 256, 0, (int)rows, a.vocab, block,
                      probs, ld, part, piece, lse, target.from(row0), wide, down_rows,
-                     sums ? sums + sum_rows * a.vocab : nullptr, first ? counts : nullptr, (int64_t)counts_n, total, clean);
+                     sums, first ? counts : nullptr, (int64_t)counts_n, total, clean);
         }
-        sum_rows += these;
         StagedOperand d;
         d.data = probs;
         d.ld = ld;
@@ -475,6 +475,9 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
         Workspace again = w;  // every piece's scratch is the same
         gemm(again, go, DT, jobs, 2, post, q);
         if (go) {
+            if (sums)
+                post.add = AddRowsTask{sums,  these, a.vocab, alpha * kDScale<DT>, count, a.db, first ? nullptr : db32,
+                                       last ? nullptr : db32};
             if (!last) post.launch(DT, q);
             continue;
         }
@@ -484,7 +487,6 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
         w.take(piece_scratch);
         return;
     }
-    if (a.db) post.add = AddRowsTask{sums, sum_rows, a.vocab, alpha * kDScale<DT>, count, a.db};
     post.loss = LossTask{loss_part, losses, counts, counts_n, a.loss};
     post.launch(DT, q);
 }

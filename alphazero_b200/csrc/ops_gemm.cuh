@@ -249,12 +249,16 @@ struct FinishTask {
     GemmEpilogue e;
     int64_t blocks;
 };
-struct AddRowsTask {  // out[c] = alpha / max(count, 1) * sum of `rows` rows of sums, in a fixed order
+// s[c] = acc[c] (if set) + the sum of `rows` rows of sums, in a fixed order:
+// out[c] = alpha / max(count, 1) * s[c], or instead acc_out[c] = s[c].
+struct AddRowsTask {
     const float* sums;
     int64_t rows, cols;
     float alpha;
     Count count;
     void* out;
+    const float* acc;
+    float* acc_out;
 };
 struct LossTask {  // loss = sum of part[0 .. n) / max(sum of counts[0 .. counts_n), 1)
     const float* part;
@@ -266,7 +270,7 @@ struct LossTask {  // loss = sum of part[0 .. n) / max(sum of counts[0 .. counts
 struct Post {
     FinishTask finish[2];
     int finishes = 0;
-    AddRowsTask add{};   // out set: to do
+    AddRowsTask add{};   // sums set: to do
     LossTask loss{};     // loss set: to do
     void launch(int dtype, Queue& q);  // if there is anything, which is then done
 };

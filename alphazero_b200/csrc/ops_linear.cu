@@ -218,7 +218,7 @@ void linear_backward(const mg_linear_backward_args& a, Workspace& w, bool go, Qu
                                     : (bf ? slope_kernel<MG_PREC_BF16, 1> : slope_kernel<MG_PREC_FP16, 1>);
             q.launch("slope_kernel", kernel, dim3((unsigned)blocks), 256, 0, a, g, ldg, rows, sums, across, down,
                      packs);
-            if (a.db) post.add = AddRowsTask{sums, down, a.n, 1.0f, Count{}, a.db};
+            if (a.db) post.add = AddRowsTask{sums, down, a.n, 1.0f, Count{}, a.db, nullptr, nullptr};
         }
     } else if (go) {
         w.require();

@@ -90,7 +90,9 @@ __device__ __forceinline__ void add_rows_block(const AddRowsTask& t, int64_t blo
             for (int i = 0; i < slices; ++i) s += shared[i * columns + lane];
     }
     if (slice > 0 || c >= t.cols) return;
-    static_cast<typename Elem<DT>::T*>(t.out)[c] = Elem<DT>::put(s * alpha);
+    if (t.acc != nullptr) s += t.acc[c];
+    if (t.acc_out != nullptr) t.acc_out[c] = s;
+    else static_cast<typename Elem<DT>::T*>(t.out)[c] = Elem<DT>::put(s * alpha);
 }
 
 __device__ __forceinline__ void loss_block(const LossTask& t, float2* shared) {
@@ -128,7 +130,7 @@ __global__ void __launch_bounds__(kPostThreads) post_kernel(Post p) {
         if (block == 0) return loss_block(p.loss, reinterpret_cast<float2*>(shared));
         --block;
     }
-    if (p.add.out != nullptr) add_rows_block<DT>(p.add, block, reinterpret_cast<float*>(shared));
+    if (p.add.sums != nullptr) add_rows_block<DT>(p.add, block, reinterpret_cast<float*>(shared));
 }
 
 }  // namespace
@@ -146,7 +148,7 @@ void Post::launch(int dtype, Queue& q) {
         blocks += t.blocks;
     }
     if (loss.loss != nullptr) ++blocks;
-    if (add.out != nullptr) {
+    if (add.sums != nullptr) {
         const int columns = kPostThreads / add_rows_slices(add.rows);
         blocks += (add.cols + columns - 1) / columns;
     }

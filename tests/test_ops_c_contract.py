@@ -1,5 +1,7 @@
 """What the C entries of the training operators check and report besides
 shapes, types and null pointers.  Nothing here reaches a GPU."""
+import ctypes
+
 import pytest
 
 from alphazero_b200 import build, ops
@@ -29,3 +31,17 @@ def test_pointers_inside_an_element_are_refused(L, name, args, words):
     for field, word in wide.items():
         if field in words:  # 2 bytes past an element of 4 or 8
             refused(L, name, args(**{field: 258}), word + " is not aligned")
+
+
+@pytest.mark.parametrize("vocab", [510, 131072, 1000003])
+@pytest.mark.parametrize("bias", [False, True])
+def test_gradient_scratch_does_not_grow_with_the_rows(L, vocab, bias):
+    """Rows are taken in pieces; what is kept between pieces has the size of
+    a gradient, and of a loss per 128 rows."""
+    need, sizes = ctypes.c_size_t(), []
+    rows = (1 << 16, 1 << 20) if vocab > 510 else (3 << 20, 24 << 20)
+    for n in rows:
+        a = entropy_args(n=n, vocab=vocab, dx=256, dw=256, b=256 * bias, db=256 * bias)
+        assert L.mg_cross_entropy_workspace(a, ctypes.byref(need)) == 0
+        sizes.append(need.value)
+    assert sizes[1] - sizes[0] < 64 << 20 and sizes[1] < 2 << 30
