@@ -22,8 +22,8 @@ namespace mgb {
 namespace ops {
 namespace {
 
-// Of a piece of the rows' probabilities at a time.  Each further piece costs
-// the fp32 sums of dw a trip through memory.
+// Of a piece of the rows' probabilities, or without gradients of its statistics,
+// at a time.  Each further piece costs the fp32 sums of dw a trip through memory.
 constexpr size_t kPieceBytes = size_t(1) << 30;
 
 // The number of counted rows, per block: only where there are several pieces
@@ -310,9 +310,10 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
         return;
     }
     const int64_t ld = (a.vocab + 7) / 8 * 8;
-    // pieces of equal length, whole tiles
-    const int64_t most = std::max<int64_t>(256, (int64_t)(kPieceBytes / 2) / ld / 256 * 256);
-    const int64_t count_pieces = grads ? (a.n + most - 1) / most : 1;
+    // pieces of equal length, whole tiles; a block of columns has at least 64 (few rows are one piece)
+    const int64_t per = grads ? 2 * ld : 8 * ((a.vocab + 63) / 64);
+    const int64_t most = std::max<int64_t>(256, (int64_t)kPieceBytes / per / 256 * 256);
+    const int64_t count_pieces = (a.n + most - 1) / most;
     const int64_t piece = std::min(a.n, ((a.n + count_pieces - 1) / count_pieces + 255) / 256 * 256);
     Packs packs;
     StagedOperand x = stage_operand(w, packs, {a.x, a.x_row, a.x_col}, a.n, a.dim);

@@ -45,3 +45,15 @@ def test_gradient_scratch_does_not_grow_with_the_rows(L, vocab, bias):
         assert L.mg_cross_entropy_workspace(a, ctypes.byref(need)) == 0
         sizes.append(need.value)
     assert sizes[1] - sizes[0] < 64 << 20 and sizes[1] < 2 << 30
+
+
+@pytest.mark.parametrize("vocab", [82, 510, 700, 65536, 1000003])
+def test_scoring_scratch_does_not_grow_with_the_rows(L, vocab):
+    """Without gradients too: statistics per row and block of columns are kept for
+    a piece of the rows."""
+    need, sizes = ctypes.c_size_t(), []
+    rows = (1 << 18, 1 << 22) if vocab > 700 else (1 << 27, 1 << 29)
+    for n in rows:
+        assert L.mg_cross_entropy_workspace(entropy_args(n=n, vocab=vocab), ctypes.byref(need)) == 0
+        sizes.append(need.value)
+    assert sizes[1] - sizes[0] < 64 << 20 and sizes[1] < 2 << 30
