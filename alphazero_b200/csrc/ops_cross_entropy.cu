@@ -63,10 +63,11 @@ __device__ __forceinline__ void join_lanes(float& m, float& s) {
     m = top;
 }
 
-// A row's loss, given that it is counted.
+// A row's loss, given that it is counted: log(s exp(m)) - at, the difference of
+// large numbers first, so that what is left of it when the target is the
+// maximum, log(s), keeps its bits.
 __device__ __forceinline__ float loss_of(float m, float s, float at) {
-    const float lse = s == 0.0f ? -INFINITY : m + logf(s);
-    return at == -INFINITY ? INFINITY : lse - at;
+    return at == -INFINITY ? INFINITY : (m - at) + logf(s);
 }
 
 // A few rows without gradients: their losses and the mean in one launch, by a
@@ -119,17 +120,17 @@ __global__ void __cluster_dims__(kFewRows / 2, 1, 1) __launch_bounds__(1024)
 
 // Bound by latency: 5 us for 13 rows of 4096 blocks of columns, 13 for 4096
 // rows of 513.
-// logsumexp and loss per row, and the loss summed per block: a thread per row
-// where a row has few blocks of columns; with many, 32 threads per row, or
-// where there are few rows too, a block per row.
-// A row of -inf has lse -inf.  counts, if set: the counted rows per block.
+// Maximum m and log2 of the sum s of exp(l - m) and the loss per row, and the
+// loss summed per block: a thread per row where a row has few blocks of
+// columns; with many, 32 threads per row, or where there are few rows too, a
+// block per row.  A row of -inf has log2 s = -inf.  counts, if set: the counted rows per block.
 enum Combine : int { kThreadPerRow, kWarpPerRow, kBlockPerRow };
 constexpr int kFewBlocks = 16;
 
 template <Combine HOW>
 __global__ void __launch_bounds__(HOW == kThreadPerRow ? 128 : 1024)
     combine_kernel(int64_t rows, int blocks, const float2* part, int64_t part_ld, Indices target,
-                   const float* logit, float* lse, float* row_loss, float* loss_part, int* counts) {
+                   const float* logit, float2* stat, float* row_loss, float* loss_part, int* counts) {
     constexpr bool FEW = HOW == kThreadPerRow;
     __shared__ float2 tile[FEW ? 1 : 32][33];
     __shared__ float losses[FEW ? 128 : 32];
@@ -167,11 +168,10 @@ __global__ void __launch_bounds__(HOW == kThreadPerRow ? 128 : 1024)
     float loss = 0.0f;
     bool counted = false;
     if (row < rows) {
-        const float l = s == 0.0f ? -INFINITY : m + logf(s);
         counted = target.at(row) >= 0;
         if (counted) loss = loss_of(m, s, logit[row]);
         if (FEW || lane == 0) {  // (a block per row: every warp has the row, and writes the same)
-            lse[row] = l;
+            stat[row] = make_float2(m, log2f(s));
             row_loss[row] = loss;
         }
     }
@@ -200,14 +200,16 @@ __global__ void __launch_bounds__(HOW == kThreadPerRow ? 128 : 1024)
 // has 8 adjacent columns; `wide` of the block's eight warps lie side by side
 // (up to 4 KB of a row at once; with one, 512 bytes, the same work took a
 // half longer), the others take further rows.  The factor from the
-// block's maximum to the row's logsumexp is one exp per thread and row.
+// block's maximum to the row's softmax, exp(m_block - m) / s, is one exp per
+// thread and row; near the row's maximum it is exact to the last bits, which
+// the difference to one where a target has nearly everything needs.
 // Bound by memory: 4096 x 65544 take 213 us, 5 TB/s read and written.
 // Block 0 also adds up counts, if set, to count; each step of rows has a block
 // that looks for rows whose x would reach dw through d = 0 (CleanRows).
 template <int DT>
 __global__ void __launch_bounds__(256)
     d_kernel(int rows, int64_t vocab, int block, uint16_t* probs, int64_t ld, const float2* part, int64_t part_ld,
-             const float* lse, Indices target, int wide, int rows_per_block, float* sums, const int* counts,
+             const float2* stat, Indices target, int wide, int rows_per_block, float* sums, const int* counts,
              int64_t counts_n, int* count, CleanRows clean) {
     using E = Elem<DT>;
     using T = typename E::T;
@@ -228,7 +230,7 @@ __global__ void __launch_bounds__(256)
     const int steps = (rows + kStepRows - 1) / kStepRows, step0 = blockIdx.y * gridDim.x + blockIdx.x;
     const auto is_bad = [&](int g) {
         const int row = g * kStepRows + threadIdx.x;
-        return threadIdx.x < kStepRows && row < rows && !isfinite(lse[row]) && target.at(row) < 0;
+        return threadIdx.x < kStepRows && row < rows && !isfinite(stat[row].y) && target.at(row) < 0;
     };
     const bool bad = step0 < steps && is_bad(step0);  // its loads are ahead of the others
     if (c < vocab) {
@@ -242,14 +244,15 @@ __global__ void __launch_bounds__(256)
         for (int r = r0 + down; r < r1; r += deep * kRows, p += kRows * step) {
             uint4 u[kRows];
             int t[kRows];
-            float f[kRows], m[kRows];
+            float2 f[kRows];
+            float m[kRows];
 #pragma unroll
             for (int q = 0; q < kRows; ++q) {
                 const int row = r + deep * q;
                 if (row >= r1) continue;
                 u[q] = *reinterpret_cast<const uint4*>(p + q * step);
                 t[q] = target.at(row);
-                f[q] = lse[row];
+                f[q] = stat[row];
                 m[q] = mine[row].x;
             }
 #pragma unroll
@@ -257,8 +260,8 @@ __global__ void __launch_bounds__(256)
                 if (r + deep * q >= r1) break;
                 const uint32_t w[4] = {u[q].x, u[q].y, u[q].z, u[q].w};
                 // a row that is not counted (whatever it holds) and one of -inf have no probabilities
-                float scale = exp2_flush((m[q] - f[q]) * 1.4426950408889634f) * 0x1p112f;  // prob16_value's
-                if (f[q] == -INFINITY || t[q] < 0) scale = 0.0f;
+                float scale = exp2_flush((m[q] - f[q].x) * 1.4426950408889634f - f[q].y) * 0x1p112f;  // prob16_value's
+                if (f[q].y == -INFINITY || t[q] < 0) scale = 0.0f;
                 float v[8];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -336,7 +339,7 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
     target.limit = a.vocab;
     const size_t per_row = rows_whole ? 0 : (size_t)piece * 4;
     float* logit = w.take<float>(per_row);
-    float* lse = w.take<float>(per_row);
+    float2* stat = w.take<float2>(2 * per_row);
     float2* part = w.take<float2>(blocks * 2 * per_row);
     uint16_t* probs = grads ? w.take<uint16_t>((size_t)piece * ld * 2) : nullptr;
     // a copy of x as x lies, of which few steps are ever written
@@ -433,7 +436,7 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
                                 : how == kBlockPerRow ? combine_kernel<kBlockPerRow>
                                                       : combine_kernel<kWarpPerRow>;
             q.launch("combine_kernel", kernel, dim3((unsigned)combine_blocks), how == kThreadPerRow ? 128 : 1024, 0, rows,
-                     blocks, part, piece, target.from(row0), logit, lse, a.row_loss + row0, loss_part + losses,
+                     blocks, part, piece, target.from(row0), logit, stat, a.row_loss + row0, loss_part + losses,
                      apart ? nullptr : counts);
             losses += combine_blocks;
         }
@@ -441,7 +444,7 @@ void run(const mg_cross_entropy_args& a, Workspace& w, bool go, Queue& q) {
         const int64_t these = rows_whole ? gemm_rows_ctas(rows) : (rows + down_rows - 1) / down_rows;
         if (go && !rows_whole) {
             q.launch("d_kernel", d_kernel<DT>, dim3((unsigned)across, (unsigned)these), 256, 0, (int)rows, a.vocab, block,
-                     probs, ld, part, piece, lse, target.from(row0), wide, down_rows,
+                     probs, ld, part, piece, stat, target.from(row0), wide, down_rows,
                      sums, first ? counts : nullptr, (int64_t)counts_n, total, clean);
         }
         StagedOperand d;
