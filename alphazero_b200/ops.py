@@ -330,6 +330,13 @@ def linear_cross_entropy_grad(x, weight, targets, bias=None, grad_scale: float =
 
 # ---- autograd ----
 
+def _recorded(*inputs) -> bool:
+    """Whether a gradient can be asked for.  (Inside a Function's forward
+    this is not to be known: gradients are off there in any case, and
+    needs_input_grad tells what inputs require, under no_grad as well.)"""
+    return torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in inputs)
+
+
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, table, scale):
@@ -367,8 +374,6 @@ class _Linear(torch.autograd.Function):
 class _CrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, targets, grad_scale):
-        if not any(ctx.needs_input_grad):
-            return linear_cross_entropy(x, weight, targets, bias)[0]
         loss, _, dx, dw, db = linear_cross_entropy_grad(x, weight, targets, bias, grad_scale)
         ctx.save_for_backward(dx, dw, db)
         ctx.grad_scale = grad_scale
@@ -384,17 +389,24 @@ class _CrossEntropy(torch.autograd.Function):
 
 def embedding(tokens, table, scale: float = 1.0):
     """``embed`` for autograd."""
+    if not _recorded(table):
+        return embed(tokens, table, float(scale))
     return _Embedding.apply(tokens, table, float(scale))
 
 
 def linear_layer(x, weight, bias=None, residual=None, activation: str = "none",
                  residual_scale: float = 1.0):
     """``linear`` for autograd."""
+    if not _recorded(x, weight, bias, residual):
+        return linear(x, weight, bias, residual, activation, float(residual_scale))
     return _Linear.apply(x, weight, bias, residual, activation, float(residual_scale))
 
 
 def cross_entropy_loss(x, weight, targets, bias=None, grad_scale: float = 1.0):
     """The loss of ``linear_cross_entropy`` for autograd.  The gradients are
     made with the loss, of grad_scale * loss, and multiplied by the incoming
-    gradient / grad_scale when the backward pass reaches them."""
+    gradient / grad_scale when the backward pass reaches them; where none can
+    be asked for, only the loss is."""
+    if not _recorded(x, weight, bias):
+        return linear_cross_entropy(x, weight, targets, bias)[0]
     return _CrossEntropy.apply(x, weight, bias, targets, float(grad_scale))
