@@ -163,6 +163,7 @@ void linear(const mg_linear_args& a, Workspace& w, bool go, Queue& q) {
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 void linear_backward(const mg_linear_backward_args& a, Workspace& w, bool go, Queue& q) {
+    if (!a.dx && !a.dw && !a.db) return;
     if (a.m == 0) {
         if (!go) return;
         if (a.dw) q.clear(a.dw, (size_t)a.n * a.k * 2);

@@ -250,9 +250,11 @@ def linear(x, weight, bias=None, residual=None, activation: str = "none",
     return (y, z) if keep_preactivation else y
 
 
-def linear_backward(grad, x, weight, preactivation=None, activation: str = "none", bias: bool = True):
+def linear_backward(grad, x, weight, preactivation=None, activation: str = "none", bias: bool = True,
+                    input_grad: bool = True, weight_grad: bool = True):
     """Gradients (dx, dw, db) of ``linear`` from grad = dL/dy [..., n] and
-    the z that it kept (needed unless activation is "none"); db is None with
+    the z that it kept (needed unless activation is "none"); dx is None, and
+    not computed, with input_grad=False, dw with weight_grad=False, db with
     bias=False.  The residual's gradient is residual_scale * grad."""
     d = _on_gpu(grad, "grad")
     dt = _dtype(grad, "grad", False)
@@ -273,12 +275,12 @@ def linear_backward(grad, x, weight, preactivation=None, activation: str = "none
                              f"{tuple(preactivation.shape)}")
         z = _matrix(preactivation, "preactivation")
         z_row, z_col = z.stride()
-    dx = x.new_empty(x.shape)
-    dw = x.new_empty((n, k))
+    dx = x.new_empty(x.shape) if input_grad else None
+    dw = x.new_empty((n, k)) if weight_grad else None
     db = x.new_empty((n,)) if bias else None
     _call("mg_linear_backward",
           _LINEAR_BACKWARD.pack(g.data_ptr(), x2.data_ptr(), weight.data_ptr(), _ptr(z),
-                                dx.data_ptr(), dw.data_ptr(), _ptr(db), g.shape[0], n, k,
+                                _ptr(dx), _ptr(dw), _ptr(db), g.shape[0], n, k,
                                 *g.stride(), *x2.stride(), *weight.stride(), z_row, z_col, act, dt,
                                 d, 0), x, d)
     return dx, dw, db
@@ -354,20 +356,22 @@ class _Embedding(torch.autograd.Function):
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, residual_scale):
-        keep = activation != "none"
+        keep = activation != "none" and any(ctx.needs_input_grad[:3])
         out = linear(x, weight, bias, residual, activation, residual_scale, keep)
         y, z = out if keep else (out, None)
         ctx.save_for_backward(x, weight, z)
         ctx.activation, ctx.residual_scale = activation, residual_scale
-        ctx.has_bias, ctx.has_residual = bias is not None, residual is not None
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         x, weight, z = ctx.saved_tensors
-        dx, dw, db = linear_backward(grad, x, weight, z, ctx.activation, ctx.has_bias)
-        dr = grad * ctx.residual_scale if ctx.has_residual else None
+        x_grad, w_grad, b_grad, r_grad = ctx.needs_input_grad[:4]
+        dx = dw = db = None
+        if x_grad or w_grad or b_grad:
+            dx, dw, db = linear_backward(grad, x, weight, z, ctx.activation, b_grad, x_grad, w_grad)
+        dr = grad * ctx.residual_scale if r_grad else None
         return dx, dw, db, dr, None, None
 
 
@@ -383,7 +387,8 @@ class _CrossEntropy(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         factor = grad / ctx.grad_scale
-        dx, dw, db = (None if t is None else (t * factor).to(t.dtype) for t in ctx.saved_tensors)
+        dx, dw, db = ((t * factor).to(t.dtype) if wanted else None
+                      for t, wanted in zip(ctx.saved_tensors, ctx.needs_input_grad))
         return dx, dw, db, None, None
 
 

@@ -3,8 +3,9 @@ gradients where none are recorded, and only the gradients that are wanted."""
 import pytest
 import torch
 
+import ops_reference as ref
 from alphazero_b200 import ops
-from test_gpu_ops import integers, make
+from test_gpu_ops import integers, laid, make
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +65,39 @@ def test_wrong_arguments_are_refused_by_the_autograd_forms_too():
             ops.embedding(torch.zeros(3, device="cuda"), w)
         with pytest.raises(ValueError):
             ops.cross_entropy_loss(x, w, integers(3, 0, 6))
+
+
+@pytest.mark.parametrize("name", ["none", "relu", "gelu"])
+@pytest.mark.parametrize("how", ["plain", "transposed", "offset"])
+@pytest.mark.parametrize("m,n,k", [(1, 16, 8), (3, 362, 722), (9, 128, 2050), (16, 96, 4096), (129, 257, 65),
+                                   (300, 128, 1024), (4099, 40, 24)])
+def test_one_gradient_at_a_time(name, how, m, n, k):
+    g, x = make(m, n, seed=4), make(m, k)
+    w, z = laid(make(n, k, seed=1, scale=k ** -0.5), how), make(m, n, seed=5)
+    want = ref.linear_backward(g, x, w, z, name)
+    for wanted in [(True, False, False), (False, True, False), (False, False, True), (True, False, True),
+                   (False, True, True), (False, False, False)]:
+        got = ops.linear_backward(g, x, w, z, name, bias=wanted[2], input_grad=wanted[0], weight_grad=wanted[1])
+        for a, (b, off), asked in zip(got, want, wanted):
+            assert (a is not None) == asked
+            if asked:
+                ref.within(a, b, off)
+
+
+def test_frozen_inputs_cost_nothing():
+    m, n, k = 64, 8192, 4096  # a gradient of w takes 64 MB, everything else under 2
+    for frozen in ("w", "x", "wx", "wxb"):
+        x, w = make(m, k), make(n, k, seed=1, scale=0.02)
+        b, r = make(n, seed=2), make(m, n, seed=3)
+        for letter, t in (("x", x), ("w", w), ("b", b), ("r", r)):
+            t.requires_grad_(letter not in frozen)
+        y = ops.linear_layer(x, w, b, r, "gelu", 0.5)
+        g = make(m, n, seed=4)
+        inputs = [t for t in (x, w, b, r) if t.requires_grad]
+        got, most = peak(lambda: torch.autograd.grad(y, inputs, g, retain_graph=True))
+        full = ops.linear_backward(g, x, w, ops.linear(x, w, b, r, "gelu", 0.5, True)[1], "gelu")
+        want = [v for t, v in zip((x, w, b, r), (*full, g * 0.5)) if t.requires_grad]
+        for a, c in zip(got, want):
+            # sums of other splits, each rounded once to 8 bits
+            assert (a.double() - c.double()).norm() <= 2.0 ** -8 * c.double().norm()
+        assert ("w" in frozen) == (most < n * k * 2)
