@@ -10,7 +10,7 @@ from alphazero_b200 import ops
 
 pytestmark = pytest.mark.gpu
 
-UNIT = {torch.bfloat16: 2.0 ** -9, torch.float16: 2.0 ** -12}
+UNIT = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
@@ -40,9 +40,10 @@ def test_confident_rows_at_large_logits(dtype, base, n, vocab, dim):
     _, _, _, dw, db = ops.linear_cross_entropy_grad(x, w, t, b, scale)
     # d is -left and left in two classes: off as above (the smaller probability to 2^-13 of
     # itself between two kernels), rounded once, summed over equal rows, rounded again
+    # by up to the type's unit roundoff each
     for got in (dw[:, 0], db):
         for v, d in ((c, -left), (c + 1, left)):
-            room = off + 2.0 ** -13 * left + 3 * UNIT[dtype] * left
+            room = off + 2.0 ** -13 * left + 2 * UNIT[dtype] * left
             assert abs(got[v].double().item() / scale - d) <= room
         rest = torch.ones(vocab, dtype=torch.bool, device="cuda")
         rest[c:c + 2] = False
@@ -63,5 +64,5 @@ def test_column_sums_of_confident_rows(n):
         left = math.exp(-gap) / (1 + math.exp(-gap))
         # each p is off by at most 2^-21 as above; sums of equal numbers at most a unit of
         # 2^-24 per addition, of which a column has fewer than 4096 in a row
-        room = 2.0 ** -21 + (2.0 ** -12 + 2.0 ** -9) * left
+        room = 2.0 ** -21 + (2.0 ** -12 + 2.0 ** -8) * left
         assert abs(db[3].item() + left) <= room and abs(db[400].item() - left) <= room
