@@ -25,6 +25,7 @@ from . import engine
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_FLOAT_LIMIT = 2.0 ** 128  # a float32 is below it
 _INDEX_BYTES = {torch.int64: 8, torch.int32: 4}
 
 # The argument structs of minigo_ops.h, field by field.
@@ -411,7 +412,10 @@ def cross_entropy_loss(x, weight, targets, bias=None, grad_scale: float = 1.0):
     """The loss of ``linear_cross_entropy`` for autograd.  The gradients are
     made with the loss, of grad_scale * loss, and multiplied by the incoming
     gradient / grad_scale when the backward pass reaches them; where none can
-    be asked for, only the loss is."""
+    be asked for, only the loss is.  So grad_scale is a finite number that is
+    not 0, in the range of float32."""
+    if not 0.0 < abs(float(grad_scale)) < _FLOAT_LIMIT:
+        raise ValueError(f"grad_scale must be finite and not 0, not {grad_scale}")
     if not _recorded(x, weight, bias):
         return linear_cross_entropy(x, weight, targets, bias)[0]
     return _CrossEntropy.apply(x, weight, bias, targets, float(grad_scale))

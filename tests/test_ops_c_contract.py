@@ -3,6 +3,7 @@ shapes, types and null pointers.  Nothing here reaches a GPU."""
 import ctypes
 
 import pytest
+import torch
 
 from alphazero_b200 import build, ops
 from test_ops_refusals import backward_args, embed_args, entropy_args, linear_args, refused
@@ -57,3 +58,10 @@ def test_scoring_scratch_does_not_grow_with_the_rows(L, vocab):
         assert L.mg_cross_entropy_workspace(entropy_args(n=n, vocab=vocab), ctypes.byref(need)) == 0
         sizes.append(need.value)
     assert sizes[1] - sizes[0] < 64 << 20 and sizes[1] < 2 << 30
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.0, float("inf"), float("nan"), 1e39])
+def test_a_gradient_scale_that_cannot_be_divided_by_is_refused(scale):
+    f, t = torch.zeros(4, 8, dtype=torch.bfloat16, requires_grad=True), torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(ValueError, match="grad_scale"):
+        ops.cross_entropy_loss(f, f, t, grad_scale=scale)
