@@ -65,6 +65,13 @@ def _raise(code: int):
 _stream = torch._C._cuda_getCurrentRawStream
 
 
+def _pack(layout: struct.Struct, *values) -> bytes:
+    try:
+        return layout.pack(*values)
+    except struct.error as e:  # everything else has been checked
+        raise TypeError("a scale must be a number") from e
+
+
 def _call(name: str, args: bytes, like, device: int) -> None:
     L = _LIB or lib()
     need = ctypes.c_size_t()
@@ -193,8 +200,8 @@ def embed(tokens, table, scale: float = 1.0):
         row = dim
     n = t.numel()
     out = table.new_empty((n, dim) if t is tokens else (*tokens.shape, dim))
-    code = (_LIB or lib()).mg_embed(_EMBED.pack(t.data_ptr(), table.data_ptr(), out.data_ptr(), n, vocab,
-                                                dim, t_stride, row, scale, dt, tb, d), _stream(d))
+    code = (_LIB or lib()).mg_embed(_pack(_EMBED, t.data_ptr(), table.data_ptr(), out.data_ptr(), n, vocab,
+                                                 dim, t_stride, row, scale, dt, tb, d), _stream(d))
     if code:
         _raise(code)
     return out
@@ -213,8 +220,8 @@ def embed_backward(grad, tokens, vocab: int, scale: float = 1.0):
     n, dim = g.shape
     out = grad.new_empty((vocab, dim))
     _call("mg_embed_backward",
-          _EMBED_BACKWARD.pack(t.data_ptr(), g.data_ptr(), out.data_ptr(), n, vocab, dim, t_stride,
-                               g.stride(0), scale, dt, tb, d), grad, d)
+          _pack(_EMBED_BACKWARD, t.data_ptr(), g.data_ptr(), out.data_ptr(), n, vocab, dim, t_stride,
+                g.stride(0), scale, dt, tb, d), grad, d)
     return out
 
 
@@ -245,9 +252,9 @@ def linear(x, weight, bias=None, residual=None, activation: str = "none",
     y = x.new_empty(shape)
     z = x.new_empty(shape) if keep_preactivation else None
     _call("mg_linear",
-          _LINEAR.pack(x2.data_ptr(), weight.data_ptr(), _ptr(b), _ptr(r), y.data_ptr(), _ptr(z),
-                       x2.shape[0], n, k, *x2.stride(), *weight.stride(), r_row, r_col,
-                       residual_scale, act, dt, d), x, d)
+          _pack(_LINEAR, x2.data_ptr(), weight.data_ptr(), _ptr(b), _ptr(r), y.data_ptr(), _ptr(z),
+                x2.shape[0], n, k, *x2.stride(), *weight.stride(), r_row, r_col, residual_scale,
+                act, dt, d), x, d)
     return (y, z) if keep_preactivation else y
 
 
@@ -280,10 +287,9 @@ def linear_backward(grad, x, weight, preactivation=None, activation: str = "none
     dw = x.new_empty((n, k)) if weight_grad else None
     db = x.new_empty((n,)) if bias else None
     _call("mg_linear_backward",
-          _LINEAR_BACKWARD.pack(g.data_ptr(), x2.data_ptr(), weight.data_ptr(), _ptr(z),
-                                _ptr(dx), _ptr(dw), _ptr(db), g.shape[0], n, k,
-                                *g.stride(), *x2.stride(), *weight.stride(), z_row, z_col, act, dt,
-                                d, 0), x, d)
+          _pack(_LINEAR_BACKWARD, g.data_ptr(), x2.data_ptr(), weight.data_ptr(), _ptr(z),
+                _ptr(dx), _ptr(dw), _ptr(db), g.shape[0], n, k, *g.stride(), *x2.stride(),
+                *weight.stride(), z_row, z_col, act, dt, d, 0), x, d)
     return dx, dw, db
 
 
@@ -308,10 +314,9 @@ def _cross_entropy(x, weight, targets, bias, grad_scale, gradients):
         dw = x.new_empty((vocab, dim))
         db = x.new_empty((vocab,)) if b is not None else None
     _call("mg_cross_entropy",
-          _CROSS_ENTROPY.pack(x2.data_ptr(), weight.data_ptr(), _ptr(b), t.data_ptr(),
-                              loss.data_ptr(), rows.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db),
-                              t.shape[0], vocab, dim, *x2.stride(), *weight.stride(), t_stride,
-                              grad_scale, dt, tb, d), x, d)
+          _pack(_CROSS_ENTROPY, x2.data_ptr(), weight.data_ptr(), _ptr(b), t.data_ptr(),
+                loss.data_ptr(), rows.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), t.shape[0], vocab,
+                dim, *x2.stride(), *weight.stride(), t_stride, grad_scale, dt, tb, d), x, d)
     return loss, rows, dx, dw, db
 
 
@@ -328,7 +333,7 @@ def linear_cross_entropy_grad(x, weight, targets, bias=None, grad_scale: float =
     """(loss, row_loss, dx, dw, db): ``linear_cross_entropy`` and the
     gradients of grad_scale * loss (db None without a bias) in one call.
     float16 gradients need a grad_scale that keeps them in range."""
-    return _cross_entropy(x, weight, targets, bias, float(grad_scale), True)
+    return _cross_entropy(x, weight, targets, bias, grad_scale, True)
 
 
 # ---- autograd ----
