@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
+from operator import index
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -218,6 +219,9 @@ def embed_backward(grad, tokens, vocab: int, scale: float = 1.0):
     g = _rows(_matrix(grad, "grad"))
     t, t_stride = _flat(tokens)
     n, dim = g.shape
+    vocab = index(vocab)
+    if not 0 < vocab < 1 << 31:
+        raise ValueError(f"vocab must be from 1 to 2^31 - 1, not {vocab}")
     out = grad.new_empty((vocab, dim))
     _call("mg_embed_backward",
           _pack(_EMBED_BACKWARD, t.data_ptr(), g.data_ptr(), out.data_ptr(), n, vocab, dim, t_stride,

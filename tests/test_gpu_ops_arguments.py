@@ -20,3 +20,12 @@ def test_scales(value):
     # whatever float32 holds is a scale
     assert torch.isinf(ops.embed(t, w, float("inf"))).all()
     assert torch.isfinite(ops.linear(x, w, residual=make(4, 6), residual_scale=torch.tensor(0.5))).all()
+
+
+@pytest.mark.parametrize("vocab,error", [(-1, ValueError), (0, ValueError), (1 << 31, ValueError), (1 << 40, ValueError),
+                                         (1 << 70, ValueError), (6.0, TypeError), ("6", TypeError), (None, TypeError)])
+def test_vocabularies(vocab, error):
+    """Refused before anything of that size is allocated."""
+    x, t = make(4, 8), integers(4, 0, 6)
+    with pytest.raises(error):
+        ops.embed_backward(x, t, vocab)
