@@ -62,8 +62,8 @@ def _raise(code: int):
     raise ValueError(message) if code == -1 else RuntimeError(message)
 
 
-# The current stream of a device by index, without a Stream object.
-_stream = torch._C._cuda_getCurrentRawStream
+# The current stream of a device by index, without a Stream object (a torch without CUDA has none).
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _pack(layout: struct.Struct, *values) -> bytes:
