@@ -311,6 +311,23 @@ def aggregate_rate(world, per_rank_units, steps, max_seconds):
     return world * per_rank_units * steps / max_seconds
 
 
+def reference_positions(board, batch, max_moves):
+    """The workload's positions, from the reference's own src/game.cpp (bit-identical
+    to the product's generator).  Where there is no reference tree to build that
+    from, a child process generates them, so that the reference arm's own process
+    maps no product library either way."""
+    import oracle
+
+    if oracle.ref_available():
+        return oracle.ref_random_positions(board, batch, 1000, max_moves)
+    with tempfile.TemporaryDirectory(prefix="mgb_bench_") as tmp:
+        path = os.path.join(tmp, "positions")
+        code = ("from alphazero_b200 import host_lib; "
+                f"host_lib.random_positions({board}, {batch}, 1000, {max_moves}).tofile({path!r})")
+        subprocess.run([sys.executable, "-c", code], cwd=ROOT, check=True)
+        return np.fromfile(path, np.float32).reshape(batch, -1)
+
+
 def run_reference(args, wl):
     world, rank, _ = dist_setup()
     if rank != 0:
@@ -321,14 +338,7 @@ def run_reference(args, wl):
     from alphazero_b200 import weights  # seeded numpy weights (no native code)
 
     sd = weights.make_state_dict(board, filters, blocks, seed=0, variant="init")
-    # the reference's own src/game.cpp generates the positions (bit-identical
-    # to the product's generator; the reference arm maps no product library
-    # where a reference tree was there to build it from)
-    if oracle.ref_available():
-        x = oracle.ref_random_positions(board, batch, 1000, max_moves)
-    else:
-        from alphazero_b200 import host_lib
-        x = host_lib.random_positions(board, batch, 1000, max_moves)
+    x = reference_positions(board, batch, max_moves)
     threads = os.cpu_count() or 1
     orc = oracle.EigenOracle(sd)
     t0 = time.perf_counter()
