@@ -8,6 +8,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <exception>
+#include <new>
 #include <string>
 
 #include "ptx_sm100.cuh"
@@ -179,6 +181,16 @@ private:
 
 std::string& last_op_error();  // of the calling thread
 
+// Leaves a message, or where there is no memory for one, none.
+inline int failed(int code, const char* what) noexcept {
+    try {
+        last_op_error().clear();
+        last_op_error() = what;
+    } catch (...) {
+    }
+    return code;
+}
+
 // Runs a C entry's body: any failure becomes a code and a message.
 template <class F>
 int guarded(F&& body) noexcept {
@@ -186,13 +198,13 @@ int guarded(F&& body) noexcept {
         body();
         return MG_OK;
     } catch (const OpFailure& f) {
-        try {
-            last_op_error() = f.what;
-        } catch (...) {
-        }
-        return f.code;
+        return failed(f.code, f.what.c_str());
+    } catch (const std::bad_alloc&) {
+        return failed(MG_E_STATE, "out of host memory");
+    } catch (const std::exception& e) {
+        return failed(MG_E_STATE, e.what());
     } catch (...) {
-        return MG_E_STATE;
+        return failed(MG_E_STATE, "unknown exception");
     }
 }
 
