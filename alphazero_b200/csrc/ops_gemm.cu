@@ -761,7 +761,7 @@ __device__ __forceinline__ bool rows_epilogue(const KernelArgs& a, const RowsEpi
         const bool any = __any_sync(~0u, bad);
         if (lane == 0) reinterpret_cast<uint8_t*>(e.clean.use)[m0 / 32] = any;
         // (two warps may copy a step, and then write the same)
-        if (any) clean_step(e.clean, m0 / kStepRows, m, e.target, lane, 32);
+        if (__builtin_expect(any, false)) clean_step(e.clean, m0 / kStepRows, m, e.target, lane, 32);
     }
     if (row >= m) return true;
     if (live && (target & 96) == first) {

@@ -85,15 +85,30 @@ struct CleanRows {
     int64_t dim = 0;
 };
 
-// One step's copy, by `count` threads.
+// One step's copy, by `count` threads (whole warps): a warp per row, 16 bytes
+// per lane where rows lie along x (a StagedOperand's are 16-byte aligned).
+// Small code, since kernels carry it that hardly ever run it: 32768 rows of 256,
+// 362 classes take 99 us instead of 54 where 3% of the rows are NaN and not counted.
 __device__ __forceinline__ void clean_step(const CleanRows& c, int step, int rows, const Indices& target, int thread,
                                            int count) {
-    const bool along = c.col == 1;  // rows of x
+    const int lane = thread & 31, first = step * kStepRows, end = min(first + kStepRows, rows);
+    const bool along = c.col == 1;
 #pragma unroll 1
-    for (int64_t e = thread; e < kStepRows * c.dim; e += count) {
-        const int64_t i = (int64_t)step * kStepRows + (along ? e / c.dim : e % kStepRows);
-        const int64_t j = along ? e % c.dim : e / kStepRows;
-        if (i < rows) c.clean[i * c.clean_row + j * c.clean_col] = target.at(i) >= 0 ? c.x[i * c.row + j * c.col] : 0;
+    for (int i = first + thread / 32; i < end; i += count / 32) {
+        const bool keep = target.at(i) >= 0;
+        const uint16_t* const in = c.x + i * c.row;
+        uint16_t* const out = c.clean + i * c.clean_row;
+        int64_t j = lane;
+        if (along) {
+#pragma unroll 1
+            for (j = lane * 8; j + 8 <= c.dim; j += 256) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(in + j));
+                *reinterpret_cast<uint4*>(out + j) = keep ? v : make_uint4(0, 0, 0, 0);
+            }
+            j = c.dim / 8 * 8 + lane;
+        }
+#pragma unroll 1
+        for (; j < c.dim; j += 32) out[j * c.clean_col] = keep ? in[j * c.col] : 0;
     }
 }
 
@@ -172,9 +187,10 @@ void encode_operand(CUtensorMap* map, int dtype, const StagedOperand& s, int64_t
 // A number in [0, 1] in 16 bits: 4 bits of exponent and 12 of fraction, no
 // sign (relative error 2^-14 from 2^-14 up, absolute 2^-28 below).  A block's
 // largest is 1, so the range is where the block's probabilities are, and the
-// rounding is far below the one to bf16 or fp16 that follows.  It is an fp32
-// value scaled by 2^-112, whose exponent then has four bits, cut to its top
-// 16 bits below the exponent's fourth.
+// rounding is far below the one to bf16 or fp16 that follows, down to 2^-19 of the
+// block's largest; what is below 2^-29 of it is lost.  It is an fp32 value scaled
+// by 2^-112, whose exponent then has four bits, cut to its top 16 bits below the
+// exponent's fourth: bits << 11, times 2^112.
 __device__ __forceinline__ uint32_t prob16(float v) {
     return (__float_as_uint(v * 0x1p-112f) + 0x400u) >> 11;
 }
@@ -183,7 +199,6 @@ __device__ __forceinline__ uint32_t prob16(float v) {
 __device__ __forceinline__ uint32_t prob16x2(float low, float high) {
     return __byte_perm(prob16(low), prob16(high), 0x5410);
 }
-__device__ __forceinline__ float prob16_value(uint32_t u) { return __uint_as_float(u << 11) * 0x1p112f; }
 
 // Copies of operands that do not lie right, made by blocks of the kernel that
 // comes first in a call (a launch of their own would cost as much as the
