@@ -72,8 +72,8 @@ __device__ __forceinline__ float loss_of(float m, float s, float at) {
 
 // A few rows without gradients: their losses and the mean in one launch, by a
 // cluster whose CTAs have two rows each and leave their losses with the first.
-// Bound by latency: 7.6 us for 13 rows of 4096 blocks of columns, where a block per
-// row and another launch for the mean took 8.8 and the step between them.
+// Bound by latency: 7 us for 13 rows of 2364 blocks of columns (65536 classes); a
+// block per row and another launch for the mean took longer.
 constexpr int kFewRows = 16;
 
 __global__ void __cluster_dims__(kFewRows / 2, 1, 1) __launch_bounds__(1024)
@@ -118,8 +118,7 @@ __global__ void __cluster_dims__(kFewRows / 2, 1, 1) __launch_bounds__(1024)
     *loss = all / fmaxf(count, 1.0f);
 }
 
-// Bound by latency: 5 us for 13 rows of 4096 blocks of columns, 13 for 4096
-// rows of 513.
+// Bound by latency: 13 us for 4096 rows of 513 blocks of columns.
 // Maximum m and log2 of the sum s of exp(l - m) and the loss per row, and the
 // loss summed per block: a thread per row where a row has few blocks of
 // columns; with many, 32 threads per row, or where there are few rows too, a
@@ -260,7 +259,7 @@ __global__ void __launch_bounds__(256)
                 if (r + deep * q >= r1) break;
                 const uint32_t w[4] = {u[q].x, u[q].y, u[q].z, u[q].w};
                 // a row that is not counted (whatever it holds) and one of -inf have no probabilities
-                float scale = exp2_flush((m[q] - f[q].x) * 1.4426950408889634f - f[q].y) * 0x1p112f;  // prob16_value's
+                float scale = exp2_flush((m[q] - f[q].x) * 1.4426950408889634f - f[q].y) * 0x1p112f;  // Prob16's
                 if (f[q].y == -INFINITY || t[q] < 0) scale = 0.0f;
                 float v[8];
 #pragma unroll

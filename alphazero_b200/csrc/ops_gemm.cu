@@ -26,12 +26,12 @@
 // The sums are double-buffered in TMEM: a tile's epilogue overlaps the next
 // tile's products.  Every wait is bounded (ptx_sm100.cuh).
 //
-// Long products are bound by the tensor cores: 8192 x 4096 x 4096 with GELU
-// 175 us, 1.57 PFLOP/s with the tensor pipe 86% active; 16384 x 4096 x 4096
-// with GELU, residual and z kept 384 us, 1.43.  In a loop both, like any such
-// product, are bound by the power cap.  A product with 256 elements to a sum
-// is bound by its epilogue's memory traffic: 184832 x 256 x 256 with a
-// residual 61 us, 4.6 TB/s.
+// Long products are bound by the tensor cores, and in a loop, as any such
+// product, by the power cap: 8192 x 4096 x 4096 with GELU 210 us a call in a loop,
+// 1.31 PFLOP/s (a profiled launch by itself 175, with the tensor pipe 86% active);
+// 16384 x 4096 x 4096 with GELU, residual and z kept 500, 1.10 (one call after a
+// pause 424, 1.30).  A product with 256 elements to a sum is bound by its
+// epilogue: 184832 x 256 x 256 with a residual 66 us, 4.3 TB/s, without it 45.
 #include "ops_gemm.cuh"
 
 #include <algorithm>

@@ -10,8 +10,10 @@ ValueError (wrong shapes or values) or TypeError (wrong types or devices);
 failures of the library raise RuntimeError.  There is no CPU fallback.
 
 ``embedding``, ``linear_layer`` and ``cross_entropy_loss`` are the same
-operators for torch's autograd (first derivatives; a second one raises).  The reference trains with torch on its own
-(scripts/train.py) and has no counterpart.
+operators for torch's autograd (first derivatives; a second one raises).  The
+others record nothing: what they return requires no gradient, whatever their
+inputs do.  The reference trains with torch on its own (scripts/train.py) and
+has no counterpart.
 """
 from __future__ import annotations
 

@@ -148,8 +148,11 @@ int mg_linear_backward(const mg_linear_backward_args* args, void* workspace, siz
  * With dx, dw (and db where there is a bias) set, also the gradients of
  * grad_scale * loss: d = (softmax(l) - onehot(t)) * grad_scale / counted
  * (softmax 0 where every logit is -inf), dx = d weight, dw = d^T x, db = sum
- * of d over rows; rows that are not counted give nothing.  d is rounded to
- * the operands' type once.  FP16 gradients are small: give a grad_scale
+ * of d over rows; rows that are not counted give nothing, whatever x holds
+ * there (an infinity or NaN in weight shows in every row's dx).  d is rounded
+ * to the operands' type once; before that, probabilities are held to 2^-14 of
+ * themselves, and to 2^-28 of the largest of up to 128 neighbouring classes
+ * where they are below 2^-14 of it.  FP16 gradients are small: give a grad_scale
  * that keeps them in range.  All three gradients, or none, except that db
  * is NULL without a bias.  n may be 0; vocab and dim may not.  n, vocab and dim
  * are below 2^31 - 1024. */
